@@ -39,9 +39,14 @@ def _hipcc() -> str:
     raise RuntimeError("hipcc not found")
 
 
-# Per-file compiler flags. conv_igemm.hip keeps its in-flight loads in accumulation registers that only inline asm names, so the
-# compiler must keep the MFMA accumulators in vector registers there (with accumulation registers in the clobber lists it would
-# otherwise select the accumulation-register form of the MFMAs). tools/check_async_loads.py verifies the generated code.
+# Packed FP32 instructions (v_pk_add / mul / fma_f32) are kept out of all device code: some of their forms have given wrong results on
+# MI355X now and then, and -O3 selects them by itself from scalar float code. The host pass does not know the feature and says so.
+HIP_FLAGS = ("-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops")
+# Compiler flags of single files, in place of HIP_FLAGS. conv_igemm.hip keeps its in-flight loads in accumulation registers that only
+# inline asm names, so the compiler must keep the MFMA accumulators in vector registers there (with accumulation registers in the clobber
+# lists it would otherwise select the accumulation-register form of the MFMAs). tools/check_async_loads.py verifies the generated code.
+# It is the one file without HIP_FLAGS: with packed math off its 128 x 128 weight-gradient kernel needs so many registers that the compiler
+# takes hidden ones (the check then names them).
 EXTRA_FLAGS = {"conv_igemm.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form")}
 
 
@@ -73,7 +78,7 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -
         o = OBJ / (s.stem + ".hip.o")
         if force or _newer(s, o, headers):
             tasks.append([hipcc, f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17", "-fvisibility=hidden",
-                          "-Wno-unused-result", "-Wno-unused-value", *EXTRA_FLAGS.get(s.name, ()), "-I", str(CSRC), "-c", str(s),
+                          "-Wno-unused-result", "-Wno-unused-value", *EXTRA_FLAGS.get(s.name, HIP_FLAGS), "-I", str(CSRC), "-c", str(s),
                           "-o", str(o)])
     for s in cpp_srcs:
         o = OBJ / (s.stem + ".cpp.o")
