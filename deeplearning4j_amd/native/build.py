@@ -47,7 +47,9 @@ HIP_FLAGS = ("-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops")
 # lists it would otherwise select the accumulation-register form of the MFMAs). tools/check_async_loads.py verifies the generated code.
 # It is the one file without HIP_FLAGS: with packed math off its 128 x 128 weight-gradient kernel needs so many registers that the compiler
 # takes hidden ones (the check then names them).
-EXTRA_FLAGS = {"conv_igemm.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form")}
+# legacy_ops.hip: the compiler cannot select code for its vector kernels with the feature off; without the vectoriser that packs scalar
+# code it emits no packed FP32 either.
+EXTRA_FLAGS = {"conv_igemm.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form"), "legacy_ops.hip": ("-fno-slp-vectorize",)}
 
 
 def _newer(src: Path, dst: Path, extra=()) -> bool:

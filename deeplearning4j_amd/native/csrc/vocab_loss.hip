@@ -10,13 +10,17 @@
 // combine_kernel joins. Backward: the same product again, piece by piece of the vocabulary; the epilogue turns the accumulators into dz
 // (a piece of at most some hundred MiB), and two products consume it: dh += dz W and dW = dz^T h. Rows without a label / teacher entry
 // are left out of all products: rows_kernel writes the list of the others, the kernels read their number on the device.
-#include "gemm_trans.h"
+//
+// fp32 operands go through the 16-bit matrix cores as scaled pairs of halves (gemm_pingpong.h); small calls keep the fp32 matrix cores,
+// which need no conversion of W.
+#include "gemm_pingpong.h"
 
 using namespace gemmcore;
 
 namespace {
 
 constexpr float NEG_INF = -__builtin_inff();
+constexpr int KMAX = 1024;                              // teacher entries per row
 
 __device__ __forceinline__ float load_f(const void* p, int64_t i, int dt) {
   if (dt == DT_F32) return reinterpret_cast<const float*>(p)[i];
@@ -27,6 +31,9 @@ __device__ __forceinline__ void store_f(void* p, int64_t i, int dt, float v) {
   if (dt == DT_F32) reinterpret_cast<float*>(p)[i] = v;
   else if (dt == DT_BF16) reinterpret_cast<uint16_t*>(p)[i] = f2bf(v);
   else reinterpret_cast<uint16_t*>(p)[i] = __builtin_bit_cast(uint16_t, (_Float16)v);
+}
+__device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int is64) {
+  return is64 ? reinterpret_cast<const int64_t*>(p)[i] : (int64_t)reinterpret_cast<const int*>(p)[i];
 }
 
 // all-lanes reductions over the 16 lanes that share the accumulator rows of a 16x16 block: rotations inside a DPP row, no LDS traffic
@@ -40,19 +47,34 @@ __device__ __forceinline__ float sum16(float v) {
   v += dpp_ror<8>(v); v += dpp_ror<4>(v); v += dpp_ror<2>(v); return v + dpp_ror<1>(v);
 }
 
+// (max, sum of exp) pairs: the join of two; a pair without a finite score has max -inf and sum 0 (or NaN)
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float nm = fmaxf(m, m2);
+  if (nm == NEG_INF) s += s2;
+  else s = s * __expf(m - nm) + s2 * __expf(m2 - nm);
+  m = nm;
+}
+
+// Factors that the halves' scaling (fp32) and the range of fp16 gradients bring in; all powers of two, 1 for other types.
+struct Scales {
+  float z;          // scores = z * product
+  float h, w;       // of the operands' halves
+  float dh, dw, db; // gradients = factor * product (sum)
+};
+
 // ------------------------------------------------------------------------------------------------------------------------ rows
 // rows[0 .. count) = rows that take part, in order; rows[count .. N) = the others; loss of the others = 0.
 // One workgroup: a scan of N flags, 1024 at a time.
-__global__ void __launch_bounds__(1024) rows_kernel(const int64_t* __restrict__ lab64, const int* __restrict__ lab32, int64_t ignore,
-                                                    const float* __restrict__ mass, int N, int* __restrict__ rows, int* __restrict__ count,
+__global__ void __launch_bounds__(1024) rows_kernel(const void* __restrict__ labels, int lab64, int64_t ignore, const float* __restrict__ mass, int N,
+                                                    int* __restrict__ rows, int* __restrict__ count, Scales* __restrict__ sc,
                                                     float* __restrict__ loss) {
   __shared__ int wsum[16];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   int done = 0;
-  for (int base = 0; base < N; base += 1024) {
-    const int n = base + tid;
+  for (int64_t base = 0; base < N; base += 1024) {
+    const int64_t n = base + tid;
     bool ok = false;
-    if (n < N) ok = lab64 ? lab64[n] != ignore : lab32 ? (int64_t)lab32[n] != ignore : mass[n] != 0.f;
+    if (n < N) ok = labels ? load_index(labels, n, lab64) != ignore : mass[n] != 0.f;
     const unsigned long long b = __ballot(ok);
     if (lane == 0) wsum[wid] = __popcll(b);
     __syncthreads();
@@ -60,146 +82,210 @@ __global__ void __launch_bounds__(1024) rows_kernel(const int64_t* __restrict__ 
     for (int w = 0; w < 16; ++w) { if (w < wid) before += wsum[w]; all += wsum[w]; }
     const int at = done + before + __popcll(b & ((1ull << lane) - 1));
     if (n < N) {
-      if (ok) rows[at] = n;
-      else { rows[N - 1 - (n - at)] = n; loss[n] = 0.f; }      // n - at rows before this one do not take part
+      if (ok) rows[at] = (int)n;
+      else { rows[N - 1 - (n - at)] = (int)n; loss[n] = 0.f; }   // n - at rows before this one do not take part
     }
     done += all;
     __syncthreads();
   }
-  if (tid == 0) *count = done;
+  if (tid == 0) { *count = done; *sc = Scales{1.f, 1.f, 1.f, 1.f, 1.f, 1.f}; }
 }
 
 // ------------------------------------------------------------------------------------------------------------------------ teacher
-// One wave per row: p = softmax(teacher / T) over the entries with an index >= 0, ent = sum p log p, mass = sum p as 1 or 0 (0: no entry
-// with a finite weight), and psum_k = the summed p of all entries with entry k's index (an index may come twice). K <= 1024.
-__global__ void __launch_bounds__(256) teacher_kernel(const void* __restrict__ idx, int idx64, const void* __restrict__ t, int tdt, int N, int K,
-                                                      float invT, float* __restrict__ p, float* __restrict__ psum, float* __restrict__ ent,
-                                                      float* __restrict__ mass) {
-  __shared__ int si[4][1024];
-  __shared__ float sp[4][1024];
+struct TeacherP {
+  const void* idx; int idx64;
+  const void* t; int tdt;
+  int N, V, K, P2;                       // P2: K rounded up to a power of two
+  float invT;
+  int tile, tiles;                       // column tiles of the score kernels
+  int* sidx; float* sp; float* psum;     // [N][K], by index
+  unsigned short* first;                 // [tiles + 1][N]: entries before column tile t
+  float* ent; float* mass;
+};
+// One wave per row: p = softmax(teacher / T) over the entries with an index >= 0, ent = sum p log p, mass = 1, or 0 where no entry has a
+// weight. The entries are sorted by index (a bitonic sort in LDS), so that a column tile finds its own between first[t] and first[t + 1],
+// and psum, the summed p of all entries with one index, is a run. An index outside the vocabulary, a NaN or +inf makes ent NaN.
+__global__ void __launch_bounds__(256) teacher_kernel(const TeacherP p) {
+  extern __shared__ char smem[];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int n = blockIdx.x * 4 + wid;
-  if (n >= N) return;                                   // waves work alone below: no block barrier
+  uint64_t* key = reinterpret_cast<uint64_t*>(smem) + wid * p.P2;            // index << 10 | entry
+  float* w = reinterpret_cast<float*>(smem + 4 * 8 * p.P2) + wid * p.P2;
+  if (n >= p.N) return;                                 // waves work alone: no block barrier below
   float m = NEG_INF;
   bool bad = false;
-  for (int k = lane; k < K; k += 64) {
-    const int64_t o = (int64_t)n * K + k;
-    const int64_t i = idx64 ? reinterpret_cast<const int64_t*>(idx)[o] : (int64_t)reinterpret_cast<const int*>(idx)[o];
-    const float v = i < 0 ? NEG_INF : load_f(t, o, tdt) * invT;
-    si[wid][k] = i > 0x7fffffff ? 0x7fffffff : (int)i;
-    sp[wid][k] = v;
-    bad |= !(v < __builtin_inff());                     // NaN or +inf
+  for (int k = lane; k < p.P2; k += 64) {
+    uint64_t q = ~0ull;
+    float v = NEG_INF;
+    if (k < p.K) {
+      const int64_t o = (int64_t)n * p.K + k, i = load_index(p.idx, o, p.idx64);
+      if (i >= 0) {
+        v = load_f(p.t, o, p.tdt) * p.invT;
+        bad |= !(v < __builtin_inff()) || (i >= p.V && v != NEG_INF);
+        if (i < p.V) q = (uint64_t)i << 10 | (uint64_t)k;
+      }
+    }
+    key[k] = q;
+    w[k] = v;
     m = fmaxf(m, v);
   }
   bad = __any(bad);
   m = wave_max(m);
   float s = 0.f;
-  for (int k = lane; k < K; k += 64) {
-    const float e = m == NEG_INF ? 0.f : __expf(sp[wid][k] - m);
-    s += e;
-  }
+  if (m != NEG_INF)
+    for (int k = lane; k < p.P2; k += 64) s += __expf(w[k] - m);
   s = wave_sum(s);
   const float inv = s > 0.f ? 1.f / s : 0.f, ls = s > 0.f ? __logf(s) : 0.f;
   float h = 0.f;
-  for (int k = lane; k < K; k += 64) {
-    const float d = sp[wid][k] - m;
-    float w = m == NEG_INF ? 0.f : __expf(d) * inv;
-    if (w > 0.f) h += w * (d - ls);
-    if (bad) w = __builtin_nanf("");
-    sp[wid][k] = w;
-    p[(int64_t)n * K + k] = w;
+  for (int k = lane; k < p.P2; k += 64) {
+    const float d = w[k] - m;
+    const float e = m == NEG_INF ? 0.f : __expf(d) * inv;
+    if (e > 0.f) h += e * (d - ls);
+    w[k] = e;
   }
   h = wave_sum(h);
   if (lane == 0) {
-    ent[n] = bad ? __builtin_nanf("") : h;
-    mass[n] = bad || s > 0.f ? 1.f : 0.f;
+    p.ent[n] = bad ? __builtin_nanf("") : h;
+    p.mass[n] = bad || s > 0.f ? 1.f : 0.f;
   }
+  for (int size = 2; size <= p.P2; size <<= 1)
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      for (int c = lane; c < p.P2 / 2; c += 64) {
+        const int i = (c / step) * 2 * step + (c % step), j = i + step;
+        const uint64_t a = key[i], b = key[j];
+        if ((a > b) == ((i & size) == 0)) { key[i] = b; key[j] = a; }
+      }
+    }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  for (int k = lane; k < K; k += 64) {
-    const int mine = si[wid][k];
-    float q = 0.f;
-    for (int j = 0; j < K; ++j) q += si[wid][j] == mine ? sp[wid][j] : 0.f;
-    psum[(int64_t)n * K + k] = q;
+  for (int k = lane; k < p.K; k += 64) {
+    const uint64_t q = key[k];
+    const bool there = q != ~0ull;
+    const int i = there ? (int)(q >> 10) : 0x7fffffff;
+    float sum = 0.f;
+    if (there) {
+      int a = k;
+      while (a > 0 && (int)(key[a - 1] >> 10) == i) --a;
+      for (; a < p.K && key[a] != ~0ull && (int)(key[a] >> 10) == i; ++a) sum += w[key[a] & 1023];
+    }
+    const int64_t o = (int64_t)n * p.K + k;
+    p.sidx[o] = i;
+    p.sp[o] = there ? w[q & 1023] : 0.f;
+    p.psum[o] = sum;
+  }
+  for (int t = lane; t <= p.tiles; t += 64) {
+    const uint64_t lim = (uint64_t)t * p.tile << 10;
+    int lo = 0, hi = p.K;                               // entries below the tile's first column
+    while (lo < hi) { const int mid = (lo + hi) >> 1; if (key[mid] < lim) lo = mid + 1; else hi = mid; }
+    p.first[(int64_t)t * p.N + n] = (unsigned short)lo;
   }
 }
 
-// z'[m, i_k] for the entries that count, and cross_n = sum_k p_k z'[n, i_k]: one wave per row, dot products along the hidden axis
-// (W rows are contiguous here; `vstride` 1 and `dstride` V walk the [D, V] layout). An index >= V makes the row NaN.
-__global__ void __launch_bounds__(256) gather_kernel(const void* __restrict__ h, int64_t ldh, const void* __restrict__ W, int64_t vstride,
-                                                     int64_t dstride, const void* __restrict__ bias, int bdt, int dt, int D, int V,
-                                                     const void* __restrict__ idx, int idx64, int K, float invT, const float* __restrict__ p,
-                                                     const int* __restrict__ rows, const int* __restrict__ count, float* __restrict__ zk,
-                                                     float* __restrict__ cross) {
-  const int lane = threadIdx.x & 63;
-  const int m = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (m >= *count) return;
-  const int n = rows[m];
-  float acc = 0.f;
-  for (int k = 0; k < K; ++k) {
-    const int64_t o = (int64_t)n * K + k;
-    const float pk = p[o];
-    if (pk == 0.f) continue;
-    const int64_t i = idx64 ? reinterpret_cast<const int64_t*>(idx)[o] : (int64_t)reinterpret_cast<const int*>(idx)[o];
-    float z = __builtin_nanf("");
-    if (i >= 0 && i < V) {
-      float s = 0.f;
-      for (int d = lane; d < D; d += 64) s += load_f(h, n * ldh + d, dt) * load_f(W, i * vstride + d * dstride, dt);
-      z = (wave_sum(s) + (bias ? load_f(bias, i, bdt) : 0.f)) * invT;
+// ------------------------------------------------------------------------------------------------------------------------ operands
+// largest finite |x| of W (workgroups 0 .. AMAX_W - 1) and of the rows of H that take part (the others): one value per workgroup
+constexpr int AMAX_W = 512, AMAX_H = 128;
+__global__ void __launch_bounds__(256) amax_kernel(const float* __restrict__ W, int64_t ldw, int wr, int wc, const float* __restrict__ H, int64_t ldh,
+                                                   int D, const int* __restrict__ rows, const int* __restrict__ count, float* __restrict__ out) {
+  __shared__ float red[16];
+  const bool is_w = blockIdx.x < AMAX_W;
+  const int R = is_w ? wr : *count, C = is_w ? wc : D, step = is_w ? AMAX_W : AMAX_H;
+  float m = 0.f;
+  for (int r = is_w ? blockIdx.x : blockIdx.x - AMAX_W; r < R; r += step) {
+    const float* x = is_w ? W + r * ldw : H + rows[r] * ldh;
+#pragma unroll 4
+    for (int c = threadIdx.x; c < C; c += 256) {
+      const float v = fabsf(x[c]);
+      m = fmaxf(m, v < __builtin_inff() ? v : 0.f);
     }
-    if (lane == 0) zk[o] = z;
-    acc += pk * z;
   }
-  if (lane == 0) cross[n] = acc;
+  m = block_max(m, red);
+  if (threadIdx.x == 0) out[blockIdx.x] = m;
+}
+
+// a power of two that puts m into [2^13, 2^14)
+__device__ __forceinline__ float scale_for(float m) {
+  if (!(m > 0.f)) return 1.f;
+  int e;
+  frexpf(m, &e);
+  return ldexpf(1.f, min(max(14 - e, -100), 100));
+}
+
+__device__ __forceinline__ void halves(float v, _Float16& hi, _Float16& lo) {
+  hi = (_Float16)v;
+  const float d = v - (float)hi;
+  lo = (_Float16)(d == d ? d : 0.f);                    // inf - inf: an infinity stays in the first half alone
+}
+
+// W and the packed rows of H as scaled halves, 4 values per thread and step; columns [C, Cp) are zeros. Workgroups [0, gw) take W, the others H.
+struct SplitP {
+  const float* W; int64_t ldw; int wr, wc, wcp; _Float16* wo;
+  const float* H; int64_t ldh; int D, Dp; _Float16* ho; int hcap;      // hcap: rows of one half of ho
+  const int* rows; const int* count; const float* amax;
+  Scales* sc;
+  int gw;
+};
+__global__ void __launch_bounds__(256) split_kernel(const SplitP p) {
+  __shared__ float red[16];
+  float mw = 0.f, mh = 0.f;
+  for (int i = threadIdx.x; i < AMAX_W; i += 256) mw = fmaxf(mw, p.amax[i]);
+  for (int i = threadIdx.x; i < AMAX_H; i += 256) mh = fmaxf(mh, p.amax[AMAX_W + i]);
+  const float sw = scale_for(block_max(mw, red)), sh = scale_for(block_max(mh, red));
+  if (blockIdx.x == 0 && threadIdx.x == 0) { p.sc->h = sh; p.sc->w = sw; p.sc->z = 1.f / sh / sw; }
+  const bool is_w = (int)blockIdx.x < p.gw;
+  const int c = *p.count;
+  const int R = is_w ? p.wr : c, C = is_w ? p.wc : p.D, q = (is_w ? p.wcp : p.Dp) / 4;
+  const float s = is_w ? sw : sh;
+  const int64_t n = (int64_t)R * q, step = (int64_t)(is_w ? p.gw : gridDim.x - p.gw) * 256;
+  _Float16* out = is_w ? p.wo : p.ho;
+  const int64_t half = (int64_t)(is_w ? p.wr : p.hcap) * q * 4;
+  for (int64_t i = (int64_t)(is_w ? blockIdx.x : blockIdx.x - p.gw) * 256 + threadIdx.x; i < n; i += step) {
+    const int r = (int)(i / q), d = (int)(i - (int64_t)r * q) * 4;
+    const float* x = is_w ? p.W + r * p.ldw + d : p.H + p.rows[r] * p.ldh + d;
+    _Float16 hi[4], lo[4];
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (d + 4 <= C && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+      const f32x4 f = *reinterpret_cast<const f32x4*>(x);
+      v[0] = f[0]; v[1] = f[1]; v[2] = f[2]; v[3] = f[3];
+    } else {
+      for (int j = 0; j < 4; ++j) v[j] = d + j < C ? x[j] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) halves(v[j] * s, hi[j], lo[j]);
+    __builtin_memcpy(out + i * 4, hi, 8);
+    __builtin_memcpy(out + half + i * 4, lo, 8);
+  }
+}
+
+// the rows that take part, packed
+__global__ void __launch_bounds__(256) pack_kernel(const char* __restrict__ h, int64_t ldh_bytes, const int* __restrict__ rows,
+                                                   const int* __restrict__ count, char* __restrict__ out, int64_t row_bytes) {
+  const int c = *count, m = blockIdx.x;
+  if (m >= c) return;
+  const char* src = h + rows[m] * ldh_bytes;
+  for (int64_t b = threadIdx.x * 16; b < row_bytes; b += 256 * 16) *reinterpret_cast<f32x4*>(out + m * row_bytes + b) = *reinterpret_cast<const f32x4*>(src + b);
 }
 
 // ------------------------------------------------------------------------------------------------------------------------ scores
 struct ScoreP {
-  const void* H; int64_t ldh;            // [N, D]
-  const void* W; int64_t ldw;            // [V, D], or [D, V] (TB)
+  Operand H, W;                          // H: [rows, D] (xlim is the count, set on the device); W: columns of the vocabulary
   const void* bias; int bdt;
-  const int* rows; const int* count;
-  const int64_t* lab64; const int* lab32;
-  int N, D, V, v0, v1;                   // columns [v0, v1) of the vocabulary
+  const int* rows; const int* count; const Scales* sc;
+  const void* labels; int lab64;
+  int N, D, v0, v1;                      // columns [v0, v1) of the vocabulary
   float invT, smooth_v;                  // 1 / T;  e / V
-  // statistics
-  float2* part; float* tz; float* zs;    // part [ntiles][N]; target score [N]; zs [ntiles][N] = sum of z * e / V (or null)
-  // gradient
-  const float* lse; const float* coef; const float* mass;   // per position in `rows` (mass per row, or null = 1)
+  float2* part; float* tz; float* zs;    // statistics: part [ntiles][N]; target score [N]; zs [ntiles][N] = sum of z * e / V (or null)
+  // gradient: coefficient and lse per position in `rows`
+  const float* lse; const float* coef;
   float keep;                            // 1 - e
-  void* G; int64_t ldg;                  // [rows up to a tile][ldg], column v at v - v0
+  char* G; int64_t ldg, glo;             // [rows up to a tile][ldg bytes], column v at v - v0; second half glo bytes behind
+  // teacher entries (first != null)
+  const unsigned short* first; const int* sidx; const float* psum; float* zk; int K;
 };
 
-__device__ __forceinline__ int64_t label_of(const ScoreP& p, int n) {
-  return p.lab64 ? p.lab64[n] : p.lab32 ? (int64_t)p.lab32[n] : -1;
-}
+template <class C> constexpr int score_lds_stats() { return C::BM * 4 * (1 + 3 * C::WN) + C::BM / C::WM * (C::BN + 4) * 4; }
+template <class C> constexpr int score_lds_grad() { return C::BM * (C::BN * C::ESZ + 16) + 3 * C::BM * 4; }
 
-template <class C, bool TB> __device__ __forceinline__ void score_src(FlexSrc<C, false, TB>& src, const ScoreP& p, int m0, int n0, int count) {
-  src.kb = 0; src.ke = p.D;
-  src.kchunk = stage_chunk(stage_row<C>(0)) * C::CH;
-  src.a_kstride = 0;
-  src.b_kstride = p.ldw * C::ESZ;
-#pragma unroll
-  for (int i = 0; i < C::PA; ++i) {
-    int m = m0 + stage_row<C>(i);
-    if (m > count - 1) m = count - 1;                   // results of the rows past the end are not used
-    src.ap[i] = (const char*)p.H + (int64_t)p.rows[m] * p.ldh * C::ESZ;
-  }
-#pragma unroll
-  for (int i = 0; i < C::PB; ++i) {
-    if constexpr (TB) {
-      int row, x;
-      tr_stage_pos<C, C::BN>(i, row, x);
-      src.brow[i] = row;
-      src.bp[i] = (n0 + x < p.v1) ? (const char*)p.W + (int64_t)(n0 + x) * C::ESZ : nullptr;
-    } else {
-      int n = n0 + stage_row<C>(i);
-      if (n > p.V - 1) n = p.V - 1;
-      src.bp[i] = (const char*)p.W + (int64_t)n * p.ldw * C::ESZ;
-    }
-  }
-}
-
-template <class C, bool TB, bool GRAD>
+template <class C, bool TB, bool GRAD, int SEG>
 __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int count = *p.count;
@@ -210,13 +296,14 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
   const int m0 = mt * C::BM, n0 = p.v0 + nt * C::BN;
   typename C::acc_t acc[C::TM][C::TN];
   {
-    FlexSrc<C, false, TB> src;
-    score_src<C, TB>(src, p, m0, n0, count);
-    mainloop_flex<C, FlexSrc<C, false, TB>, false, TB>(smem, src, (p.D + C::BK - 1) / C::BK, acc);
+    Operand H = p.H;
+    H.xlim = count;
+    product<C, false, TB, SEG>(smem, H, p.W, m0, n0, p.D, 0, k_tiles<C, SEG>(p.D), acc);
   }
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int wm = wid / C::WN, wn = wid - wm * C::WN, lc = lane & 15;
   const int row0 = wm * (C::BM / C::WM) + (lane >> 4) * 4, col0 = wn * (C::BN / C::WN) + lc;
+  const float zscale = p.sc->z * p.invT;
   float bv[C::TN];
 #pragma unroll
   for (int j = 0; j < C::TN; ++j) {
@@ -231,11 +318,12 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
     int lab = -1;
     float c = 0.f, l = 0.f;
     if (m < count) {
-      const int n = p.rows[m];
-      const int64_t y = label_of(p, n) - n0;
-      lab = y >= 0 && y < C::BN && y + n0 < p.v1 ? (int)y : -1;
-      if constexpr (GRAD) { c = p.coef[m]; l = p.lse[m]; if (p.mass) sf[3 * C::BM + r] = c * p.mass[n]; else sf[3 * C::BM + r] = c; }
-    } else if constexpr (GRAD) sf[3 * C::BM + r] = 0.f;
+      if (p.labels) {
+        const int64_t y = load_index(p.labels, p.rows[m], p.lab64) - n0;
+        lab = y >= 0 && y < C::BN && y + n0 < p.v1 ? (int)y : -1;
+      }
+      if constexpr (GRAD) { c = p.coef[m]; l = p.lse[m]; }
+    }
     slab[r] = lab;
     if constexpr (GRAD) { sf[C::BM + r] = c; sf[2 * C::BM + r] = l; }
   }
@@ -250,62 +338,131 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
       for (int q = 0; q < 4; ++q) {
         const int r = row0 + i * 16 + q;
         const int lab = slab[r] - col0;
-        float z[C::TN], m = NEG_INF, zsum = 0.f;
+        float z[C::TN], m = NEG_INF;
 #pragma unroll
         for (int j = 0; j < C::TN; ++j) {
-          z[j] = acc[i][j][q] * p.invT + bv[j];
+          z[j] = acc[i][j][q] * zscale + bv[j];
           m = fmaxf(m, z[j]);
           if (lab == j * 16) p.tz[m0 + r] = z[j];
-          if (p.zs && n0 + col0 + j * 16 < p.v1) zsum += z[j] * p.smooth_v;
+          acc[i][j][q] = z[j];
         }
-        float mm = max16(m);
+        const float mm = max16(m);
         const float ref = mm == NEG_INF ? 0.f : mm;
         float s = 0.f;
 #pragma unroll
         for (int j = 0; j < C::TN; ++j) s += __expf(z[j] - ref);  // the maximum passes over a NaN score, the sum keeps it
         s = sum16(s);
-        if (p.zs) zsum = sum16(zsum);
-        if (lc == 0) { sM[wn * C::BM + r] = mm; sS[wn * C::BM + r] = s; if (p.zs) sZ[wn * C::BM + r] = zsum; }
+        if (lc == 0) { sM[wn * C::BM + r] = mm; sS[wn * C::BM + r] = s; }
       }
+    if (p.zs) {                                                  // label smoothing
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float zsum = 0.f;
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j)
+            if (n0 + col0 + j * 16 < p.v1) zsum += acc[i][j][q] * p.smooth_v;
+          zsum = sum16(zsum);
+          if (lc == 0) sZ[wn * C::BM + row0 + i * 16 + q] = zsum;
+        }
+    }
     __syncthreads();
     for (int r = tid; r < C::BM; r += C::NT) {
       if (m0 + r >= count) continue;
       float m = NEG_INF, s = 0.f, z = 0.f;
 #pragma unroll
-      for (int w = 0; w < C::WN; ++w) m = fmaxf(m, sM[w * C::BM + r]);
-#pragma unroll
       for (int w = 0; w < C::WN; ++w) {
-        const float mw = sM[w * C::BM + r], sw = sS[w * C::BM + r];
-        s += mw == NEG_INF ? sw : sw * __expf(mw - m);
+        join(m, s, sM[w * C::BM + r], sS[w * C::BM + r]);
         if (p.zs) z += sZ[w * C::BM + r];
       }
       p.part[(int64_t)nt * p.N + m0 + r] = make_float2(m, s);
       if (p.zs) p.zs[(int64_t)nt * p.N + m0 + r] = z;
     }
+    if (p.first) {
+      // the scores of the teacher's entries: the tile passes through LDS, one row of waves at a time, and every row picks its own
+      constexpr int RW = C::BM / C::WM, P4 = C::BN + 4, TPR = C::NT / RW;
+      float* sz = sf + C::BM * (1 + 3 * C::WN);
+      for (int half = 0; half < C::WM; ++half) {
+        if (wm == half) {
+#pragma unroll
+          for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int j = 0; j < C::TN; ++j) sz[(row0 - wm * RW + i * 16 + q) * P4 + col0 + j * 16] = acc[i][j][q];
+        }
+        __syncthreads();
+        const int r = tid / TPR, m = m0 + half * RW + r;
+        if (m < count) {
+          const int n = p.rows[m];
+          const int64_t t = nt + p.v0 / C::BN;
+          const int e1 = p.first[(t + 1) * p.N + n];
+          for (int e = p.first[t * p.N + n] + tid % TPR; e < e1; e += TPR) {
+            const int64_t o = (int64_t)n * p.K + e;
+            p.zk[o] = sz[r * P4 + p.sidx[o] - n0];
+          }
+        }
+        __syncthreads();
+      }
+    }
   } else {
-    typedef typename Out<C::DT == DT_F32 ? OT_F32 : C::DT == DT_F16 ? OT_F16 : OT_BF16>::T OTy;
     typedef Out<C::DT == DT_F32 ? OT_F32 : C::DT == DT_F16 ? OT_F16 : OT_BF16> O;
+    typedef typename O::T OTy;
 #pragma unroll
     for (int i = 0; i < C::TM; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int r = row0 + i * 16 + q;
         const int lab = slab[r] - col0;
-        const float c = sf[C::BM + r], l = sf[2 * C::BM + r], cm = sf[3 * C::BM + r];
+        const float c = sf[C::BM + r], l = sf[2 * C::BM + r];
 #pragma unroll
         for (int j = 0; j < C::TN; ++j) {
-          float g = cm * __expf(acc[i][j][q] * p.invT + bv[j] - l) - c * p.smooth_v;
+          float g = c * (__expf(acc[i][j][q] * zscale + bv[j] - l) - p.smooth_v);
           if (lab == j * 16) g -= c * p.keep;
           if (n0 + col0 + j * 16 >= p.v1 || m0 + r >= count) g = 0.f;
-          *reinterpret_cast<OTy*>(smem + r * PITCH + (col0 + j * 16) * OSZ) = O::cv(g);
+          const OTy hi = O::cv(g);
+          *reinterpret_cast<OTy*>(smem + r * PITCH + (col0 + j * 16) * OSZ) = hi;
+          if constexpr (SEG == 3) acc[i][j][q] = g - O::fl(hi);
         }
       }
-    __syncthreads();
     constexpr int CPR = C::BN * OSZ / 16;
-    char* out = (char*)p.G + ((int64_t)m0 * p.ldg + (n0 - p.v0)) * OSZ;
-    for (int idx = tid; idx < C::BM * CPR; idx += C::NT) {
-      const int r = idx / CPR, ch = idx - r * CPR;
-      *reinterpret_cast<f32x4*>(out + (int64_t)r * p.ldg * OSZ + ch * 16) = *reinterpret_cast<const f32x4*>(smem + r * PITCH + ch * 16);
+    char* out = p.G + (int64_t)m0 * p.ldg + (int64_t)(n0 - p.v0) * OSZ;
+#pragma unroll
+    for (int half = 0; half < (SEG == 3 ? 2 : 1); ++half) {
+      if (half == 1) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < C::TN; ++j)
+              *reinterpret_cast<OTy*>(smem + (row0 + i * 16 + q) * PITCH + (col0 + j * 16) * OSZ) = O::cv(acc[i][j][q]);
+      }
+      __syncthreads();
+      if (p.first) {
+        // the teacher's entries of this tile, from their exact scores: entries with one index write the same value
+        for (int r = tid; r < C::BM; r += C::NT) {
+          const int m = m0 + r;
+          if (m >= count) break;
+          const int n = p.rows[m];
+          const int64_t t = nt + p.v0 / C::BN;
+          const int e1 = p.first[(t + 1) * p.N + n];
+          for (int e = p.first[t * p.N + n]; e < e1; ++e) {
+            const int64_t o = (int64_t)n * p.K + e;
+            float g = sf[C::BM + r] * (__expf(p.zk[o] - sf[2 * C::BM + r]) - p.psum[o]);
+            if (half == 1) g -= O::fl(O::cv(g));
+            *reinterpret_cast<OTy*>(smem + r * PITCH + (p.sidx[o] - n0) * OSZ) = O::cv(g);
+          }
+        }
+        __syncthreads();
+      }
+      char* o = out + half * p.glo;
+      for (int idx = tid; idx < C::BM * CPR; idx += C::NT) {
+        const int r = idx / CPR, ch = idx - r * CPR;
+        *reinterpret_cast<f32x4*>(o + r * p.ldg + ch * 16) = *reinterpret_cast<const f32x4*>(smem + r * PITCH + ch * 16);
+      }
     }
   }
 }
@@ -314,8 +471,8 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
 struct CombineP {
   const float2* part; const float* zs; const float* tz;
   const int* rows; const int* count;
-  const int64_t* lab64; const int* lab32;
-  const float* ent; const float* cross; const float* mass;      // distillation (ent != null)
+  const void* labels; int lab64;
+  const float* ent; const float* sp; const float* zk; int K;    // distillation (ent != null)
   int N, V, ntiles;
   float keep, T;
   float* lse; float* loss;
@@ -327,47 +484,53 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineP p) {
   const int r = threadIdx.x % R, g = threadIdx.x / R;
   const int m = blockIdx.x * R + r, count = *p.count;
   if ((int)blockIdx.x * R >= count) return;
-  float mx = NEG_INF, s = 0.f, z = 0.f;
+  float mx = NEG_INF, s = 0.f, z = 0.f;                          // z: smoothing term, or sum of p * score over the teacher's entries
+  int n = 0;
   if (m < count) {
+    n = p.rows[m];
 #pragma unroll 4
     for (int t = g; t < p.ntiles; t += GR) {
       const float2 v = p.part[(int64_t)t * p.N + m];
-      const float nm = fmaxf(mx, v.x);
-      if (nm == NEG_INF) s += v.y;
-      else s = s * __expf(mx - nm) + v.y * __expf(v.x - nm);     // exp(-inf) = 0 for a tile without a finite score
-      mx = nm;
-      if (p.zs) z += p.zs[(int64_t)t * p.N + m];
+      join(mx, s, v.x, v.y);
     }
+    if (p.zs)
+      for (int t = g; t < p.ntiles; t += GR) z += p.zs[(int64_t)t * p.N + m];
+    if (p.ent)
+      for (int k = g; k < p.K; k += GR) {
+        const float w = p.sp[(int64_t)n * p.K + k];
+        if (w > 0.f) z += w * p.zk[(int64_t)n * p.K + k];
+      }
   }
   sm[g][r] = mx; ss[g][r] = s; sz[g][r] = z;
-  __syncthreads();
-  if (g != 0 || m >= count) return;
-  for (int w = 1; w < GR; ++w) {
-    const float mw = sm[w][r], nm = fmaxf(mx, mw);
-    if (nm == NEG_INF) s += ss[w][r];
-    else s = s * __expf(mx - nm) + ss[w][r] * __expf(mw - nm);
-    mx = nm;
-    z += sz[w][r];
+  for (int w = GR / 2; w > 0; w >>= 1) {
+    __syncthreads();
+    if (g < w) {
+      join(mx, s, sm[g + w][r], ss[g + w][r]);
+      z += sz[g + w][r];
+      sm[g][r] = mx; ss[g][r] = s; sz[g][r] = z;
+    }
   }
-  const int n = p.rows[m];
+  if (g != 0 || m >= count) return;
   float lse = mx + __logf(s), loss;
   if (p.ent) {
-    loss = p.T * p.T * (p.ent[n] - p.cross[n] + lse * p.mass[n]);
-    if (p.cross[n] != p.cross[n]) lse = p.cross[n];
+    const float h = p.ent[n];
+    loss = p.T * p.T * (h - z + lse);
+    if (h != h) lse = h;                                         // nothing sound to distil from: the row's gradient is NaN too
   } else {
-    const int64_t y = p.lab64 ? p.lab64[n] : (int64_t)p.lab32[n];
-    if (y < 0 || y >= p.V) lse = __builtin_nanf("");            // a label outside the vocabulary: loss and gradient of the row are NaN
-    loss = lse - p.keep * (y < 0 || y >= p.V ? 0.f : p.tz[m]) - z;
+    const int64_t y = load_index(p.labels, n, p.lab64);
+    const bool in = y >= 0 && y < p.V;
+    if (!in) lse = __builtin_nanf("");                           // a label outside the vocabulary: loss and gradient of the row are NaN
+    loss = lse - (in ? p.keep * p.tz[m] : 0.f) - z;
   }
   p.lse[m] = lse;
   p.loss[n] = loss;
 }
 
 // ------------------------------------------------------------------------------------------------------------------------ backward
-// coef[m] = dloss[rows[m]] * T * s,  scale = 1 / s.  s = 1, or for fp16 the power of two that puts the largest coefficient into
-// [2^13, 2^14): dz is at most that large then, and entries down to 2^-38 of it stay above fp16's smallest step.
+// coef[m] = dloss[rows[m]] * T * s.  s = 1, or where the scores' gradient is kept in fp16 the power of two that puts the largest
+// coefficient into [2^13, 2^14): no entry is larger then, and entries down to 2^-38 of it stay above fp16's smallest step.
 __global__ void __launch_bounds__(1024) coef_kernel(const float* __restrict__ dloss, const int* __restrict__ rows, const int* __restrict__ count,
-                                                    float T, int scaled, float* __restrict__ coef, float* __restrict__ scale) {
+                                                    float T, int scaled, float* __restrict__ coef, Scales* __restrict__ sc) {
   __shared__ float red[16];
   const int c = *count;
   float s = 1.f;
@@ -377,120 +540,52 @@ __global__ void __launch_bounds__(1024) coef_kernel(const float* __restrict__ dl
       const float v = fabsf(dloss[rows[m]] * T);
       if (v < __builtin_inff()) mx = fmaxf(mx, v);
     }
-    mx = block_max(mx, red);
-    if (mx > 0.f) {
-      int e;
-      frexpf(mx, &e);                                            // mx in [2^(e-1), 2^e)
-      e = min(max(14 - e, -100), 100);
-      s = ldexpf(1.f, e);
-    }
+    s = scale_for(block_max(mx, red));
   }
   for (int m = threadIdx.x; m < c; m += 1024) coef[m] = dloss[rows[m]] * T * s;
-  if (threadIdx.x == 0) *scale = 1.f / s;
+  if (threadIdx.x == 0) { sc->db = 1.f / s; sc->dh = 1.f / s / sc->w; sc->dw = 1.f / s / sc->h; }
 }
 
-// the rows that take part, packed; zeros up to the next multiple of 256 rows
-__global__ void __launch_bounds__(256) pack_kernel(const char* __restrict__ h, int64_t ldh_bytes, const int* __restrict__ rows,
-                                                   const int* __restrict__ count, char* __restrict__ out, int64_t row_bytes) {
-  const int c = *count, m = blockIdx.x;
-  if (m >= (c + 255) / 256 * 256) return;
-  const char* src = m < c ? h + rows[m] * ldh_bytes : nullptr;
-  for (int64_t b = threadIdx.x * 16; b < row_bytes; b += 256 * 16) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (src) v = *reinterpret_cast<const f32x4*>(src + b);
-    *reinterpret_cast<f32x4*>(out + m * row_bytes + b) = v;
-  }
-}
-
-// the teacher's entries of a piece of dz: dz[m, i_k] = c_m (P q - psum_k), from the exact scores (entries with the same index write the
-// same value)
-__global__ void __launch_bounds__(256) entries_kernel(const void* __restrict__ idx, int idx64, int K, const float* __restrict__ p,
-                                                      const float* __restrict__ psum, const float* __restrict__ zk, const float* __restrict__ lse,
-                                                      const float* __restrict__ coef, const float* __restrict__ mass,
-                                                      const int* __restrict__ rows, const int* __restrict__ count, int v0, int v1, void* G,
-                                                      int64_t ldg, int dt) {
-  const int lane = threadIdx.x & 63, m = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (m >= *count) return;
-  const int n = rows[m];
-  for (int k = lane; k < K; k += 64) {
-    const int64_t o = (int64_t)n * K + k;
-    const int64_t i = idx64 ? reinterpret_cast<const int64_t*>(idx)[o] : (int64_t)reinterpret_cast<const int*>(idx)[o];
-    if (i < v0 || i >= v1 || p[o] == 0.f) continue;
-    store_f(G, (int64_t)m * ldg + (i - v0), dt, coef[m] * (mass[n] * __expf(zk[o] - lse[m]) - psum[o]));
-  }
-}
-
-// db[v0 + v] = scale * column sum of dz: 8 columns per thread, 32 row lanes, one workgroup per 64 columns
-__global__ void __launch_bounds__(256) colsum_kernel(const void* __restrict__ G, int64_t ldg, int dt, int vc, const int* __restrict__ count,
-                                                     const float* __restrict__ scale, void* __restrict__ db, int bdt) {
+// db[v] = scale * column sum of the scores' gradient (of both its halves): 8 columns per thread, 32 row lanes, 64 columns per workgroup
+__global__ void __launch_bounds__(256) colsum_kernel(const char* __restrict__ G, int64_t ldg, int64_t glo, int dt, int vc, const int* __restrict__ count,
+                                                     const Scales* __restrict__ sc, void* __restrict__ db, int bdt) {
   __shared__ float red[32][65];
   const int cg = threadIdx.x & 7, rl = threadIdx.x >> 3, c = *count;
   const int v = blockIdx.x * 64 + cg * 8;
   float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (v < vc)                                                    // dz is zero between vc and its row stride (a multiple of 64)
-    for (int m = rl; m < c; m += 32)
+  if (v < vc)                                                    // rows are zero between vc and the next multiple of 128 columns
+    for (int m = rl; m < c; m += 32) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] += load_f(G, (int64_t)m * ldg + v + e, dt);
+      for (int e = 0; e < 8; ++e) s[e] += load_f(G + m * ldg, v + e, dt);
+      if (glo)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += load_f(G + glo + m * ldg, v + e, dt);
+    }
 #pragma unroll
   for (int e = 0; e < 8; ++e) red[rl][cg * 8 + e] = s[e];
   __syncthreads();
   if (threadIdx.x < 64 && (int)(blockIdx.x * 64 + threadIdx.x) < vc) {
     float a = 0.f;
     for (int r = 0; r < 32; ++r) a += red[r][threadIdx.x];
-    store_f(db, blockIdx.x * 64 + threadIdx.x, bdt, a * *scale);
+    store_f(db, blockIdx.x * 64 + threadIdx.x, bdt, a * sc->db);
   }
 }
 
-// dh partial products: unit u of the grid owns output tile u % tiles and share u / tiles of the piece's columns; its fp32 tile lives in
-// slab u and is added to by the following pieces. Which unit owns what depends on the number of rows alone, so the sum's order is fixed.
+// dh: unit u of the grid owns output tile u % tiles and share u / tiles of the piece's columns; its fp32 tile lives in slab u and is added
+// to by the following pieces. Which unit owns what depends on the number of rows alone, so the sum's order is fixed.
 struct DhP {
-  const void* G; int64_t ldg;
-  const void* W; int64_t ldw;            // first row (column) of the piece
+  Operand G, W;                          // G: xlim set on the device
   const int* count;
   int D, vc, units, accum;
   float* slab;
 };
-__device__ __forceinline__ int dh_shares(int tiles, int units) { return tiles >= units ? 1 : units / tiles; }
+__device__ __forceinline__ int shares_of(int tiles, int units) { return tiles >= units ? 1 : units / tiles; }
 
-template <class C, bool TB>
-__global__ void __launch_bounds__(C::NT) dh_kernel(const DhP p) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int count = *p.count;
-  const int mtiles = (count + C::BM - 1) / C::BM, ntiles = (p.D + C::BN - 1) / C::BN, tiles = mtiles * ntiles;
-  if (tiles == 0) return;
-  const int shares = dh_shares(tiles, p.units);
-  if ((int)blockIdx.x >= tiles * shares) return;
-  const int u = xcd_remap(blockIdx.x, tiles * shares);
-  const int share = u / tiles, t = u - share * tiles;
-  int mt, nt;
-  tile_coords(t, mtiles, ntiles, 8, mt, nt);
-  const int m0 = mt * C::BM, n0 = nt * C::BN;
-  const int ktiles = (p.vc + C::BK - 1) / C::BK, per = (ktiles + shares - 1) / shares;
-  const int k0 = min(ktiles, share * per), k1 = min(ktiles, k0 + per);
-  FlexSrc<C, false, TB> src;
-  src.kb = k0 * C::BK; src.ke = min(p.vc, k1 * C::BK);
-  src.kchunk = stage_chunk(stage_row<C>(0)) * C::CH;
-  src.a_kstride = 0; src.b_kstride = p.ldw * C::ESZ;
-#pragma unroll
-  for (int i = 0; i < C::PA; ++i) src.ap[i] = (const char*)p.G + (int64_t)(m0 + stage_row<C>(i)) * p.ldg * C::ESZ;
-#pragma unroll
-  for (int i = 0; i < C::PB; ++i) {
-    if constexpr (TB) {
-      int row, x;
-      tr_stage_pos<C, C::BN>(i, row, x);
-      src.brow[i] = row;
-      src.bp[i] = (n0 + x < p.D) ? (const char*)p.W + (int64_t)(n0 + x) * C::ESZ : nullptr;
-    } else {
-      int n = n0 + stage_row<C>(i);
-      if (n > p.D - 1) n = p.D - 1;
-      src.bp[i] = (const char*)p.W + (int64_t)n * p.ldw * C::ESZ;
-    }
-  }
-  typename C::acc_t acc[C::TM][C::TN];
-  mainloop_flex<C, FlexSrc<C, false, TB>, false, TB>(smem, src, k1 - k0, acc);
+// accumulators to (or onto) a tile of a slab
+template <class C> __device__ __forceinline__ void to_slab(float* tile, typename C::acc_t (&acc)[C::TM][C::TN], bool add) {
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int wm = wid / C::WN, wn = wid - wm * C::WN;
-  float* out = p.slab + (int64_t)u * C::BM * C::BN + (wm * (C::BM / C::WM) + (lane >> 4) * 4) * C::BN + wn * (C::BN / C::WN) + (lane & 15);
+  float* out = tile + (wm * (C::BM / C::WM) + (lane >> 4) * 4) * C::BN + wn * (C::BN / C::WN) + (lane & 15);
 #pragma unroll
   for (int i = 0; i < C::TM; ++i)
 #pragma unroll
@@ -498,257 +593,437 @@ __global__ void __launch_bounds__(C::NT) dh_kernel(const DhP p) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         float* o = out + (i * 16 + q) * C::BN + j * 16;
-        *o = p.accum ? *o + acc[i][j][q] : acc[i][j][q];
+        *o = add ? *o + acc[i][j][q] : acc[i][j][q];
       }
+}
+
+template <class C, bool TB, int SEG>
+__global__ void __launch_bounds__(C::NT) dh_kernel(const DhP p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int count = *p.count;
+  const int mtiles = (count + C::BM - 1) / C::BM, ntiles = (p.D + C::BN - 1) / C::BN, tiles = mtiles * ntiles;
+  if (tiles == 0) return;
+  const int shares = shares_of(tiles, p.units);
+  if ((int)blockIdx.x >= tiles * shares) return;
+  const int u = xcd_remap(blockIdx.x, tiles * shares);
+  const int share = u / tiles;
+  int mt, nt;
+  tile_coords(u - share * tiles, mtiles, ntiles, 8, mt, nt);
+  const int ktiles = k_tiles<C, SEG>(p.vc), per = (ktiles + shares - 1) / shares;
+  const int k0 = min(ktiles, share * per), k1 = min(ktiles, k0 + per);
+  typename C::acc_t acc[C::TM][C::TN];
+  Operand G = p.G;
+  G.xlim = mtiles * C::BM;                                       // rows up to the tile's end are there (zeros)
+  product<C, false, TB, SEG>(smem, G, p.W, mt * C::BM, nt * C::BN, p.vc, k0, k1, acc);
+  to_slab<C>(p.slab + (int64_t)u * C::BM * C::BN, acc, p.accum);
 }
 
 // dh rows from the slabs, in the order of the shares; rows that take no part get zeros. One workgroup per row.
 template <int BM, int BN>
 __global__ void __launch_bounds__(256) dh_rows_kernel(const float* __restrict__ slab, const int* __restrict__ rows, const int* __restrict__ count,
-                                                      const float* __restrict__ scale, int D, int units, void* __restrict__ dh, int64_t ldo, int dt) {
+                                                      const Scales* __restrict__ sc, int D, int units, void* __restrict__ dh, int64_t ldo, int dt) {
   const int m = blockIdx.x, c = *count, n = rows[m];
   const int mtiles = (c + BM - 1) / BM, ntiles = (D + BN - 1) / BN, tiles = mtiles * ntiles;
-  const int shares = tiles ? dh_shares(tiles, units) : 1;
-  const float s = *scale;
-  for (int d = threadIdx.x; d < D; d += 256) {
-    float v = 0.f;
+  const int shares = tiles ? shares_of(tiles, units) : 1;
+  const float s = sc->dh;
+  for (int d = threadIdx.x * 4; d < D; d += 1024) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (m < c) {
       const int mt = m / BM, nt = d / BN;
       const int g = mt / 8, rowsg = min(8, mtiles - g * 8);       // tile_coords with 8 row tiles to a group
       const int t = g * 8 * ntiles + nt * rowsg + (mt - g * 8);
-      for (int k = 0; k < shares; ++k) v += slab[(int64_t)(k * tiles + t) * BM * BN + (m - mt * BM) * BN + (d - nt * BN)];
+      const float* x = slab + ((int64_t)t * BM + (m - mt * BM)) * BN + (d - nt * BN);
+#pragma unroll 4
+      for (int k = 0; k < shares; ++k) v += *reinterpret_cast<const f32x4*>(x + (int64_t)k * tiles * BM * BN);
       v *= s;
     }
-    store_f(dh, (int64_t)n * ldo + d, dt, v);
+    const int64_t o = (int64_t)n * ldo + d;
+    for (int j = 0; j < 4 && d + j < D; ++j) store_f(dh, o + j, dt, v[j]);
   }
 }
 
-// dW[v0 .. v0 + vc) = scale * dz^T h (SWAP 0, [V, D]) or its transpose (SWAP 1, [D, V]): both operands are walked along their rows
+// dW[v0 .. v0 + vc) = scale * dz^T h (SWAP 0, [V, D]) or its transpose (SWAP 1, [D, V]): both operands are walked along their rows.
+// shares > 1 (small outputs): the rows' range is cut, fp32 tiles go to a slab and dw_sum_kernel adds them in order.
 struct DwP {
-  const void* G; int64_t ldg;
-  const void* H; int64_t ldh;            // packed rows
-  const int* count; const float* scale;
+  Operand G, H;
+  const int* count; const Scales* sc;
   void* out; int64_t ldo;
-  int D, vc;
+  int D, vc, shares;
+  float* slab;
 };
-template <class C, int OT, bool SWAP>
+template <class C, int OT, bool SWAP, int SEG>
 __global__ void __launch_bounds__(C::NT) dw_kernel(const DwP p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int K = (*p.count + 63) / 64 * 64;
+  const int K = *p.count;                                        // rows past it are not read
   const int M = SWAP ? p.D : p.vc, N = SWAP ? p.vc : p.D;
-  const int mtiles = (M + C::BM - 1) / C::BM, ntiles = (N + C::BN - 1) / C::BN;
+  const int mtiles = (M + C::BM - 1) / C::BM, ntiles = (N + C::BN - 1) / C::BN, tiles = mtiles * ntiles;
+  const int u = xcd_remap(blockIdx.x, gridDim.x), share = u / tiles;
   int mt, nt;
-  tile_coords(xcd_remap(blockIdx.x, gridDim.x), mtiles, ntiles, 8, mt, nt);
+  tile_coords(u - share * tiles, mtiles, ntiles, 8, mt, nt);
   const int m0 = mt * C::BM, n0 = nt * C::BN;
-  const char* A = (const char*)(SWAP ? p.H : p.G);
-  const char* B = (const char*)(SWAP ? p.G : p.H);
-  const int mlim = SWAP ? p.D : (int)p.ldg, nlim = SWAP ? (int)p.ldg : p.D;   // dz is zero from vc to ldg
-  FlexSrc<C, true, true> src;
-  src.kb = 0; src.ke = K; src.kchunk = 0;
-  src.a_kstride = (SWAP ? p.ldh : p.ldg) * C::ESZ;
-  src.b_kstride = (SWAP ? p.ldg : p.ldh) * C::ESZ;
-#pragma unroll
-  for (int i = 0; i < C::PA; ++i) {
-    int row, x;
-    tr_stage_pos<C, C::BM>(i, row, x);
-    src.arow[i] = row;
-    src.ap[i] = m0 + x < mlim ? A + (int64_t)(m0 + x) * C::ESZ : nullptr;
-  }
-#pragma unroll
-  for (int i = 0; i < C::PB; ++i) {
-    int row, x;
-    tr_stage_pos<C, C::BN>(i, row, x);
-    src.brow[i] = row;
-    src.bp[i] = n0 + x < nlim ? B + (int64_t)(n0 + x) * C::ESZ : nullptr;
-  }
+  const int ktiles = k_tiles<C, SEG>(K), per = (ktiles + p.shares - 1) / p.shares;
+  const int k0 = min(ktiles, share * per), k1 = min(ktiles, k0 + per);
   typename C::acc_t acc[C::TM][C::TN];
-  mainloop_flex<C, FlexSrc<C, true, true>, true, true>(smem, src, K / C::BK, acc);
+  product<C, true, true, SEG>(smem, SWAP ? p.H : p.G, SWAP ? p.G : p.H, m0, n0, K, k0, k1, acc);
+  if (p.shares > 1) { to_slab<C>(p.slab + (int64_t)u * C::BM * C::BN, acc, false); return; }
   EpiP e;
   e.out = p.out; e.residual = nullptr; e.bias = nullptr; e.stats = nullptr; e.stat_shift = nullptr;
-  e.alpha = *p.scale; e.act = ACT_NONE; e.accum = 0;
+  e.alpha = p.sc->dw; e.act = ACT_NONE; e.accum = 0;
   const int64_t ldo = p.ldo;
   epilogue_impl<C, OT, ACT_NONE, 0>(smem, acc, mt, n0, N, M - m0, e, [=](int r) -> int64_t {
     return m0 + r < M ? (int64_t)(m0 + r) * ldo + n0 : (int64_t)-1;
   });
 }
-
-template <int DT> using Tile = Cfg<128, 128, 2, 2, 2, 16, DT>;
-
-template <typename F> void allow_lds(F* fn, int bytes, DeviceOnceLds& once) { once.ensure(reinterpret_cast<const void*>(fn), bytes); }
-
-template <int DT, bool TB, bool GRAD> int launch_score(const ScoreP& p, hipStream_t st) {
-  typedef Tile<DT> C;
-  const int64_t grid = (int64_t)((p.N + C::BM - 1) / C::BM) * ((p.v1 - p.v0 + C::BN - 1) / C::BN);
-  constexpr int EPI = GRAD ? C::BM * (C::BN * C::ESZ + 16) + 4 * C::BM * 4 : C::BM * 4 * (1 + 3 * C::WN);
-  constexpr int MAIN = C::STAGES * C::STAGE_BYTES, LDS = MAIN > EPI ? MAIN : EPI;
-  static DeviceOnceLds once;
-  allow_lds(&score_kernel<C, TB, GRAD>, LDS, once);
-  hipLaunchKernelGGL((score_kernel<C, TB, GRAD>), dim3(grid), dim3(C::NT), LDS, st, p);
-  return (int)hipGetLastError();
-}
-template <bool GRAD> int dispatch_score(const ScoreP& p, int dt, int tb, hipStream_t st) {
-  switch (dt) {
-    case DT_BF16: return tb ? launch_score<DT_BF16, true, GRAD>(p, st) : launch_score<DT_BF16, false, GRAD>(p, st);
-    case DT_F16: return tb ? launch_score<DT_F16, true, GRAD>(p, st) : launch_score<DT_F16, false, GRAD>(p, st);
-    case DT_F32: return tb ? launch_score<DT_F32, true, GRAD>(p, st) : launch_score<DT_F32, false, GRAD>(p, st);
+template <int BM, int BN>
+__global__ void __launch_bounds__(256) dw_sum_kernel(const float* __restrict__ slab, int shares, int M, int N, const Scales* __restrict__ sc,
+                                                     void* __restrict__ out, int64_t ldo, int dt) {
+  const int mtiles = (M + BM - 1) / BM, ntiles = (N + BN - 1) / BN, tiles = mtiles * ntiles;
+  const int m = blockIdx.x, mt = m / BM, g = mt / 8, rowsg = min(8, mtiles - g * 8);
+  for (int n = threadIdx.x; n < N; n += 256) {
+    const int nt = n / BN, t = g * 8 * ntiles + nt * rowsg + (mt - g * 8);
+    const float* x = slab + ((int64_t)t * BM + (m - mt * BM)) * BN + (n - nt * BN);
+    float v = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < shares; ++k) v += x[(int64_t)k * tiles * BM * BN];
+    store_f(out, (int64_t)m * ldo + n, dt, v * sc->dw);
   }
-  return -2;
 }
 
-template <int DT, bool TB> int launch_dh(const DhP& p, int grid, hipStream_t st) {
-  typedef Tile<DT> C;
-  constexpr int LDS = C::STAGES * C::STAGE_BYTES;
-  static DeviceOnceLds once;
-  allow_lds(&dh_kernel<C, TB>, LDS, once);
-  hipLaunchKernelGGL((dh_kernel<C, TB>), dim3(grid), dim3(C::NT), LDS, st, p);
-  return (int)hipGetLastError();
+// ------------------------------------------------------------------------------------------------------------------------ host side
+template <int DT> using Big = Cfg<256, 256, 2, 4, 2, 16, DT>;
+template <int DT> using Mid = Cfg<128, 128, 2, 2, 2, 16, DT>;
+template <int DT> using Few = Cfg<32, 128, 1, 4, 4, 16, DT>;
+enum { TILE_BIG = 0, TILE_MID = 1, TILE_FEW = 2 };
+
+// One call: sizes, layout and pointers (ops/vocab_loss.py _ARGS lists the same fields in the same order)
+struct Args {
+  int64_t N, D, V, dt, split, wt, bdt, ldh, ldw, lab64, ignore, idx64, tdt, K, want_h, want_w, want_b;
+  const void *H, *W, *bias, *labels, *idx, *t;
+  float* loss; char* state; char* ws;
+  const float* dloss; void *dh, *dw, *db;
+};
+
+int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+#ifdef VL_TUNE
+int g_tune[8] = {-1, -1, -1, -1, -1, -1, -1, -1};
+#define TUNE(i, v) (g_tune[i] >= 0 ? g_tune[i] : (v))
+#else
+#define TUNE(i, v) (v)
+#endif
+
+struct Plan {
+  int tile, dh_tile, dw_tile;            // TILE_*
+  int op;                                // operand type of the products
+  int bn, tiles;                         // column tiles of the scores
+  int64_t np, dp, wcp, wrows;            // padded rows / columns of the packed H and of the halves of W
+  int pieces, step;
+  int units, shares;
+  int64_t gcols;
+};
+
+Plan plan(const Args& a) {
+  Plan p;
+  p.op = a.split ? DT_F16 : (int)a.dt;
+  const bool bits16 = p.op != DT_F32;
+  const int64_t big_tiles = up(a.N, 256) / 256 * (up(a.V, 256) / 256);
+  // 256 x 256 tiles once they cover two thirds of the 256 CUs, 32 rows for the fewest rows (W streams through: one tile per CU at a
+  // vocabulary of 32768), 128 x 128 between them and for fp32
+  p.tile = TUNE(0, bits16 && big_tiles >= 176 && a.N > 128 ? TILE_BIG : a.N <= 32 ? TILE_FEW : TILE_MID);
+  if (a.split && p.tile == TILE_FEW) p.tile = TILE_MID;
+  if (!bits16 && p.tile == TILE_BIG) p.tile = TILE_MID;
+  p.bn = p.tile == TILE_BIG ? 256 : 128;
+  p.tiles = (int)(up(a.V, p.bn) / p.bn);
+  p.np = up(a.N, 256);
+  p.dp = up(a.D, 8);
+  p.wrows = a.wt ? a.D : a.V;
+  p.wcp = up(a.wt ? a.V : a.D, 8);
+  const int64_t esz = a.dt == DT_F32 ? 4 : 2;                    // halves take as much as fp32
+  const int64_t most = TUNE(4, 256) * (int64_t)(1 << 20) / (p.np * esz) / 256 * 256;
+  p.pieces = (int)(most >= 256 ? (a.V + most - 1) / most : up(a.V, 256) / 256);
+  p.step = (int)up((a.V + p.pieces - 1) / p.pieces, 256);
+  p.pieces = (int)((a.V + p.step - 1) / p.step);
+  p.gcols = up(a.V < p.step ? a.V : p.step, 256);
+  p.dh_tile = TUNE(1, bits16 && a.N > 128 && a.D >= 256 ? TILE_BIG : TILE_MID);
+  if (!bits16) p.dh_tile = TILE_MID;
+  const int ht = p.dh_tile == TILE_BIG ? 256 : 128;
+  const int64_t htiles = up(a.N, ht) / ht * (up(a.D, ht) / ht);
+  const int want = p.dh_tile == TILE_BIG ? 256 : 512;
+  p.units = (int)(htiles > want ? htiles : want);
+  const int64_t wbig = up(p.gcols, 256) / 256 * (up(a.D, 256) / 256);
+  p.dw_tile = TUNE(2, bits16 && wbig >= 176 ? TILE_BIG : TILE_MID);
+  if (!bits16) p.dw_tile = TILE_MID;
+  const int wt = p.dw_tile == TILE_BIG ? 256 : 128;
+  const int64_t wtiles = up(p.gcols < a.V ? p.gcols : a.V, wt) / wt * (up(a.D, wt) / wt);
+  const int64_t ks = up(a.N, 64) / 64;
+  int64_t sh = p.dw_tile == TILE_BIG ? 1 : 512 / wtiles;         // shares of at least 4 k-tiles
+  if (sh > ks / 4) sh = ks / 4;
+  p.shares = (int)(sh < 1 ? 1 : sh);
+  return p;
 }
-template <int DT, bool SWAP> int launch_dw(const DwP& p, hipStream_t st) {
-  typedef Tile<DT> C;
-  constexpr int OT = DT == DT_F32 ? OT_F32 : DT == DT_F16 ? OT_F16 : OT_BF16;
-  const int M = SWAP ? p.D : p.vc, N = SWAP ? p.vc : p.D;
-  constexpr int LDS = C::lds_bytes(Out<OT>::SZ);
-  static DeviceOnceLds once;
-  allow_lds(&dw_kernel<C, OT, SWAP>, LDS, once);
-  hipLaunchKernelGGL((dw_kernel<C, OT, SWAP>), dim3(((M + C::BM - 1) / C::BM) * ((N + C::BN - 1) / C::BN)), dim3(C::NT), LDS, st, p);
-  return (int)hipGetLastError();
-}
+
+// buffers carved from one allocation each: state (kept from forward to backward), forward and backward workspace
+struct Carve {
+  char* base; int64_t at = 0;
+  explicit Carve(char* b) : base(b) {}
+  template <typename T> T* take(int64_t n) {
+    T* r = reinterpret_cast<T*>(base + at);
+    at += up(n * (int64_t)sizeof(T), 256);
+    return r;
+  }
+};
+struct State {
+  Scales* sc; int* count; int* rows; float* lse;
+  int* sidx; float *sp, *psum, *zk, *ent, *mass; unsigned short* first;
+  _Float16 *wo, *ho;
+  int64_t bytes;
+  State(const Args& a, const Plan& p) {
+    Carve c(a.state);
+    sc = c.take<Scales>(1); count = c.take<int>(1); rows = c.take<int>(a.N); lse = c.take<float>(a.N);
+    const int64_t nk = a.K ? a.N * a.K : 0;
+    sidx = c.take<int>(nk); sp = c.take<float>(nk); psum = c.take<float>(nk); zk = c.take<float>(nk);
+    ent = c.take<float>(a.K ? a.N : 0); mass = c.take<float>(a.K ? a.N : 0);
+    first = c.take<unsigned short>(a.K ? (int64_t)(p.tiles + 1) * a.N : 0);
+    wo = c.take<_Float16>(a.split ? 2 * p.wrows * p.wcp : 0);
+    ho = c.take<_Float16>(a.split ? 2 * p.np * p.dp : 0);
+    bytes = c.at;
+  }
+};
+struct Work {
+  float2* part; float *tz, *zs, *amax;                           // forward
+  float* coef; char* G; char* packed; float *dh_slab, *dw_slab;  // backward
+  int64_t fwd, bwd;
+  Work(const Args& a, const Plan& p) {
+    Carve c(a.ws);
+    part = c.take<float2>((int64_t)p.tiles * a.N); tz = c.take<float>(a.N); zs = c.take<float>((int64_t)p.tiles * a.N);
+    amax = c.take<float>(a.split ? AMAX_W + AMAX_H : 0);
+    fwd = c.at;
+    c.at = 0;
+    const int64_t esz = a.dt == DT_F32 ? 4 : 2;
+    coef = c.take<float>(a.N); G = c.take<char>(p.np * p.gcols * esz);
+    packed = c.take<char>(a.want_w && !a.split ? p.np * up(a.D, 16 / esz) * esz : 0);
+    const int64_t ht = p.dh_tile == TILE_BIG ? 256 : 128;
+    dh_slab = c.take<float>(a.want_h ? p.units * ht * ht : 0);
+    const int64_t wt = p.dw_tile == TILE_BIG ? 256 : 128;
+    const int64_t wtiles = up(p.gcols < a.V ? p.gcols : a.V, wt) / wt * (up(a.D, wt) / wt);
+    dw_slab = c.take<float>(a.want_w && p.shares > 1 ? wtiles * p.shares * wt * wt : 0);
+    bwd = c.at;
+  }
+};
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+#define VL_CHECK() do { const int e_ = (int)hipGetLastError(); if (e_) return e_; } while (0)
+
+template <class C, bool TB, bool GRAD, int SEG> int launch_score(const ScoreP& p, hipStream_t st) {
+  const int64_t grid = (int64_t)((p.N + C::BM - 1) / C::BM) * ((p.v1 - p.v0 + C::BN - 1) / C::BN);
+  if (grid > 0x7fffffff) return -2;
+  constexpr int EPI = GRAD ? score_lds_grad<C>() : score_lds_stats<C>();
+  constexpr int MAIN = C::STAGES * C::STAGE_BYTES, LDS = MAIN > EPI ? MAIN : EPI;
+  static_assert(LDS <= 160 * 1024, "tile does not fit the 160 KiB LDS");
+  static DeviceOnceLds once;
+  once.ensure(reinterpret_cast<const void*>(&score_kernel<C, TB, GRAD, SEG>), LDS);
+  hipLaunchKernelGGL((score_kernel<C, TB, GRAD, SEG>), dim3((unsigned)grid), dim3(C::NT), LDS, st, p);
+  return (int)hipGetLastError();
+}
+template <bool TB, bool GRAD> int dispatch_score(const ScoreP& p, int tile, int op, bool split, hipStream_t st) {
+  if (split) return tile == TILE_BIG ? launch_score<Big<DT_F16>, TB, GRAD, 3>(p, st) : launch_score<Mid<DT_F16>, TB, GRAD, 3>(p, st);
+  if (op == DT_F32) return tile == TILE_FEW ? launch_score<Few<DT_F32>, TB, GRAD, 1>(p, st) : launch_score<Mid<DT_F32>, TB, GRAD, 1>(p, st);
+  if (op == DT_BF16)
+    return tile == TILE_BIG ? launch_score<Big<DT_BF16>, TB, GRAD, 1>(p, st) : tile == TILE_FEW ? launch_score<Few<DT_BF16>, TB, GRAD, 1>(p, st)
+                            : launch_score<Mid<DT_BF16>, TB, GRAD, 1>(p, st);
+  return tile == TILE_BIG ? launch_score<Big<DT_F16>, TB, GRAD, 1>(p, st) : tile == TILE_FEW ? launch_score<Few<DT_F16>, TB, GRAD, 1>(p, st)
+                          : launch_score<Mid<DT_F16>, TB, GRAD, 1>(p, st);
+}
+template <bool GRAD> int scores(const ScoreP& p, int tile, int op, bool split, bool tb, hipStream_t st) {
+  return tb ? dispatch_score<true, GRAD>(p, tile, op, split, st) : dispatch_score<false, GRAD>(p, tile, op, split, st);
+}
+
+template <class C, bool TB, int SEG> int launch_dh(const DhP& p, hipStream_t st) {
+  constexpr int LDS = C::STAGES * C::STAGE_BYTES;
+  static DeviceOnceLds once;
+  once.ensure(reinterpret_cast<const void*>(&dh_kernel<C, TB, SEG>), LDS);
+  hipLaunchKernelGGL((dh_kernel<C, TB, SEG>), dim3(p.units), dim3(C::NT), LDS, st, p);
+  return (int)hipGetLastError();
+}
+template <bool TB> int dispatch_dh(const DhP& p, int tile, int op, bool split, hipStream_t st) {
+  const bool big = tile == TILE_BIG;
+  if (split) return big ? launch_dh<Big<DT_F16>, TB, 3>(p, st) : launch_dh<Mid<DT_F16>, TB, 3>(p, st);
+  if (op == DT_F32) return launch_dh<Mid<DT_F32>, TB, 1>(p, st);
+  if (op == DT_BF16) return big ? launch_dh<Big<DT_BF16>, TB, 1>(p, st) : launch_dh<Mid<DT_BF16>, TB, 1>(p, st);
+  return big ? launch_dh<Big<DT_F16>, TB, 1>(p, st) : launch_dh<Mid<DT_F16>, TB, 1>(p, st);
+}
+
+template <class C, int OT, bool SWAP, int SEG> int launch_dw(const DwP& p, hipStream_t st) {
+  const int M = SWAP ? p.D : p.vc, N = SWAP ? p.vc : p.D;
+  const int tiles = ((M + C::BM - 1) / C::BM) * ((N + C::BN - 1) / C::BN);
+  constexpr int LDS = C::lds_bytes(Out<OT>::SZ);
+  static_assert(LDS <= 160 * 1024, "tile does not fit the 160 KiB LDS");
+  static DeviceOnceLds once;
+  once.ensure(reinterpret_cast<const void*>(&dw_kernel<C, OT, SWAP, SEG>), LDS);
+  hipLaunchKernelGGL((dw_kernel<C, OT, SWAP, SEG>), dim3(tiles * p.shares), dim3(C::NT), LDS, st, p);
+  VL_CHECK();
+  if (p.shares > 1)
+    hipLaunchKernelGGL((dw_sum_kernel<C::BM, C::BN>), dim3(M), dim3(256), 0, st, p.slab, p.shares, M, N, p.sc, p.out, p.ldo,
+                       OT == OT_F32 ? (int)DT_F32 : OT == OT_F16 ? (int)DT_F16 : (int)DT_BF16);
+  return (int)hipGetLastError();
+}
+template <bool SWAP> int dispatch_dw(const DwP& p, int tile, int op, bool split, hipStream_t st) {
+  const bool big = tile == TILE_BIG;
+  if (split) return launch_dw<Mid<DT_F16>, OT_F32, SWAP, 3>(p, st);
+  if (op == DT_F32) return launch_dw<Mid<DT_F32>, OT_F32, SWAP, 1>(p, st);
+  if (op == DT_BF16) return big ? launch_dw<Big<DT_BF16>, OT_BF16, SWAP, 1>(p, st) : launch_dw<Mid<DT_BF16>, OT_BF16, SWAP, 1>(p, st);
+  return big ? launch_dw<Big<DT_F16>, OT_F16, SWAP, 1>(p, st) : launch_dw<Mid<DT_F16>, OT_F16, SWAP, 1>(p, st);
+}
+
+// 0 where the arguments are what the kernels assume
+int check(const Args& a, bool bwd) {
+  if (a.N <= 0 || a.N > 0x7fffffff - 512 || a.D <= 0 || a.D > 0x7fffffff - 512 || a.V <= 0 || a.V > 0x7fffffff - 512) return -2;
+  if (a.dt < 0 || a.dt > 2 || a.bdt < 0 || a.bdt > 2 || (a.split && a.dt != DT_F32) || a.K < 0 || a.K > KMAX) return -2;
+  if (!a.H || !a.W || !a.state || !a.ws || !a.loss || !aligned16(a.state) || !aligned16(a.ws)) return -2;
+  if (a.K ? !a.idx || !a.t || a.tdt < 0 || a.tdt > 2 : !a.labels) return -2;
+  const int64_t ch = a.dt == DT_F32 ? 4 : 8, wc = a.wt ? a.V : a.D;
+  if (a.split ? a.ldh < a.D || a.ldw < wc                        // halves are made from any row stride
+              : a.ldh % ch || a.ldw % ch || a.ldh < up(a.D, ch) || a.ldw < up(wc, ch) || !aligned16(a.H) || !aligned16(a.W)) return -2;
+  if (bwd && (!a.dloss || (a.want_h && !a.dh) || (a.want_w && !a.dw) || (a.want_b && (!a.db || !a.bias)))) return -2;
+  return 0;
+}
+
+void operands(const Args& a, const Plan& p, const State& s, Operand& H, Operand& W) {
+  const int esz = a.dt == DT_F32 ? 4 : 2;
+  if (a.split) {
+    H = Operand{(const char*)s.ho, p.dp * 2, p.np * p.dp * 2, 0, nullptr};
+    W = Operand{(const char*)s.wo, p.wcp * 2, p.wrows * p.wcp * 2, 0, nullptr};
+  } else {
+    H = Operand{(const char*)a.H, a.ldh * esz, 0, 0, s.rows};
+    W = Operand{(const char*)a.W, a.ldw * esz, 0, 0, nullptr};
+  }
+}
+
+ScoreP score_args(const Args& a, const State& s, const float* f) {
+  ScoreP q = {};
+  q.bias = a.bias; q.bdt = (int)a.bdt; q.rows = s.rows; q.count = s.count; q.sc = s.sc;
+  q.labels = a.K ? nullptr : a.labels; q.lab64 = (int)a.lab64;
+  q.N = (int)a.N; q.D = (int)a.D;
+  q.invT = 1.f / f[0]; q.smooth_v = f[1] / (float)a.V; q.keep = 1.f - f[1];
+  if (a.K) { q.first = s.first; q.sidx = s.sidx; q.psum = s.psum; q.zk = s.zk; q.K = (int)a.K; q.keep = 0.f; q.smooth_v = 0.f; }
+  return q;
+}
+
+int forward(const Args& a, const float* f, hipStream_t st) {
+  if (const int e = check(a, false)) return e;
+  const Plan p = plan(a);
+  const State s(a, p);
+  const Work w(a, p);
+  if (a.K) {
+    int p2 = 2;
+    while (p2 < a.K) p2 <<= 1;
+    TeacherP t{a.idx, (int)a.idx64, a.t, (int)a.tdt, (int)a.N, (int)a.V, (int)a.K, p2, 1.f / f[0], p.bn, p.tiles, s.sidx, s.sp, s.psum, s.first, s.ent, s.mass};
+    hipLaunchKernelGGL(teacher_kernel, dim3((unsigned)((a.N + 3) / 4)), dim3(256), 4 * 12 * p2, st, t);
+    VL_CHECK();
+  }
+  hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, a.K ? nullptr : a.labels, (int)a.lab64, a.ignore, s.mass, (int)a.N, s.rows, s.count, s.sc, a.loss);
+  VL_CHECK();
+  if (a.split) {
+    const int wr = (int)p.wrows, wc = (int)(a.wt ? a.V : a.D);
+    hipLaunchKernelGGL(amax_kernel, dim3(AMAX_W + AMAX_H), dim3(256), 0, st, (const float*)a.W, a.ldw, wr, wc, (const float*)a.H, a.ldh, (int)a.D, s.rows,
+                       s.count, w.amax);
+    VL_CHECK();
+    SplitP q{(const float*)a.W, a.ldw, wr, wc, (int)p.wcp, s.wo, (const float*)a.H, a.ldh, (int)a.D, (int)p.dp, s.ho, (int)p.np, s.rows, s.count, w.amax, s.sc, 2048};
+    hipLaunchKernelGGL(split_kernel, dim3(2048 + 256), dim3(256), 0, st, q);
+    VL_CHECK();
+  }
+  ScoreP q = score_args(a, s, f);
+  operands(a, p, s, q.H, q.W);
+  q.W.xlim = (int)a.V;
+  q.v0 = 0; q.v1 = (int)a.V;
+  q.part = w.part; q.tz = w.tz; q.zs = q.smooth_v != 0.f ? w.zs : nullptr;
+  if (const int e = scores<false>(q, p.tile, p.op, a.split, a.wt, st)) return e;
+  CombineP c{w.part, q.zs, w.tz, s.rows, s.count, q.labels, (int)a.lab64, a.K ? s.ent : nullptr, s.sp, s.zk, (int)a.K, (int)a.N, (int)a.V, p.tiles, q.keep, f[0],
+             s.lse, a.loss};
+  if (a.N <= 256) hipLaunchKernelGGL((combine_kernel<1>), dim3((unsigned)a.N), dim3(256), 0, st, c);
+  else hipLaunchKernelGGL((combine_kernel<8>), dim3((unsigned)((a.N + 7) / 8)), dim3(256), 0, st, c);
+  return (int)hipGetLastError();
+}
+
+int backward(const Args& a, const float* f, hipStream_t st) {
+  if (const int e = check(a, true)) return e;
+  const Plan p = plan(a);
+  const State s(a, p);
+  const Work w(a, p);
+  const int esz = a.dt == DT_F32 ? 4 : 2, gsz = a.split ? 2 : esz;
+  hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, st, a.dloss, s.rows, s.count, f[0], (int)(p.op == DT_F16), w.coef, s.sc);
+  VL_CHECK();
+  Operand H, W;
+  operands(a, p, s, H, W);
+  Operand packed = H;
+  if (a.want_w && !a.split) {
+    const int64_t rb = up(a.D, 16 / esz) * esz;
+    hipLaunchKernelGGL(pack_kernel, dim3((unsigned)a.N), dim3(256), 0, st, (const char*)a.H, a.ldh * esz, s.rows, s.count, w.packed, rb);
+    VL_CHECK();
+    packed = Operand{w.packed, rb, 0, 0, nullptr};
+  }
+  packed.xlim = (int)a.D;
+  const int64_t ldg = p.gcols * gsz, glo = a.split ? p.np * ldg : 0;
+  for (int k = 0; k < p.pieces; ++k) {
+    const int v0 = k * p.step, v1 = (int)(a.V < v0 + (int64_t)p.step ? a.V : v0 + p.step), vc = v1 - v0;
+    ScoreP q = score_args(a, s, f);
+    q.H = H; q.W = W;
+    q.W.xlim = (int)a.V;
+    q.v0 = v0; q.v1 = v1; q.lse = s.lse; q.coef = w.coef; q.G = w.G; q.ldg = ldg; q.glo = glo;
+    if (const int e = scores<true>(q, p.tile, p.op, a.split, a.wt, st)) return e;
+    if (a.want_b) {
+      hipLaunchKernelGGL(colsum_kernel, dim3((vc + 63) / 64), dim3(256), 0, st, w.G, ldg, glo, a.split ? (int)DT_F16 : (int)a.dt, vc, s.count, s.sc,
+                         (char*)a.db + (int64_t)v0 * (a.bdt == DT_F32 ? 4 : 2), (int)a.bdt);
+      VL_CHECK();
+    }
+    Operand G{w.G, ldg, glo, 0, nullptr};
+    if (a.want_h) {
+      DhP d;
+      d.G = G; d.W = W;
+      d.W.p += a.wt ? (int64_t)v0 * gsz : v0 * W.ld;
+      d.W.xlim = (int)a.D;
+      d.count = s.count; d.D = (int)a.D; d.vc = vc; d.units = p.units; d.accum = k > 0; d.slab = w.dh_slab;
+      const int e = a.wt ? dispatch_dh<false>(d, p.dh_tile, p.op, a.split, st) : dispatch_dh<true>(d, p.dh_tile, p.op, a.split, st);
+      if (e) return e;
+    }
+    if (a.want_w) {
+      DwP d;
+      d.G = G; d.G.xlim = (int)up(vc, p.bn);                      // zeros from vc on
+      d.H = packed; d.count = s.count; d.sc = s.sc;
+      d.out = (char*)a.dw + (a.wt ? (int64_t)v0 : v0 * a.D) * esz;
+      d.ldo = a.wt ? a.V : a.D;
+      d.D = (int)a.D; d.vc = vc; d.shares = p.shares; d.slab = w.dw_slab;
+      const int e = a.wt ? dispatch_dw<true>(d, p.dw_tile, p.op, a.split, st) : dispatch_dw<false>(d, p.dw_tile, p.op, a.split, st);
+      if (e) return e;
+    }
+  }
+  if (a.want_h) {
+    if (p.dh_tile == TILE_BIG)
+      hipLaunchKernelGGL((dh_rows_kernel<256, 256>), dim3((unsigned)a.N), dim3(256), 0, st, w.dh_slab, s.rows, s.count, s.sc, (int)a.D, p.units, a.dh, a.D, (int)a.dt);
+    else
+      hipLaunchKernelGGL((dh_rows_kernel<128, 128>), dim3((unsigned)a.N), dim3(256), 0, st, w.dh_slab, s.rows, s.count, s.sc, (int)a.D, p.units, a.dh, a.D, (int)a.dt);
+  }
+  return (int)hipGetLastError();
+}
+
 }  // namespace
 
-// rows that take part: label != ignore (labels64 / labels32), or mass != 0
-DL4J_API int dl4j_vl_rows(const int64_t* labels64, const int* labels32, int64_t ignore, const float* mass, int N, int* rows, int* count,
-                          float* loss, hipStream_t st) {
-  if (N <= 0 || !rows || !count || !loss || (!labels64 && !labels32 && !mass)) return -2;
-  hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, labels64, labels32, ignore, mass, N, rows, count, loss);
-  return (int)hipGetLastError();
+#ifdef VL_TUNE
+DL4J_API void dl4j_vl_tune(int i, int v) { g_tune[i] = v; }
+#endif
+
+// bytes of the state (0), the forward workspace (1) and the backward workspace (2)
+DL4J_API int64_t dl4j_linear_loss_bytes(const int64_t* args, int which) {
+  const Args& a = *reinterpret_cast<const Args*>(args);
+  const Plan p = plan(a);
+  return which == 0 ? State(a, p).bytes : which == 1 ? Work(a, p).fwd : Work(a, p).bwd;
 }
-
-DL4J_API int dl4j_vl_teacher(const void* idx, int idx64, const void* t, int tdt, int N, int K, float invT, float* p, float* psum, float* ent,
-                             float* mass, hipStream_t st) {
-  if (N <= 0 || K <= 0 || K > 1024 || tdt < 0 || tdt > 2 || !idx || !t || !p || !psum || !ent || !mass) return -2;
-  hipLaunchKernelGGL(teacher_kernel, dim3((N + 3) / 4), dim3(256), 0, st, idx, idx64, t, tdt, N, K, invT, p, psum, ent, mass);
-  return (int)hipGetLastError();
+// loss [N] of cross entropy (K = 0) or of distillation; f: temperature, label smoothing
+DL4J_API int dl4j_linear_loss_fwd(const int64_t* args, const float* f, hipStream_t st) {
+  return forward(*reinterpret_cast<const Args*>(args), f, st);
 }
-
-// sizes: N D V ldh vstride dstride dt bdt idx64 K
-DL4J_API int dl4j_vl_gather(const void* h, const void* W, const void* bias, const void* idx, const float* p, const int* rows, const int* count,
-                            float invT, float* zk, float* cross, const int64_t* d, hipStream_t st) {
-  if (d[0] <= 0 || d[1] <= 0 || d[2] <= 0 || d[9] <= 0 || !h || !W || !idx) return -2;
-  hipLaunchKernelGGL(gather_kernel, dim3((d[0] + 3) / 4), dim3(256), 0, st, h, d[3], W, d[4], d[5], bias, (int)d[7], (int)d[6], (int)d[1], (int)d[2],
-                     idx, (int)d[8], (int)d[9], invT, p, rows, count, zk, cross);
-  return (int)hipGetLastError();
-}
-
-// column tiles that the statistics of V columns take (rows of `part`)
-DL4J_API int dl4j_vl_tiles(int V, int dt) { return (V + Tile<DT_BF16>::BN - 1) / Tile<DT_BF16>::BN; }
-
-// d: N D V v0 v1 ldh ldw ldg dt wt bdt (wt: W is [D, V]);  f: 1/T, e/V, 1-e
-// grad = 0: part / tz / zs are written; grad = 1: G [N rounded up to 128 rows][ldg]
-DL4J_API int dl4j_vl_scores(int grad, const void* H, const void* W, const void* bias, const int* rows, const int* count, const int64_t* labels64,
-                            const int* labels32, float* part, float* tz, float* zs, const float* lse, const float* coef, const float* mass, void* G,
-                            const int64_t* d, const float* f, hipStream_t st) {
-  ScoreP p;
-  p.H = H; p.W = W; p.bias = bias; p.rows = rows; p.count = count; p.lab64 = labels64; p.lab32 = labels32;
-  p.N = (int)d[0]; p.D = (int)d[1]; p.V = (int)d[2]; p.v0 = (int)d[3]; p.v1 = (int)d[4];
-  p.ldh = d[5]; p.ldw = d[6]; p.ldg = d[7]; p.bdt = (int)d[10];
-  p.invT = f[0]; p.smooth_v = f[1]; p.keep = f[2];
-  p.part = (float2*)part; p.tz = tz; p.zs = zs; p.lse = lse; p.coef = coef; p.mass = mass; p.G = G;
-  const int dt = (int)d[8], wt = (int)d[9], ch = dt == DT_F32 ? 4 : 8;
-  if (p.N <= 0 || p.D <= 0 || p.V <= 0 || p.v0 < 0 || p.v1 > p.V || p.v0 >= p.v1 || dt < 0 || dt > 2) return -2;
-  const int Dp = (p.D + ch - 1) / ch * ch;                       // rows are read in 16-byte chunks, zeros behind D (V)
-  if (p.ldh % ch || p.ldh < Dp || p.ldw % ch || !aligned16(H) || !aligned16(W)) return -2;
-  if (wt ? p.ldw < (p.V + ch - 1) / ch * ch || p.v0 % ch : p.ldw < Dp) return -2;
-  if (grad ? (!G || !lse || !coef || p.ldg % Tile<DT_BF16>::BN || p.ldg < p.v1 - p.v0 || !aligned16(G)) : (!part || !tz)) return -2;
-  return grad ? dispatch_score<true>(p, dt, wt, st) : dispatch_score<false>(p, dt, wt, st);
-}
-
-DL4J_API int dl4j_vl_combine(const float* part, const float* zs, const float* tz, const int* rows, const int* count, const int64_t* labels64,
-                             const int* labels32, const float* ent, const float* cross, const float* mass, int N, int V, int ntiles, float keep,
-                             float T, float* lse, float* loss, hipStream_t st) {
-  if (N <= 0 || ntiles <= 0 || !part || !lse || !loss || (!ent && !labels64 && !labels32)) return -2;
-  CombineP p{(const float2*)part, zs, tz, rows, count, labels64, labels32, ent, cross, mass, N, V, ntiles, keep, T, lse, loss};
-  if (N <= 256) hipLaunchKernelGGL((combine_kernel<1>), dim3(N), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((combine_kernel<8>), dim3((N + 7) / 8), dim3(256), 0, st, p);
-  return (int)hipGetLastError();
-}
-
-DL4J_API int dl4j_vl_coef(const float* dloss, const int* rows, const int* count, float T, int scaled, float* coef, float* scale, hipStream_t st) {
-  if (!dloss || !rows || !count || !coef || !scale) return -2;
-  hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, st, dloss, rows, count, T, scaled, coef, scale);
-  return (int)hipGetLastError();
-}
-
-// out: [N rounded up to 256][row_bytes]
-DL4J_API int dl4j_vl_pack(const void* h, int64_t ldh_bytes, const int* rows, const int* count, void* out, int64_t row_bytes, int N, hipStream_t st) {
-  if (N <= 0 || row_bytes % 16 || ldh_bytes % 16 || !aligned16(h) || !aligned16(out)) return -2;
-  hipLaunchKernelGGL(pack_kernel, dim3((N + 255) / 256 * 256), dim3(256), 0, st, (const char*)h, ldh_bytes, rows, count, (char*)out, row_bytes);
-  return (int)hipGetLastError();
-}
-
-DL4J_API int dl4j_vl_entries(const void* idx, int idx64, int K, const float* p, const float* psum, const float* zk, const float* lse,
-                             const float* coef, const float* mass, const int* rows, const int* count, int N, int v0, int v1, void* G, int64_t ldg,
-                             int dt, hipStream_t st) {
-  if (N <= 0 || K <= 0 || !G || !zk) return -2;
-  hipLaunchKernelGGL(entries_kernel, dim3((N + 3) / 4), dim3(256), 0, st, idx, idx64, K, p, psum, zk, lse, coef, mass, rows, count, v0, v1, G, ldg, dt);
-  return (int)hipGetLastError();
-}
-
-DL4J_API int dl4j_vl_colsum(const void* G, int64_t ldg, int dt, int vc, const int* count, const float* scale, void* db, int bdt, hipStream_t st) {
-  if (vc <= 0 || ldg % 64 || ldg < vc || !db) return -2;
-  hipLaunchKernelGGL(colsum_kernel, dim3((vc + 63) / 64), dim3(256), 0, st, G, ldg, dt, vc, count, scale, db, bdt);
-  return (int)hipGetLastError();
-}
-
-// units of the dh product's grid for N rows at most; the slab takes units * 128 * 128 floats
-DL4J_API int dl4j_vl_dh_units(int N, int D) {
-  const int tiles = ((N + 127) / 128) * ((D + 127) / 128);
-  return tiles > 512 ? tiles : 512;
-}
-
-// d: N D vc ldg ldw dt wt accum units ; W points at the piece's first row (column)
-DL4J_API int dl4j_vl_dh(const void* G, const void* W, const int* count, float* slab, const int64_t* d, hipStream_t st) {
-  DhP p;
-  p.G = G; p.W = W; p.count = count; p.slab = slab;
-  p.D = (int)d[1]; p.vc = (int)d[2]; p.ldg = d[3]; p.ldw = d[4]; p.accum = (int)d[7]; p.units = (int)d[8];
-  const int dt = (int)d[5], wt = (int)d[6], ch = dt == DT_F32 ? 4 : 8;
-  if (d[0] <= 0 || p.D <= 0 || p.vc <= 0 || p.ldw % ch || p.ldg % 128 || p.ldg < p.vc || !aligned16(G) || !aligned16(W)) return -2;
-  if (p.ldw < ((wt ? p.vc : p.D) + ch - 1) / ch * ch) return -2;
-  if (p.units != dl4j_vl_dh_units((int)d[0], p.D) || !slab) return -2;
-  switch (dt * 2 + wt) {
-    case DT_BF16 * 2: return launch_dh<DT_BF16, true>(p, p.units, st);
-    case DT_BF16 * 2 + 1: return launch_dh<DT_BF16, false>(p, p.units, st);
-    case DT_F16 * 2: return launch_dh<DT_F16, true>(p, p.units, st);
-    case DT_F16 * 2 + 1: return launch_dh<DT_F16, false>(p, p.units, st);
-    case DT_F32 * 2: return launch_dh<DT_F32, true>(p, p.units, st);
-    case DT_F32 * 2 + 1: return launch_dh<DT_F32, false>(p, p.units, st);
-  }
-  return -2;
-}
-
-DL4J_API int dl4j_vl_dh_rows(const float* slab, const int* rows, const int* count, const float* scale, int N, int D, void* dh, int64_t ldo, int dt,
-                             hipStream_t st) {
-  if (N <= 0 || D <= 0 || !slab || !dh) return -2;
-  hipLaunchKernelGGL((dh_rows_kernel<128, 128>), dim3(N), dim3(256), 0, st, slab, rows, count, scale, D, dl4j_vl_dh_units(N, D), dh, ldo, dt);
-  return (int)hipGetLastError();
-}
-
-// d: D vc ldg ldh ldo dt wt ; out points at the piece's first row (column)
-DL4J_API int dl4j_vl_dw(const void* G, const void* H, const int* count, const float* scale, void* out, const int64_t* d, hipStream_t st) {
-  DwP p;
-  p.G = G; p.H = H; p.count = count; p.scale = scale; p.out = out;
-  p.D = (int)d[0]; p.vc = (int)d[1]; p.ldg = d[2]; p.ldh = d[3]; p.ldo = d[4];
-  const int dt = (int)d[5], wt = (int)d[6], ch = dt == DT_F32 ? 4 : 8;
-  if (p.D <= 0 || p.vc <= 0 || p.ldg % 128 || p.ldg < p.vc || p.ldh % ch || p.ldh < (p.D + ch - 1) / ch * ch || !aligned16(G) || !aligned16(H)) return -2;
-  switch (dt * 2 + wt) {
-    case DT_BF16 * 2: return launch_dw<DT_BF16, false>(p, st);
-    case DT_BF16 * 2 + 1: return launch_dw<DT_BF16, true>(p, st);
-    case DT_F16 * 2: return launch_dw<DT_F16, false>(p, st);
-    case DT_F16 * 2 + 1: return launch_dw<DT_F16, true>(p, st);
-    case DT_F32 * 2: return launch_dw<DT_F32, false>(p, st);
-    case DT_F32 * 2 + 1: return launch_dw<DT_F32, true>(p, st);
-  }
-  return -2;
+// dh [N, D], dw [V, D] ([D, V] with wt), db [V] from dloss [N] and the forward call's state
+DL4J_API int dl4j_linear_loss_bwd(const int64_t* args, const float* f, hipStream_t st) {
+  return backward(*reinterpret_cast<const Args*>(args), f, st);
 }

@@ -25,7 +25,6 @@ from ..nd4j.exceptions import ND4JIllegalArgumentException
 
 _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}      # operand codes of the GEMM core
 MAX_TEACHER = 1024                                                  # entries per row the kernels keep on chip
-PIECE_BYTES = 256 << 20                                             # gradient of the scores held at a time: fits the last-level cache
 
 
 def _need(ok, what):
@@ -120,8 +119,11 @@ def linear_topk_distillation_reference(hidden, weights, teacher_indices, teacher
 
 
 # ------------------------------------------------------------------------------------------------------------------ kernel calls
-def _i64(*v):
-    return (ctypes.c_int64 * len(v))(*[int(x) for x in v])
+# the fields of struct Args in native/csrc/vocab_loss.hip, in order
+_ARGS = ("N D V dt split wt bdt ldh ldw lab64 ignore idx64 tdt K want_h want_w want_b "
+         "H W bias labels idx t loss state ws dloss dh dw db").split()
+_AT = {n: k for k, n in enumerate(_ARGS)}
+_Block = ctypes.c_int64 * len(_ARGS)
 
 
 def _up(n, m):
@@ -144,162 +146,66 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else _up(t.shape[1], 16 // t.element_size())
 
 
-def _weights16(w):
-    """(operand, is_dv): W [V, D] row by row, or as the rows of its [D, V] transpose where that is how it lies in memory."""
-    if w.stride(1) != 1 and w.stride(0) == 1:
-        return _rows16(w.t()), 1
-    return _rows16(w), 0
-
-
-def _label_ptrs(labels):
-    return (L.ptr(labels), L.ptr(None)) if labels.dtype == torch.int64 else (L.ptr(None), L.ptr(labels))
-
-
-class _Rows:
-    """What both losses know about their rows: the list of those that take part, their number (on the device), and the loss' own terms."""
-    __slots__ = ("N", "rows", "count", "labels", "ignore", "keep", "smooth_v", "T", "idx", "p", "psum", "ent", "mass", "zk", "cross", "K")
-
-
-def _f32(n, like):
-    return torch.empty(n, dtype=torch.float32, device=like.device)
-
-
-def _cross_entropy_rows(labels, ignore, smoothing, V, loss):
-    r = _Rows()
-    r.N, r.labels, r.ignore, r.keep, r.smooth_v, r.T = labels.numel(), labels, ignore, 1.0 - smoothing, smoothing / V, 1.0
-    r.idx = r.p = r.psum = r.ent = r.mass = r.zk = r.cross = None
-    r.K = 0
-    buf = torch.empty(r.N + 1, dtype=torch.int32, device=labels.device)
-    r.rows, r.count = buf[1:], buf[:1]
-    l64, l32 = _label_ptrs(labels)
-    L.check(L.hip().dl4j_vl_rows(l64, l32, L.c_int64(ignore), L.ptr(None), L.c_int(r.N), L.ptr(r.rows), L.ptr(r.count), L.ptr(loss), L.stream()), "vl_rows")
-    return r
-
-
-def _distillation_rows(idx, t, temperature, loss):
-    r = _Rows()
-    N, K = idx.shape
-    r.N, r.K, r.labels, r.ignore, r.keep, r.smooth_v, r.T = N, K, None, 0, 0.0, 0.0, temperature
-    buf = torch.empty(N + 1, dtype=torch.int32, device=idx.device)
-    r.rows, r.count, r.idx = buf[1:], buf[:1], idx
-    r.p, r.psum, r.zk = _f32(N * K, idx), _f32(N * K, idx), _f32(N * K, idx)
-    r.ent, r.mass, r.cross = _f32(N, idx), _f32(N, idx), _f32(N, idx)
-    L.check(L.hip().dl4j_vl_teacher(L.ptr(idx), L.c_int(idx.dtype == torch.int64), L.ptr(t), L.c_int(_DT[t.dtype]), L.c_int(N), L.c_int(K),
-                                    L.c_float(1.0 / temperature), L.ptr(r.p), L.ptr(r.psum), L.ptr(r.ent), L.ptr(r.mass), L.stream()), "vl_teacher")
-    L.check(L.hip().dl4j_vl_rows(L.ptr(None), L.ptr(None), L.c_int64(0), L.ptr(r.mass), L.c_int(N), L.ptr(r.rows), L.ptr(r.count), L.ptr(loss), L.stream()),
-            "vl_rows")
-    return r
-
-
-def _scores(grad, r, h, w, dv, bias, v0, v1, part=None, tz=None, zs=None, lse=None, coef=None, G=None):
-    l64, l32 = _label_ptrs(r.labels) if r.labels is not None else (L.ptr(None), L.ptr(None))
-    V = w.shape[1] if dv else w.shape[0]
-    d = _i64(r.N, h.shape[1], V, v0, v1, _ld(h), _ld(w), G.stride(0) if G is not None else 0, _DT[h.dtype], dv, _DT[bias.dtype] if bias is not None else 0)
-    f = (ctypes.c_float * 3)(1.0 / r.T, r.smooth_v, r.keep)
-    L.check(L.hip().dl4j_vl_scores(L.c_int(grad), L.ptr(h), L.ptr(w), L.ptr(bias), L.ptr(r.rows), L.ptr(r.count), l64, l32, L.ptr(part), L.ptr(tz),
-                                   L.ptr(zs), L.ptr(lse), L.ptr(coef), L.ptr(r.mass), L.ptr(G), d, f, L.stream()), "vl_scores")
-
-
-def _forward(r, h, w, dv, bias, loss):
-    V = w.shape[1] if dv else w.shape[0]
-    N = r.N
-    tiles = L.hip().dl4j_vl_tiles(L.c_int(V), L.c_int(_DT[h.dtype]))
-    part, tz = _f32(tiles * N * 2, h), _f32(N, h)
-    zs = _f32(tiles * N, h) if r.smooth_v else None
-    lse = _f32(N, h)
-    if r.idx is not None:
-        g = _i64(N, h.shape[1], V, _ld(h), 1 if dv else _ld(w), _ld(w) if dv else 1, _DT[h.dtype], _DT[bias.dtype] if bias is not None else 0,
-                 r.idx.dtype == torch.int64, r.K)
-        L.check(L.hip().dl4j_vl_gather(L.ptr(h), L.ptr(w), L.ptr(bias), L.ptr(r.idx), L.ptr(r.p), L.ptr(r.rows), L.ptr(r.count), L.c_float(1.0 / r.T),
-                                       L.ptr(r.zk), L.ptr(r.cross), g, L.stream()), "vl_gather")
-    _scores(0, r, h, w, dv, bias, 0, V, part=part, tz=tz, zs=zs)
-    l64, l32 = _label_ptrs(r.labels) if r.labels is not None else (L.ptr(None), L.ptr(None))
-    L.check(L.hip().dl4j_vl_combine(L.ptr(part), L.ptr(zs), L.ptr(tz), L.ptr(r.rows), L.ptr(r.count), l64, l32, L.ptr(r.ent), L.ptr(r.cross),
-                                    L.ptr(r.mass), L.c_int(N), L.c_int(V), L.c_int(tiles), L.c_float(r.keep), L.c_float(r.T), L.ptr(lse),
-                                    L.ptr(loss), L.stream()), "vl_combine")
-    return lse
-
-
-def _pieces(V, rows, esz):
-    """Column ranges of the vocabulary whose score gradients fit PIECE_BYTES, of equal size up to a tile."""
-    most = max(256, PIECE_BYTES // (rows * esz) // 256 * 256)
-    n = (V + most - 1) // most
-    step = _up((V + n - 1) // n, 256)
-    return [(a, min(V, a + step)) for a in range(0, V, step)]
-
-
-def _backward(r, h, w, dv, bias, lse, dloss, shape, want_h, want_w, want_b):
-    N, D, V, dt = r.N, h.shape[1], (w.shape[1] if dv else w.shape[0]), h.dtype
-    dev, esz, code = h.device, h.element_size(), _DT[h.dtype]
-    coef, scale = _f32(N, h), _f32(1, h)
-    L.check(L.hip().dl4j_vl_coef(L.ptr(dloss), L.ptr(r.rows), L.ptr(r.count), L.c_float(r.T), L.c_int(dt == torch.float16), L.ptr(coef), L.ptr(scale),
-                                 L.stream()), "vl_coef")
-    Np = _up(N, 256)
-    pieces = _pieces(V, Np, esz)
-    G = torch.empty(Np, _up(pieces[0][1] - pieces[0][0], 256), dtype=dt, device=dev)
-    dh = dw = db = packed = slab = None
-    if want_w:
-        Dp = _up(D, 16 // esz)
-        packed = torch.empty(Np, Dp, dtype=dt, device=dev)
-        L.check(L.hip().dl4j_vl_pack(L.ptr(h), L.c_int64(_ld(h) * esz), L.ptr(r.rows), L.ptr(r.count), L.ptr(packed), L.c_int64(Dp * esz), L.c_int(N),
-                                     L.stream()), "vl_pack")
-        dw = torch.empty((D, V) if dv else (V, D), dtype=dt, device=dev)
-    if want_h:
-        units = L.hip().dl4j_vl_dh_units(L.c_int(N), L.c_int(D))
-        slab = _f32(units * 128 * 128, h)
-        dh = torch.empty(N, D, dtype=dt, device=dev)
-    if want_b:
-        db = torch.empty(V, dtype=bias.dtype, device=dev)
-    for k, (a, b) in enumerate(pieces):
-        _scores(1, r, h, w, dv, bias, a, b, lse=lse, coef=coef, G=G)
-        if r.idx is not None:
-            L.check(L.hip().dl4j_vl_entries(L.ptr(r.idx), L.c_int(r.idx.dtype == torch.int64), L.c_int(r.K), L.ptr(r.p), L.ptr(r.psum), L.ptr(r.zk), L.ptr(lse),
-                                            L.ptr(coef), L.ptr(r.mass), L.ptr(r.rows), L.ptr(r.count), L.c_int(N), L.c_int(a), L.c_int(b), L.ptr(G),
-                                            L.c_int64(G.stride(0)), L.c_int(code), L.stream()), "vl_entries")
-        if want_b:
-            L.check(L.hip().dl4j_vl_colsum(L.ptr(G), L.c_int64(G.stride(0)), L.c_int(code), L.c_int(b - a), L.ptr(r.count), L.ptr(scale), L.ptr(db[a:b]),
-                                           L.c_int(_DT[db.dtype]), L.stream()), "vl_colsum")
-        if want_h:
-            wp = w[:, a:b] if dv else w[a:b]
-            L.check(L.hip().dl4j_vl_dh(L.ptr(G), L.ptr(wp), L.ptr(r.count), L.ptr(slab), _i64(N, D, b - a, G.stride(0), _ld(w), code, dv, k > 0, units),
-                                       L.stream()), "vl_dh")
-        if want_w:
-            out = dw[:, a:b] if dv else dw[a:b]
-            L.check(L.hip().dl4j_vl_dw(L.ptr(G), L.ptr(packed), L.ptr(r.count), L.ptr(scale), L.ptr(out),
-                                       _i64(D, b - a, G.stride(0), packed.stride(0), dw.stride(0), code, dv), L.stream()), "vl_dw")
-    if want_h:
-        L.check(L.hip().dl4j_vl_dh_rows(L.ptr(slab), L.ptr(r.rows), L.ptr(r.count), L.ptr(scale), L.c_int(N), L.c_int(D), L.ptr(dh), L.c_int64(D),
-                                        L.c_int(code), L.stream()), "vl_dh_rows")
-        dh = dh.view(shape)
-    return dh, (dw.t() if dw is not None and dv else dw), db
+def _split(rows, training):
+    """fp32 operands as pairs of halves on the 16-bit matrix cores (three products, twice to three times the rate of the fp32 ones), once
+    the rows pay for the conversion of the weights."""
+    return rows >= (48 if training else 128)
 
 
 class _LinearLoss(torch.autograd.Function):
-    """hidden [..., D], weights [V, D], bias [V] or None; the rest describes the rows (labels, or teacher entries)."""
+    """hidden [..., D], weights [V, D], bias [V] or None; first / second: labels and None, or the teacher's indices and logits."""
 
     @staticmethod
     def forward(ctx, hidden, weights, bias, first, second, ignore, smoothing, temperature):
-        h = _rows16(hidden.reshape(-1, hidden.shape[-1]))
-        w, dv = _weights16(weights)
-        loss = _f32(h.shape[0], h)
-        if second is None:
-            r = _cross_entropy_rows(first, ignore, smoothing, weights.shape[0], loss)
+        lib = L.hip()
+        h = hidden.reshape(-1, hidden.shape[-1])
+        dv = int(weights.stride(1) != 1 and weights.stride(0) == 1)     # [V, D] row by row, or as the rows of its [D, V] transpose
+        w = weights.t() if dv else weights
+        training = any(ctx.needs_input_grad)
+        split = h.dtype == torch.float32 and _split(h.shape[0], training)
+        if split:                                                       # the conversion takes rows of any stride
+            h = h if h.stride(1) == 1 and (h.shape[0] == 1 or h.stride(0) >= h.shape[1]) else h.contiguous()
+            w = w if w.stride(1) == 1 and (w.shape[0] == 1 or w.stride(0) >= w.shape[1]) else w.contiguous()
         else:
-            r = _distillation_rows(first, second, temperature, loss)
-        lse = _forward(r, h, w, dv, bias, loss)
-        ctx.save_for_backward(h, w, bias, lse, first, second)
-        ctx.r, ctx.dv, ctx.shape = r, dv, hidden.shape
+            h, w = _rows16(h), _rows16(w)
+        N, dev = h.shape[0], h.device
+        loss = torch.empty(N, dtype=torch.float32, device=dev)
+        teacher = second is not None
+        a = _Block(N, h.shape[1], w.shape[1] if dv else w.shape[0], _DT[h.dtype], split, dv, _DT[bias.dtype] if bias is not None else 0, _ld(h), _ld(w),
+                   first.dtype == torch.int64, ignore, first.dtype == torch.int64, _DT[second.dtype] if teacher else 0, first.shape[1] if teacher else 0,
+                   *ctx.needs_input_grad[:3],
+                   h.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if teacher else first.data_ptr(), first.data_ptr() if teacher else 0,
+                   second.data_ptr() if teacher else 0, loss.data_ptr(), 0, 0, 0, 0, 0, 0)
+        f = (ctypes.c_float * 2)(temperature, smoothing)
+        state = torch.empty(lib.dl4j_linear_loss_bytes(a, 0), dtype=torch.uint8, device=dev)
+        ws = torch.empty(lib.dl4j_linear_loss_bytes(a, 1), dtype=torch.uint8, device=dev)
+        a[_AT["state"]], a[_AT["ws"]] = state.data_ptr(), ws.data_ptr()
+        L.check(lib.dl4j_linear_loss_fwd(a, f, L.stream()), "linear_loss_fwd")
+        if training:
+            ctx.save_for_backward(h, w, bias, first, second, loss, state)
+            ctx.call, ctx.dv, ctx.shape = (a, f), dv, hidden.shape
         return loss.view(hidden.shape[:-1])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        h, w, bias, lse, _, _ = ctx.saved_tensors
-        with torch.cuda.device(h.device):
+        lib = L.hip()
+        h, w, bias, _, _, _, _ = ctx.saved_tensors
+        a, f = ctx.call
+        a = _Block(*a)                                                  # (a graph kept alive may be walked from two threads)
+        dev = h.device
+        with torch.cuda.device(dev):
             g = dloss.reshape(-1)
             g = g if g.dtype == torch.float32 and g.is_contiguous() else g.float().contiguous()
-            dh, dw, db = _backward(ctx.r, h, w, ctx.dv, bias, lse, g, ctx.shape, *ctx.needs_input_grad[:3])
-        return dh, dw, db, None, None, None, None, None
+            want_h, want_w, want_b = ctx.needs_input_grad[:3]
+            dh = torch.empty(ctx.shape, dtype=h.dtype, device=dev) if want_h else None
+            dw = torch.empty(w.shape, dtype=h.dtype, device=dev) if want_w else None
+            db = torch.empty_like(bias) if want_b else None
+            ws = torch.empty(lib.dl4j_linear_loss_bytes(a, 2), dtype=torch.uint8, device=dev)
+            for name, t in (("ws", ws), ("dloss", g), ("dh", dh), ("dw", dw), ("db", db)):
+                a[_AT[name]] = 0 if t is None else t.data_ptr()
+            L.check(lib.dl4j_linear_loss_bwd(a, f, L.stream()), "linear_loss_bwd")
+        return dh, (dw.t() if want_w and ctx.dv else dw), db, None, None, None, None, None
 
 
 class _TopkDistillation(torch.autograd.Function):
@@ -309,7 +215,7 @@ class _TopkDistillation(torch.autograd.Function):
     def forward(ctx, logits, idx, t, temperature):
         z = logits.reshape(-1, logits.shape[-1])
         z = z if z.stride(1) == 1 and z.stride(0) >= z.shape[1] else z.contiguous()
-        loss, lse = _f32(z.shape[0], z), _f32(z.shape[0], z)
+        loss, lse = torch.empty(2, z.shape[0], dtype=torch.float32, device=z.device)
         c = _TopkDistillation.CODE
         L.check(L.hip().dl4j_topk_distill_fwd(L.ptr(z), L.c_int64(z.stride(0)), L.ptr(idx), L.c_int(idx.dtype == torch.int64), L.ptr(t), L.c_int(c[t.dtype]),
                                               L.c_int(z.shape[0]), L.c_int(z.shape[1]), L.c_int(idx.shape[1]), L.c_int(c[z.dtype]),
