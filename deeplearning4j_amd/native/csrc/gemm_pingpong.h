@@ -1,5 +1,8 @@
-// The ping-pong 256 x 256 loop of gemm_core.h (mainloop_pingpong_deep: phases, staging order, counted waits and hazards are those) for
-// operands in either layout, and product sources that take an operand as the sum of two 16-bit halves.
+// The ping-pong 256 x 256 loop of gemm_core.h (mainloop_pingpong_deep: wave groups, staging order and hazards are those) for operands in
+// either layout, and product sources that take an operand as the sum of two 16-bit halves.
+//
+// Phases of a k-tile read 8, 4, 8 and 4 fragments (32, 16, 32, 16 KiB for the four waves of a group; LDS gives 128 bytes a cycle, a phase's
+// MFMAs take 256 cycles): A-lo | B-hi | A-hi | B-lo of the NEXT k-tile, into the registers that B-hi has left. (With B-lo read beside A-lo, 12 / 4 / 8 / 0, the first phase waits for LDS.)
 //
 //   K-contiguous operand   the core's image: 256 rows x 128 bytes, half-tile h = rows g * 128 + h * 64 + 0..63 (A) / cols wn * 64 + h * 32 + 0..31 (B)
 //   K-major operand        each half-tile is an image of its own, [64 k][128 x] with a pitch of 256 bytes: 16 KiB, two 1-KiB pieces per
@@ -14,7 +17,7 @@
 namespace gemmcore {
 
 template <class C, bool TA, bool TB, class Src>
-__device__ __forceinline__ void mainloop_pp(char* smem, const Src& src, int KT, typename C::acc_t (&acc)[C::TM][C::TN]) {
+__device__ __forceinline__ void mainloop_pp(char* smem, const Src& src, int KT, typename C::acc_t (&acc)[C::TM][C::TN], const float (&init)[C::TN]) {
   static_assert(C::BM == 256 && C::BN == 256 && C::WM == 2 && C::WN == 4 && C::MF == 16 && C::STAGES == 2 && C::ESZ == 2, "ping-pong geometry");
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -24,7 +27,7 @@ __device__ __forceinline__ void mainloop_pp(char* smem, const Src& src, int KT, 
 #pragma unroll
     for (int j = 0; j < C::TN; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = init[j];
 
   constexpr int HALF = 16384;
   int oa[2][2], ob[2][2];
@@ -74,9 +77,14 @@ __device__ __forceinline__ void mainloop_pp(char* smem, const Src& src, int KT, 
   stage_ah(0, 1); stage_bh(0, 1); stage_bh(1, 1);
   wait_vmcnt<6>();                        // k-tile 0 landed
   PP_BAR();
+  bf16x8_t af[4][2], bx[2][2], by[2][2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) bx[j][ks] = frag_b(smem, 0, j, ks);
   if (grp == 1) PP_BAR();                 // stagger: group 1 runs one barrier behind group 0
 
-  bf16x8_t af[4][2], b0[2][2], b1[2][2];
+  // bx holds the k-tile's B-lo fragments; by takes its B-hi ones and, once those are used, B-lo of the next k-tile
   for (int t = 0; t < KT; ++t) {
     const char* cs = smem + (t & 1) * C::STAGE_BYTES;
     // ---- phase 0
@@ -84,36 +92,41 @@ __device__ __forceinline__ void mainloop_pp(char* smem, const Src& src, int KT, 
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) af[i][ks] = frag_a(cs, 0, i, ks);
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) b0[j][ks] = frag_b(cs, 0, j, ks);
     stage_ah(1, t + 1);
-    wait_vmcnt<10>();
+    wait_vmcnt<10>();                     // B-hi(t) landed
     PP_LOAD_END();
-    PP_MMA(0, 0, b0);
+    PP_MMA(0, 0, bx);
     // ---- phase 1
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) b1[j][ks] = frag_b(cs, 1, j, ks);
+      for (int ks = 0; ks < 2; ++ks) by[j][ks] = frag_b(cs, 1, j, ks);
     stage_ah(0, t + 2);
-    wait_vmcnt<10>();
+    wait_vmcnt<10>();                     // A-hi(t)
     PP_LOAD_END();
-    PP_MMA(0, 2, b1);
+    PP_MMA(0, 2, by);
     // ---- phase 2
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) af[i][ks] = frag_a(cs, 1, i, ks);
     stage_bh(0, t + 2);
+    wait_vmcnt<8>();                      // A-lo(t + 1) and B-lo(t + 1)
     PP_LOAD_END();
-    PP_MMA(4, 2, b1);
+    PP_MMA(4, 2, by);
     // ---- phase 3
+    const char* ns = smem + ((t + 1) & 1) * C::STAGE_BYTES;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) by[j][ks] = frag_b(ns, 0, j, ks);
     stage_bh(1, t + 2);
-    wait_vmcnt<10>();
     PP_LOAD_END();
-    PP_MMA(4, 0, b0);
+    PP_MMA(4, 0, bx);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) bx[j][ks] = by[j][ks];
   }
   wait_vmcnt<0>();                        // the stages past the end: the epilogue reuses the staging memory
   if (grp == 0) PP_BAR();                 // re-align the two groups: every LDS read of the main loop is complete behind this
@@ -213,14 +226,28 @@ template <class C, bool TA, bool TB, int SEG, bool PP> struct ProductSrc {
 
 template <class C> constexpr bool is_pp() { return C::BM == 256 && C::BN == 256; }
 
-// acc = k-tiles [t0, t1) of A . B^T at rows m0.., columns n0..
+// acc = init (a value per column of the lane) + k-tiles [t0, t1) of A . B^T at rows m0.., columns n0..
+template <class C, bool TA, bool TB, int SEG>
+__device__ __forceinline__ void product(char* smem, const Operand& A, const Operand& B, int m0, int n0, int K, int t0, int t1,
+                                        typename C::acc_t (&acc)[C::TM][C::TN], const float (&init)[C::TN]) {
+  ProductSrc<C, TA, TB, SEG, is_pp<C>()> src;
+  src.set(A, B, m0, n0, K, t0);
+  if constexpr (is_pp<C>()) mainloop_pp<C, TA, TB>(smem, src, t1 - t0, acc, init);
+  else {
+    mainloop_flex<C, decltype(src), TA, TB>(smem, src, t1 - t0, acc);
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) acc[i][j] += init[j];
+  }
+}
 template <class C, bool TA, bool TB, int SEG>
 __device__ __forceinline__ void product(char* smem, const Operand& A, const Operand& B, int m0, int n0, int K, int t0, int t1,
                                         typename C::acc_t (&acc)[C::TM][C::TN]) {
-  ProductSrc<C, TA, TB, SEG, is_pp<C>()> src;
-  src.set(A, B, m0, n0, K, t0);
-  if constexpr (is_pp<C>()) mainloop_pp<C, TA, TB>(smem, src, t1 - t0, acc);
-  else mainloop_flex<C, decltype(src), TA, TB>(smem, src, t1 - t0, acc);
+  float zero[C::TN];
+#pragma unroll
+  for (int j = 0; j < C::TN; ++j) zero[j] = 0.f;
+  product<C, TA, TB, SEG>(smem, A, B, m0, n0, K, t0, t1, acc, zero);
 }
 
 }  // namespace gemmcore

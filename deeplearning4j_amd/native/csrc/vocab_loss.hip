@@ -20,6 +20,10 @@ using namespace gemmcore;
 namespace {
 
 constexpr float NEG_INF = -__builtin_inff();
+// Scores are kept in units of log 2 (z' = z / T / ln 2): every exponential is one v_exp_f32, every normaliser one v_log_f32.
+constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x); }
 constexpr int KMAX = 1024;                              // teacher entries per row
 
 __device__ __forceinline__ float load_f(const void* p, int64_t i, int dt) {
@@ -51,11 +55,11 @@ __device__ __forceinline__ float sum16(float v) {
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   const float nm = fmaxf(m, m2);
   if (nm == NEG_INF) s += s2;
-  else s = s * __expf(m - nm) + s2 * __expf(m2 - nm);
+  else s = s * exp2_(m - nm) + s2 * exp2_(m2 - nm);
   m = nm;
 }
 
-// Factors that the halves' scaling (fp32) and the range of fp16 gradients bring in; all powers of two, 1 for other types.
+// Factors that the halves' scaling (fp32, powers of two) and the normalised coefficients of the backward pass bring in.
 struct Scales {
   float z;          // scores = z * product
   float h, w;       // of the operands' halves
@@ -63,18 +67,21 @@ struct Scales {
 };
 
 // ------------------------------------------------------------------------------------------------------------------------ rows
-// rows[0 .. count) = rows that take part, in order; rows[count .. N) = the others; loss of the others = 0.
+// rows[0 .. count) = rows that take part, in order, lab their labels (-1: outside the vocabulary, or none); rows[count .. N) = the others;
+// loss of the others = 0.
 // One workgroup: a scan of N flags, 1024 at a time.
 __global__ void __launch_bounds__(1024) rows_kernel(const void* __restrict__ labels, int lab64, int64_t ignore, const float* __restrict__ mass, int N,
-                                                    int* __restrict__ rows, int* __restrict__ count, Scales* __restrict__ sc,
-                                                    float* __restrict__ loss) {
+                                                    int V, int* __restrict__ rows, int* __restrict__ lab, int* __restrict__ count,
+                                                    Scales* __restrict__ sc, float* __restrict__ loss) {
   __shared__ int wsum[16];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   int done = 0;
   for (int64_t base = 0; base < N; base += 1024) {
     const int64_t n = base + tid;
     bool ok = false;
-    if (n < N) ok = labels ? load_index(labels, n, lab64) != ignore : mass[n] != 0.f;
+    int64_t y = -1;
+    if (n < N && labels) { y = load_index(labels, n, lab64); ok = y != ignore; }
+    else if (n < N) ok = mass[n] != 0.f;
     const unsigned long long b = __ballot(ok);
     if (lane == 0) wsum[wid] = __popcll(b);
     __syncthreads();
@@ -82,7 +89,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(const void* __restrict__ lab
     for (int w = 0; w < 16; ++w) { if (w < wid) before += wsum[w]; all += wsum[w]; }
     const int at = done + before + __popcll(b & ((1ull << lane) - 1));
     if (n < N) {
-      if (ok) rows[at] = (int)n;
+      if (ok) { rows[at] = (int)n; lab[at] = y >= 0 && y < V ? (int)y : -1; }
       else { rows[N - 1 - (n - at)] = (int)n; loss[n] = 0.f; }   // n - at rows before this one do not take part
     }
     done += all;
@@ -183,20 +190,27 @@ __global__ void __launch_bounds__(256) teacher_kernel(const TeacherP p) {
 
 // ------------------------------------------------------------------------------------------------------------------------ operands
 // largest finite |x| of W (workgroups 0 .. AMAX_W - 1) and of the rows of H that take part (the others): one value per workgroup
-constexpr int AMAX_W = 512, AMAX_H = 128;
+constexpr int AMAX_W = 1024, AMAX_H = 128;
 __global__ void __launch_bounds__(256) amax_kernel(const float* __restrict__ W, int64_t ldw, int wr, int wc, const float* __restrict__ H, int64_t ldh,
                                                    int D, const int* __restrict__ rows, const int* __restrict__ count, float* __restrict__ out) {
   __shared__ float red[16];
   const bool is_w = blockIdx.x < AMAX_W;
-  const int R = is_w ? wr : *count, C = is_w ? wc : D, step = is_w ? AMAX_W : AMAX_H;
+  const int R = is_w ? wr : *count, C = is_w ? wc : D, q = (C + 3) / 4;
+  const int64_t n = (int64_t)R * q, step = (is_w ? AMAX_W : AMAX_H) * 256;
   float m = 0.f;
-  for (int r = is_w ? blockIdx.x : blockIdx.x - AMAX_W; r < R; r += step) {
-    const float* x = is_w ? W + r * ldw : H + rows[r] * ldh;
 #pragma unroll 4
-    for (int c = threadIdx.x; c < C; c += 256) {
-      const float v = fabsf(x[c]);
-      m = fmaxf(m, v < __builtin_inff() ? v : 0.f);
+  for (int64_t i = (int64_t)(is_w ? blockIdx.x : blockIdx.x - AMAX_W) * 256 + threadIdx.x; i < n; i += step) {
+    const int r = (int)(i / q), c = (int)(i - (int64_t)r * q) * 4;
+    const float* x = (is_w ? W + r * ldw : H + rows[r] * ldh) + c;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c + 4 <= C && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+      const f32x4 f = *reinterpret_cast<const f32x4*>(x);
+      v[0] = f[0]; v[1] = f[1]; v[2] = f[2]; v[3] = f[3];
+    } else {
+      for (int j = 0; j < 4; ++j) v[j] = c + j < C ? x[j] : 0.f;
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { const float t = fabsf(v[j]); m = fmaxf(m, t < __builtin_inff() ? t : 0.f); }
   }
   m = block_max(m, red);
   if (threadIdx.x == 0) out[blockIdx.x] = m;
@@ -258,11 +272,47 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitP p) {
 
 // the rows that take part, packed
 __global__ void __launch_bounds__(256) pack_kernel(const char* __restrict__ h, int64_t ldh_bytes, const int* __restrict__ rows,
-                                                   const int* __restrict__ count, char* __restrict__ out, int64_t row_bytes) {
+                                                   const int* __restrict__ count, char* __restrict__ out, int64_t row_bytes, int64_t ldo_bytes) {
   const int c = *count, m = blockIdx.x;
   if (m >= c) return;
   const char* src = h + rows[m] * ldh_bytes;
-  for (int64_t b = threadIdx.x * 16; b < row_bytes; b += 256 * 16) *reinterpret_cast<f32x4*>(out + m * row_bytes + b) = *reinterpret_cast<const f32x4*>(src + b);
+  for (int64_t b = threadIdx.x * 16; b < row_bytes; b += 256 * 16) *reinterpret_cast<f32x4*>(out + m * ldo_bytes + b) = *reinterpret_cast<const f32x4*>(src + b);
+}
+
+// out[c][r] = in[row r][c] of 16-bit values, R x C, 64 x 64 at a time through LDS; blockIdx.z: the halves of a pair. `count`: R on the device,
+// and `rows` the row of position r (both or none); positions from R to the next multiple of 64 become zeros.
+struct TransposeP {
+  const uint16_t* in; int64_t ldi, half_in;
+  uint16_t* out; int64_t ldo, half_out;
+  int R, C;
+  const int* count; const int* rows;
+};
+__global__ void __launch_bounds__(256) transpose_kernel(const TransposeP p) {
+  __shared__ uint16_t tile[64][64 + 2];
+  const int R = p.count ? *p.count : p.R, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+  if (r0 >= R) return;
+  const uint16_t* in = p.in + blockIdx.z * p.half_in;
+  uint16_t* out = p.out + blockIdx.z * p.half_out;
+  const int r = threadIdx.x >> 2, q = (threadIdx.x & 3) * 16;      // 16 values of a row
+  const uint16_t* src = r0 + r < R ? in + (int64_t)(p.rows ? p.rows[r0 + r] : r0 + r) * p.ldi + c0 + q : nullptr;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (src && c0 + q + h * 8 < p.C) v = *reinterpret_cast<const s16x8*>(src + h * 8);      // rows are readable in whole chunks
+#pragma unroll
+    for (int e = 0; e < 8; ++e) tile[r][q + h * 8 + e] = (uint16_t)v[e];
+  }
+  __syncthreads();
+  const int c = threadIdx.x >> 2;
+  if (c0 + c >= p.C) return;
+  uint16_t* dst = out + (c0 + c) * p.ldo + r0 + q;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    s16x8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (short)tile[q + h * 8 + e][c];
+    *reinterpret_cast<s16x8*>(dst + h * 8) = v;
+  }
 }
 
 // ------------------------------------------------------------------------------------------------------------------------ scores
@@ -270,21 +320,39 @@ struct ScoreP {
   Operand H, W;                          // H: [rows, D] (xlim is the count, set on the device); W: columns of the vocabulary
   const void* bias; int bdt;
   const int* rows; const int* count; const Scales* sc;
-  const void* labels; int lab64;
+  const int* lab;                        // per position in `rows`
   int N, D, v0, v1;                      // columns [v0, v1) of the vocabulary
   float invT, smooth_v;                  // 1 / T;  e / V
   float2* part; float* tz; float* zs;    // statistics: part [ntiles][N]; target score [N]; zs [ntiles][N] = sum of z * e / V (or null)
   // gradient: coefficient and lse per position in `rows`
   const float* lse; const float* coef;
   float keep;                            // 1 - e
-  char* G; int64_t ldg, glo;             // [rows up to a tile][ldg bytes], column v at v - v0; second half glo bytes behind
+  char* G; int64_t ldg, glo;             // [v - v0][ldg bytes]: position m at element m; second half glo bytes behind
+  char* R; int64_t ldr, rlo;             // the gradient once more, row by row: [m][v - v0] (or null; 256 x 256 tiles)
+  float* colsum; int64_t ldc;            // [row tiles][ldc] column sums of the gradient, or null
   // teacher entries (first != null)
   const unsigned short* first; const int* sidx; const float* psum; float* zk; int K;
 };
 
-template <class C> constexpr int score_lds_stats() { return C::BM * 4 * (1 + 3 * C::WN) + C::BM / C::WM * (C::BN + 4) * 4; }
-template <class C> constexpr int score_lds_grad() { return C::BM * (C::BN * C::ESZ + 16) + 3 * C::BM * 4; }
+// pitch of a vocabulary row of the staged gradient: 4 positions of 16 columns leave the accumulators at a time, 8 banks (of fp32 16) apart
+template <class C> constexpr int grad_pitch() { return C::BM * C::ESZ + 16 * C::ESZ; }
+constexpr int larger(int a, int b) { return a > b ? a : b; }
+// The epilogue lays over the operand stages: the gradient; or the lanes' sums of exponentials, then the scores of the teacher's entries.
+// Behind them: the rows' side arrays.
+template <class C> constexpr int score_over(bool grad) {
+  return larger(C::STAGES * C::STAGE_BYTES, grad ? C::BN * grad_pitch<C>() : larger(C::WN * 16 * (C::BM + 16), C::BM / C::WM * (C::BN + 4)) * 4);
+}
+template <class C> constexpr int score_lds(bool grad) {
+  return score_over<C>(grad) + (grad ? 3 * C::BM + C::WM * C::BN : C::BM * (1 + 3 * C::WN) + 4 * C::NW + 1) * 4;
+}
 
+// The bias is where the accumulators start (-inf for columns past the vocabulary), so that a score is accumulator * zscale.
+//
+// Statistics: every exponential is taken against ONE reference per quarter wave, the largest score of its 32 rows x 64 columns (on the large
+// tile), instead of the row's maximum: four cross-lane steps in all instead of four per row, and no row waits for its own maximum. A sum of
+// exponentials 2^-100 below the reference is still a sound fp32 number; a row that lies lower makes the workgroup take the tile again with a
+// reference per row. The 16 lanes that share a row leave their partial sums in LDS, where one thread per row adds them.
+// Epilogue of a 256 x 256 tile: 11 us with a maximum and a sum reduced over the lanes for every row (product of one k-tile: 1.5 us).
 template <class C, bool TB, bool GRAD, int SEG>
 __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -294,67 +362,110 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
   int mt, nt;
   tile_coords(xcd_remap(blockIdx.x, mtiles * ntiles), mtiles, ntiles, 8, mt, nt);
   const int m0 = mt * C::BM, n0 = p.v0 + nt * C::BN;
-  typename C::acc_t acc[C::TM][C::TN];
-  {
-    Operand H = p.H;
-    H.xlim = count;
-    product<C, false, TB, SEG>(smem, H, p.W, m0, n0, p.D, 0, k_tiles<C, SEG>(p.D), acc);
-  }
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int wm = wid / C::WN, wn = wid - wm * C::WN, lc = lane & 15;
   const int row0 = wm * (C::BM / C::WM) + (lane >> 4) * 4, col0 = wn * (C::BN / C::WN) + lc;
-  const float zscale = p.sc->z * p.invT;
-  float bv[C::TN];
-#pragma unroll
-  for (int j = 0; j < C::TN; ++j) {
-    const int col = n0 + col0 + j * 16;
-    bv[j] = col < p.v1 ? (p.bias ? load_f(p.bias, col, p.bdt) * p.invT : 0.f) : NEG_INF;
+  constexpr int OSZ = C::ESZ, PITCH = grad_pitch<C>(), RW = C::BM / C::WM, CW = C::BN / C::WN;
+  const float zscale = p.sc->z * p.invT * LOG2E;
+  // the rows' label, coefficient and normaliser: on their way while the product runs
+  int lab = -1;
+  float rc = 0.f, rl = 3e38f;                                      // rows past the end: exp2(z - l) = 0
+  if (tid < C::BM && m0 + tid < count) {
+    lab = p.lab[m0 + tid] - n0;
+    if constexpr (GRAD) { rc = p.coef[m0 + tid]; rl = p.lse[m0 + tid]; }
   }
-  constexpr int OSZ = C::ESZ, PITCH = C::BN * OSZ + 16;
-  float* sf = reinterpret_cast<float*>(smem + (GRAD ? C::BM * PITCH : 0));
-  int* slab = reinterpret_cast<int*>(sf);                        // label's column inside the tile, or -1
-  for (int r = tid; r < C::BM; r += C::NT) {
-    const int m = m0 + r;
-    int lab = -1;
-    float c = 0.f, l = 0.f;
-    if (m < count) {
-      if (p.labels) {
-        const int64_t y = load_index(p.labels, p.rows[m], p.lab64) - n0;
-        lab = y >= 0 && y < C::BN && y + n0 < p.v1 ? (int)y : -1;
-      }
-      if constexpr (GRAD) { c = p.coef[m]; l = p.lse[m]; }
+  typename C::acc_t acc[C::TM][C::TN];
+  {
+    float init[C::TN];
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+      const int col = n0 + col0 + j * 16;
+      init[j] = col < p.v1 ? (p.bias ? load_f(p.bias, col, p.bdt) / p.sc->z : 0.f) : NEG_INF;
     }
-    slab[r] = lab;
-    if constexpr (GRAD) { sf[C::BM + r] = c; sf[2 * C::BM + r] = l; }
+    Operand H = p.H;
+    H.xlim = count;
+    product<C, false, TB, SEG>(smem, H, p.W, m0, n0, p.D, 0, k_tiles<C, SEG>(p.D), acc, init);
+  }
+  float* sf = reinterpret_cast<float*>(smem + score_over<C>(GRAD));
+  int* slab = reinterpret_cast<int*>(sf);                          // label's column inside the tile, or none of them
+  if (tid < C::BM) {
+    slab[tid] = lab < C::BN && lab + n0 < p.v1 ? lab : -1;
+    if constexpr (GRAD) { sf[C::BM + tid] = rc; sf[2 * C::BM + tid] = rl; }
   }
   __syncthreads();
+  // a label's score is rare in a wave's part of the tile: whether there is one at all is asked once
+  bool labelled = false;
+  for (int r = lane; r < RW; r += 64) labelled |= (unsigned)(slab[wm * RW + r] - wn * CW) < (unsigned)CW;
+  labelled = __any(labelled);
   if constexpr (!GRAD) {
-    float* sM = sf + C::BM;                                      // [WN][BM]
+    float* sM = sf + C::BM;                                        // [WN][BM] maximum (reference) and sum of a row in a wave's columns
     float* sS = sM + C::WN * C::BM;
     float* sZ = sS + C::WN * C::BM;
+    float* sR = sZ + C::WN * C::BM;                                // [NW][4] references
+    int* again = reinterpret_cast<int*>(sR + 4 * C::NW);
+    float* sP = reinterpret_cast<float*>(smem);                    // [WN][16][BM + 16] partial sums
+    float m = NEG_INF;
 #pragma unroll
     for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int r = row0 + i * 16 + q;
-        const int lab = slab[r] - col0;
-        float z[C::TN], m = NEG_INF;
+      for (int j = 0; j < C::TN; ++j) m = fmaxf(fmaxf(fmaxf(m, acc[i][j][0]), fmaxf(acc[i][j][1], acc[i][j][2])), acc[i][j][3]);
+    m = max16(m) * zscale;
+    const float ref = m == NEG_INF ? 0.f : m;
+    if (lc == 0) sR[wid * 4 + (lane >> 4)] = ref;
+    if (tid == 0) *again = 0;
 #pragma unroll
-        for (int j = 0; j < C::TN; ++j) {
-          z[j] = acc[i][j][q] * zscale + bv[j];
-          m = fmaxf(m, z[j]);
-          if (lab == j * 16) p.tz[m0 + r] = z[j];
-          acc[i][j][q] = z[j];
-        }
-        const float mm = max16(m);
-        const float ref = mm == NEG_INF ? 0.f : mm;
+    for (int i = 0; i < C::TM; ++i) {
+      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s[q] += exp2_(acc[i][j][q] * zscale - ref);   // (the reference passes over a NaN score, the sum keeps it)
+      *reinterpret_cast<f32x4*>(sP + (wn * 16 + lc) * (C::BM + 16) + row0 + i * 16) = s;
+    }
+    __syncthreads();
+    if (tid < C::BM && m0 + tid < count) {
+      bool low = false;
+#pragma unroll
+      for (int w = 0; w < C::WN; ++w) {
         float s = 0.f;
 #pragma unroll
-        for (int j = 0; j < C::TN; ++j) s += __expf(z[j] - ref);  // the maximum passes over a NaN score, the sum keeps it
-        s = sum16(s);
-        if (lc == 0) { sM[wn * C::BM + r] = mm; sS[wn * C::BM + r] = s; }
+        for (int k = 0; k < 16; ++k) s += sP[(w * 16 + k) * (C::BM + 16) + tid];
+        sM[w * C::BM + tid] = sR[(tid / RW * C::WN + w) * 4 + ((tid >> 2) & 3)];
+        sS[w * C::BM + tid] = s;
+        low |= s < 0x1p-100f && n0 + w * CW < p.v1;
       }
-    if (p.zs) {                                                  // label smoothing
+      if (low) *again = 1;
+    }
+    __syncthreads();
+    if (*again) {                                                  // a reference per row
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float mr = NEG_INF, s = 0.f;
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j) mr = fmaxf(mr, acc[i][j][q]);
+          mr = max16(mr) * zscale;
+          const float rr = mr == NEG_INF ? 0.f : mr;
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j) s += exp2_(acc[i][j][q] * zscale - rr);
+          s = sum16(s);
+          if (lc == 0) { sM[wn * C::BM + row0 + i * 16 + q] = mr; sS[wn * C::BM + row0 + i * 16 + q] = s; }
+        }
+    }
+    if (labelled) {
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = row0 + i * 16 + q, at = slab[r] - col0;
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j)
+            if (at == j * 16) p.tz[m0 + r] = acc[i][j][q] * zscale;
+        }
+    }
+    if (p.zs) {                                                    // label smoothing
+      const float k = zscale * p.smooth_v;
 #pragma unroll
       for (int i = 0; i < C::TM; ++i)
 #pragma unroll
@@ -362,27 +473,26 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
           float zsum = 0.f;
 #pragma unroll
           for (int j = 0; j < C::TN; ++j)
-            if (n0 + col0 + j * 16 < p.v1) zsum += acc[i][j][q] * p.smooth_v;
+            if (n0 + col0 + j * 16 < p.v1) zsum += acc[i][j][q] * k;
           zsum = sum16(zsum);
           if (lc == 0) sZ[wn * C::BM + row0 + i * 16 + q] = zsum;
         }
     }
     __syncthreads();
-    for (int r = tid; r < C::BM; r += C::NT) {
-      if (m0 + r >= count) continue;
-      float m = NEG_INF, s = 0.f, z = 0.f;
+    if (tid < C::BM && m0 + tid < count) {
+      float mx = NEG_INF, s = 0.f, z = 0.f;
 #pragma unroll
       for (int w = 0; w < C::WN; ++w) {
-        join(m, s, sM[w * C::BM + r], sS[w * C::BM + r]);
-        if (p.zs) z += sZ[w * C::BM + r];
+        join(mx, s, sM[w * C::BM + tid], sS[w * C::BM + tid]);
+        if (p.zs) z += sZ[w * C::BM + tid];
       }
-      p.part[(int64_t)nt * p.N + m0 + r] = make_float2(m, s);
-      if (p.zs) p.zs[(int64_t)nt * p.N + m0 + r] = z;
+      p.part[(int64_t)nt * p.N + m0 + tid] = make_float2(mx, s);
+      if (p.zs) p.zs[(int64_t)nt * p.N + m0 + tid] = z;
     }
     if (p.first) {
       // the scores of the teacher's entries: the tile passes through LDS, one row of waves at a time, and every row picks its own
-      constexpr int RW = C::BM / C::WM, P4 = C::BN + 4, TPR = C::NT / RW;
-      float* sz = sf + C::BM * (1 + 3 * C::WN);
+      constexpr int P4 = C::BN + 4, TPR = C::NT / RW;
+      float* sz = reinterpret_cast<float*>(smem);
       for (int half = 0; half < C::WM; ++half) {
         if (wm == half) {
 #pragma unroll
@@ -393,14 +503,14 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
               for (int j = 0; j < C::TN; ++j) sz[(row0 - wm * RW + i * 16 + q) * P4 + col0 + j * 16] = acc[i][j][q];
         }
         __syncthreads();
-        const int r = tid / TPR, m = m0 + half * RW + r;
-        if (m < count) {
-          const int n = p.rows[m];
+        const int r = tid / TPR, at = m0 + half * RW + r;
+        if (at < count) {
+          const int n = p.rows[at];
           const int64_t t = nt + p.v0 / C::BN;
           const int e1 = p.first[(t + 1) * p.N + n];
           for (int e = p.first[t * p.N + n] + tid % TPR; e < e1; e += TPR) {
             const int64_t o = (int64_t)n * p.K + e;
-            p.zk[o] = sz[r * P4 + p.sidx[o] - n0];
+            p.zk[o] = sz[r * P4 + p.sidx[o] - n0] * zscale;
           }
         }
         __syncthreads();
@@ -409,59 +519,114 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
   } else {
     typedef Out<C::DT == DT_F32 ? OT_F32 : C::DT == DT_F16 ? OT_F16 : OT_BF16> O;
     typedef typename O::T OTy;
+    typedef OTy Pack __attribute__((ext_vector_type(4)));
 #pragma unroll
-    for (int i = 0; i < C::TM; ++i)
+    for (int i = 0; i < C::TM; ++i) {
+      const f32x4 c = *reinterpret_cast<const f32x4*>(sf + C::BM + row0 + i * 16), l = *reinterpret_cast<const f32x4*>(sf + 2 * C::BM + row0 + i * 16);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int r = row0 + i * 16 + q;
-        const int lab = slab[r] - col0;
-        const float c = sf[C::BM + r], l = sf[2 * C::BM + r];
+      for (int q = 0; q < 4; ++q)
 #pragma unroll
-        for (int j = 0; j < C::TN; ++j) {
-          float g = c * (__expf(acc[i][j][q] * zscale + bv[j] - l) - p.smooth_v);
-          if (lab == j * 16) g -= c * p.keep;
-          if (n0 + col0 + j * 16 >= p.v1 || m0 + r >= count) g = 0.f;
-          const OTy hi = O::cv(g);
-          *reinterpret_cast<OTy*>(smem + r * PITCH + (col0 + j * 16) * OSZ) = hi;
-          if constexpr (SEG == 3) acc[i][j][q] = g - O::fl(hi);
-        }
-      }
-    constexpr int CPR = C::BN * OSZ / 16;
-    char* out = p.G + (int64_t)m0 * p.ldg + (int64_t)(n0 - p.v0) * OSZ;
+        for (int j = 0; j < C::TN; ++j) acc[i][j][q] = c[q] * exp2_(acc[i][j][q] * zscale - l[q]);
+    }
+    if (p.smooth_v != 0.f) {
 #pragma unroll
-    for (int half = 0; half < (SEG == 3 ? 2 : 1); ++half) {
-      if (half == 1) {
-        __syncthreads();
+      for (int j = 0; j < C::TN; ++j) {
+        const float sv = n0 + col0 + j * 16 < p.v1 ? p.smooth_v : 0.f;
 #pragma unroll
         for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int j = 0; j < C::TN; ++j)
-              *reinterpret_cast<OTy*>(smem + (row0 + i * 16 + q) * PITCH + (col0 + j * 16) * OSZ) = O::cv(acc[i][j][q]);
+          for (int q = 0; q < 4; ++q) acc[i][j][q] -= sf[C::BM + row0 + i * 16 + q] * sv;
       }
+    }
+    if (labelled) {
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = row0 + i * 16 + q, at = slab[r] - col0;
+          const float ck = sf[C::BM + r] * p.keep;
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j)
+            if (at == j * 16) acc[i][j][q] -= ck;
+        }
+    }
+    if (p.colsum) {                                                // a lane's rows, the four lane groups of a column, the wave rows
+      float* sC = sf + 3 * C::BM;
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) s += (acc[i][j][0] + acc[i][j][1]) + (acc[i][j][2] + acc[i][j][3]);
+        s += __shfl_xor(s, 16, 64);
+        s += __shfl_xor(s, 32, 64);
+        if (lane < 16) sC[wm * C::BN + col0 + j * 16] = s;
+      }
+    }
+    char* out = p.G + (int64_t)(n0 - p.v0) * p.ldg + (int64_t)m0 * OSZ;
+    constexpr int CPR = C::BM * OSZ / 16;
+#pragma unroll
+    for (int half = 0; half < (SEG == 3 ? 2 : 1); ++half) {
+      if (half == 1) __syncthreads();
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j) {
+          Pack v;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            v[q] = O::cv(acc[i][j][q]);
+            if constexpr (SEG == 3) acc[i][j][q] -= O::fl(v[q]);
+          }
+          *reinterpret_cast<Pack*>(smem + (col0 + j * 16) * PITCH + (row0 + i * 16) * OSZ) = v;
+        }
       __syncthreads();
       if (p.first) {
         // the teacher's entries of this tile, from their exact scores: entries with one index write the same value
-        for (int r = tid; r < C::BM; r += C::NT) {
-          const int m = m0 + r;
-          if (m >= count) break;
-          const int n = p.rows[m];
+        if (tid < C::BM && m0 + tid < count) {
+          const int n = p.rows[m0 + tid];
           const int64_t t = nt + p.v0 / C::BN;
           const int e1 = p.first[(t + 1) * p.N + n];
           for (int e = p.first[t * p.N + n]; e < e1; ++e) {
             const int64_t o = (int64_t)n * p.K + e;
-            float g = sf[C::BM + r] * (__expf(p.zk[o] - sf[2 * C::BM + r]) - p.psum[o]);
+            float g = sf[C::BM + tid] * (exp2_(p.zk[o] - sf[2 * C::BM + tid]) - p.psum[o]);
             if (half == 1) g -= O::fl(O::cv(g));
-            *reinterpret_cast<OTy*>(smem + r * PITCH + (p.sidx[o] - n0) * OSZ) = O::cv(g);
+            *reinterpret_cast<OTy*>(smem + (p.sidx[o] - n0) * PITCH + tid * OSZ) = O::cv(g);
           }
         }
         __syncthreads();
       }
       char* o = out + half * p.glo;
-      for (int idx = tid; idx < C::BM * CPR; idx += C::NT) {
-        const int r = idx / CPR, ch = idx - r * CPR;
-        *reinterpret_cast<f32x4*>(o + r * p.ldg + ch * 16) = *reinterpret_cast<const f32x4*>(smem + r * PITCH + ch * 16);
+      for (int idx = tid; idx < C::BN * CPR; idx += C::NT) {
+        const int v = idx / CPR, ch = idx - v * CPR;
+        if (n0 + v < p.v1) *reinterpret_cast<f32x4*>(o + v * p.ldg + ch * 16) = *reinterpret_cast<const f32x4*>(smem + v * PITCH + ch * 16);
+      }
+      if constexpr (is_pp<C>()) {
+        if (p.R) {
+          // rows again: transposing LDS reads give a lane 4 + 4 words of one position; a wave writes 16 positions x 32 words at a time
+          char* orow = p.R + half * p.rlo + (int64_t)m0 * p.ldr + (int64_t)(n0 - p.v0) * OSZ;
+          const int x = lane & 15, g4 = lane >> 4;
+          const char* base = smem + (g4 * 8 + (x >> 2)) * PITCH + (x & 3) * 8;
+#pragma unroll 4
+          for (int b = wid; b < 128; b += 8) {
+            const int v = (b & 7) * 32, m = (b >> 3) * 16;
+            const char* a0 = base + v * PITCH + m * 2;
+            typedef s16x4 __attribute__((address_space(3))) * lds_ptr_t;
+            const s16x4 t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr_t)(a0));
+            const s16x4 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr_t)(a0 + 4 * PITCH));
+            s16x8 t;
+            t[0] = t0[0]; t[1] = t0[1]; t[2] = t0[2]; t[3] = t0[3]; t[4] = t1[0]; t[5] = t1[1]; t[6] = t1[2]; t[7] = t1[3];
+            *reinterpret_cast<s16x8*>(orow + (int64_t)(m + x) * p.ldr + (v + g4 * 8) * 2) = t;
+          }
+        }
+      }
+    }
+    if (p.colsum) {
+      const float* sC = sf + 3 * C::BM;
+      for (int v = tid; v < C::BN; v += C::NT) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < C::WM; ++w) s += sC[w * C::BN + v];
+        if (n0 + v < p.v1) p.colsum[mt * p.ldc + n0 + v] = s;
       }
     }
   }
@@ -471,9 +636,9 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
 struct CombineP {
   const float2* part; const float* zs; const float* tz;
   const int* rows; const int* count;
-  const void* labels; int lab64;
+  const int* lab;
   const float* ent; const float* sp; const float* zk; int K;    // distillation (ent != null)
-  int N, V, ntiles;
+  int N, ntiles;
   float keep, T;
   float* lse; float* loss;
 };
@@ -511,70 +676,70 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineP p) {
     }
   }
   if (g != 0 || m >= count) return;
-  float lse = mx + __logf(s), loss;
+  float lse = mx + log2_(s), loss;
   if (p.ent) {
     const float h = p.ent[n];
-    loss = p.T * p.T * (h - z + lse);
+    loss = p.T * p.T * (h + LN2 * (lse - z));
     if (h != h) lse = h;                                         // nothing sound to distil from: the row's gradient is NaN too
   } else {
-    const int64_t y = load_index(p.labels, n, p.lab64);
-    const bool in = y >= 0 && y < p.V;
+    const bool in = p.lab[m] >= 0;
     if (!in) lse = __builtin_nanf("");                           // a label outside the vocabulary: loss and gradient of the row are NaN
-    loss = lse - (in ? p.keep * p.tz[m] : 0.f) - z;
+    loss = LN2 * (lse - (in ? p.keep * p.tz[m] : 0.f) - z);
   }
   p.lse[m] = lse;
   p.loss[n] = loss;
 }
 
 // ------------------------------------------------------------------------------------------------------------------------ backward
-// coef[m] = dloss[rows[m]] * T * s.  s = 1, or where the scores' gradient is kept in fp16 the power of two that puts the largest
-// coefficient into [2^13, 2^14): no entry is larger then, and entries down to 2^-38 of it stay above fp16's smallest step.
+// coef[m] = dloss[rows[m]] * T * s with the largest at `top` (0: s = 1). The scores' gradient is rounded to 16 bits: at a label it is close to
+// its coefficient, and with the largest coefficient at a power of two the large ones sit at the end of their binade, where a rounding counts
+// least; fp16 takes 2^14, so that entries down to 2^-38 of the largest stay above its smallest step.
 __global__ void __launch_bounds__(1024) coef_kernel(const float* __restrict__ dloss, const int* __restrict__ rows, const int* __restrict__ count,
-                                                    float T, int scaled, float* __restrict__ coef, Scales* __restrict__ sc) {
+                                                    float T, float top, float* __restrict__ coef, Scales* __restrict__ sc) {
   __shared__ float red[16];
   const int c = *count;
   float s = 1.f;
-  if (scaled) {
+  if (top > 0.f) {
     float mx = 0.f;
     for (int m = threadIdx.x; m < c; m += 1024) {
       const float v = fabsf(dloss[rows[m]] * T);
       if (v < __builtin_inff()) mx = fmaxf(mx, v);
     }
-    s = scale_for(block_max(mx, red));
+    mx = block_max(mx, red);
+    if (mx > 0.f) s = fminf(top / mx, 1e37f);
   }
   for (int m = threadIdx.x; m < c; m += 1024) coef[m] = dloss[rows[m]] * T * s;
   if (threadIdx.x == 0) { sc->db = 1.f / s; sc->dh = 1.f / s / sc->w; sc->dw = 1.f / s / sc->h; }
 }
 
-// db[v] = scale * column sum of the scores' gradient (of both its halves): 8 columns per thread, 32 row lanes, 64 columns per workgroup
-__global__ void __launch_bounds__(256) colsum_kernel(const char* __restrict__ G, int64_t ldg, int64_t glo, int dt, int vc, const int* __restrict__ count,
-                                                     const Scales* __restrict__ sc, void* __restrict__ db, int bdt) {
-  __shared__ float red[32][65];
-  const int cg = threadIdx.x & 7, rl = threadIdx.x >> 3, c = *count;
-  const int v = blockIdx.x * 64 + cg * 8;
-  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (v < vc)                                                    // rows are zero between vc and the next multiple of 128 columns
-    for (int m = rl; m < c; m += 32) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] += load_f(G + m * ldg, v + e, dt);
-      if (glo)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] += load_f(G + glo + m * ldg, v + e, dt);
-    }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) red[rl][cg * 8 + e] = s[e];
-  __syncthreads();
-  if (threadIdx.x < 64 && (int)(blockIdx.x * 64 + threadIdx.x) < vc) {
-    float a = 0.f;
-    for (int r = 0; r < 32; ++r) a += red[r][threadIdx.x];
-    store_f(db, blockIdx.x * 64 + threadIdx.x, bdt, a * sc->db);
+// db[v] = scale * sum over the row tiles' column sums
+__global__ void __launch_bounds__(256) bias_kernel(const float* __restrict__ colsum, int64_t ldc, int bm, int V, const int* __restrict__ count,
+                                                   const Scales* __restrict__ sc, void* __restrict__ db, int bdt) {
+  const int v = blockIdx.x * 256 + threadIdx.x, tiles = (*count + bm - 1) / bm;
+  if (v >= V) return;
+  float s = 0.f;
+#pragma unroll 4
+  for (int t = 0; t < tiles; ++t) s += colsum[t * ldc + v];
+  store_f(db, v, bdt, s * sc->db);
+}
+// the same from the gradient itself (both halves), one wave per word: with teacher entries the tiles' sums do not hold them
+__global__ void __launch_bounds__(256) bias_rows_kernel(const char* __restrict__ G, int64_t ldg, int64_t glo, int dt, int vc, const int* __restrict__ count,
+                                                        const Scales* __restrict__ sc, void* __restrict__ db, int bdt) {
+  const int v = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, c = *count;
+  if (v >= vc) return;
+  float s = 0.f;
+  for (int m = lane; m < c; m += 64) {
+    s += load_f(G + v * ldg, m, dt);
+    if (glo) s += load_f(G + glo + v * ldg, m, dt);
   }
+  s = wave_sum(s);
+  if (lane == 0) store_f(db, v, bdt, s * sc->db);
 }
 
 // dh: unit u of the grid owns output tile u % tiles and share u / tiles of the piece's columns; its fp32 tile lives in slab u and is added
 // to by the following pieces. Which unit owns what depends on the number of rows alone, so the sum's order is fixed.
 struct DhP {
-  Operand G, W;                          // G: xlim set on the device
+  Operand G, W;
   const int* count;
   int D, vc, units, accum;
   float* slab;
@@ -597,7 +762,7 @@ template <class C> __device__ __forceinline__ void to_slab(float* tile, typename
       }
 }
 
-template <class C, bool TB, int SEG>
+template <class C, bool TA, bool TB, int SEG>
 __global__ void __launch_bounds__(C::NT) dh_kernel(const DhP p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int count = *p.count;
@@ -612,9 +777,7 @@ __global__ void __launch_bounds__(C::NT) dh_kernel(const DhP p) {
   const int ktiles = k_tiles<C, SEG>(p.vc), per = (ktiles + shares - 1) / shares;
   const int k0 = min(ktiles, share * per), k1 = min(ktiles, k0 + per);
   typename C::acc_t acc[C::TM][C::TN];
-  Operand G = p.G;
-  G.xlim = mtiles * C::BM;                                       // rows up to the tile's end are there (zeros)
-  product<C, false, TB, SEG>(smem, G, p.W, mt * C::BM, nt * C::BN, p.vc, k0, k1, acc);
+  product<C, TA, TB, SEG>(smem, p.G, p.W, mt * C::BM, nt * C::BN, p.vc, k0, k1, acc);
   to_slab<C>(p.slab + (int64_t)u * C::BM * C::BN, acc, p.accum);
 }
 
@@ -642,7 +805,8 @@ __global__ void __launch_bounds__(256) dh_rows_kernel(const float* __restrict__ 
   }
 }
 
-// dW[v0 .. v0 + vc) = scale * dz^T h (SWAP 0, [V, D]) or its transpose (SWAP 1, [D, V]): both operands are walked along their rows.
+// dW[v0 .. v0 + vc) = scale * dz^T h (SWAP 0, [V, D]) or its transpose (SWAP 1, [D, V]): the gradient is read along its
+// rows (the sum's axis); h is walked row by row by the 128 x 128 tiles, and read along the rows of its transpose by the 256 x 256 ones.
 // shares > 1 (small outputs): the rows' range is cut, fp32 tiles go to a slab and dw_sum_kernel adds them in order.
 struct DwP {
   Operand G, H;
@@ -664,8 +828,21 @@ __global__ void __launch_bounds__(C::NT) dw_kernel(const DwP p) {
   const int ktiles = k_tiles<C, SEG>(K), per = (ktiles + p.shares - 1) / p.shares;
   const int k0 = min(ktiles, share * per), k1 = min(ktiles, k0 + per);
   typename C::acc_t acc[C::TM][C::TN];
-  product<C, true, true, SEG>(smem, SWAP ? p.H : p.G, SWAP ? p.G : p.H, m0, n0, K, k0, k1, acc);
+  product<C, SWAP && !is_pp<C>(), !SWAP && !is_pp<C>(), SEG>(smem, SWAP ? p.H : p.G, SWAP ? p.G : p.H, m0, n0, K, k0, k1, acc);
   if (p.shares > 1) { to_slab<C>(p.slab + (int64_t)u * C::BM * C::BN, acc, false); return; }
+  if constexpr (is_pp<C>() && OT == OT_F32) {                      // an fp32 tile is more than LDS: stores of 16 columns from the accumulators
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, wm = wid / C::WN, wn = wid - wm * C::WN;
+    const int r0 = m0 + wm * (C::BM / C::WM) + (lane >> 4) * 4, c0 = n0 + wn * (C::BN / C::WN) + (lane & 15);
+    const float s = p.sc->dw;
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j)
+          if (r0 + i * 16 + q < M && c0 + j * 16 < N) reinterpret_cast<float*>(p.out)[(r0 + i * 16 + q) * p.ldo + c0 + j * 16] = acc[i][j][q] * s;
+    return;
+  }
   EpiP e;
   e.out = p.out; e.residual = nullptr; e.bias = nullptr; e.stats = nullptr; e.stat_shift = nullptr;
   e.alpha = p.sc->dw; e.act = ACT_NONE; e.accum = 0;
@@ -715,8 +892,9 @@ int g_tune[8] = {-1, -1, -1, -1, -1, -1, -1, -1};
 struct Plan {
   int tile, dh_tile, dw_tile;            // TILE_*
   int op;                                // operand type of the products
-  int bn, tiles;                         // column tiles of the scores
-  int64_t np, dp, wcp, wrows;            // padded rows / columns of the packed H and of the halves of W
+  bool nt;                               // backward products on 256 x 256 tiles from operands laid out along the sum's axis
+  int bm, bn, tiles;                     // tiles of the scores
+  int64_t np, dp, wcp, wrows, vp;           // padded rows / columns of the packed H and of the halves of W
   int pieces, step;
   int units, shares;
   int64_t gcols;
@@ -732,27 +910,26 @@ Plan plan(const Args& a) {
   p.tile = TUNE(0, bits16 && big_tiles >= 176 && a.N > 128 ? TILE_BIG : a.N <= 32 ? TILE_FEW : TILE_MID);
   if (a.split && p.tile == TILE_FEW) p.tile = TILE_MID;
   if (!bits16 && p.tile == TILE_BIG) p.tile = TILE_MID;
+  p.bm = p.tile == TILE_BIG ? 256 : p.tile == TILE_FEW ? 32 : 128;
   p.bn = p.tile == TILE_BIG ? 256 : 128;
   p.tiles = (int)(up(a.V, p.bn) / p.bn);
   p.np = up(a.N, 256);
+  p.vp = up(a.V, 64);
   p.dp = up(a.D, 8);
   p.wrows = a.wt ? a.D : a.V;
   p.wcp = up(a.wt ? a.V : a.D, 8);
   const int64_t esz = a.dt == DT_F32 ? 4 : 2;                    // halves take as much as fp32
-  const int64_t most = TUNE(4, 256) * (int64_t)(1 << 20) / (p.np * esz) / 256 * 256;
+  const int64_t most = TUNE(4, 512) * (int64_t)(1 << 20) / (p.np * esz) / 256 * 256;
   p.pieces = (int)(most >= 256 ? (a.V + most - 1) / most : up(a.V, 256) / 256);
   p.step = (int)up((a.V + p.pieces - 1) / p.pieces, 256);
   p.pieces = (int)((a.V + p.step - 1) / p.step);
   p.gcols = up(a.V < p.step ? a.V : p.step, 256);
-  p.dh_tile = TUNE(1, bits16 && a.N > 128 && a.D >= 256 ? TILE_BIG : TILE_MID);
-  if (!bits16) p.dh_tile = TILE_MID;
+  p.nt = p.tile == TILE_BIG && TUNE(1, a.N >= 512 && a.D >= 256);
+  p.dh_tile = p.dw_tile = p.nt ? TILE_BIG : TILE_MID;
   const int ht = p.dh_tile == TILE_BIG ? 256 : 128;
   const int64_t htiles = up(a.N, ht) / ht * (up(a.D, ht) / ht);
   const int want = p.dh_tile == TILE_BIG ? 256 : 512;
   p.units = (int)(htiles > want ? htiles : want);
-  const int64_t wbig = up(p.gcols, 256) / 256 * (up(a.D, 256) / 256);
-  p.dw_tile = TUNE(2, bits16 && wbig >= 176 ? TILE_BIG : TILE_MID);
-  if (!bits16) p.dw_tile = TILE_MID;
   const int wt = p.dw_tile == TILE_BIG ? 256 : 128;
   const int64_t wtiles = up(p.gcols < a.V ? p.gcols : a.V, wt) / wt * (up(a.D, wt) / wt);
   const int64_t ks = up(a.N, 64) / 64;
@@ -773,13 +950,13 @@ struct Carve {
   }
 };
 struct State {
-  Scales* sc; int* count; int* rows; float* lse;
+  Scales* sc; int *count, *rows, *lab; float* lse;
   int* sidx; float *sp, *psum, *zk, *ent, *mass; unsigned short* first;
   _Float16 *wo, *ho;
   int64_t bytes;
   State(const Args& a, const Plan& p) {
     Carve c(a.state);
-    sc = c.take<Scales>(1); count = c.take<int>(1); rows = c.take<int>(a.N); lse = c.take<float>(a.N);
+    sc = c.take<Scales>(1); count = c.take<int>(1); rows = c.take<int>(a.N); lab = c.take<int>(a.N); lse = c.take<float>(a.N);
     const int64_t nk = a.K ? a.N * a.K : 0;
     sidx = c.take<int>(nk); sp = c.take<float>(nk); psum = c.take<float>(nk); zk = c.take<float>(nk);
     ent = c.take<float>(a.K ? a.N : 0); mass = c.take<float>(a.K ? a.N : 0);
@@ -791,7 +968,7 @@ struct State {
 };
 struct Work {
   float2* part; float *tz, *zs, *amax;                           // forward
-  float* coef; char* G; char* packed; float *dh_slab, *dw_slab;  // backward
+  float *coef, *colsum; char* G; char* packed; uint16_t *ht, *wtr; float *dh_slab, *dw_slab;  // backward
   int64_t fwd, bwd;
   Work(const Args& a, const Plan& p) {
     Carve c(a.ws);
@@ -800,8 +977,11 @@ struct Work {
     fwd = c.at;
     c.at = 0;
     const int64_t esz = a.dt == DT_F32 ? 4 : 2;
-    coef = c.take<float>(a.N); G = c.take<char>(p.np * p.gcols * esz);
-    packed = c.take<char>(a.want_w && !a.split ? p.np * up(a.D, 16 / esz) * esz : 0);
+    coef = c.take<float>(a.N); G = c.take<char>(p.np * p.gcols * esz * (p.nt ? 2 : 1));
+    colsum = c.take<float>(a.want_b && !a.K ? (a.N + p.bm - 1) / p.bm * a.V : 0);
+    packed = c.take<char>(a.want_w && !a.split && !p.nt ? a.N * p.dp * esz : 0);
+    ht = c.take<uint16_t>(a.want_w && p.nt ? a.D * p.np * (a.split ? 2 : 1) : 0);
+    wtr = c.take<uint16_t>(a.want_h && p.nt && !a.wt ? a.D * p.vp * (a.split ? 2 : 1) : 0);
     const int64_t ht = p.dh_tile == TILE_BIG ? 256 : 128;
     dh_slab = c.take<float>(a.want_h ? p.units * ht * ht : 0);
     const int64_t wt = p.dw_tile == TILE_BIG ? 256 : 128;
@@ -818,8 +998,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 template <class C, bool TB, bool GRAD, int SEG> int launch_score(const ScoreP& p, hipStream_t st) {
   const int64_t grid = (int64_t)((p.N + C::BM - 1) / C::BM) * ((p.v1 - p.v0 + C::BN - 1) / C::BN);
   if (grid > 0x7fffffff) return -2;
-  constexpr int EPI = GRAD ? score_lds_grad<C>() : score_lds_stats<C>();
-  constexpr int MAIN = C::STAGES * C::STAGE_BYTES, LDS = MAIN > EPI ? MAIN : EPI;
+  constexpr int LDS = score_lds<C>(GRAD);
   static_assert(LDS <= 160 * 1024, "tile does not fit the 160 KiB LDS");
   static DeviceOnceLds once;
   once.ensure(reinterpret_cast<const void*>(&score_kernel<C, TB, GRAD, SEG>), LDS);
@@ -839,25 +1018,28 @@ template <bool GRAD> int scores(const ScoreP& p, int tile, int op, bool split, b
   return tb ? dispatch_score<true, GRAD>(p, tile, op, split, st) : dispatch_score<false, GRAD>(p, tile, op, split, st);
 }
 
-template <class C, bool TB, int SEG> int launch_dh(const DhP& p, hipStream_t st) {
+template <class C, bool TA, bool TB, int SEG> int launch_dh(const DhP& p, hipStream_t st) {
   constexpr int LDS = C::STAGES * C::STAGE_BYTES;
   static DeviceOnceLds once;
-  once.ensure(reinterpret_cast<const void*>(&dh_kernel<C, TB, SEG>), LDS);
-  hipLaunchKernelGGL((dh_kernel<C, TB, SEG>), dim3(p.units), dim3(C::NT), LDS, st, p);
+  once.ensure(reinterpret_cast<const void*>(&dh_kernel<C, TA, TB, SEG>), LDS);
+  hipLaunchKernelGGL((dh_kernel<C, TA, TB, SEG>), dim3(p.units), dim3(C::NT), LDS, st, p);
   return (int)hipGetLastError();
 }
-template <bool TB> int dispatch_dh(const DhP& p, int tile, int op, bool split, hipStream_t st) {
-  const bool big = tile == TILE_BIG;
-  if (split) return big ? launch_dh<Big<DT_F16>, TB, 3>(p, st) : launch_dh<Mid<DT_F16>, TB, 3>(p, st);
-  if (op == DT_F32) return launch_dh<Mid<DT_F32>, TB, 1>(p, st);
-  if (op == DT_BF16) return big ? launch_dh<Big<DT_BF16>, TB, 1>(p, st) : launch_dh<Mid<DT_BF16>, TB, 1>(p, st);
-  return big ? launch_dh<Big<DT_F16>, TB, 1>(p, st) : launch_dh<Mid<DT_F16>, TB, 1>(p, st);
+// 256 x 256: both operands K-contiguous (p.nt); 128 x 128: the gradient and the [V, D] table are walked row by row
+int dispatch_dh(const DhP& p, int tile, int op, bool split, bool wt, hipStream_t st) {
+  if (tile == TILE_BIG)
+    return split ? launch_dh<Big<DT_F16>, false, false, 3>(p, st) : op == DT_BF16 ? launch_dh<Big<DT_BF16>, false, false, 1>(p, st)
+                                                                                 : launch_dh<Big<DT_F16>, false, false, 1>(p, st);
+  if (split) return wt ? launch_dh<Mid<DT_F16>, true, false, 3>(p, st) : launch_dh<Mid<DT_F16>, true, true, 3>(p, st);
+  if (op == DT_F32) return wt ? launch_dh<Mid<DT_F32>, true, false, 1>(p, st) : launch_dh<Mid<DT_F32>, true, true, 1>(p, st);
+  if (op == DT_BF16) return wt ? launch_dh<Mid<DT_BF16>, true, false, 1>(p, st) : launch_dh<Mid<DT_BF16>, true, true, 1>(p, st);
+  return wt ? launch_dh<Mid<DT_F16>, true, false, 1>(p, st) : launch_dh<Mid<DT_F16>, true, true, 1>(p, st);
 }
 
 template <class C, int OT, bool SWAP, int SEG> int launch_dw(const DwP& p, hipStream_t st) {
   const int M = SWAP ? p.D : p.vc, N = SWAP ? p.vc : p.D;
   const int tiles = ((M + C::BM - 1) / C::BM) * ((N + C::BN - 1) / C::BN);
-  constexpr int LDS = C::lds_bytes(Out<OT>::SZ);
+  constexpr int LDS = is_pp<C>() && OT == OT_F32 ? C::STAGES * C::STAGE_BYTES : C::lds_bytes(Out<OT>::SZ);
   static_assert(LDS <= 160 * 1024, "tile does not fit the 160 KiB LDS");
   static DeviceOnceLds once;
   once.ensure(reinterpret_cast<const void*>(&dw_kernel<C, OT, SWAP, SEG>), LDS);
@@ -870,7 +1052,7 @@ template <class C, int OT, bool SWAP, int SEG> int launch_dw(const DwP& p, hipSt
 }
 template <bool SWAP> int dispatch_dw(const DwP& p, int tile, int op, bool split, hipStream_t st) {
   const bool big = tile == TILE_BIG;
-  if (split) return launch_dw<Mid<DT_F16>, OT_F32, SWAP, 3>(p, st);
+  if (split) return big ? launch_dw<Big<DT_F16>, OT_F32, SWAP, 3>(p, st) : launch_dw<Mid<DT_F16>, OT_F32, SWAP, 3>(p, st);
   if (op == DT_F32) return launch_dw<Mid<DT_F32>, OT_F32, SWAP, 1>(p, st);
   if (op == DT_BF16) return big ? launch_dw<Big<DT_BF16>, OT_BF16, SWAP, 1>(p, st) : launch_dw<Mid<DT_BF16>, OT_BF16, SWAP, 1>(p, st);
   return big ? launch_dw<Big<DT_F16>, OT_F16, SWAP, 1>(p, st) : launch_dw<Mid<DT_F16>, OT_F16, SWAP, 1>(p, st);
@@ -903,7 +1085,7 @@ void operands(const Args& a, const Plan& p, const State& s, Operand& H, Operand&
 ScoreP score_args(const Args& a, const State& s, const float* f) {
   ScoreP q = {};
   q.bias = a.bias; q.bdt = (int)a.bdt; q.rows = s.rows; q.count = s.count; q.sc = s.sc;
-  q.labels = a.K ? nullptr : a.labels; q.lab64 = (int)a.lab64;
+  q.lab = s.lab;
   q.N = (int)a.N; q.D = (int)a.D;
   q.invT = 1.f / f[0]; q.smooth_v = f[1] / (float)a.V; q.keep = 1.f - f[1];
   if (a.K) { q.first = s.first; q.sidx = s.sidx; q.psum = s.psum; q.zk = s.zk; q.K = (int)a.K; q.keep = 0.f; q.smooth_v = 0.f; }
@@ -922,7 +1104,7 @@ int forward(const Args& a, const float* f, hipStream_t st) {
     hipLaunchKernelGGL(teacher_kernel, dim3((unsigned)((a.N + 3) / 4)), dim3(256), 4 * 12 * p2, st, t);
     VL_CHECK();
   }
-  hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, a.K ? nullptr : a.labels, (int)a.lab64, a.ignore, s.mass, (int)a.N, s.rows, s.count, s.sc, a.loss);
+  hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, a.K ? nullptr : a.labels, (int)a.lab64, a.ignore, s.mass, (int)a.N, (int)a.V, s.rows, s.lab, s.count, s.sc, a.loss);
   VL_CHECK();
   if (a.split) {
     const int wr = (int)p.wrows, wc = (int)(a.wt ? a.V : a.D);
@@ -939,7 +1121,7 @@ int forward(const Args& a, const float* f, hipStream_t st) {
   q.v0 = 0; q.v1 = (int)a.V;
   q.part = w.part; q.tz = w.tz; q.zs = q.smooth_v != 0.f ? w.zs : nullptr;
   if (const int e = scores<false>(q, p.tile, p.op, a.split, a.wt, st)) return e;
-  CombineP c{w.part, q.zs, w.tz, s.rows, s.count, q.labels, (int)a.lab64, a.K ? s.ent : nullptr, s.sp, s.zk, (int)a.K, (int)a.N, (int)a.V, p.tiles, q.keep, f[0],
+  CombineP c{w.part, q.zs, w.tz, s.rows, s.count, s.lab, a.K ? s.ent : nullptr, s.sp, s.zk, (int)a.K, (int)a.N, p.tiles, q.keep, f[0],
              s.lse, a.loss};
   if (a.N <= 256) hipLaunchKernelGGL((combine_kernel<1>), dim3((unsigned)a.N), dim3(256), 0, st, c);
   else hipLaunchKernelGGL((combine_kernel<8>), dim3((unsigned)((a.N + 7) / 8)), dim3(256), 0, st, c);
@@ -952,44 +1134,62 @@ int backward(const Args& a, const float* f, hipStream_t st) {
   const State s(a, p);
   const Work w(a, p);
   const int esz = a.dt == DT_F32 ? 4 : 2, gsz = a.split ? 2 : esz;
-  hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, st, a.dloss, s.rows, s.count, f[0], (int)(p.op == DT_F16), w.coef, s.sc);
+  hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, st, a.dloss, s.rows, s.count, f[0], p.op == DT_F16 ? 16384.f : p.op == DT_BF16 ? 1.f : 0.f, w.coef, s.sc);
   VL_CHECK();
   Operand H, W;
   operands(a, p, s, H, W);
   Operand packed = H;
-  if (a.want_w && !a.split) {
-    const int64_t rb = up(a.D, 16 / esz) * esz;
-    hipLaunchKernelGGL(pack_kernel, dim3((unsigned)a.N), dim3(256), 0, st, (const char*)a.H, a.ldh * esz, s.rows, s.count, w.packed, rb);
+  if (a.want_w && p.nt) {
+    TransposeP t{(const uint16_t*)H.p, H.ld / 2, H.lo / 2, w.ht, p.np, a.D * p.np, (int)a.N, (int)a.D, s.count, H.rows};
+    hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)((a.N + 63) / 64), (unsigned)((a.D + 63) / 64), a.split ? 2 : 1), dim3(256), 0, st, t);
     VL_CHECK();
-    packed = Operand{w.packed, rb, 0, 0, nullptr};
+    packed = Operand{(const char*)w.ht, p.np * 2, a.split ? a.D * p.np * 2 : 0, 0, nullptr};
+  } else if (a.want_w && !a.split) {
+    const int64_t rb = up(a.D, 16 / esz) * esz;
+    const int64_t ld = p.dp * esz;
+    hipLaunchKernelGGL(pack_kernel, dim3((unsigned)a.N), dim3(256), 0, st, (const char*)a.H, a.ldh * esz, s.rows, s.count, w.packed, rb, ld);
+    VL_CHECK();
+    packed = Operand{w.packed, ld, 0, 0, nullptr};
   }
   packed.xlim = (int)a.D;
-  const int64_t ldg = p.gcols * gsz, glo = a.split ? p.np * ldg : 0;
+  Operand wh = W;                                                  // W for the dh product
+  if (a.want_h && p.nt && !a.wt) {
+    TransposeP t{(const uint16_t*)W.p, W.ld / 2, W.lo / 2, w.wtr, p.vp, a.D * p.vp, (int)a.V, (int)a.D, nullptr, nullptr};
+    hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)((a.V + 63) / 64), (unsigned)((a.D + 63) / 64), a.split ? 2 : 1), dim3(256), 0, st, t);
+    VL_CHECK();
+    wh = Operand{(const char*)w.wtr, p.vp * 2, a.split ? a.D * p.vp * 2 : 0, 0, nullptr};
+  }
+  const int64_t ldg = p.np * gsz, glo = a.split ? p.gcols * ldg : 0;
+  const int64_t ldr = p.gcols * gsz, rlo = a.split ? p.np * ldr : 0;   // the same row by row (p.nt)
+  char* rows_g = w.G + p.np * p.gcols * esz;
   for (int k = 0; k < p.pieces; ++k) {
     const int v0 = k * p.step, v1 = (int)(a.V < v0 + (int64_t)p.step ? a.V : v0 + p.step), vc = v1 - v0;
     ScoreP q = score_args(a, s, f);
     q.H = H; q.W = W;
     q.W.xlim = (int)a.V;
     q.v0 = v0; q.v1 = v1; q.lse = s.lse; q.coef = w.coef; q.G = w.G; q.ldg = ldg; q.glo = glo;
+    if (p.nt && a.want_h) { q.R = rows_g; q.ldr = ldr; q.rlo = rlo; }
+    if (a.want_b && !a.K) { q.colsum = w.colsum; q.ldc = a.V; }
     if (const int e = scores<true>(q, p.tile, p.op, a.split, a.wt, st)) return e;
-    if (a.want_b) {
-      hipLaunchKernelGGL(colsum_kernel, dim3((vc + 63) / 64), dim3(256), 0, st, w.G, ldg, glo, a.split ? (int)DT_F16 : (int)a.dt, vc, s.count, s.sc,
+    if (a.want_b && a.K) {
+      hipLaunchKernelGGL(bias_rows_kernel, dim3((vc + 3) / 4), dim3(256), 0, st, w.G, ldg, glo, a.split ? (int)DT_F16 : (int)a.dt, vc, s.count, s.sc,
                          (char*)a.db + (int64_t)v0 * (a.bdt == DT_F32 ? 4 : 2), (int)a.bdt);
       VL_CHECK();
     }
     Operand G{w.G, ldg, glo, 0, nullptr};
     if (a.want_h) {
       DhP d;
-      d.G = G; d.W = W;
-      d.W.p += a.wt ? (int64_t)v0 * gsz : v0 * W.ld;
+      d.G = p.nt ? Operand{rows_g, ldr, rlo, 0, nullptr} : G;
+      d.G.xlim = (int)p.np; d.W = wh;
+      d.W.p += p.nt || a.wt ? (int64_t)v0 * gsz : v0 * wh.ld;
       d.W.xlim = (int)a.D;
       d.count = s.count; d.D = (int)a.D; d.vc = vc; d.units = p.units; d.accum = k > 0; d.slab = w.dh_slab;
-      const int e = a.wt ? dispatch_dh<false>(d, p.dh_tile, p.op, a.split, st) : dispatch_dh<true>(d, p.dh_tile, p.op, a.split, st);
+      const int e = dispatch_dh(d, p.dh_tile, p.op, a.split, a.wt, st);
       if (e) return e;
     }
     if (a.want_w) {
       DwP d;
-      d.G = G; d.G.xlim = (int)up(vc, p.bn);                      // zeros from vc on
+      d.G = G; d.G.xlim = vc;
       d.H = packed; d.count = s.count; d.sc = s.sc;
       d.out = (char*)a.dw + (a.wt ? (int64_t)v0 : v0 * a.D) * esz;
       d.ldo = a.wt ? a.V : a.D;
@@ -997,6 +1197,10 @@ int backward(const Args& a, const float* f, hipStream_t st) {
       const int e = a.wt ? dispatch_dw<true>(d, p.dw_tile, p.op, a.split, st) : dispatch_dw<false>(d, p.dw_tile, p.op, a.split, st);
       if (e) return e;
     }
+  }
+  if (a.want_b && !a.K) {
+    hipLaunchKernelGGL(bias_kernel, dim3((unsigned)((a.V + 255) / 256)), dim3(256), 0, st, w.colsum, a.V, p.bm, (int)a.V, s.count, s.sc, a.db, (int)a.bdt);
+    VL_CHECK();
   }
   if (a.want_h) {
     if (p.dh_tile == TILE_BIG)
