@@ -196,13 +196,16 @@ int dispatch(bool bwd, const void* z, int64_t ldz, const void* idx, int idx64, c
 
 }  // namespace
 
-// z [N][ldz], idx / t [N][K]; loss, lse [N] (lse of z / T, for the backward call). Types: 0 fp32, 1 bf16, 2 fp16.
-DL4J_API int dl4j_topk_distill_fwd(const void* z, int64_t ldz, const void* idx, int idx64, const void* t, int tdt, int N, int V, int K, int dt,
-                                   float T, float* loss, float* lse, hipStream_t st) {
-  return dispatch(false, z, ldz, idx, idx64, t, tdt, N, V, K, dt, T, loss, lse, nullptr, nullptr, st);
-}
-// dz [N][V]
-DL4J_API int dl4j_topk_distill_bwd(const void* z, int64_t ldz, const void* idx, int idx64, const void* t, int tdt, int N, int V, int K, int dt,
-                                   float T, const float* lse, const float* dloss, void* dz, hipStream_t st) {
-  return dispatch(true, z, ldz, idx, idx64, t, tdt, N, V, K, dt, T, nullptr, const_cast<float*>(lse), dloss, dz, st);
+// One call (ops/vocab_loss.py lists the same fields in the same order). Types: 0 fp32, 1 bf16, 2 fp16.
+// loss != null: loss [N] and lse [N] (of z / T, for the backward call); else dz [N][V] from dloss [N] and lse.
+struct DistillArgs {
+  int64_t N, V, K, ldz, dt, idx64, tdt;
+  const void *z, *idx, *t;
+  float *loss, *lse; const float* dloss; void* dz;
+};
+DL4J_API int dl4j_topk_distill(const int64_t* args, const float* f, hipStream_t st) {
+  const DistillArgs& a = *reinterpret_cast<const DistillArgs*>(args);
+  if (a.N > 0x7fffffff || a.V > 0x7fffffff || a.K > KMAX) return -2;
+  return dispatch(a.loss == nullptr, a.z, a.ldz, a.idx, (int)a.idx64, a.t, (int)a.tdt, (int)a.N, (int)a.V, (int)a.K, (int)a.dt, f[0], a.loss, a.lse, a.dloss,
+                  a.dz, st);
 }

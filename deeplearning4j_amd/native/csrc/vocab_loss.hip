@@ -1217,11 +1217,14 @@ int backward(const Args& a, const float* f, hipStream_t st) {
 DL4J_API void dl4j_vl_tune(int i, int v) { g_tune[i] = v; }
 #endif
 
-// bytes of the state (0), the forward workspace (1) and the backward workspace (2)
-DL4J_API int64_t dl4j_linear_loss_bytes(const int64_t* args, int which) {
+// bytes of the state, the forward workspace and the backward workspace
+DL4J_API void dl4j_linear_loss_bytes(const int64_t* args, int64_t* out) {
   const Args& a = *reinterpret_cast<const Args*>(args);
   const Plan p = plan(a);
-  return which == 0 ? State(a, p).bytes : which == 1 ? Work(a, p).fwd : Work(a, p).bwd;
+  const Work w(a, p);
+  out[0] = State(a, p).bytes;
+  out[1] = w.fwd;
+  out[2] = w.bwd;
 }
 // loss [N] of cross entropy (K = 0) or of distillation; f: temperature, label smoothing
 DL4J_API int dl4j_linear_loss_fwd(const int64_t* args, const float* f, hipStream_t st) {

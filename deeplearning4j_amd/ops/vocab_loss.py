@@ -152,16 +152,42 @@ def _split(rows, training):
     return rows >= (48 if training else 128)
 
 
+def _launch(fn, what, dev, *args):
+    """One native call on the current stream of ``dev``, with ``dev`` as the current device."""
+    if dev.index == torch.cuda.current_device():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if code:
+        L.check(code, what)
+
+
+def _lib():
+    lib = L.hip()
+    if lib.dl4j_linear_loss_fwd.argtypes is None:
+        for fn in (lib.dl4j_linear_loss_fwd, lib.dl4j_linear_loss_bwd, lib.dl4j_topk_distill):
+            fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+        lib.dl4j_linear_loss_bytes.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    return lib
+
+
+def _dloss(g):
+    g = g.reshape(-1)
+    return g if g.dtype == torch.float32 and g.is_contiguous() else g.float().contiguous()
+
+
 class _LinearLoss(torch.autograd.Function):
     """hidden [..., D], weights [V, D], bias [V] or None; first / second: labels and None, or the teacher's indices and logits."""
 
     @staticmethod
     def forward(ctx, hidden, weights, bias, first, second, ignore, smoothing, temperature):
-        lib = L.hip()
+        lib = _lib()
         h = hidden.reshape(-1, hidden.shape[-1])
-        dv = int(weights.stride(1) != 1 and weights.stride(0) == 1)     # [V, D] row by row, or as the rows of its [D, V] transpose
+        dv = weights.stride(1) != 1 and weights.stride(0) == 1          # [V, D] row by row, or as the rows of its [D, V] transpose
         w = weights.t() if dv else weights
-        training = any(ctx.needs_input_grad)
+        want = ctx.needs_input_grad[:3]
+        training = any(want)
         split = h.dtype == torch.float32 and _split(h.shape[0], training)
         if split:                                                       # the conversion takes rows of any stride
             h = h if h.stride(1) == 1 and (h.shape[0] == 1 or h.stride(0) >= h.shape[1]) else h.contiguous()
@@ -169,43 +195,53 @@ class _LinearLoss(torch.autograd.Function):
         else:
             h, w = _rows16(h), _rows16(w)
         N, dev = h.shape[0], h.device
-        loss = torch.empty(N, dtype=torch.float32, device=dev)
+        loss = torch.empty(hidden.shape[:-1], dtype=torch.float32, device=dev)
         teacher = second is not None
-        a = _Block(N, h.shape[1], w.shape[1] if dv else w.shape[0], _DT[h.dtype], split, dv, _DT[bias.dtype] if bias is not None else 0, _ld(h), _ld(w),
-                   first.dtype == torch.int64, ignore, first.dtype == torch.int64, _DT[second.dtype] if teacher else 0, first.shape[1] if teacher else 0,
-                   *ctx.needs_input_grad[:3],
+        is64 = first.dtype == torch.int64
+        a = _Block(N, h.shape[1], weights.shape[0], _DT[h.dtype], split, dv, 0 if bias is None else _DT[bias.dtype], _ld(h), _ld(w), is64, ignore, is64,
+                   _DT[second.dtype] if teacher else 0, first.shape[1] if teacher else 0, *want,
                    h.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if teacher else first.data_ptr(), first.data_ptr() if teacher else 0,
                    second.data_ptr() if teacher else 0, loss.data_ptr(), 0, 0, 0, 0, 0, 0)
         f = (ctypes.c_float * 2)(temperature, smoothing)
-        state = torch.empty(lib.dl4j_linear_loss_bytes(a, 0), dtype=torch.uint8, device=dev)
-        ws = torch.empty(lib.dl4j_linear_loss_bytes(a, 1), dtype=torch.uint8, device=dev)
+        size = (ctypes.c_int64 * 3)()
+        lib.dl4j_linear_loss_bytes(a, size)
+        state = torch.empty(size[0], dtype=torch.uint8, device=dev)
+        ws = torch.empty(size[1], dtype=torch.uint8, device=dev)
         a[_AT["state"]], a[_AT["ws"]] = state.data_ptr(), ws.data_ptr()
-        L.check(lib.dl4j_linear_loss_fwd(a, f, L.stream()), "linear_loss_fwd")
+        _launch(lib.dl4j_linear_loss_fwd, "linear_loss_fwd", dev, a, f)
         if training:
             ctx.save_for_backward(h, w, bias, first, second, loss, state)
-            ctx.call, ctx.dv, ctx.shape = (a, f), dv, hidden.shape
-        return loss.view(hidden.shape[:-1])
+            ctx.call, ctx.dv, ctx.shape = (a, f, size[2]), dv, hidden.shape
+        return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dloss):
-        lib = L.hip()
-        h, w, bias, _, _, _, _ = ctx.saved_tensors
-        a, f = ctx.call
-        a = _Block(*a)                                                  # (a graph kept alive may be walked from two threads)
-        dev = h.device
-        with torch.cuda.device(dev):
-            g = dloss.reshape(-1)
-            g = g if g.dtype == torch.float32 and g.is_contiguous() else g.float().contiguous()
-            want_h, want_w, want_b = ctx.needs_input_grad[:3]
-            dh = torch.empty(ctx.shape, dtype=h.dtype, device=dev) if want_h else None
-            dw = torch.empty(w.shape, dtype=h.dtype, device=dev) if want_w else None
-            db = torch.empty_like(bias) if want_b else None
-            ws = torch.empty(lib.dl4j_linear_loss_bytes(a, 2), dtype=torch.uint8, device=dev)
-            for name, t in (("ws", ws), ("dloss", g), ("dh", dh), ("dw", dw), ("db", db)):
-                a[_AT[name]] = 0 if t is None else t.data_ptr()
-            L.check(lib.dl4j_linear_loss_bwd(a, f, L.stream()), "linear_loss_bwd")
-        return dh, (dw.t() if want_w and ctx.dv else dw), db, None, None, None, None, None
+        return _once(_linear_backward, ctx, dloss) if torch.is_grad_enabled() else _linear_backward(ctx, dloss)
+
+
+def _linear_backward(ctx, dloss):
+    h, w, bias = ctx.saved_tensors[:3]
+    a, f, size = ctx.call
+    a = _Block(*a)                                                      # (a graph kept alive may be walked from two threads)
+    dev = h.device
+    g = _dloss(dloss)
+    want_h, want_w, want_b = ctx.needs_input_grad[:3]
+    dh = torch.empty(ctx.shape, dtype=h.dtype, device=dev) if want_h else None
+    dw = torch.empty(w.shape, dtype=h.dtype, device=dev) if want_w else None
+    db = torch.empty_like(bias) if want_b else None
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    for name, t in (("ws", ws), ("dloss", g), ("dh", dh), ("dw", dw), ("db", db)):
+        if t is not None:
+            a[_AT[name]] = t.data_ptr()
+    _launch(_lib().dl4j_linear_loss_bwd, "linear_loss_bwd", dev, a, f)
+    return dh, (dw.t() if want_w and ctx.dv else dw), db, None, None, None, None, None
+
+
+def _once(fn, ctx, dloss):
+    """``fn`` where the caller asked for a graph of the gradients: differentiating them raises."""
+    class Once:
+        call = once_differentiable(lambda c, g: fn(c, g))
+    return Once.call(ctx, dloss)
 
 
 class _TopkDistillation(torch.autograd.Function):
@@ -215,29 +251,33 @@ class _TopkDistillation(torch.autograd.Function):
     def forward(ctx, logits, idx, t, temperature):
         z = logits.reshape(-1, logits.shape[-1])
         z = z if z.stride(1) == 1 and z.stride(0) >= z.shape[1] else z.contiguous()
-        loss, lse = torch.empty(2, z.shape[0], dtype=torch.float32, device=z.device)
+        N = z.shape[0]
+        loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=z.device)
+        lse = torch.empty(N, dtype=torch.float32, device=z.device)
         c = _TopkDistillation.CODE
-        L.check(L.hip().dl4j_topk_distill_fwd(L.ptr(z), L.c_int64(z.stride(0)), L.ptr(idx), L.c_int(idx.dtype == torch.int64), L.ptr(t), L.c_int(c[t.dtype]),
-                                              L.c_int(z.shape[0]), L.c_int(z.shape[1]), L.c_int(idx.shape[1]), L.c_int(c[z.dtype]),
-                                              L.c_float(temperature), L.ptr(loss), L.ptr(lse), L.stream()), "topk_distill_fwd")
-        ctx.save_for_backward(z, idx, t, lse)
-        ctx.temperature, ctx.shape = temperature, logits.shape
-        return loss.view(logits.shape[:-1])
+        a = (ctypes.c_int64 * 14)(N, z.shape[1], idx.shape[1], z.stride(0), c[z.dtype], idx.dtype == torch.int64, c[t.dtype], z.data_ptr(), idx.data_ptr(),
+                                  t.data_ptr(), loss.data_ptr(), lse.data_ptr(), 0, 0)
+        f = (ctypes.c_float * 1)(temperature)
+        _launch(_lib().dl4j_topk_distill, "topk_distill", z.device, a, f)
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(z, idx, t, lse)
+            ctx.call, ctx.shape = (a, f), logits.shape
+        return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dloss):
-        z, idx, t, lse = ctx.saved_tensors
-        c = _TopkDistillation.CODE
-        with torch.cuda.device(z.device):
-            g = dloss.reshape(-1)
-            g = g if g.dtype == torch.float32 and g.is_contiguous() else g.float().contiguous()
-            dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-            L.check(L.hip().dl4j_topk_distill_bwd(L.ptr(z), L.c_int64(z.stride(0)), L.ptr(idx), L.c_int(idx.dtype == torch.int64), L.ptr(t),
-                                                  L.c_int(c[t.dtype]), L.c_int(z.shape[0]), L.c_int(z.shape[1]), L.c_int(idx.shape[1]),
-                                                  L.c_int(c[z.dtype]), L.c_float(ctx.temperature), L.ptr(lse), L.ptr(g), L.ptr(dz), L.stream()),
-                    "topk_distill_bwd")
-        return dz.view(ctx.shape), None, None, None
+        return _once(_topk_backward, ctx, dloss) if torch.is_grad_enabled() else _topk_backward(ctx, dloss)
+
+
+def _topk_backward(ctx, dloss):
+    z = ctx.saved_tensors[0]                                            # (unpacked: a changed tensor is refused)
+    a, f = ctx.call
+    a = (ctypes.c_int64 * 14)(*a)
+    g = _dloss(dloss)
+    dz = torch.empty(ctx.shape, dtype=z.dtype, device=z.device)
+    a[10], a[12], a[13] = 0, g.data_ptr(), dz.data_ptr()
+    _launch(_lib().dl4j_topk_distill, "topk_distill", z.device, a, f)
+    return dz, None, None, None
 
 
 # ------------------------------------------------------------------------------------------------------------------ entry points
@@ -274,9 +314,8 @@ def linear_cross_entropy(hidden, weights, labels, bias=None, ignore_index=-100, 
     _need(0.0 <= label_smoothing < 1.0, "%s: label smoothing must be in [0, 1)" % name)
     if not usable(hidden, weights, labels, bias):
         return linear_cross_entropy_reference(hidden, weights, labels, bias, ignore_index, label_smoothing)
-    with torch.cuda.device(hidden.device):
-        return _LinearLoss.apply(hidden, weights, None if bias is None else bias.contiguous(), labels.reshape(-1).contiguous(), None, int(ignore_index),
-                                 float(label_smoothing), 1.0)
+    return _LinearLoss.apply(hidden, weights, None if bias is None else bias.contiguous(), labels.reshape(-1).contiguous(), None, int(ignore_index),
+                             float(label_smoothing), 1.0)
 
 
 def linear_topk_distillation(hidden, weights, teacher_indices, teacher_logits, bias=None, temperature=1.0):
@@ -292,9 +331,8 @@ def linear_topk_distillation(hidden, weights, teacher_indices, teacher_logits, b
     _check_teacher(hidden.shape[:-1], hidden.device, teacher_indices, teacher_logits, temperature, name)
     if not usable(hidden, weights, teacher_indices, teacher_logits, bias):
         return linear_topk_distillation_reference(hidden, weights, teacher_indices, teacher_logits, bias, temperature)
-    with torch.cuda.device(hidden.device):
-        idx, t = _teacher_operands(teacher_indices, teacher_logits)
-        return _LinearLoss.apply(hidden, weights, None if bias is None else bias.contiguous(), idx, t, 0, 0.0, float(temperature))
+    idx, t = _teacher_operands(teacher_indices, teacher_logits)
+    return _LinearLoss.apply(hidden, weights, None if bias is None else bias.contiguous(), idx, t, 0, 0.0, float(temperature))
 
 
 def topk_distillation(logits, teacher_indices, teacher_logits, temperature=1.0):
@@ -304,6 +342,5 @@ def topk_distillation(logits, teacher_indices, teacher_logits, temperature=1.0):
     _check_teacher(logits.shape[:-1], logits.device, teacher_indices, teacher_logits, temperature, name)
     if not usable(logits, teacher_indices, teacher_logits):
         return topk_distillation_reference(logits, teacher_indices, teacher_logits, temperature)
-    with torch.cuda.device(logits.device):
-        idx, t = _teacher_operands(teacher_indices, teacher_logits)
-        return _TopkDistillation.apply(logits, idx, t, float(temperature))
+    idx, t = _teacher_operands(teacher_indices, teacher_logits)
+    return _TopkDistillation.apply(logits, idx, t, float(temperature))
