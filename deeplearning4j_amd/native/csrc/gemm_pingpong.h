@@ -146,7 +146,7 @@ struct Operand {
   const int* rows;
 };
 
-// k-tiles of a product over K: SEG * ceil(K / BK); SEG 3 = halves
+// k-tiles of a product over K: SEG * ceil(K / BK); SEG 3: both operands are pairs of halves, SEG 2: one is (the other's `lo` is 0)
 template <class C, int SEG> __host__ __device__ __forceinline__ int k_tiles(int K) { return SEG * ((K + C::BK - 1) / C::BK); }
 
 // Source of both loops: k-tiles [t0, ..) of the product; k >= K reads zeros, whatever the tile index.
@@ -163,7 +163,12 @@ template <class C, bool TA, bool TB, int SEG, bool PP> struct ProductSrc {
     t += t0;
     At at;
     if constexpr (SEG == 1) { at.k = t * C::BK; at.a = at.b = 0; }
-    else {
+    else if constexpr (SEG == 2) {
+      const int seg = t >= KT1 ? 1 : 0;
+      at.k = (t - seg * KT1) * C::BK;
+      at.a = seg ? alo : 0;
+      at.b = seg ? blo : 0;
+    } else {
       const int seg = t >= 2 * KT1 ? 2 : t >= KT1 ? 1 : 0;
       at.k = (t - seg * KT1) * C::BK;
       at.a = seg == 2 ? alo : 0;

@@ -353,6 +353,8 @@ template <class C> constexpr int score_lds(bool grad) {
 // exponentials 2^-100 below the reference is still a sound fp32 number; a row that lies lower makes the workgroup take the tile again with a
 // reference per row. The 16 lanes that share a row leave their partial sums in LDS, where one thread per row adds them.
 // Epilogue of a 256 x 256 tile: 11 us with a maximum and a sum reduced over the lanes for every row (product of one k-tile: 1.5 us).
+// SEG 3: operands and gradient in halves; 2: the gradient in halves (its rounding to 16 bits then counts for nothing: few rows do not
+// average it out, and for them a second pass over the gradient costs little beside W).
 template <class C, bool TB, bool GRAD, int SEG>
 __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -384,7 +386,8 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
     }
     Operand H = p.H;
     H.xlim = count;
-    product<C, false, TB, SEG>(smem, H, p.W, m0, n0, p.D, 0, k_tiles<C, SEG>(p.D), acc, init);
+    constexpr int PSEG = SEG == 3 ? 3 : 1;
+    product<C, false, TB, PSEG>(smem, H, p.W, m0, n0, p.D, 0, k_tiles<C, PSEG>(p.D), acc, init);
   }
   float* sf = reinterpret_cast<float*>(smem + score_over<C>(GRAD));
   int* slab = reinterpret_cast<int*>(sf);                          // label's column inside the tile, or none of them
@@ -565,7 +568,7 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
     char* out = p.G + (int64_t)(n0 - p.v0) * p.ldg + (int64_t)m0 * OSZ;
     constexpr int CPR = C::BM * OSZ / 16;
 #pragma unroll
-    for (int half = 0; half < (SEG == 3 ? 2 : 1); ++half) {
+    for (int half = 0; half < (SEG > 1 ? 2 : 1); ++half) {
       if (half == 1) __syncthreads();
 #pragma unroll
       for (int i = 0; i < C::TM; ++i)
@@ -575,7 +578,7 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             v[q] = O::cv(acc[i][j][q]);
-            if constexpr (SEG == 3) acc[i][j][q] -= O::fl(v[q]);
+            if constexpr (SEG > 1) acc[i][j][q] -= O::fl(v[q]);
           }
           *reinterpret_cast<Pack*>(smem + (col0 + j * 16) * PITCH + (row0 + i * 16) * OSZ) = v;
         }
@@ -712,17 +715,34 @@ __global__ void __launch_bounds__(1024) coef_kernel(const float* __restrict__ dl
   if (threadIdx.x == 0) { sc->db = 1.f / s; sc->dh = 1.f / s / sc->w; sc->dw = 1.f / s / sc->h; }
 }
 
-// db[v] = scale * sum over the row tiles' column sums
-__global__ void __launch_bounds__(256) bias_kernel(const float* __restrict__ colsum, int64_t ldc, int bm, int V, const int* __restrict__ count,
-                                                   const Scales* __restrict__ sc, void* __restrict__ db, int bdt) {
-  const int v = blockIdx.x * 256 + threadIdx.x, tiles = (*count + bm - 1) / bm;
-  if (v >= V) return;
-  float s = 0.f;
-#pragma unroll 4
-  for (int t = 0; t < tiles; ++t) s += colsum[t * ldc + v];
-  store_f(db, v, bdt, s * sc->db);
+// coef_kernel and pack_kernel in one launch for few rows: a workgroup per row, each finds the largest coefficient for itself
+__global__ void __launch_bounds__(256) prepare_kernel(const float* __restrict__ dloss, const int* __restrict__ rows, const int* __restrict__ count,
+                                                      float T, float top, float* __restrict__ coef, Scales* __restrict__ sc,
+                                                      const char* __restrict__ h, int64_t ldh_bytes, char* __restrict__ out, int64_t row_bytes,
+                                                      int64_t ldo_bytes) {
+  __shared__ float red[16];
+  const int c = *count, m = blockIdx.x;
+  if (m >= c && m > 0) return;
+  float s = 1.f;
+  if (top > 0.f) {
+    float mx = 0.f;
+    for (int k = threadIdx.x; k < c; k += 256) {
+      const float v = fabsf(dloss[rows[k]] * T);
+      if (v < __builtin_inff()) mx = fmaxf(mx, v);
+    }
+    mx = block_max(mx, red);
+    if (mx > 0.f) s = fminf(top / mx, 1e37f);
+  }
+  if (m == 0 && threadIdx.x == 0) { sc->db = 1.f / s; sc->dh = 1.f / s / sc->w; sc->dw = 1.f / s / sc->h; }
+  if (m >= c) return;
+  const int n = rows[m];
+  if (threadIdx.x == 0) coef[m] = dloss[n] * T * s;
+  const char* src = h + n * ldh_bytes;
+  if (out)
+    for (int64_t b = threadIdx.x * 16; b < row_bytes; b += 256 * 16) *reinterpret_cast<f32x4*>(out + m * ldo_bytes + b) = *reinterpret_cast<const f32x4*>(src + b);
 }
-// the same from the gradient itself (both halves), one wave per word: with teacher entries the tiles' sums do not hold them
+
+// db from the gradient itself (both halves), one wave per word: with teacher entries the tiles' column sums do not hold them
 __global__ void __launch_bounds__(256) bias_rows_kernel(const char* __restrict__ G, int64_t ldg, int64_t glo, int dt, int vc, const int* __restrict__ count,
                                                         const Scales* __restrict__ sc, void* __restrict__ db, int bdt) {
   const int v = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, c = *count;
@@ -781,27 +801,44 @@ __global__ void __launch_bounds__(C::NT) dh_kernel(const DhP p) {
   to_slab<C>(p.slab + (int64_t)u * C::BM * C::BN, acc, p.accum);
 }
 
-// dh rows from the slabs, in the order of the shares; rows that take no part get zeros. One workgroup per row.
+// What is left: workgroups [0, N) one row of dh each from the slabs, in the order of the shares (rows that take no part get zeros), those
+// behind them 256 words of db = scale * sum over the row tiles' column sums.
+struct FinishP {
+  const float* slab; const int* rows; const int* count; const Scales* sc;
+  int N, D, units;
+  void* dh; int dt;
+  const float* colsum; int bm; int V;
+  void* db; int bdt;
+};
 template <int BM, int BN>
-__global__ void __launch_bounds__(256) dh_rows_kernel(const float* __restrict__ slab, const int* __restrict__ rows, const int* __restrict__ count,
-                                                      const Scales* __restrict__ sc, int D, int units, void* __restrict__ dh, int64_t ldo, int dt) {
-  const int m = blockIdx.x, c = *count, n = rows[m];
-  const int mtiles = (c + BM - 1) / BM, ntiles = (D + BN - 1) / BN, tiles = mtiles * ntiles;
-  const int shares = tiles ? shares_of(tiles, units) : 1;
-  const float s = sc->dh;
-  for (int d = threadIdx.x * 4; d < D; d += 1024) {
+__global__ void __launch_bounds__(256) finish_kernel(const FinishP p) {
+  const int c = *p.count;
+  if ((int)blockIdx.x >= p.N) {
+    const int v = ((int)blockIdx.x - p.N) * 256 + threadIdx.x, tiles = (c + p.bm - 1) / p.bm;
+    if (v >= p.V) return;
+    float s = 0.f;
+#pragma unroll 4
+    for (int t = 0; t < tiles; ++t) s += p.colsum[(int64_t)t * p.V + v];
+    store_f(p.db, v, p.bdt, s * p.sc->db);
+    return;
+  }
+  const int m = blockIdx.x, n = p.rows[m];
+  const int mtiles = (c + BM - 1) / BM, ntiles = (p.D + BN - 1) / BN, tiles = mtiles * ntiles;
+  const int shares = tiles ? shares_of(tiles, p.units) : 1;
+  const float s = p.sc->dh;
+  for (int d = threadIdx.x * 4; d < p.D; d += 1024) {
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (m < c) {
       const int mt = m / BM, nt = d / BN;
       const int g = mt / 8, rowsg = min(8, mtiles - g * 8);       // tile_coords with 8 row tiles to a group
       const int t = g * 8 * ntiles + nt * rowsg + (mt - g * 8);
-      const float* x = slab + ((int64_t)t * BM + (m - mt * BM)) * BN + (d - nt * BN);
+      const float* x = p.slab + ((int64_t)t * BM + (m - mt * BM)) * BN + (d - nt * BN);
 #pragma unroll 4
       for (int k = 0; k < shares; ++k) v += *reinterpret_cast<const f32x4*>(x + (int64_t)k * tiles * BM * BN);
       v *= s;
     }
-    const int64_t o = (int64_t)n * ldo + d;
-    for (int j = 0; j < 4 && d + j < D; ++j) store_f(dh, o + j, dt, v[j]);
+    const int64_t o = (int64_t)n * p.D + d;
+    for (int j = 0; j < 4 && d + j < p.D; ++j) store_f(p.dh, o + j, p.dt, v[j]);
   }
 }
 
@@ -892,6 +929,7 @@ int g_tune[8] = {-1, -1, -1, -1, -1, -1, -1, -1};
 struct Plan {
   int tile, dh_tile, dw_tile;            // TILE_*
   int op;                                // operand type of the products
+  bool pair;                             // 16-bit operands: the scores' gradient in two halves
   bool nt;                               // backward products on 256 x 256 tiles from operands laid out along the sum's axis
   int bm, bn, tiles;                     // tiles of the scores
   int64_t np, dp, wcp, wrows, vp;           // padded rows / columns of the packed H and of the halves of W
@@ -925,6 +963,7 @@ Plan plan(const Args& a) {
   p.pieces = (int)((a.V + p.step - 1) / p.step);
   p.gcols = up(a.V < p.step ? a.V : p.step, 256);
   p.nt = p.tile == TILE_BIG && TUNE(1, a.N >= 512 && a.D >= 256);
+  p.pair = bits16 && !a.split && a.N <= 256;
   p.dh_tile = p.dw_tile = p.nt ? TILE_BIG : TILE_MID;
   const int ht = p.dh_tile == TILE_BIG ? 256 : 128;
   const int64_t htiles = up(a.N, ht) / ht * (up(a.D, ht) / ht);
@@ -977,7 +1016,7 @@ struct Work {
     fwd = c.at;
     c.at = 0;
     const int64_t esz = a.dt == DT_F32 ? 4 : 2;
-    coef = c.take<float>(a.N); G = c.take<char>(p.np * p.gcols * esz * (p.nt ? 2 : 1));
+    coef = c.take<float>(a.N); G = c.take<char>(p.np * p.gcols * esz * (p.nt || p.pair ? 2 : 1));
     colsum = c.take<float>(a.want_b && !a.K ? (a.N + p.bm - 1) / p.bm * a.V : 0);
     packed = c.take<char>(a.want_w && !a.split && !p.nt ? a.N * p.dp * esz : 0);
     ht = c.take<uint16_t>(a.want_w && p.nt ? a.D * p.np * (a.split ? 2 : 1) : 0);
@@ -1005,17 +1044,19 @@ template <class C, bool TB, bool GRAD, int SEG> int launch_score(const ScoreP& p
   hipLaunchKernelGGL((score_kernel<C, TB, GRAD, SEG>), dim3((unsigned)grid), dim3(C::NT), LDS, st, p);
   return (int)hipGetLastError();
 }
-template <bool TB, bool GRAD> int dispatch_score(const ScoreP& p, int tile, int op, bool split, hipStream_t st) {
+template <int DT, bool TB, bool GRAD> int score16(const ScoreP& p, int tile, bool pair, hipStream_t st) {
+  if (tile == TILE_BIG) return launch_score<Big<DT>, TB, GRAD, 1>(p, st);
+  if constexpr (GRAD)
+    if (pair) return tile == TILE_FEW ? launch_score<Few<DT>, TB, GRAD, 2>(p, st) : launch_score<Mid<DT>, TB, GRAD, 2>(p, st);
+  return tile == TILE_FEW ? launch_score<Few<DT>, TB, GRAD, 1>(p, st) : launch_score<Mid<DT>, TB, GRAD, 1>(p, st);
+}
+template <bool TB, bool GRAD> int dispatch_score(const ScoreP& p, int tile, int op, bool split, bool pair, hipStream_t st) {
   if (split) return tile == TILE_BIG ? launch_score<Big<DT_F16>, TB, GRAD, 3>(p, st) : launch_score<Mid<DT_F16>, TB, GRAD, 3>(p, st);
   if (op == DT_F32) return tile == TILE_FEW ? launch_score<Few<DT_F32>, TB, GRAD, 1>(p, st) : launch_score<Mid<DT_F32>, TB, GRAD, 1>(p, st);
-  if (op == DT_BF16)
-    return tile == TILE_BIG ? launch_score<Big<DT_BF16>, TB, GRAD, 1>(p, st) : tile == TILE_FEW ? launch_score<Few<DT_BF16>, TB, GRAD, 1>(p, st)
-                            : launch_score<Mid<DT_BF16>, TB, GRAD, 1>(p, st);
-  return tile == TILE_BIG ? launch_score<Big<DT_F16>, TB, GRAD, 1>(p, st) : tile == TILE_FEW ? launch_score<Few<DT_F16>, TB, GRAD, 1>(p, st)
-                          : launch_score<Mid<DT_F16>, TB, GRAD, 1>(p, st);
+  return op == DT_BF16 ? score16<DT_BF16, TB, GRAD>(p, tile, pair, st) : score16<DT_F16, TB, GRAD>(p, tile, pair, st);
 }
-template <bool GRAD> int scores(const ScoreP& p, int tile, int op, bool split, bool tb, hipStream_t st) {
-  return tb ? dispatch_score<true, GRAD>(p, tile, op, split, st) : dispatch_score<false, GRAD>(p, tile, op, split, st);
+template <bool GRAD> int scores(const ScoreP& p, int tile, int op, bool split, bool pair, bool tb, hipStream_t st) {
+  return tb ? dispatch_score<true, GRAD>(p, tile, op, split, pair, st) : dispatch_score<false, GRAD>(p, tile, op, split, pair, st);
 }
 
 template <class C, bool TA, bool TB, int SEG> int launch_dh(const DhP& p, hipStream_t st) {
@@ -1026,14 +1067,15 @@ template <class C, bool TA, bool TB, int SEG> int launch_dh(const DhP& p, hipStr
   return (int)hipGetLastError();
 }
 // 256 x 256: both operands K-contiguous (p.nt); 128 x 128: the gradient and the [V, D] table are walked row by row
-int dispatch_dh(const DhP& p, int tile, int op, bool split, bool wt, hipStream_t st) {
+template <class C, int SEG> int mid_dh(const DhP& p, bool wt, hipStream_t st) { return wt ? launch_dh<C, true, false, SEG>(p, st) : launch_dh<C, true, true, SEG>(p, st); }
+int dispatch_dh(const DhP& p, int tile, int op, bool split, bool pair, bool wt, hipStream_t st) {
   if (tile == TILE_BIG)
     return split ? launch_dh<Big<DT_F16>, false, false, 3>(p, st) : op == DT_BF16 ? launch_dh<Big<DT_BF16>, false, false, 1>(p, st)
                                                                                  : launch_dh<Big<DT_F16>, false, false, 1>(p, st);
-  if (split) return wt ? launch_dh<Mid<DT_F16>, true, false, 3>(p, st) : launch_dh<Mid<DT_F16>, true, true, 3>(p, st);
-  if (op == DT_F32) return wt ? launch_dh<Mid<DT_F32>, true, false, 1>(p, st) : launch_dh<Mid<DT_F32>, true, true, 1>(p, st);
-  if (op == DT_BF16) return wt ? launch_dh<Mid<DT_BF16>, true, false, 1>(p, st) : launch_dh<Mid<DT_BF16>, true, true, 1>(p, st);
-  return wt ? launch_dh<Mid<DT_F16>, true, false, 1>(p, st) : launch_dh<Mid<DT_F16>, true, true, 1>(p, st);
+  if (split) return mid_dh<Mid<DT_F16>, 3>(p, wt, st);
+  if (op == DT_F32) return mid_dh<Mid<DT_F32>, 1>(p, wt, st);
+  if (op == DT_BF16) return pair ? mid_dh<Mid<DT_BF16>, 2>(p, wt, st) : mid_dh<Mid<DT_BF16>, 1>(p, wt, st);
+  return pair ? mid_dh<Mid<DT_F16>, 2>(p, wt, st) : mid_dh<Mid<DT_F16>, 1>(p, wt, st);
 }
 
 template <class C, int OT, bool SWAP, int SEG> int launch_dw(const DwP& p, hipStream_t st) {
@@ -1050,12 +1092,13 @@ template <class C, int OT, bool SWAP, int SEG> int launch_dw(const DwP& p, hipSt
                        OT == OT_F32 ? (int)DT_F32 : OT == OT_F16 ? (int)DT_F16 : (int)DT_BF16);
   return (int)hipGetLastError();
 }
-template <bool SWAP> int dispatch_dw(const DwP& p, int tile, int op, bool split, hipStream_t st) {
+template <bool SWAP> int dispatch_dw(const DwP& p, int tile, int op, bool split, bool pair, hipStream_t st) {
   const bool big = tile == TILE_BIG;
   if (split) return big ? launch_dw<Big<DT_F16>, OT_F32, SWAP, 3>(p, st) : launch_dw<Mid<DT_F16>, OT_F32, SWAP, 3>(p, st);
   if (op == DT_F32) return launch_dw<Mid<DT_F32>, OT_F32, SWAP, 1>(p, st);
-  if (op == DT_BF16) return big ? launch_dw<Big<DT_BF16>, OT_BF16, SWAP, 1>(p, st) : launch_dw<Mid<DT_BF16>, OT_BF16, SWAP, 1>(p, st);
-  return big ? launch_dw<Big<DT_F16>, OT_F16, SWAP, 1>(p, st) : launch_dw<Mid<DT_F16>, OT_F16, SWAP, 1>(p, st);
+  if (op == DT_BF16)
+    return big ? launch_dw<Big<DT_BF16>, OT_BF16, SWAP, 1>(p, st) : pair ? launch_dw<Mid<DT_BF16>, OT_BF16, SWAP, 2>(p, st) : launch_dw<Mid<DT_BF16>, OT_BF16, SWAP, 1>(p, st);
+  return big ? launch_dw<Big<DT_F16>, OT_F16, SWAP, 1>(p, st) : pair ? launch_dw<Mid<DT_F16>, OT_F16, SWAP, 2>(p, st) : launch_dw<Mid<DT_F16>, OT_F16, SWAP, 1>(p, st);
 }
 
 // 0 where the arguments are what the kernels assume
@@ -1120,7 +1163,7 @@ int forward(const Args& a, const float* f, hipStream_t st) {
   q.W.xlim = (int)a.V;
   q.v0 = 0; q.v1 = (int)a.V;
   q.part = w.part; q.tz = w.tz; q.zs = q.smooth_v != 0.f ? w.zs : nullptr;
-  if (const int e = scores<false>(q, p.tile, p.op, a.split, a.wt, st)) return e;
+  if (const int e = scores<false>(q, p.tile, p.op, a.split, false, a.wt, st)) return e;
   CombineP c{w.part, q.zs, w.tz, s.rows, s.count, s.lab, a.K ? s.ent : nullptr, s.sp, s.zk, (int)a.K, (int)a.N, p.tiles, q.keep, f[0],
              s.lse, a.loss};
   if (a.N <= 256) hipLaunchKernelGGL((combine_kernel<1>), dim3((unsigned)a.N), dim3(256), 0, st, c);
@@ -1134,22 +1177,30 @@ int backward(const Args& a, const float* f, hipStream_t st) {
   const State s(a, p);
   const Work w(a, p);
   const int esz = a.dt == DT_F32 ? 4 : 2, gsz = a.split ? 2 : esz;
-  hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, st, a.dloss, s.rows, s.count, f[0], p.op == DT_F16 ? 16384.f : p.op == DT_BF16 ? 1.f : 0.f, w.coef, s.sc);
-  VL_CHECK();
+  const float top = p.op == DT_F16 ? 16384.f : p.op == DT_BF16 ? 1.f : 0.f;
   Operand H, W;
   operands(a, p, s, H, W);
   Operand packed = H;
+  const int64_t rb = up(a.D, 16 / esz) * esz;
+  const bool pack = a.want_w && !a.split && !p.nt;
+  if (a.N <= 1024) {
+    hipLaunchKernelGGL(prepare_kernel, dim3((unsigned)a.N), dim3(256), 0, st, a.dloss, s.rows, s.count, f[0], top, w.coef, s.sc, (const char*)a.H, a.ldh * esz,
+                       pack ? w.packed : nullptr, rb, p.dp * esz);
+    VL_CHECK();
+  } else {
+    hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, st, a.dloss, s.rows, s.count, f[0], top, w.coef, s.sc);
+    VL_CHECK();
+    if (pack) {
+      hipLaunchKernelGGL(pack_kernel, dim3((unsigned)a.N), dim3(256), 0, st, (const char*)a.H, a.ldh * esz, s.rows, s.count, w.packed, rb, p.dp * esz);
+      VL_CHECK();
+    }
+  }
+  if (pack) packed = Operand{w.packed, p.dp * esz, 0, 0, nullptr};
   if (a.want_w && p.nt) {
     TransposeP t{(const uint16_t*)H.p, H.ld / 2, H.lo / 2, w.ht, p.np, a.D * p.np, (int)a.N, (int)a.D, s.count, H.rows};
     hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)((a.N + 63) / 64), (unsigned)((a.D + 63) / 64), a.split ? 2 : 1), dim3(256), 0, st, t);
     VL_CHECK();
     packed = Operand{(const char*)w.ht, p.np * 2, a.split ? a.D * p.np * 2 : 0, 0, nullptr};
-  } else if (a.want_w && !a.split) {
-    const int64_t rb = up(a.D, 16 / esz) * esz;
-    const int64_t ld = p.dp * esz;
-    hipLaunchKernelGGL(pack_kernel, dim3((unsigned)a.N), dim3(256), 0, st, (const char*)a.H, a.ldh * esz, s.rows, s.count, w.packed, rb, ld);
-    VL_CHECK();
-    packed = Operand{w.packed, ld, 0, 0, nullptr};
   }
   packed.xlim = (int)a.D;
   Operand wh = W;                                                  // W for the dh product
@@ -1159,7 +1210,7 @@ int backward(const Args& a, const float* f, hipStream_t st) {
     VL_CHECK();
     wh = Operand{(const char*)w.wtr, p.vp * 2, a.split ? a.D * p.vp * 2 : 0, 0, nullptr};
   }
-  const int64_t ldg = p.np * gsz, glo = a.split ? p.gcols * ldg : 0;
+  const int64_t ldg = p.np * gsz, glo = a.split || p.pair ? p.gcols * ldg : 0;
   const int64_t ldr = p.gcols * gsz, rlo = a.split ? p.np * ldr : 0;   // the same row by row (p.nt)
   char* rows_g = w.G + p.np * p.gcols * esz;
   for (int k = 0; k < p.pieces; ++k) {
@@ -1170,7 +1221,7 @@ int backward(const Args& a, const float* f, hipStream_t st) {
     q.v0 = v0; q.v1 = v1; q.lse = s.lse; q.coef = w.coef; q.G = w.G; q.ldg = ldg; q.glo = glo;
     if (p.nt && a.want_h) { q.R = rows_g; q.ldr = ldr; q.rlo = rlo; }
     if (a.want_b && !a.K) { q.colsum = w.colsum; q.ldc = a.V; }
-    if (const int e = scores<true>(q, p.tile, p.op, a.split, a.wt, st)) return e;
+    if (const int e = scores<true>(q, p.tile, p.op, a.split, p.pair, a.wt, st)) return e;
     if (a.want_b && a.K) {
       hipLaunchKernelGGL(bias_rows_kernel, dim3((vc + 3) / 4), dim3(256), 0, st, w.G, ldg, glo, a.split ? (int)DT_F16 : (int)a.dt, vc, s.count, s.sc,
                          (char*)a.db + (int64_t)v0 * (a.bdt == DT_F32 ? 4 : 2), (int)a.bdt);
@@ -1184,7 +1235,7 @@ int backward(const Args& a, const float* f, hipStream_t st) {
       d.W.p += p.nt || a.wt ? (int64_t)v0 * gsz : v0 * wh.ld;
       d.W.xlim = (int)a.D;
       d.count = s.count; d.D = (int)a.D; d.vc = vc; d.units = p.units; d.accum = k > 0; d.slab = w.dh_slab;
-      const int e = dispatch_dh(d, p.dh_tile, p.op, a.split, a.wt, st);
+      const int e = dispatch_dh(d, p.dh_tile, p.op, a.split, p.pair, a.wt, st);
       if (e) return e;
     }
     if (a.want_w) {
@@ -1194,19 +1245,16 @@ int backward(const Args& a, const float* f, hipStream_t st) {
       d.out = (char*)a.dw + (a.wt ? (int64_t)v0 : v0 * a.D) * esz;
       d.ldo = a.wt ? a.V : a.D;
       d.D = (int)a.D; d.vc = vc; d.shares = p.shares; d.slab = w.dw_slab;
-      const int e = a.wt ? dispatch_dw<true>(d, p.dw_tile, p.op, a.split, st) : dispatch_dw<false>(d, p.dw_tile, p.op, a.split, st);
+      const int e = a.wt ? dispatch_dw<true>(d, p.dw_tile, p.op, a.split, p.pair, st) : dispatch_dw<false>(d, p.dw_tile, p.op, a.split, p.pair, st);
       if (e) return e;
     }
   }
-  if (a.want_b && !a.K) {
-    hipLaunchKernelGGL(bias_kernel, dim3((unsigned)((a.V + 255) / 256)), dim3(256), 0, st, w.colsum, a.V, p.bm, (int)a.V, s.count, s.sc, a.db, (int)a.bdt);
-    VL_CHECK();
-  }
-  if (a.want_h) {
-    if (p.dh_tile == TILE_BIG)
-      hipLaunchKernelGGL((dh_rows_kernel<256, 256>), dim3((unsigned)a.N), dim3(256), 0, st, w.dh_slab, s.rows, s.count, s.sc, (int)a.D, p.units, a.dh, a.D, (int)a.dt);
-    else
-      hipLaunchKernelGGL((dh_rows_kernel<128, 128>), dim3((unsigned)a.N), dim3(256), 0, st, w.dh_slab, s.rows, s.count, s.sc, (int)a.D, p.units, a.dh, a.D, (int)a.dt);
+  const bool sums = a.want_b && !a.K;
+  if (a.want_h || sums) {
+    const FinishP q{w.dh_slab, s.rows, s.count, s.sc, a.want_h ? (int)a.N : 0, (int)a.D, p.units, a.dh, (int)a.dt, w.colsum, p.bm, (int)a.V, a.db, (int)a.bdt};
+    const dim3 grid((unsigned)(q.N + (sums ? (a.V + 255) / 256 : 0)));
+    if (p.dh_tile == TILE_BIG) hipLaunchKernelGGL((finish_kernel<256, 256>), grid, dim3(256), 0, st, q);
+    else hipLaunchKernelGGL((finish_kernel<128, 128>), grid, dim3(256), 0, st, q);
   }
   return (int)hipGetLastError();
 }

@@ -124,6 +124,10 @@ _ARGS = ("N D V dt split wt bdt ldh ldw lab64 ignore idx64 tdt K want_h want_w w
          "H W bias labels idx t loss state ws dloss dh dw db").split()
 _AT = {n: k for k, n in enumerate(_ARGS)}
 _Block = ctypes.c_int64 * len(_ARGS)
+_Floats = ctypes.c_float * 2
+_Sizes = ctypes.c_int64 * 3
+# struct DistillArgs in native/csrc/topk_distill.hip: N V K ldz dt idx64 tdt z idx t loss lse dloss dz
+_TopkBlock = ctypes.c_int64 * 14
 
 
 def _up(n, m):
@@ -202,8 +206,8 @@ class _LinearLoss(torch.autograd.Function):
                    _DT[second.dtype] if teacher else 0, first.shape[1] if teacher else 0, *want,
                    h.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if teacher else first.data_ptr(), first.data_ptr() if teacher else 0,
                    second.data_ptr() if teacher else 0, loss.data_ptr(), 0, 0, 0, 0, 0, 0)
-        f = (ctypes.c_float * 2)(temperature, smoothing)
-        size = (ctypes.c_int64 * 3)()
+        f = _Floats(temperature, smoothing)
+        size = _Sizes()
         lib.dl4j_linear_loss_bytes(a, size)
         state = torch.empty(size[0], dtype=torch.uint8, device=dev)
         ws = torch.empty(size[1], dtype=torch.uint8, device=dev)
@@ -255,9 +259,9 @@ class _TopkDistillation(torch.autograd.Function):
         loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=z.device)
         lse = torch.empty(N, dtype=torch.float32, device=z.device)
         c = _TopkDistillation.CODE
-        a = (ctypes.c_int64 * 14)(N, z.shape[1], idx.shape[1], z.stride(0), c[z.dtype], idx.dtype == torch.int64, c[t.dtype], z.data_ptr(), idx.data_ptr(),
-                                  t.data_ptr(), loss.data_ptr(), lse.data_ptr(), 0, 0)
-        f = (ctypes.c_float * 1)(temperature)
+        a = _TopkBlock(N, z.shape[1], idx.shape[1], z.stride(0), c[z.dtype], idx.dtype == torch.int64, c[t.dtype], z.data_ptr(), idx.data_ptr(),
+                       t.data_ptr(), loss.data_ptr(), lse.data_ptr(), 0, 0)
+        f = _Floats(temperature, 0.0)
         _launch(_lib().dl4j_topk_distill, "topk_distill", z.device, a, f)
         if ctx.needs_input_grad[0]:
             ctx.save_for_backward(z, idx, t, lse)
@@ -272,7 +276,7 @@ class _TopkDistillation(torch.autograd.Function):
 def _topk_backward(ctx, dloss):
     z = ctx.saved_tensors[0]                                            # (unpacked: a changed tensor is refused)
     a, f = ctx.call
-    a = (ctypes.c_int64 * 14)(*a)
+    a = _TopkBlock(*a)
     g = _dloss(dloss)
     dz = torch.empty(ctx.shape, dtype=z.dtype, device=z.device)
     a[10], a[12], a[13] = 0, g.data_ptr(), dz.data_ptr()
@@ -291,9 +295,11 @@ def usable(operand, *others):
 
 def _teacher_operands(indices, logits):
     K = indices.shape[-1]
-    t = logits.detach()
+    t = logits.detach() if logits.requires_grad else logits
     t = t.float() if t.dtype not in _DT else t
-    return indices.reshape(-1, K).contiguous(), t.reshape(-1, K).contiguous()
+    if t.dim() != 2:
+        indices, t = indices.reshape(-1, K), t.reshape(-1, K)
+    return indices.contiguous(), t.contiguous()
 
 
 def linear_cross_entropy(hidden, weights, labels, bias=None, ignore_index=-100, label_smoothing=0.0):
