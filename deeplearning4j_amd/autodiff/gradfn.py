@@ -136,6 +136,17 @@ for _n in ("softmax_cross_entropy_loss", "sigm_cross_entropy_loss", "mean_sqerr_
     RULES[_n] = _loss_rule
 
 
+@rule("linear_softmax_cross_entropy_loss", "linear_topk_distillation_loss", "topk_distillation_loss")
+def _vocab_loss(sd, o, ins, outs, gs):
+    # <name>_bp(inputs..., dL/dloss per row) -> gradients of hidden, weights and bias (of the logits); labels and teacher get none
+    at = [0] if o.opName == "topk_distillation_loss" else [0, 1] + ([len(ins) - 1] if len(ins) > (3 if "cross" in o.opName else 4) else [])
+    res = sd._op(o.opName + "_bp", list(ins) + [gs[0]], nOut=len(at), name=o.name + "_bp", **_args(o))
+    out = [None] * len(ins)
+    for k, r in zip(at, res):
+        out[k] = r
+    return out
+
+
 def _static_shape(sd, v):
     a = sd._arrays.get(v.name)
     if a is not None:

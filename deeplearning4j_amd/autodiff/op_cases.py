@@ -419,6 +419,27 @@ def cases() -> Dict[str, List[Case]]:
     add("softmax_cross_entropy_loss_with_logits_grad", Case([x34, oh], ref=None))
     add("sparse_softmax_cross_entropy_loss_with_logits_grad", Case([I(0, 2, 3), x34], ref=None))
     add("ctc_loss_grad", Case([torch.tensor([[1, 2]]), R(1, 5, 4, seed=113).log_softmax(-1), I(2), I(5)], i=[0], ref=None))
+    # ---- losses on an output layer whose logits are not kept (codegen/ops/loss.py)
+    vh, vw, vb = R(5, 6, seed=301), R(7, 6, seed=302), R(7, seed=303)
+    vl = I(0, -100, 6, 3, 3)
+
+    def _lce(h, w, l, b=None, eps=0.0, dv=False):
+        z = d64(h) @ (d64(w) if dv else d64(w).t()) + (0 if b is None else d64(b))
+        tgt = torch.full_like(z, eps / z.shape[1])
+        tgt[torch.arange(len(l)), l.clamp(min=0)] += 1 - eps
+        return torch.where(l == -100, 0.0, -(tgt * torch.log_softmax(z, 1)).sum(1))
+    add("linear_softmax_cross_entropy_loss",
+        Case([vh, vw, vl], ref=lambda h, w, l: _lce(h, w, l), rtol=1e-4, grad=True, gin=[0, 1]),
+        Case([vh, vw.t().contiguous(), vl, vb], i=[-100, 1], t=[0.2], ref=lambda h, w, l, b: _lce(h, w, l, b, 0.2, True), rtol=1e-4, grad=True, gin=[0, 1, 3]))
+    ti, tt = torch.tensor([[0, 3, 6], [2, 2, -1], [-1, -1, -1], [5, 1, 0], [4, -1, 6]]), R(5, 3, seed=304)
+
+    def _kd(z, i, t, T):
+        p = torch.nan_to_num(torch.softmax(torch.where(i >= 0, d64(t) / T, -math.inf), 1), nan=0.0)
+        return T * T * (torch.xlogy(p, p) - p * torch.log_softmax(z / T, 1).gather(1, i.clamp(min=0))).sum(1)
+    add("topk_distillation_loss", Case([R(5, 7, seed=305), ti, tt], t=[1.5], ref=lambda z, i, t: _kd(d64(z), i, t, 1.5), rtol=1e-4, grad=True, gin=[0]))
+    add("linear_topk_distillation_loss",
+        Case([vh, vw, ti, tt, vb], i=[0], t=[2.0], ref=lambda h, w, i, t, b: _kd(d64(h) @ d64(w).t() + d64(b), i, t, 2.0), rtol=1e-4, grad=True, gin=[0, 1, 4]),
+        Case([vh, vw.t().contiguous(), ti, tt], i=[1], ref=lambda h, w, i, t: _kd(d64(h) @ d64(w), i, t, 1.0), rtol=1e-4, grad=True, gin=[0, 1]))
     # ---- updaters (closed forms of SURVEY appendix B.5)
     gr, z2 = I(0.1, -0.2, dtype=torch.float32), torch.zeros(2)
     add("sgd_updater", Case([gr], t=[0.1], ref=lambda g: 0.1 * d64(g)))

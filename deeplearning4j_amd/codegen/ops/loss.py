@@ -35,6 +35,31 @@ _weighted("meanSquaredError", "mean_sqerr_loss", "Mean squared error.").output("
 (ns.op("sparseSoftmaxCrossEntropy", libnd4j="sparse_softmax_cross_entropy_loss_with_logits", doc="Softmax cross entropy against integer class labels.")
    .input("logits", D.NUMERIC, "Logits [..., nClasses]").input("labels", D.INT, "Class indices [...]").nativeOrder("labels", "logits")
    .output("output", D.NUMERIC, "Per-example loss"))
+# losses on a vocabulary-sized output layer that do not keep its logits (deeplearning4j_amd/ops/vocab_loss.py); not ops of the reference
+(ns.op("linearSoftmaxCrossEntropy", libnd4j="linear_softmax_cross_entropy_loss",
+       doc="Softmax cross entropy of the logits hidden . weights^T + bias against integer class labels; the logits are not kept.")
+   .input("hidden", D.FLOATING_POINT, "Hidden states [..., D]")
+   .input("weights", D.FLOATING_POINT, "Output weights [V, D] (an embedding table), or [D, V] with transposeWeights, in the type of hidden")
+   .input("labels", D.INT, "Class indices [...]; a row labelled ignoreIndex has loss 0 and no gradient, one labelled otherwise outside [0, V) gives NaN")
+   .input("bias", D.FLOATING_POINT, "Output bias [V]", optional=True)
+   .arg("labelSmoothing", D.FLOATING_POINT, "Label smoothing factor in [0, 1)", default=0.0)
+   .arg("ignoreIndex", D.INT, "Label of the rows that take no part", default=-100)
+   .arg("transposeWeights", D.BOOL, "Weights are [D, V], as a dense layer holds them", default=False, slot="i", convert="int")
+   .output("output", D.FLOATING_POINT, "Per-row loss [...], FLOAT (DOUBLE for DOUBLE operands)"))
+(ns.op("linearTopKDistillation", libnd4j="linear_topk_distillation_loss",
+       doc="Distillation from a teacher's top logits, T^2 KL(softmax(teacher / T) || softmax(student / T)), for student logits "
+           "hidden . weights^T + bias that are not kept.")
+   .input("hidden", D.FLOATING_POINT, "Hidden states [..., D]").input("weights", D.FLOATING_POINT, "Output weights [V, D], or [D, V] with transposeWeights")
+   .input("teacherIndices", D.INT, "Words of the teacher's K best logits [..., K], negative: padding")
+   .input("teacherLogits", D.FLOATING_POINT, "Their logits [..., K]").input("bias", D.FLOATING_POINT, "Output bias [V]", optional=True)
+   .arg("temperature", D.FLOATING_POINT, "Temperature T", default=1.0)
+   .arg("transposeWeights", D.BOOL, "Weights are [D, V], as a dense layer holds them", default=False, slot="i", convert="int")
+   .output("output", D.FLOATING_POINT, "Per-row loss [...]"))
+(ns.op("topKDistillation", libnd4j="topk_distillation_loss",
+       doc="Distillation from a teacher's top logits, T^2 KL(softmax(teacher / T) || softmax(student / T)), on student logits.")
+   .input("logits", D.FLOATING_POINT, "Student logits [..., V]").input("teacherIndices", D.INT, "Words of the teacher's K best logits [..., K], negative: padding")
+   .input("teacherLogits", D.FLOATING_POINT, "Their logits [..., K]").arg("temperature", D.FLOATING_POINT, "Temperature T", default=1.0)
+   .output("output", D.FLOATING_POINT, "Per-row loss [...]"))
 (ns.op("l2Loss", libnd4j="l2_loss", doc="Half the sum of squares: sum(x^2) / 2.").input("var", D.NUMERIC, "Input").output("output", D.NUMERIC, "Scalar loss"))
 (ns.op("ctcLoss", libnd4j="ctc_loss", doc="Connectionist temporal classification loss.")
    .input("targetLabels", D.INT, "Label sequences [batch, maxLabelLength]").input("logitInput", D.NUMERIC, "Logits [batch, time, nClasses]")

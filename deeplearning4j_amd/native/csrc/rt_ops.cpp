@@ -4,7 +4,7 @@
 // or by 64-bit name hash — and HashHelper::getLongHash (helpers/impl/helper_hash.cpp; the hash is
 // stored as FlatNode.opNum for custom ops, so it must be bit-compatible), plus the
 // getAllCustomOps descriptor string parsed by OpExecutioner.getCustomOperations.
-// The table itself is generated (tools/gen_op_table.py → op_table.inc).
+// The reference's table is generated (tools/gen_op_table.py → op_table.inc), the framework's own ops follow it (op_table_own.inc).
 #include "rt_common.h"
 
 #include <mutex>
@@ -72,6 +72,7 @@ void init_ops() {
     }                                                         \
   }
 #include "op_table.inc"
+#include "op_table_own.inc"
 #undef OPDEF
 #undef OPSYN
 }

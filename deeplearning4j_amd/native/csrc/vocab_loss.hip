@@ -761,10 +761,10 @@ __global__ void __launch_bounds__(256) bias_rows_kernel(const char* __restrict__
 struct DhP {
   Operand G, W;
   const int* count;
-  int D, vc, units, accum;
+  int D, vc, units, most, accum;         // most: shares at most (each has some k-tiles to work on)
   float* slab;
 };
-__device__ __forceinline__ int shares_of(int tiles, int units) { return tiles >= units ? 1 : units / tiles; }
+__device__ __forceinline__ int shares_of(int tiles, int units, int most) { return tiles >= units ? 1 : min(most, units / tiles); }
 
 // accumulators to (or onto) a tile of a slab
 template <class C> __device__ __forceinline__ void to_slab(float* tile, typename C::acc_t (&acc)[C::TM][C::TN], bool add) {
@@ -788,7 +788,7 @@ __global__ void __launch_bounds__(C::NT) dh_kernel(const DhP p) {
   const int count = *p.count;
   const int mtiles = (count + C::BM - 1) / C::BM, ntiles = (p.D + C::BN - 1) / C::BN, tiles = mtiles * ntiles;
   if (tiles == 0) return;
-  const int shares = shares_of(tiles, p.units);
+  const int shares = shares_of(tiles, p.units, p.most);
   if ((int)blockIdx.x >= tiles * shares) return;
   const int u = xcd_remap(blockIdx.x, tiles * shares);
   const int share = u / tiles;
@@ -805,7 +805,7 @@ __global__ void __launch_bounds__(C::NT) dh_kernel(const DhP p) {
 // behind them 256 words of db = scale * sum over the row tiles' column sums.
 struct FinishP {
   const float* slab; const int* rows; const int* count; const Scales* sc;
-  int N, D, units;
+  int N, D, units, most;
   void* dh; int dt;
   const float* colsum; int bm; int V;
   void* db; int bdt;
@@ -824,7 +824,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishP p) {
   }
   const int m = blockIdx.x, n = p.rows[m];
   const int mtiles = (c + BM - 1) / BM, ntiles = (p.D + BN - 1) / BN, tiles = mtiles * ntiles;
-  const int shares = tiles ? shares_of(tiles, p.units) : 1;
+  const int shares = tiles ? shares_of(tiles, p.units, p.most) : 1;
   const float s = p.sc->dh;
   for (int d = threadIdx.x * 4; d < p.D; d += 1024) {
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
@@ -907,7 +907,10 @@ __global__ void __launch_bounds__(256) dw_sum_kernel(const float* __restrict__ s
 template <int DT> using Big = Cfg<256, 256, 2, 4, 2, 16, DT>;
 template <int DT> using Mid = Cfg<128, 128, 2, 2, 2, 16, DT>;
 template <int DT> using Few = Cfg<32, 128, 1, 4, 4, 16, DT>;
-enum { TILE_BIG = 0, TILE_MID = 1, TILE_FEW = 2 };
+template <int DT> using Small = Cfg<64, 64, 2, 2, 4, 16, DT>;
+enum { TILE_BIG = 0, TILE_MID = 1, TILE_FEW = 2, TILE_SMALL = 3 };
+int tile_rows(int tile) { return tile == TILE_BIG ? 256 : tile == TILE_MID ? 128 : tile == TILE_FEW ? 32 : 64; }
+int tile_cols(int tile) { return tile == TILE_BIG ? 256 : tile == TILE_SMALL ? 64 : 128; }
 
 // One call: sizes, layout and pointers (ops/vocab_loss.py _ARGS lists the same fields in the same order)
 struct Args {
@@ -934,7 +937,7 @@ struct Plan {
   int bm, bn, tiles;                     // tiles of the scores
   int64_t np, dp, wcp, wrows, vp;           // padded rows / columns of the packed H and of the halves of W
   int pieces, step;
-  int units, shares;
+  int units, most, shares;
   int64_t gcols;
 };
 
@@ -943,13 +946,14 @@ Plan plan(const Args& a) {
   p.op = a.split ? DT_F16 : (int)a.dt;
   const bool bits16 = p.op != DT_F32;
   const int64_t big_tiles = up(a.N, 256) / 256 * (up(a.V, 256) / 256);
-  // 256 x 256 tiles once they cover two thirds of the 256 CUs, 32 rows for the fewest rows (W streams through: one tile per CU at a
-  // vocabulary of 32768), 128 x 128 between them and for fp32
-  p.tile = TUNE(0, bits16 && big_tiles >= 176 && a.N > 128 ? TILE_BIG : a.N <= 32 ? TILE_FEW : TILE_MID);
+  const int64_t mid_tiles = up(a.N, 128) / 128 * (up(a.V, 128) / 128);
+  // 256 x 256 tiles once they cover two thirds of the 256 CUs; 32 rows where few rows meet a large vocabulary (W streams through, a tile per
+  // CU at 32768 words); 64 x 64 tiles with four stages where 128 x 128 ones would leave CUs idle (the time is a chain of k-tiles then)
+  p.tile = TUNE(0, bits16 && big_tiles >= 176 && a.N > 128 ? TILE_BIG : a.N <= 32 && a.V >= 16384 ? TILE_FEW : mid_tiles < 176 ? TILE_SMALL : TILE_MID);
   if (a.split && p.tile == TILE_FEW) p.tile = TILE_MID;
   if (!bits16 && p.tile == TILE_BIG) p.tile = TILE_MID;
-  p.bm = p.tile == TILE_BIG ? 256 : p.tile == TILE_FEW ? 32 : 128;
-  p.bn = p.tile == TILE_BIG ? 256 : 128;
+  p.bm = tile_rows(p.tile);
+  p.bn = tile_cols(p.tile);
   p.tiles = (int)(up(a.V, p.bn) / p.bn);
   p.np = up(a.N, 256);
   p.vp = up(a.V, 64);
@@ -964,16 +968,19 @@ Plan plan(const Args& a) {
   p.gcols = up(a.V < p.step ? a.V : p.step, 256);
   p.nt = p.tile == TILE_BIG && TUNE(1, a.N >= 512 && a.D >= 256);
   p.pair = bits16 && !a.split && a.N <= 256;
-  p.dh_tile = p.dw_tile = p.nt ? TILE_BIG : TILE_MID;
-  const int ht = p.dh_tile == TILE_BIG ? 256 : 128;
-  const int64_t htiles = up(a.N, ht) / ht * (up(a.D, ht) / ht);
-  const int want = p.dh_tile == TILE_BIG ? 256 : 512;
-  p.units = (int)(htiles > want ? htiles : want);
-  const int wt = p.dw_tile == TILE_BIG ? 256 : 128;
-  const int64_t wtiles = up(p.gcols < a.V ? p.gcols : a.V, wt) / wt * (up(a.D, wt) / wt);
-  const int64_t ks = up(a.N, 64) / 64;
-  int64_t sh = p.dw_tile == TILE_BIG ? 1 : 512 / wtiles;         // shares of at least 4 k-tiles
-  if (sh > ks / 4) sh = ks / 4;
+  const int seg = a.split ? 3 : p.pair ? 2 : 1, bk = bits16 ? 64 : 32;
+  const int64_t vk = seg * (up(p.step, bk) / bk), nk = seg * (up(a.N, bk) / bk);   // k-tiles of the two products' sums
+  const int64_t cols = p.gcols < a.V ? p.gcols : a.V;
+  auto tiles = [](int64_t m, int64_t n, int t) { return up(m, t) / t * (up(n, t) / t); };
+  // the same for the backward products, whose sums can be cut into shares of four k-tiles
+  p.dh_tile = p.nt ? TILE_BIG : TUNE(2, tiles(a.N, a.D, 128) * (vk / 4 + 1) < 256 ? TILE_SMALL : TILE_MID);
+  p.dw_tile = p.nt ? TILE_BIG : TUNE(3, tiles(cols, a.D, 128) * (nk / 4 + 1) < 256 ? TILE_SMALL : TILE_MID);
+  const int want_h = p.dh_tile == TILE_BIG ? 256 : p.dh_tile == TILE_SMALL ? 1024 : 512, want_w = p.dw_tile == TILE_SMALL ? 1024 : 512;
+  const int64_t ht = tiles(a.N, a.D, tile_rows(p.dh_tile)), wt = tiles(cols, a.D, tile_rows(p.dw_tile));
+  p.units = (int)(ht > want_h ? ht : want_h);
+  p.most = (int)((vk + 3) / 4);
+  int64_t sh = p.dw_tile == TILE_BIG ? 1 : want_w / wt;
+  if (sh > nk / 4) sh = nk / 4;
   p.shares = (int)(sh < 1 ? 1 : sh);
   return p;
 }
@@ -1021,11 +1028,9 @@ struct Work {
     packed = c.take<char>(a.want_w && !a.split && !p.nt ? a.N * p.dp * esz : 0);
     ht = c.take<uint16_t>(a.want_w && p.nt ? a.D * p.np * (a.split ? 2 : 1) : 0);
     wtr = c.take<uint16_t>(a.want_h && p.nt && !a.wt ? a.D * p.vp * (a.split ? 2 : 1) : 0);
-    const int64_t ht = p.dh_tile == TILE_BIG ? 256 : 128;
+    const int64_t ht = tile_rows(p.dh_tile), wt = tile_rows(p.dw_tile), cols = p.gcols < a.V ? p.gcols : a.V;
     dh_slab = c.take<float>(a.want_h ? p.units * ht * ht : 0);
-    const int64_t wt = p.dw_tile == TILE_BIG ? 256 : 128;
-    const int64_t wtiles = up(p.gcols < a.V ? p.gcols : a.V, wt) / wt * (up(a.D, wt) / wt);
-    dw_slab = c.take<float>(a.want_w && p.shares > 1 ? wtiles * p.shares * wt * wt : 0);
+    dw_slab = c.take<float>(a.want_w && p.shares > 1 ? up(cols, wt) * up(a.D, wt) * p.shares : 0);
     bwd = c.at;
   }
 };
@@ -1044,15 +1049,22 @@ template <class C, bool TB, bool GRAD, int SEG> int launch_score(const ScoreP& p
   hipLaunchKernelGGL((score_kernel<C, TB, GRAD, SEG>), dim3((unsigned)grid), dim3(C::NT), LDS, st, p);
   return (int)hipGetLastError();
 }
+template <int DT, bool TB, bool GRAD, int SEG> int score_tile(const ScoreP& p, int tile, hipStream_t st) {
+  if (tile == TILE_FEW) return launch_score<Few<DT>, TB, GRAD, SEG>(p, st);
+  return tile == TILE_SMALL ? launch_score<Small<DT>, TB, GRAD, SEG>(p, st) : launch_score<Mid<DT>, TB, GRAD, SEG>(p, st);
+}
 template <int DT, bool TB, bool GRAD> int score16(const ScoreP& p, int tile, bool pair, hipStream_t st) {
   if (tile == TILE_BIG) return launch_score<Big<DT>, TB, GRAD, 1>(p, st);
   if constexpr (GRAD)
-    if (pair) return tile == TILE_FEW ? launch_score<Few<DT>, TB, GRAD, 2>(p, st) : launch_score<Mid<DT>, TB, GRAD, 2>(p, st);
-  return tile == TILE_FEW ? launch_score<Few<DT>, TB, GRAD, 1>(p, st) : launch_score<Mid<DT>, TB, GRAD, 1>(p, st);
+    if (pair) return score_tile<DT, TB, GRAD, 2>(p, tile, st);
+  if (GRAD || tile != TILE_FEW) return tile == TILE_SMALL ? launch_score<Small<DT>, TB, GRAD, 1>(p, st) : launch_score<Mid<DT>, TB, GRAD, 1>(p, st);
+  return launch_score<Few<DT>, TB, false, 1>(p, st);
 }
 template <bool TB, bool GRAD> int dispatch_score(const ScoreP& p, int tile, int op, bool split, bool pair, hipStream_t st) {
-  if (split) return tile == TILE_BIG ? launch_score<Big<DT_F16>, TB, GRAD, 3>(p, st) : launch_score<Mid<DT_F16>, TB, GRAD, 3>(p, st);
-  if (op == DT_F32) return tile == TILE_FEW ? launch_score<Few<DT_F32>, TB, GRAD, 1>(p, st) : launch_score<Mid<DT_F32>, TB, GRAD, 1>(p, st);
+  if (split)
+    return tile == TILE_BIG ? launch_score<Big<DT_F16>, TB, GRAD, 3>(p, st) : tile == TILE_SMALL ? launch_score<Small<DT_F16>, TB, GRAD, 3>(p, st)
+                            : launch_score<Mid<DT_F16>, TB, GRAD, 3>(p, st);
+  if (op == DT_F32) return score_tile<DT_F32, TB, GRAD, 1>(p, tile, st);
   return op == DT_BF16 ? score16<DT_BF16, TB, GRAD>(p, tile, pair, st) : score16<DT_F16, TB, GRAD>(p, tile, pair, st);
 }
 template <bool GRAD> int scores(const ScoreP& p, int tile, int op, bool split, bool pair, bool tb, hipStream_t st) {
@@ -1066,16 +1078,19 @@ template <class C, bool TA, bool TB, int SEG> int launch_dh(const DhP& p, hipStr
   hipLaunchKernelGGL((dh_kernel<C, TA, TB, SEG>), dim3(p.units), dim3(C::NT), LDS, st, p);
   return (int)hipGetLastError();
 }
-// 256 x 256: both operands K-contiguous (p.nt); 128 x 128: the gradient and the [V, D] table are walked row by row
-template <class C, int SEG> int mid_dh(const DhP& p, bool wt, hipStream_t st) { return wt ? launch_dh<C, true, false, SEG>(p, st) : launch_dh<C, true, true, SEG>(p, st); }
+// 256 x 256: both operands K-contiguous (p.nt); smaller tiles: the gradient and the [V, D] table are walked row by row
+template <int DT, int SEG> int rows_dh(const DhP& p, int tile, bool wt, hipStream_t st) {
+  if (tile == TILE_SMALL) return wt ? launch_dh<Small<DT>, true, false, SEG>(p, st) : launch_dh<Small<DT>, true, true, SEG>(p, st);
+  return wt ? launch_dh<Mid<DT>, true, false, SEG>(p, st) : launch_dh<Mid<DT>, true, true, SEG>(p, st);
+}
 int dispatch_dh(const DhP& p, int tile, int op, bool split, bool pair, bool wt, hipStream_t st) {
   if (tile == TILE_BIG)
     return split ? launch_dh<Big<DT_F16>, false, false, 3>(p, st) : op == DT_BF16 ? launch_dh<Big<DT_BF16>, false, false, 1>(p, st)
                                                                                  : launch_dh<Big<DT_F16>, false, false, 1>(p, st);
-  if (split) return mid_dh<Mid<DT_F16>, 3>(p, wt, st);
-  if (op == DT_F32) return mid_dh<Mid<DT_F32>, 1>(p, wt, st);
-  if (op == DT_BF16) return pair ? mid_dh<Mid<DT_BF16>, 2>(p, wt, st) : mid_dh<Mid<DT_BF16>, 1>(p, wt, st);
-  return pair ? mid_dh<Mid<DT_F16>, 2>(p, wt, st) : mid_dh<Mid<DT_F16>, 1>(p, wt, st);
+  if (split) return rows_dh<DT_F16, 3>(p, tile, wt, st);
+  if (op == DT_F32) return rows_dh<DT_F32, 1>(p, tile, wt, st);
+  if (op == DT_BF16) return pair ? rows_dh<DT_BF16, 2>(p, tile, wt, st) : rows_dh<DT_BF16, 1>(p, tile, wt, st);
+  return pair ? rows_dh<DT_F16, 2>(p, tile, wt, st) : rows_dh<DT_F16, 1>(p, tile, wt, st);
 }
 
 template <class C, int OT, bool SWAP, int SEG> int launch_dw(const DwP& p, hipStream_t st) {
@@ -1092,13 +1107,16 @@ template <class C, int OT, bool SWAP, int SEG> int launch_dw(const DwP& p, hipSt
                        OT == OT_F32 ? (int)DT_F32 : OT == OT_F16 ? (int)DT_F16 : (int)DT_BF16);
   return (int)hipGetLastError();
 }
+template <int DT, int OT, bool SWAP, int SEG> int rows_dw(const DwP& p, int tile, hipStream_t st) {
+  return tile == TILE_SMALL ? launch_dw<Small<DT>, OT, SWAP, SEG>(p, st) : launch_dw<Mid<DT>, OT, SWAP, SEG>(p, st);
+}
 template <bool SWAP> int dispatch_dw(const DwP& p, int tile, int op, bool split, bool pair, hipStream_t st) {
   const bool big = tile == TILE_BIG;
-  if (split) return big ? launch_dw<Big<DT_F16>, OT_F32, SWAP, 3>(p, st) : launch_dw<Mid<DT_F16>, OT_F32, SWAP, 3>(p, st);
-  if (op == DT_F32) return launch_dw<Mid<DT_F32>, OT_F32, SWAP, 1>(p, st);
+  if (split) return big ? launch_dw<Big<DT_F16>, OT_F32, SWAP, 3>(p, st) : rows_dw<DT_F16, OT_F32, SWAP, 3>(p, tile, st);
+  if (op == DT_F32) return rows_dw<DT_F32, OT_F32, SWAP, 1>(p, tile, st);
   if (op == DT_BF16)
-    return big ? launch_dw<Big<DT_BF16>, OT_BF16, SWAP, 1>(p, st) : pair ? launch_dw<Mid<DT_BF16>, OT_BF16, SWAP, 2>(p, st) : launch_dw<Mid<DT_BF16>, OT_BF16, SWAP, 1>(p, st);
-  return big ? launch_dw<Big<DT_F16>, OT_F16, SWAP, 1>(p, st) : pair ? launch_dw<Mid<DT_F16>, OT_F16, SWAP, 2>(p, st) : launch_dw<Mid<DT_F16>, OT_F16, SWAP, 1>(p, st);
+    return big ? launch_dw<Big<DT_BF16>, OT_BF16, SWAP, 1>(p, st) : pair ? rows_dw<DT_BF16, OT_BF16, SWAP, 2>(p, tile, st) : rows_dw<DT_BF16, OT_BF16, SWAP, 1>(p, tile, st);
+  return big ? launch_dw<Big<DT_F16>, OT_F16, SWAP, 1>(p, st) : pair ? rows_dw<DT_F16, OT_F16, SWAP, 2>(p, tile, st) : rows_dw<DT_F16, OT_F16, SWAP, 1>(p, tile, st);
 }
 
 // 0 where the arguments are what the kernels assume
@@ -1234,7 +1252,7 @@ int backward(const Args& a, const float* f, hipStream_t st) {
       d.G.xlim = (int)p.np; d.W = wh;
       d.W.p += p.nt || a.wt ? (int64_t)v0 * gsz : v0 * wh.ld;
       d.W.xlim = (int)a.D;
-      d.count = s.count; d.D = (int)a.D; d.vc = vc; d.units = p.units; d.accum = k > 0; d.slab = w.dh_slab;
+      d.count = s.count; d.D = (int)a.D; d.vc = vc; d.units = p.units; d.most = p.most; d.accum = k > 0; d.slab = w.dh_slab;
       const int e = dispatch_dh(d, p.dh_tile, p.op, a.split, p.pair, a.wt, st);
       if (e) return e;
     }
@@ -1251,9 +1269,10 @@ int backward(const Args& a, const float* f, hipStream_t st) {
   }
   const bool sums = a.want_b && !a.K;
   if (a.want_h || sums) {
-    const FinishP q{w.dh_slab, s.rows, s.count, s.sc, a.want_h ? (int)a.N : 0, (int)a.D, p.units, a.dh, (int)a.dt, w.colsum, p.bm, (int)a.V, a.db, (int)a.bdt};
+    const FinishP q{w.dh_slab, s.rows, s.count, s.sc, a.want_h ? (int)a.N : 0, (int)a.D, p.units, p.most, a.dh, (int)a.dt, w.colsum, p.bm, (int)a.V, a.db, (int)a.bdt};
     const dim3 grid((unsigned)(q.N + (sums ? (a.V + 255) / 256 : 0)));
     if (p.dh_tile == TILE_BIG) hipLaunchKernelGGL((finish_kernel<256, 256>), grid, dim3(256), 0, st, q);
+    else if (p.dh_tile == TILE_SMALL) hipLaunchKernelGGL((finish_kernel<64, 64>), grid, dim3(256), 0, st, q);
     else hipLaunchKernelGGL((finish_kernel<128, 128>), grid, dim3(256), 0, st, q);
   }
   return (int)hipGetLastError();

@@ -170,6 +170,54 @@ class SparseSoftmaxCrossEntropy(_b.GeneratedCustomOp):
         super().__init__('sparse_softmax_cross_entropy_loss_with_logits', [_t(v) for v in [labels, logits]], outputs)
 
 
+class LinearSoftmaxCrossEntropy(_b.GeneratedCustomOp):
+    """Softmax cross entropy of the logits hidden . weights^T + bias against integer class labels; the logits are not kept.
+    :param hidden: Hidden states [..., D] (FLOATING_POINT)
+    :param weights: Output weights [V, D] (an embedding table), or [D, V] with transposeWeights, in the type of hidden (FLOATING_POINT)
+    :param labels: Class indices [...]; a row labelled ignoreIndex has loss 0 and no gradient, one labelled otherwise outside [0, V) gives NaN (INT)
+    :param bias: Output bias [V] (FLOATING_POINT, optional)
+    :param labelSmoothing: Label smoothing factor in [0, 1) (FLOATING_POINT, default 0.0)
+    :param ignoreIndex: Label of the rows that take no part (INT, default -100)
+    :param transposeWeights: Weights are [D, V], as a dense layer holds them (BOOL, default False)
+    :return output: Per-row loss [...], FLOAT (DOUBLE for DOUBLE operands) (FLOATING_POINT)
+    """
+    OP, NAMESPACE, N_OUT = 'linear_softmax_cross_entropy_loss', 'loss', 1
+
+    def __init__(self, hidden, weights, labels, bias=None, labelSmoothing=0.0, ignoreIndex=-100, transposeWeights=False, outputs=None):
+        super().__init__('linear_softmax_cross_entropy_loss', [_t(v) for v in [hidden, weights, labels] + ([bias] if bias is not None else [])], outputs, iArgs=[ignoreIndex, int(transposeWeights)], tArgs=[labelSmoothing])
+
+
+class LinearTopKDistillation(_b.GeneratedCustomOp):
+    """Distillation from a teacher's top logits, T^2 KL(softmax(teacher / T) || softmax(student / T)), for student logits hidden . weights^T + bias that are not kept.
+    :param hidden: Hidden states [..., D] (FLOATING_POINT)
+    :param weights: Output weights [V, D], or [D, V] with transposeWeights (FLOATING_POINT)
+    :param teacherIndices: Words of the teacher's K best logits [..., K], negative: padding (INT)
+    :param teacherLogits: Their logits [..., K] (FLOATING_POINT)
+    :param bias: Output bias [V] (FLOATING_POINT, optional)
+    :param temperature: Temperature T (FLOATING_POINT, default 1.0)
+    :param transposeWeights: Weights are [D, V], as a dense layer holds them (BOOL, default False)
+    :return output: Per-row loss [...] (FLOATING_POINT)
+    """
+    OP, NAMESPACE, N_OUT = 'linear_topk_distillation_loss', 'loss', 1
+
+    def __init__(self, hidden, weights, teacherIndices, teacherLogits, bias=None, temperature=1.0, transposeWeights=False, outputs=None):
+        super().__init__('linear_topk_distillation_loss', [_t(v) for v in [hidden, weights, teacherIndices, teacherLogits] + ([bias] if bias is not None else [])], outputs, iArgs=[int(transposeWeights)], tArgs=[temperature])
+
+
+class TopKDistillation(_b.GeneratedCustomOp):
+    """Distillation from a teacher's top logits, T^2 KL(softmax(teacher / T) || softmax(student / T)), on student logits.
+    :param logits: Student logits [..., V] (FLOATING_POINT)
+    :param teacherIndices: Words of the teacher's K best logits [..., K], negative: padding (INT)
+    :param teacherLogits: Their logits [..., K] (FLOATING_POINT)
+    :param temperature: Temperature T (FLOATING_POINT, default 1.0)
+    :return output: Per-row loss [...] (FLOATING_POINT)
+    """
+    OP, NAMESPACE, N_OUT = 'topk_distillation_loss', 'loss', 1
+
+    def __init__(self, logits, teacherIndices, teacherLogits, temperature=1.0, outputs=None):
+        super().__init__('topk_distillation_loss', [_t(v) for v in [logits, teacherIndices, teacherLogits]], outputs, tArgs=[temperature])
+
+
 class L2Loss(_b.GeneratedCustomOp):
     """Half the sum of squares: sum(x^2) / 2.
     :param var: Input (NUMERIC)
@@ -209,4 +257,4 @@ class WeightedCrossEntropyWithLogits(_b.GeneratedCustomOp):
         super().__init__('weighted_cross_entropy_with_logits', [_t(v) for v in [targets, inputs, weights]], outputs)
 
 
-CLASSES = (AbsoluteDifference, CosineDistance, HingeLoss, HuberLoss, LogLoss, LogPoisson, MeanPairwiseSquaredError, MeanSquaredError, SigmoidCrossEntropy, SoftmaxCrossEntropy, SparseSoftmaxCrossEntropy, L2Loss, CtcLoss, WeightedCrossEntropyWithLogits, )
+CLASSES = (AbsoluteDifference, CosineDistance, HingeLoss, HuberLoss, LogLoss, LogPoisson, MeanPairwiseSquaredError, MeanSquaredError, SigmoidCrossEntropy, SoftmaxCrossEntropy, SparseSoftmaxCrossEntropy, LinearSoftmaxCrossEntropy, LinearTopKDistillation, TopKDistillation, L2Loss, CtcLoss, WeightedCrossEntropyWithLogits, )

@@ -1212,6 +1212,54 @@ op("weighted_cross_entropy_with_logits")(lambda ins, i, t, b, d: (1 - ins[0]) * 
     torch.log1p(torch.exp(-ins[1].abs())) + F.relu(-ins[1])))
 
 
+# ----------------------------------------------------------------------------- losses on an output layer whose logits are not kept
+# (ops/vocab_loss.py; not ops of the reference). Generic form here, kernels in impl_platform.py. iArgs / tArgs as the loss namespace
+# emits them: cross entropy [ignoreIndex, transposeWeights] / [labelSmoothing], distillation [transposeWeights] / [temperature].
+def vocab_loss_call(name, ins, i, t, plain):
+    """(function of the differentiable inputs, those inputs) of a vocabulary loss op."""
+    from ...ops import vocab_loss as VL
+    if name == "topk_distillation_loss":
+        T = float(t[0]) if t else 1.0
+        return (lambda z: VL.topk_distillation(z, ins[1], ins[2], T, plain=plain)), [ins[0]]
+    w_t = (lambda w: w.t()) if (i and int(i[-1])) else (lambda w: w)
+    if name == "linear_softmax_cross_entropy_loss":
+        n_fixed, ignore, eps = 3, int(i[0]) if i else -100, float(t[0]) if t else 0.0
+        w_t = (lambda w: w.t()) if (i and len(i) > 1 and int(i[1])) else (lambda w: w)
+        f = lambda h, w, b=None: VL.linear_cross_entropy(h, w_t(w), ins[2], b, ignore, eps, plain=plain)                  # noqa: E731
+    else:
+        n_fixed, T = 4, float(t[0]) if t else 1.0
+        f = lambda h, w, b=None: VL.linear_topk_distillation(h, w_t(w), ins[2], ins[3], b, T, plain=plain)               # noqa: E731
+    bias = [ins[n_fixed]] if len(ins) > n_fixed and ins[n_fixed] is not None else []
+    return f, [ins[0], ins[1]] + bias
+
+
+def vocab_loss_grad(name, ins, i, t, plain):
+    f, leaves = vocab_loss_call(name, ins[:-1], i, t, plain)
+    leaves = [x.detach().requires_grad_(True) for x in leaves]
+    with torch.enable_grad():
+        y = f(*leaves)
+    return tuple(torch.autograd.grad(y, leaves, ins[-1].to(y.dtype).reshape(y.shape)))
+
+
+def _vocab_loss(name):
+    def f(ins, i, t, b, d):
+        if ins[0].is_meta:
+            return torch.empty(ins[0].shape[:-1], dtype=torch.float64 if ins[0].dtype == torch.float64 else torch.float32, device="meta")
+        g, leaves = vocab_loss_call(name, ins, i, t, True)
+        return g(*leaves)
+
+    def bp(ins, i, t, b, d):
+        if ins[0].is_meta:
+            return tuple(torch.empty_like(x) for x in vocab_loss_call(name, ins[:-1], i, t, True)[1])
+        return vocab_loss_grad(name, ins, i, t, True)
+    op(name)(f)
+    op(name + "_bp")(bp)
+
+
+for _n in ("linear_softmax_cross_entropy_loss", "linear_topk_distillation_loss", "topk_distillation_loss"):
+    _vocab_loss(_n)
+
+
 @op("ctc_loss")
 def _ctc_loss(ins, i, t, b, d):
     """targetLabels [B, L], logitInput [B, T, C], targetLabelLengths [B], logitInputLengths [B]; iArgs [blankIndex]."""

@@ -845,6 +845,29 @@ def _fused_dense_hip(ins, i, t, b, d):
     return LIN.fused_dense(x, w, bias, res, act)
 
 
+# ----------------------------------------------------------------------------- losses on an output layer whose logits are not kept
+# (native/csrc/vocab_loss.hip, topk_distill.hip; generic forms and argument conventions in impl_nn.py)
+def _vocab_platform(name, n_fixed):
+    from .impl_nn import vocab_loss_call, vocab_loss_grad
+
+    def ok(ins, i, t, b, d):
+        from ...ops import vocab_loss as VL
+        return len(ins) >= n_fixed and all(isinstance(x, torch.Tensor) for x in ins) and ins[0].dim() >= 1 and VL.usable(*ins)
+
+    @platform(name, ok, differentiable=True)
+    def _f(ins, i, t, b, d):
+        f, leaves = vocab_loss_call(name, ins, i, t, False)
+        return f(*leaves)
+
+    @platform(name + "_bp", ok)
+    def _bp(ins, i, t, b, d):
+        return vocab_loss_grad(name, ins, i, t, False)
+
+
+for _n, _k in (("linear_softmax_cross_entropy_loss", 3), ("linear_topk_distillation_loss", 4), ("topk_distillation_loss", 3)):
+    _vocab_platform(_n, _k)
+
+
 # ----------------------------------------------------------------------------- helpers_misc.hip family
 # order statistics, generators, TF-exact bicubic / area resize, adjust_contrast, draw_bounding_boxes, t-SNE steps, word2vec batch
 from ...ops import misc_kernels as MK  # noqa: E402

@@ -150,10 +150,12 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else _up(t.shape[1], 16 // t.element_size())
 
 
-def _split(rows, training):
-    """fp32 operands as pairs of halves on the 16-bit matrix cores (three products, twice to three times the rate of the fp32 ones), once
-    the rows pay for the conversion of the weights."""
-    return rows >= (48 if training else 128)
+def _split(rows, hidden, vocabulary, training):
+    """fp32 operands as pairs of halves on the 16-bit matrix cores: three products there take a quarter of one on the fp32 cores, once the rows
+    pay for the conversion of the weights (12 bytes an element) and the call for its two launches. Step with 98 words x 1600 rows x 512:
+    @A us in fp32, @B us in halves; 30522 x 96 x 768: @C and @D us; one forward of 512 rows: @E and @F us."""
+    work = hidden * vocabulary
+    return (rows - 40) * work > 150e6 if training else (rows - 150) * work > 600e6
 
 
 def _launch(fn, what, dev, *args):
@@ -192,7 +194,7 @@ class _LinearLoss(torch.autograd.Function):
         w = weights.t() if dv else weights
         want = ctx.needs_input_grad[:3]
         training = any(want)
-        split = h.dtype == torch.float32 and _split(h.shape[0], training)
+        split = h.dtype == torch.float32 and _split(h.shape[0], h.shape[1], weights.shape[0], training)
         if split:                                                       # the conversion takes rows of any stride
             h = h if h.stride(1) == 1 and (h.shape[0] == 1 or h.stride(0) >= h.shape[1]) else h.contiguous()
             w = w if w.stride(1) == 1 and (w.shape[0] == 1 or w.stride(0) >= w.shape[1]) else w.contiguous()
@@ -226,7 +228,7 @@ class _LinearLoss(torch.autograd.Function):
 def _linear_backward(ctx, dloss):
     h, w, bias = ctx.saved_tensors[:3]
     a, f, size = ctx.call
-    a = _Block(*a)                                                      # (a graph kept alive may be walked from two threads)
+    a = _Block.from_buffer_copy(a)                                      # (a graph kept alive may be walked from two threads)
     dev = h.device
     g = _dloss(dloss)
     want_h, want_w, want_b = ctx.needs_input_grad[:3]
@@ -276,7 +278,7 @@ class _TopkDistillation(torch.autograd.Function):
 def _topk_backward(ctx, dloss):
     z = ctx.saved_tensors[0]                                            # (unpacked: a changed tensor is refused)
     a, f = ctx.call
-    a = _TopkBlock(*a)
+    a = _TopkBlock.from_buffer_copy(a)
     g = _dloss(dloss)
     dz = torch.empty(ctx.shape, dtype=z.dtype, device=z.device)
     a[10], a[12], a[13] = 0, g.data_ptr(), dz.data_ptr()
@@ -302,7 +304,7 @@ def _teacher_operands(indices, logits):
     return indices.contiguous(), t.contiguous()
 
 
-def linear_cross_entropy(hidden, weights, labels, bias=None, ignore_index=-100, label_smoothing=0.0):
+def linear_cross_entropy(hidden, weights, labels, bias=None, ignore_index=-100, label_smoothing=0.0, plain=False):
     """Softmax cross entropy of the logits ``hidden . weights^T + bias`` against integer labels, without keeping the logits.
 
     hidden [..., D]; weights [V, D] in hidden's type (an embedding table, or ``w.t()`` of a dense layer's [nIn, nOut] weights: both layouts
@@ -311,20 +313,20 @@ def linear_cross_entropy(hidden, weights, labels, bias=None, ignore_index=-100, 
     Returns the rows' losses (fp32; fp64 for fp64 operands). Differentiable in hidden, weights and bias.
 
     16-bit operands: scores, softmax and all sums in fp32, the scores' gradient is rounded to the operands' type for the two gradient
-    products (fp16: scaled to its range first)."""
+    products (fp16: scaled to its range first; up to 256 rows it is kept in two halves). ``plain``: the plain form, whatever the operands."""
     name = "linear_cross_entropy"
     _check_linear(hidden, weights, bias, name)
     _need(labels.dtype in (torch.int32, torch.int64), "%s: labels must be INT32 or INT64" % name)
     _need(labels.shape == hidden.shape[:-1], "%s: labels %s must have the shape of hidden's rows %s" % (name, list(labels.shape), list(hidden.shape[:-1])))
     _need(labels.device == hidden.device, "%s: labels are on another device" % name)
     _need(0.0 <= label_smoothing < 1.0, "%s: label smoothing must be in [0, 1)" % name)
-    if not usable(hidden, weights, labels, bias):
+    if plain or not usable(hidden, weights, labels, bias):
         return linear_cross_entropy_reference(hidden, weights, labels, bias, ignore_index, label_smoothing)
     return _LinearLoss.apply(hidden, weights, None if bias is None else bias.contiguous(), labels.reshape(-1).contiguous(), None, int(ignore_index),
                              float(label_smoothing), 1.0)
 
 
-def linear_topk_distillation(hidden, weights, teacher_indices, teacher_logits, bias=None, temperature=1.0):
+def linear_topk_distillation(hidden, weights, teacher_indices, teacher_logits, bias=None, temperature=1.0, plain=False):
     """Distillation from a teacher's top logits: T^2 KL(softmax(teacher_logits / T) || softmax(z / T)) per row for the student's logits
     ``z = hidden . weights^T + bias``, which are not kept.
 
@@ -335,18 +337,18 @@ def linear_topk_distillation(hidden, weights, teacher_indices, teacher_logits, b
     name = "linear_topk_distillation"
     _check_linear(hidden, weights, bias, name)
     _check_teacher(hidden.shape[:-1], hidden.device, teacher_indices, teacher_logits, temperature, name)
-    if not usable(hidden, weights, teacher_indices, teacher_logits, bias):
+    if plain or not usable(hidden, weights, teacher_indices, teacher_logits, bias):
         return linear_topk_distillation_reference(hidden, weights, teacher_indices, teacher_logits, bias, temperature)
     idx, t = _teacher_operands(teacher_indices, teacher_logits)
     return _LinearLoss.apply(hidden, weights, None if bias is None else bias.contiguous(), idx, t, 0, 0.0, float(temperature))
 
 
-def topk_distillation(logits, teacher_indices, teacher_logits, temperature=1.0):
+def topk_distillation(logits, teacher_indices, teacher_logits, temperature=1.0, plain=False):
     """:func:`linear_topk_distillation` for a student whose logits [..., V] are there already. Differentiable in the logits."""
     name = "topk_distillation"
     _need(logits.dim() >= 1 and _floating(logits) and logits.shape[-1] > 0, "%s: logits must be a floating point tensor [..., V]" % name)
     _check_teacher(logits.shape[:-1], logits.device, teacher_indices, teacher_logits, temperature, name)
-    if not usable(logits, teacher_indices, teacher_logits):
+    if plain or not usable(logits, teacher_indices, teacher_logits):
         return topk_distillation_reference(logits, teacher_indices, teacher_logits, temperature)
     idx, t = _teacher_operands(teacher_indices, teacher_logits)
     return _TopkDistillation.apply(logits, idx, t, float(temperature))
