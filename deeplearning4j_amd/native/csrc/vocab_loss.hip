@@ -946,10 +946,12 @@ Plan plan(const Args& a) {
   p.op = a.split ? DT_F16 : (int)a.dt;
   const bool bits16 = p.op != DT_F32;
   const int64_t big_tiles = up(a.N, 256) / 256 * (up(a.V, 256) / 256);
+  // (its operands are addressed with 32-bit offsets: rows of all of them, and H's indirect ones together, have to be short of that)
+  const bool near = up(a.N, 256) * 2 < BUF_LD && up(a.V, 256) * 2 < BUF_LD && a.ldh * 4 < BUF_LD && a.ldw * 4 < BUF_LD && (a.split || a.N * a.ldh * 2 < BUF_SPAN);
   const int64_t mid_tiles = up(a.N, 128) / 128 * (up(a.V, 128) / 128);
   // 256 x 256 tiles once they cover two thirds of the 256 CUs; 32 rows where few rows meet a large vocabulary (W streams through, a tile per
   // CU at 32768 words); 64 x 64 tiles with four stages where 128 x 128 ones would leave CUs idle (the time is a chain of k-tiles then)
-  p.tile = TUNE(0, bits16 && big_tiles >= 176 && a.N > 128 ? TILE_BIG : a.N <= 32 && a.V >= 16384 ? TILE_FEW : mid_tiles < 176 ? TILE_SMALL : TILE_MID);
+  p.tile = TUNE(0, bits16 && big_tiles >= 176 && a.N > 128 && near ? TILE_BIG : a.N <= 32 && a.V >= 16384 ? TILE_FEW : mid_tiles < 176 ? TILE_SMALL : TILE_MID);
   if (a.split && p.tile == TILE_FEW) p.tile = TILE_MID;
   if (!bits16 && p.tile == TILE_BIG) p.tile = TILE_MID;
   p.bm = tile_rows(p.tile);
