@@ -126,6 +126,7 @@ _AT = {n: k for k, n in enumerate(_ARGS)}
 _Block = ctypes.c_int64 * len(_ARGS)
 _Floats = ctypes.c_float * 2
 _Sizes = ctypes.c_int64 * 3
+_STATE, _WS = _AT["state"], _AT["ws"]
 # struct DistillArgs in native/csrc/topk_distill.hip: N V K ldz dt idx64 tdt z idx t loss lse dloss dz
 _TopkBlock = ctypes.c_int64 * 14
 
@@ -183,42 +184,57 @@ def _dloss(g):
     return g if g.dtype == torch.float32 and g.is_contiguous() else g.float().contiguous()
 
 
+def _linear_forward(hidden, weights, bias, first, second, ignore, smoothing, temperature, want=(False, False, False)):
+    """(loss, what the backward pass needs: tensors, call) - the latter None where no gradient is wanted."""
+    lib = _lib()
+    h = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
+    dv = weights.stride(1) != 1 and weights.stride(0) == 1              # [V, D] row by row, or as the rows of its [D, V] transpose
+    w = weights.t() if dv else weights
+    training = any(want)
+    N, D = h.shape
+    split = h.dtype == torch.float32 and _split(N, D, weights.shape[0], training)
+    if split:                                                           # the conversion takes rows of any stride
+        h = h if h.stride(1) == 1 and (N == 1 or h.stride(0) >= D) else h.contiguous()
+        w = w if w.stride(1) == 1 and (w.shape[0] == 1 or w.stride(0) >= w.shape[1]) else w.contiguous()
+    else:
+        h, w = _rows16(h), _rows16(w)
+    dev = h.device
+    loss = torch.empty(hidden.shape[:-1], dtype=torch.float32, device=dev)
+    teacher = second is not None
+    is64, at = first.dtype == torch.int64, first.data_ptr()
+    a = _Block(N, D, weights.shape[0], _DT[h.dtype], split, dv, 0 if bias is None else _DT[bias.dtype], _ld(h), _ld(w), is64, ignore, is64,
+               _DT[second.dtype] if teacher else 0, first.shape[1] if teacher else 0, *want,
+               h.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if teacher else at, at if teacher else 0,
+               second.data_ptr() if teacher else 0, loss.data_ptr(), 0, 0, 0, 0, 0, 0)
+    f = _Floats(temperature, smoothing)
+    size = _Sizes()
+    lib.dl4j_linear_loss_bytes(a, size)
+    if training:
+        state, ws = torch.empty(size[0], dtype=torch.uint8, device=dev), torch.empty(size[1], dtype=torch.uint8, device=dev)
+        a[_STATE], a[_WS] = state.data_ptr(), ws.data_ptr()
+    else:
+        both = torch.empty(size[0] + size[1], dtype=torch.uint8, device=dev)
+        a[_STATE] = both.data_ptr()
+        a[_WS] = a[_STATE] + size[0]
+    _launch(lib.dl4j_linear_loss_fwd, "linear_loss_fwd", dev, a, f)
+    return loss, ((h, w, state), (a, f, size[2], dv)) if training else None
+
+
 class _LinearLoss(torch.autograd.Function):
     """hidden [..., D], weights [V, D], bias [V] or None; first / second: labels and None, or the teacher's indices and logits."""
 
     @staticmethod
     def forward(ctx, hidden, weights, bias, first, second, ignore, smoothing, temperature):
-        lib = _lib()
-        h = hidden.reshape(-1, hidden.shape[-1])
-        dv = weights.stride(1) != 1 and weights.stride(0) == 1          # [V, D] row by row, or as the rows of its [D, V] transpose
-        w = weights.t() if dv else weights
-        want = ctx.needs_input_grad[:3]
-        training = any(want)
-        split = h.dtype == torch.float32 and _split(h.shape[0], h.shape[1], weights.shape[0], training)
-        if split:                                                       # the conversion takes rows of any stride
-            h = h if h.stride(1) == 1 and (h.shape[0] == 1 or h.stride(0) >= h.shape[1]) else h.contiguous()
-            w = w if w.stride(1) == 1 and (w.shape[0] == 1 or w.stride(0) >= w.shape[1]) else w.contiguous()
-        else:
-            h, w = _rows16(h), _rows16(w)
-        N, dev = h.shape[0], h.device
-        loss = torch.empty(hidden.shape[:-1], dtype=torch.float32, device=dev)
-        teacher = second is not None
-        is64 = first.dtype == torch.int64
-        a = _Block(N, h.shape[1], weights.shape[0], _DT[h.dtype], split, dv, 0 if bias is None else _DT[bias.dtype], _ld(h), _ld(w), is64, ignore, is64,
-                   _DT[second.dtype] if teacher else 0, first.shape[1] if teacher else 0, *want,
-                   h.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if teacher else first.data_ptr(), first.data_ptr() if teacher else 0,
-                   second.data_ptr() if teacher else 0, loss.data_ptr(), 0, 0, 0, 0, 0, 0)
-        f = _Floats(temperature, smoothing)
-        size = _Sizes()
-        lib.dl4j_linear_loss_bytes(a, size)
-        state = torch.empty(size[0], dtype=torch.uint8, device=dev)
-        ws = torch.empty(size[1], dtype=torch.uint8, device=dev)
-        a[_AT["state"]], a[_AT["ws"]] = state.data_ptr(), ws.data_ptr()
-        _launch(lib.dl4j_linear_loss_fwd, "linear_loss_fwd", dev, a, f)
-        if training:
-            ctx.save_for_backward(h, w, bias, first, second, loss, state)
-            ctx.call, ctx.dv, ctx.shape = (a, f, size[2]), dv, hidden.shape
+        loss, ((h, w, state), call) = _linear_forward(hidden, weights, bias, first, second, ignore, smoothing, temperature, ctx.needs_input_grad[:3])
+        ctx.save_for_backward(h, w, bias, first, second, loss, state)
+        ctx.call, ctx.shape = call, hidden.shape
         return loss
+
+    @staticmethod
+    def apply_or_run(hidden, weights, bias, *rest):
+        if torch.is_grad_enabled() and (hidden.requires_grad or weights.requires_grad or (bias is not None and bias.requires_grad)):
+            return _LinearLoss.apply(hidden, weights, bias, *rest)
+        return _linear_forward(hidden, weights, bias, *rest)[0]
 
     @staticmethod
     def backward(ctx, dloss):
@@ -227,7 +243,7 @@ class _LinearLoss(torch.autograd.Function):
 
 def _linear_backward(ctx, dloss):
     h, w, bias = ctx.saved_tensors[:3]
-    a, f, size = ctx.call
+    a, f, size, dv = ctx.call
     a = _Block.from_buffer_copy(a)                                      # (a graph kept alive may be walked from two threads)
     dev = h.device
     g = _dloss(dloss)
@@ -240,7 +256,7 @@ def _linear_backward(ctx, dloss):
         if t is not None:
             a[_AT[name]] = t.data_ptr()
     _launch(_lib().dl4j_linear_loss_bwd, "linear_loss_bwd", dev, a, f)
-    return dh, (dw.t() if want_w and ctx.dv else dw), db, None, None, None, None, None
+    return dh, (dw.t() if want_w and dv else dw), db, None, None, None, None, None
 
 
 def _once(fn, ctx, dloss):
@@ -250,24 +266,28 @@ def _once(fn, ctx, dloss):
     return Once.call(ctx, dloss)
 
 
-class _TopkDistillation(torch.autograd.Function):
-    CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_TOPK_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
+
+def _topk_forward(logits, idx, t, temperature):
+    z = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
+    z = z if z.stride(1) == 1 and z.stride(0) >= z.shape[1] else z.contiguous()
+    N, dev = z.shape[0], z.device
+    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
+    lse = torch.empty(N, dtype=torch.float32, device=dev)
+    a = _TopkBlock(N, z.shape[1], idx.shape[1], z.stride(0), _TOPK_DT[z.dtype], idx.dtype == torch.int64, _TOPK_DT[t.dtype], z.data_ptr(), idx.data_ptr(),
+                   t.data_ptr(), loss.data_ptr(), lse.data_ptr(), 0, 0)
+    f = _Floats(temperature, 0.0)
+    _launch(_lib().dl4j_topk_distill, "topk_distill", dev, a, f)
+    return loss, z, lse, (a, f)
+
+
+class _TopkDistillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, idx, t, temperature):
-        z = logits.reshape(-1, logits.shape[-1])
-        z = z if z.stride(1) == 1 and z.stride(0) >= z.shape[1] else z.contiguous()
-        N = z.shape[0]
-        loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=z.device)
-        lse = torch.empty(N, dtype=torch.float32, device=z.device)
-        c = _TopkDistillation.CODE
-        a = _TopkBlock(N, z.shape[1], idx.shape[1], z.stride(0), c[z.dtype], idx.dtype == torch.int64, c[t.dtype], z.data_ptr(), idx.data_ptr(),
-                       t.data_ptr(), loss.data_ptr(), lse.data_ptr(), 0, 0)
-        f = _Floats(temperature, 0.0)
-        _launch(_lib().dl4j_topk_distill, "topk_distill", z.device, a, f)
-        if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(z, idx, t, lse)
-            ctx.call, ctx.shape = (a, f), logits.shape
+        loss, z, lse, ctx.call = _topk_forward(logits, idx, t, temperature)
+        ctx.save_for_backward(z, idx, t, lse)
+        ctx.shape = logits.shape
         return loss
 
     @staticmethod
@@ -322,8 +342,8 @@ def linear_cross_entropy(hidden, weights, labels, bias=None, ignore_index=-100, 
     _need(0.0 <= label_smoothing < 1.0, "%s: label smoothing must be in [0, 1)" % name)
     if plain or not usable(hidden, weights, labels, bias):
         return linear_cross_entropy_reference(hidden, weights, labels, bias, ignore_index, label_smoothing)
-    return _LinearLoss.apply(hidden, weights, None if bias is None else bias.contiguous(), labels.reshape(-1).contiguous(), None, int(ignore_index),
-                             float(label_smoothing), 1.0)
+    return _LinearLoss.apply_or_run(hidden, weights, None if bias is None else bias.contiguous(), labels.reshape(-1).contiguous(), None,
+                                    int(ignore_index), float(label_smoothing), 1.0)
 
 
 def linear_topk_distillation(hidden, weights, teacher_indices, teacher_logits, bias=None, temperature=1.0, plain=False):
@@ -340,7 +360,7 @@ def linear_topk_distillation(hidden, weights, teacher_indices, teacher_logits, b
     if plain or not usable(hidden, weights, teacher_indices, teacher_logits, bias):
         return linear_topk_distillation_reference(hidden, weights, teacher_indices, teacher_logits, bias, temperature)
     idx, t = _teacher_operands(teacher_indices, teacher_logits)
-    return _LinearLoss.apply(hidden, weights, None if bias is None else bias.contiguous(), idx, t, 0, 0.0, float(temperature))
+    return _LinearLoss.apply_or_run(hidden, weights, None if bias is None else bias.contiguous(), idx, t, 0, 0.0, float(temperature))
 
 
 def topk_distillation(logits, teacher_indices, teacher_logits, temperature=1.0, plain=False):
@@ -351,4 +371,6 @@ def topk_distillation(logits, teacher_indices, teacher_logits, temperature=1.0, 
     if plain or not usable(logits, teacher_indices, teacher_logits):
         return topk_distillation_reference(logits, teacher_indices, teacher_logits, temperature)
     idx, t = _teacher_operands(teacher_indices, teacher_logits)
-    return _TopkDistillation.apply(logits, idx, t, float(temperature))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _TopkDistillation.apply(logits, idx, t, float(temperature))
+    return _topk_forward(logits, idx, t, float(temperature))[0]
