@@ -23,7 +23,7 @@
 //
 // A product of fp32 operands runs on the 16-bit matrix cores as three products of halves, a = a1 + a2 with a1 = fp16(a), a2 = fp16(a - a1)
 // (operands scaled by a power of two so that the largest is below 2^14):  a . b = a1 b1 + a1 b2 + a2 b1, what is left out is 2^-24 of |a||b|.
-// The three are one long product: k-tile t of 3 KT reads halves (t / KT == 2, t / KT == 1) of A and B.
+// The three are one long product whose k-tiles come in threes, (a1, b1), (a1, b2), (a2, b1), so that what a k-tile reads again is still in L2.
 #pragma once
 #include "gemm_trans.h"
 
@@ -49,22 +49,19 @@ template <class C, int SEG> __host__ __device__ __forceinline__ int k_tiles(int 
 // k-tile t of the product: first k, and the halves' byte offsets
 template <class C, int SEG> struct KWalk {
   int64_t alo, blo;
-  int K, KT1, t0;
+  int K, t0;
   struct At { int k; int64_t a, b; };
   __device__ __forceinline__ At tile(int t) const {
     t += t0;
     At at;
-    if constexpr (SEG == 1) { at.k = t * C::BK; at.a = at.b = 0; }
-    else {
-      const int seg = SEG == 3 && t >= 2 * KT1 ? 2 : t >= KT1 ? 1 : 0;
-      at.k = (t - seg * KT1) * C::BK;
-      at.a = SEG == 3 ? (seg == 2 ? alo : 0) : (seg ? alo : 0);
-      at.b = seg == 1 ? blo : 0;
-    }
+    const int k = t / SEG, seg = t - k * SEG;
+    at.k = k * C::BK;
+    at.a = seg == SEG - 1 && SEG > 1 ? alo : 0;
+    at.b = seg == 1 ? blo : 0;
     return at;
   }
   __device__ __forceinline__ void walk(const Operand& A, const Operand& B, int K_, int first) {
-    alo = A.lo; blo = B.lo; K = K_; KT1 = (K_ + C::BK - 1) / C::BK; t0 = first;
+    alo = A.lo; blo = B.lo; K = K_; t0 = first;
   }
 };
 

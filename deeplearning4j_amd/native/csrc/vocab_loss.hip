@@ -324,8 +324,8 @@ struct ScoreP {
   int N, D, v0, v1;                      // columns [v0, v1) of the vocabulary
   float invT, smooth_v;                  // 1 / T;  e / V
   float2* part; float* tz; float* zs;    // statistics: part [ntiles][N]; target score [N]; zs [ntiles][N] = sum of z * e / V (or null)
-  // gradient: coefficient and lse per position in `rows`
-  const float* lse; const float* coef;
+  // gradient, per position in `rows`: coefficient; q = exp2(z - ref) * inv
+  const float* ref; const float* inv; const float* coef;
   float keep;                            // 1 - e
   char* G; int64_t ldg, glo;             // [v - v0][ldg bytes]: position m at element m; second half glo bytes behind
   char* R; int64_t ldr, rlo;             // the gradient once more, row by row: [m][v - v0] (or null; 256 x 256 tiles)
@@ -343,7 +343,7 @@ template <class C> constexpr int score_over(bool grad) {
   return larger(C::STAGES * C::STAGE_BYTES, grad ? C::BN * grad_pitch<C>() : larger(C::WN * 16 * (C::BM + 16), C::BM / C::WM * (C::BN + 4)) * 4);
 }
 template <class C> constexpr int score_lds(bool grad) {
-  return score_over<C>(grad) + (grad ? 3 * C::BM + C::WM * C::BN : C::BM * (1 + 3 * C::WN) + 4 * C::NW + 1) * 4;
+  return score_over<C>(grad) + (grad ? 4 * C::BM + C::WM * C::BN : C::BM * (1 + 3 * C::WN) + 4 * C::NW + 1) * 4;
 }
 
 // The bias is where the accumulators start (-inf for columns past the vocabulary), so that a score is accumulator * zscale.
@@ -371,10 +371,10 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
   const float zscale = p.sc->z * p.invT * LOG2E;
   // the rows' label, coefficient and normaliser: on their way while the product runs
   int lab = -1;
-  float rc = 0.f, rl = 3e38f;                                      // rows past the end: exp2(z - l) = 0
+  float rc = 0.f, rl = 3e38f, rq = 0.f;                            // rows past the end: exp2(z - ref) = 0
   if (tid < C::BM && m0 + tid < count) {
     lab = p.lab[m0 + tid] - n0;
-    if constexpr (GRAD) { rc = p.coef[m0 + tid]; rl = p.lse[m0 + tid]; }
+    if constexpr (GRAD) { rc = p.coef[m0 + tid]; rl = p.ref[m0 + tid]; rq = rc * p.inv[m0 + tid]; }
   }
   typename C::acc_t acc[C::TM][C::TN];
   {
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
   int* slab = reinterpret_cast<int*>(sf);                          // label's column inside the tile, or none of them
   if (tid < C::BM) {
     slab[tid] = lab < C::BN && lab + n0 < p.v1 ? lab : -1;
-    if constexpr (GRAD) { sf[C::BM + tid] = rc; sf[2 * C::BM + tid] = rl; }
+    if constexpr (GRAD) { sf[C::BM + tid] = rc; sf[2 * C::BM + tid] = rl; sf[3 * C::BM + tid] = rq; }
   }
   __syncthreads();
   // a label's score is rare in a wave's part of the tile: whether there is one at all is asked once
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
     typedef OTy Pack __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int i = 0; i < C::TM; ++i) {
-      const f32x4 c = *reinterpret_cast<const f32x4*>(sf + C::BM + row0 + i * 16), l = *reinterpret_cast<const f32x4*>(sf + 2 * C::BM + row0 + i * 16);
+      const f32x4 c = *reinterpret_cast<const f32x4*>(sf + 3 * C::BM + row0 + i * 16), l = *reinterpret_cast<const f32x4*>(sf + 2 * C::BM + row0 + i * 16);
 #pragma unroll
       for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
         }
     }
     if (p.colsum) {                                                // a lane's rows, the four lane groups of a column, the wave rows
-      float* sC = sf + 3 * C::BM;
+      float* sC = sf + 4 * C::BM;
 #pragma unroll
       for (int j = 0; j < C::TN; ++j) {
         float s = 0.f;
@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
           const int e1 = p.first[(t + 1) * p.N + n];
           for (int e = p.first[t * p.N + n]; e < e1; ++e) {
             const int64_t o = (int64_t)n * p.K + e;
-            float g = sf[C::BM + tid] * (exp2_(p.zk[o] - sf[2 * C::BM + tid]) - p.psum[o]);
+            float g = sf[3 * C::BM + tid] * exp2_(p.zk[o] - sf[2 * C::BM + tid]) - sf[C::BM + tid] * p.psum[o];
             if (half == 1) g -= O::fl(O::cv(g));
             *reinterpret_cast<OTy*>(smem + (p.sidx[o] - n0) * PITCH + tid * OSZ) = O::cv(g);
           }
@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
       }
     }
     if (p.colsum) {
-      const float* sC = sf + 3 * C::BM;
+      const float* sC = sf + 4 * C::BM;
       for (int v = tid; v < C::BN; v += C::NT) {
         float s = 0.f;
 #pragma unroll
@@ -654,7 +654,7 @@ struct CombineP {
   const float* ent; const float* sp; const float* zk; int K;    // distillation (ent != null)
   int N, ntiles;
   float keep, T;
-  float* lse; float* loss;
+  float* ref; float* inv; float* loss;
 };
 template <int R>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineP p) {
@@ -690,17 +690,20 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineP p) {
     }
   }
   if (g != 0 || m >= count) return;
-  float lse = mx + log2_(s), loss;
+  // The normaliser is kept as (reference, 1 / sum): as one number of the size of the scores its rounding would be the row's, some 2^-24 |lse|
+  // of every probability at once.
+  float loss;
   if (p.ent) {
     const float h = p.ent[n];
-    loss = p.T * p.T * (h + LN2 * (lse - z));
-    if (h != h) lse = h;                                         // nothing sound to distil from: the row's gradient is NaN too
+    loss = p.T * p.T * (h + LN2 * ((mx - z) + log2_(s)));
+    if (h != h) mx = h;                                          // nothing sound to distil from: the row's gradient is NaN too
   } else {
     const bool in = p.lab[m] >= 0;
-    if (!in) lse = __builtin_nanf("");                           // a label outside the vocabulary: loss and gradient of the row are NaN
-    loss = LN2 * (lse - (in ? p.keep * p.tz[m] : 0.f) - z);
+    loss = in ? LN2 * ((mx - p.keep * p.tz[m] - z) + log2_(s)) : __builtin_nanf("");
+    if (!in) mx = loss;                                          // a label outside the vocabulary: loss and gradient of the row are NaN
   }
-  p.lse[m] = lse;
+  p.ref[m] = mx;
+  p.inv[m] = 1.f / s;
   p.loss[n] = loss;
 }
 
@@ -919,8 +922,9 @@ template <int DT> using Big = Cfg<256, 256, 2, 4, 2, 16, DT>;
 template <int DT> using Mid = Cfg<128, 128, 2, 2, 2, 16, DT>;
 template <int DT> using Few = Cfg<32, 128, 1, 4, 4, 16, DT>;
 template <int DT> using Small = Cfg<64, 64, 2, 2, 4, 16, DT>;
-enum { TILE_BIG = 0, TILE_MID = 1, TILE_FEW = 2, TILE_SMALL = 3 };
-int tile_rows(int tile) { return tile == TILE_BIG ? 256 : tile == TILE_MID ? 128 : tile == TILE_FEW ? 32 : 64; }
+template <int DT> using Thin = Cfg<128, 128, 2, 2, 1, 16, DT>;
+enum { TILE_BIG = 0, TILE_MID = 1, TILE_FEW = 2, TILE_SMALL = 3, TILE_THIN = 4 };
+int tile_rows(int tile) { return tile == TILE_BIG ? 256 : tile == TILE_FEW ? 32 : tile == TILE_SMALL ? 64 : 128; }
 int tile_cols(int tile) { return tile == TILE_BIG ? 256 : tile == TILE_SMALL ? 64 : 128; }
 
 // One call: sizes, layout and pointers (ops/vocab_loss.py _ARGS lists the same fields in the same order)
@@ -987,7 +991,8 @@ Plan plan(const Args& a) {
   auto tiles = [](int64_t m, int64_t n, int t) { return up(m, t) / t * (up(n, t) / t); };
   // the same for the backward products, whose sums can be cut into shares of four k-tiles
   p.dh_tile = p.nt ? TILE_BIG : TUNE(2, tiles(a.N, a.D, 128) * (vk / 4 + 1) < 256 ? TILE_SMALL : TILE_MID);
-  p.dw_tile = p.nt ? TILE_BIG : TUNE(3, tiles(cols, a.D, 128) * (nk / 4 + 1) < 256 ? TILE_SMALL : TILE_MID);
+  // a few k-tiles only: dW's writes are the work, and one stage of LDS leaves room for four workgroups on a CU
+  p.dw_tile = p.nt ? TILE_BIG : TUNE(3, tiles(cols, a.D, 128) * (nk / 4 + 1) < 256 ? TILE_SMALL : nk <= 4 ? TILE_THIN : TILE_MID);
   const int want_h = p.dh_tile == TILE_BIG ? 256 : p.dh_tile == TILE_SMALL ? 1024 : 512, want_w = p.dw_tile == TILE_SMALL ? 1024 : 512;
   const int64_t ht = tiles(a.N, a.D, tile_rows(p.dh_tile)), wt = tiles(cols, a.D, tile_rows(p.dw_tile));
   p.units = (int)(ht > want_h ? ht : want_h);
@@ -1009,13 +1014,13 @@ struct Carve {
   }
 };
 struct State {
-  Scales* sc; int *count, *rows, *lab; float* lse;
+  Scales* sc; int *count, *rows, *lab; float *ref, *inv;
   int* sidx; float *sp, *psum, *zk, *ent, *mass; unsigned short* first;
   _Float16 *wo, *ho;
   int64_t bytes;
   State(const Args& a, const Plan& p) {
     Carve c(a.state);
-    sc = c.take<Scales>(1); count = c.take<int>(1); rows = c.take<int>(a.N); lab = c.take<int>(a.N); lse = c.take<float>(a.N);
+    sc = c.take<Scales>(1); count = c.take<int>(1); rows = c.take<int>(a.N); lab = c.take<int>(a.N); ref = c.take<float>(a.N); inv = c.take<float>(a.N);
     const int64_t nk = a.K ? a.N * a.K : 0;
     sidx = c.take<int>(nk); sp = c.take<float>(nk); psum = c.take<float>(nk); zk = c.take<float>(nk);
     ent = c.take<float>(a.K ? a.N : 0); mass = c.take<float>(a.K ? a.N : 0);
@@ -1121,7 +1126,8 @@ template <class C, int OT, bool SWAP, int SEG> int launch_dw(const DwP& p, hipSt
   return (int)hipGetLastError();
 }
 template <int DT, int OT, bool SWAP, int SEG> int rows_dw(const DwP& p, int tile, hipStream_t st) {
-  return tile == TILE_SMALL ? launch_dw<Small<DT>, OT, SWAP, SEG>(p, st) : launch_dw<Mid<DT>, OT, SWAP, SEG>(p, st);
+  return tile == TILE_SMALL ? launch_dw<Small<DT>, OT, SWAP, SEG>(p, st) : tile == TILE_THIN ? launch_dw<Thin<DT>, OT, SWAP, SEG>(p, st)
+                            : launch_dw<Mid<DT>, OT, SWAP, SEG>(p, st);
 }
 template <bool SWAP> int dispatch_dw(const DwP& p, int tile, int op, bool split, bool pair, hipStream_t st) {
   const bool big = tile == TILE_BIG;
@@ -1196,7 +1202,7 @@ int forward(const Args& a, const float* f, hipStream_t st) {
   q.part = w.part; q.tz = w.tz; q.zs = q.smooth_v != 0.f ? w.zs : nullptr;
   if (const int e = scores<false>(q, p.tile, p.op, a.split, false, a.wt, st)) return e;
   CombineP c{w.part, q.zs, w.tz, s.rows, s.count, s.lab, a.K ? s.ent : nullptr, s.sp, s.zk, (int)a.K, (int)a.N, p.tiles, q.keep, f[0],
-             s.lse, a.loss};
+             s.ref, s.inv, a.loss};
   if (a.N <= 256) hipLaunchKernelGGL((combine_kernel<1>), dim3((unsigned)a.N), dim3(256), 0, st, c);
   else hipLaunchKernelGGL((combine_kernel<8>), dim3((unsigned)((a.N + 7) / 8)), dim3(256), 0, st, c);
   return (int)hipGetLastError();
@@ -1249,7 +1255,7 @@ int backward(const Args& a, const float* f, hipStream_t st) {
     ScoreP q = score_args(a, s, f);
     q.H = H; q.W = W;
     q.W.xlim = (int)a.V;
-    q.v0 = v0; q.v1 = v1; q.lse = s.lse; q.coef = w.coef; q.G = w.G; q.ldg = ldg; q.glo = glo;
+    q.v0 = v0; q.v1 = v1; q.ref = s.ref; q.inv = s.inv; q.coef = w.coef; q.G = w.G; q.ldg = ldg; q.glo = glo;
     if (p.nt && a.want_h) { q.R = rows_g; q.ldr = ldr; q.rlo = rlo; }
     if (a.want_b && !a.K) { q.colsum = w.colsum; q.ldc = a.V; }
     if (const int e = scores<true>(q, p.tile, p.op, a.split, p.pair, a.wt, st)) return e;
