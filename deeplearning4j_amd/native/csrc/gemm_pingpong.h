@@ -186,6 +186,7 @@ __device__ __forceinline__ void mainloop_pp(char* smem, const Src& src, int KT, 
   if (grp == 1) PP_BAR();                 // stagger: group 1 runs one barrier behind group 0
 
   bf16x8_t af[4][2], bf[2][2][2];
+#pragma unroll 1
   for (int t = 0; t < KT; ++t) {
     const char* cs = smem + (t & 1) * C::STAGE_BYTES;
     // ---- phase 0
@@ -222,7 +223,7 @@ __device__ __forceinline__ void mainloop_pp(char* smem, const Src& src, int KT, 
 }
 
 // ------------------------------------------------------------------------------------------------------------- smaller tiles
-// Source of gemm_trans.h's loop: a pointer per piece.
+// Source of the loop below: a pointer per piece.
 template <class C, bool TA, bool TB, int SEG> struct PtrSrc : KWalk<C, SEG> {
   typedef typename KWalk<C, SEG>::At At;
   const char* ap[C::PA];
@@ -259,6 +260,82 @@ template <class C, bool TA, bool TB, int SEG> struct PtrSrc : KWalk<C, SEG> {
   }
 };
 
+// The multi-stage loop of gemm_trans.h (mainloop_flex). fp32 operands: a matrix instruction adds four products, so a sum over K is a chain of
+// K / 4 roundings; every four k-tiles (128 k) the chain ends in a second set of accumulators, which leaves 32 + K / 128 of them.
+template <class C, class Src, bool TA, bool TB>
+__device__ __forceinline__ void mainloop_stages(char* smem, const Src& src, int KT, typename C::acc_t (&acc)[C::TM][C::TN]) {
+  static_assert(C::MF == 16 && C::STAGES > 1, "16x16 MFMA geometry");
+  constexpr bool FLUSH = C::DT == DT_F32;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wid / C::WN, wn = wid - wm * C::WN;
+  typename C::acc_t part[FLUSH ? C::TM : 1][FLUSH ? C::TN : 1];
+#pragma unroll
+  for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+      for (int e = 0; e < C::ACC; ++e) { acc[i][j][e] = 0.f; if constexpr (FLUSH) part[i][j][e] = 0.f; }
+  auto stage = [&](int t) {
+    char* sb = smem + (t % C::STAGES) * C::STAGE_BYTES;
+    const auto ts = src.tile(t);
+#pragma unroll
+    for (int i = 0; i < C::PA; ++i) glds16(src.a(i, ts), sb + (wid + i * C::NW) * 1024);
+#pragma unroll
+    for (int i = 0; i < C::PB; ++i) glds16(src.b(i, ts), sb + C::A_BYTES + (wid + i * C::NW) * 1024);
+  };
+  const int lr = lane & 15, lq = lane >> 4, sw = (lr >> 1) & 7;
+  int foff[2];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) foff[ks] = lr * 128 + (((ks * 4 + lq) ^ sw) << 4);
+  const int a_row0 = wm * (C::BM / C::WM), b_row0 = wn * (C::BN / C::WN);
+  constexpr int BLK = 16 * 128;
+#pragma unroll
+  for (int s = 0; s < C::STAGES - 1; ++s)
+    if (s < KT) stage(s);
+  for (int t = 0; t < KT; ++t) {
+    const int ahead = KT - 1 - t;                 // k-tiles issued behind this one may stay in flight
+    if (C::STAGES >= 4 && ahead >= 2) wait_vmcnt<2 * C::LPT>();
+    else if (C::STAGES >= 3 && ahead >= 1) wait_vmcnt<C::LPT>();
+    else wait_vmcnt<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the slot staged below has been read by this wave
+    __builtin_amdgcn_s_barrier();
+    if (t + C::STAGES - 1 < KT) stage(t + C::STAGES - 1);
+    const char* cs = smem + (t % C::STAGES) * C::STAGE_BYTES;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      bf16x8_t af[C::TM], bfr[C::TN];
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        if constexpr (TA) af[i] = tr_frag16<C, C::BM>(cs, a_row0 + i * 16, ks, lane);
+        else af[i] = *reinterpret_cast<const bf16x8_t*>(cs + a_row0 * 128 + i * BLK + foff[ks]);
+      }
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) {
+        if constexpr (TB) bfr[j] = tr_frag16<C, C::BN>(cs + C::A_BYTES, b_row0 + j * 16, ks, lane);
+        else bfr[j] = *reinterpret_cast<const bf16x8_t*>(cs + C::A_BYTES + b_row0 * 128 + j * BLK + foff[ks]);
+      }
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j) {
+          if constexpr (FLUSH) mma<C>(af[i], bfr[j], part[i][j]);
+          else mma<C>(af[i], bfr[j], acc[i][j]);
+        }
+    }
+    if constexpr (FLUSH)
+      if ((t & 3) == 3 || t == KT - 1) {
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+            for (int e = 0; e < C::ACC; ++e) { acc[i][j][e] += part[i][j][e]; part[i][j][e] = 0.f; }
+      }
+  }
+  __builtin_amdgcn_s_barrier();
+}
+
 // acc = init (a value per column of the lane) + k-tiles [t0, t1) of A . B^T at rows m0.., columns n0..
 template <class C, bool TA, bool TB, int SEG>
 __device__ __forceinline__ void product(char* smem, const Operand& A, const Operand& B, int m0, int n0, int K, int t0, int t1,
@@ -270,7 +347,7 @@ __device__ __forceinline__ void product(char* smem, const Operand& A, const Oper
   } else {
     PtrSrc<C, TA, TB, SEG> src;
     src.set(A, B, m0, n0, K, t0);
-    mainloop_flex<C, decltype(src), TA, TB>(smem, src, t1 - t0, acc);
+    mainloop_stages<C, decltype(src), TA, TB>(smem, src, t1 - t0, acc);
 #pragma unroll
     for (int j = 0; j < C::TN; ++j)
 #pragma unroll

@@ -270,6 +270,44 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitP p) {
   }
 }
 
+// Copies of operands whose rows do not start on 16 bytes or do not end on them: rows of Cp elements with zeros behind C. Workgroups [0, gw)
+// take W, the others the rows of H that take part, one after the other.
+struct PadP {
+  const char* W; int64_t ldw; int wr, wc; char* wo; int64_t wcp;       // elements
+  const char* H; int64_t ldh; int D; char* ho; int64_t dp;
+  const int* rows; const int* count;
+  int gw;
+};
+template <int ESZ>
+__global__ void __launch_bounds__(256) pad_kernel(const PadP p) {
+  constexpr int CH = 16 / ESZ;
+  const bool is_w = (int)blockIdx.x < p.gw;
+  const int count = *p.count;
+  if (count == 0) return;                                          // nothing reads the copies then
+  const int R = is_w ? p.wr : count, C = is_w ? p.wc : p.D;
+  const int64_t q = (is_w ? p.wcp : p.dp) / CH;
+  const int lane = threadIdx.x & 63, step = (is_w ? p.gw : gridDim.x - p.gw) * 4;
+  for (int r = (is_w ? blockIdx.x : blockIdx.x - p.gw) * 4 + (threadIdx.x >> 6); r < R; r += step) {   // a wave to a row
+    const char* row = is_w ? p.W + r * p.ldw * ESZ : p.H + p.rows[r] * p.ldh * ESZ;
+    char* out = is_w ? p.wo + r * p.wcp * ESZ : p.ho + r * p.dp * ESZ;
+    for (int64_t i = lane; i < q; i += 64) {
+      const int c = (int)i * CH;
+      const char* x = row + i * 16;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (ESZ == 4) {
+#pragma unroll
+        for (int j = 0; j < CH; ++j) v[j] = c + j < C ? reinterpret_cast<const float*>(x)[j] : 0.f;
+      } else {
+        s16x8 t = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < CH; ++j) t[j] = c + j < C ? reinterpret_cast<const short*>(x)[j] : (short)0;
+        v = __builtin_bit_cast(f32x4, t);
+      }
+      *reinterpret_cast<f32x4*>(out + i * 16) = v;
+    }
+  }
+}
+
 // the rows that take part, packed
 __global__ void __launch_bounds__(256) pack_kernel(const char* __restrict__ h, int64_t ldh_bytes, const int* __restrict__ rows,
                                                    const int* __restrict__ count, char* __restrict__ out, int64_t row_bytes, int64_t ldo_bytes) {
@@ -922,8 +960,7 @@ template <int DT> using Big = Cfg<256, 256, 2, 4, 2, 16, DT>;
 template <int DT> using Mid = Cfg<128, 128, 2, 2, 2, 16, DT>;
 template <int DT> using Few = Cfg<32, 128, 1, 4, 4, 16, DT>;
 template <int DT> using Small = Cfg<64, 64, 2, 2, 4, 16, DT>;
-template <int DT> using Thin = Cfg<128, 128, 2, 2, 1, 16, DT>;
-enum { TILE_BIG = 0, TILE_MID = 1, TILE_FEW = 2, TILE_SMALL = 3, TILE_THIN = 4 };
+enum { TILE_BIG = 0, TILE_MID = 1, TILE_FEW = 2, TILE_SMALL = 3 };
 int tile_rows(int tile) { return tile == TILE_BIG ? 256 : tile == TILE_FEW ? 32 : tile == TILE_SMALL ? 64 : 128; }
 int tile_cols(int tile) { return tile == TILE_BIG ? 256 : tile == TILE_SMALL ? 64 : 128; }
 
@@ -936,17 +973,12 @@ struct Args {
 };
 
 int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
-
-#ifdef VL_TUNE
-int g_tune[8] = {-1, -1, -1, -1, -1, -1, -1, -1};
-#define TUNE(i, v) (g_tune[i] >= 0 ? g_tune[i] : (v))
-#else
-#define TUNE(i, v) (v)
-#endif
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 struct Plan {
   int tile, dh_tile, dw_tile;            // TILE_*
   int op;                                // operand type of the products
+  bool pad_w, pad_h;                     // operands that are copied to whole 16-byte chunks (H: packed) by the forward call
   bool pair;                             // 16-bit operands: the scores' gradient in two halves
   bool nt;                               // backward products on 256 x 256 tiles from operands laid out along the sum's axis
   int bm, bn, tiles;                     // tiles of the scores
@@ -962,11 +994,11 @@ Plan plan(const Args& a) {
   const bool bits16 = p.op != DT_F32;
   const int64_t big_tiles = up(a.N, 256) / 256 * (up(a.V, 256) / 256);
   // (its operands are addressed with 32-bit offsets: rows of all of them, and H's indirect ones together, have to be short of that)
-  const bool near = up(a.N, 256) * 2 < BUF_LD && up(a.V, 256) * 2 < BUF_LD && a.ldh * 4 < BUF_LD && a.ldw * 4 < BUF_LD && (a.split || a.N * a.ldh * 2 < BUF_SPAN);
+  const bool near = up(a.N, 256) * 2 < BUF_LD && up(a.V, 256) * 2 < BUF_LD && a.ldh * 4 < BUF_LD && a.ldw * 4 < BUF_LD && up(a.D, 8) * 4 < BUF_LD && (a.split || a.N * a.ldh * 2 < BUF_SPAN);
   const int64_t mid_tiles = up(a.N, 128) / 128 * (up(a.V, 128) / 128);
   // 256 x 256 tiles once they cover two thirds of the 256 CUs; 32 rows where few rows meet a large vocabulary (W streams through, a tile per
   // CU at 32768 words); 64 x 64 tiles with four stages where 128 x 128 ones would leave CUs idle (the time is a chain of k-tiles then)
-  p.tile = TUNE(0, bits16 && big_tiles >= 176 && a.N > 128 && near ? TILE_BIG : a.N <= 32 && a.V >= 16384 ? TILE_FEW : mid_tiles < 176 ? TILE_SMALL : TILE_MID);
+  p.tile = bits16 && big_tiles >= 176 && a.N > 128 && near ? TILE_BIG : a.N <= 32 && a.V >= 16384 ? TILE_FEW : mid_tiles < 176 ? TILE_SMALL : TILE_MID;
   if (a.split && p.tile == TILE_FEW) p.tile = TILE_MID;
   if (!bits16 && p.tile == TILE_BIG) p.tile = TILE_MID;
   p.bm = tile_rows(p.tile);
@@ -976,23 +1008,25 @@ Plan plan(const Args& a) {
   p.vp = up(a.V, 64);
   p.dp = up(a.D, 8);
   p.wrows = a.wt ? a.D : a.V;
+  const int64_t ch = a.dt == DT_F32 ? 4 : 8, wc = a.wt ? a.V : a.D;
+  p.pad_w = !a.split && (wc % ch || a.ldw % ch || !aligned16(a.W));
+  p.pad_h = !a.split && (a.D % ch || a.ldh % ch || !aligned16(a.H));
   p.wcp = up(a.wt ? a.V : a.D, 8);
   const int64_t esz = a.dt == DT_F32 ? 4 : 2;                    // halves take as much as fp32
-  const int64_t most = TUNE(4, 512) * (int64_t)(1 << 20) / (p.np * esz) / 256 * 256;
+  const int64_t most = ((int64_t)512 << 20) / (p.np * esz) / 256 * 256;
   p.pieces = (int)(most >= 256 ? (a.V + most - 1) / most : up(a.V, 256) / 256);
   p.step = (int)up((a.V + p.pieces - 1) / p.pieces, 256);
   p.pieces = (int)((a.V + p.step - 1) / p.step);
   p.gcols = up(a.V < p.step ? a.V : p.step, 256);
-  p.nt = p.tile == TILE_BIG && TUNE(1, a.N >= 512 && a.D >= 256);
+  p.nt = p.tile == TILE_BIG && a.N >= 512 && a.D >= 256;
   p.pair = bits16 && !a.split && a.N <= 256;
   const int seg = a.split ? 3 : p.pair ? 2 : 1, bk = bits16 ? 64 : 32;
   const int64_t vk = seg * (up(p.step, bk) / bk), nk = seg * (up(a.N, bk) / bk);   // k-tiles of the two products' sums
   const int64_t cols = p.gcols < a.V ? p.gcols : a.V;
   auto tiles = [](int64_t m, int64_t n, int t) { return up(m, t) / t * (up(n, t) / t); };
   // the same for the backward products, whose sums can be cut into shares of four k-tiles
-  p.dh_tile = p.nt ? TILE_BIG : TUNE(2, tiles(a.N, a.D, 128) * (vk / 4 + 1) < 256 ? TILE_SMALL : TILE_MID);
-  // a few k-tiles only: dW's writes are the work, and one stage of LDS leaves room for four workgroups on a CU
-  p.dw_tile = p.nt ? TILE_BIG : TUNE(3, tiles(cols, a.D, 128) * (nk / 4 + 1) < 256 ? TILE_SMALL : nk <= 4 ? TILE_THIN : TILE_MID);
+  p.dh_tile = p.nt ? TILE_BIG : tiles(a.N, a.D, 128) * (vk / 4 + 1) < 256 ? TILE_SMALL : TILE_MID;
+  p.dw_tile = p.nt ? TILE_BIG : tiles(cols, a.D, 128) * (nk / 4 + 1) < 256 ? TILE_SMALL : TILE_MID;
   const int want_h = p.dh_tile == TILE_BIG ? 256 : p.dh_tile == TILE_SMALL ? 1024 : 512, want_w = p.dw_tile == TILE_SMALL ? 1024 : 512;
   const int64_t ht = tiles(a.N, a.D, tile_rows(p.dh_tile)), wt = tiles(cols, a.D, tile_rows(p.dw_tile));
   p.units = (int)(ht > want_h ? ht : want_h);
@@ -1016,7 +1050,7 @@ struct Carve {
 struct State {
   Scales* sc; int *count, *rows, *lab; float *ref, *inv;
   int* sidx; float *sp, *psum, *zk, *ent, *mass; unsigned short* first;
-  _Float16 *wo, *ho;
+  char *wo, *ho;
   int64_t bytes;
   State(const Args& a, const Plan& p) {
     Carve c(a.state);
@@ -1025,8 +1059,9 @@ struct State {
     sidx = c.take<int>(nk); sp = c.take<float>(nk); psum = c.take<float>(nk); zk = c.take<float>(nk);
     ent = c.take<float>(a.K ? a.N : 0); mass = c.take<float>(a.K ? a.N : 0);
     first = c.take<unsigned short>(a.K ? (int64_t)(p.tiles + 1) * a.N : 0);
-    wo = c.take<_Float16>(a.split ? 2 * p.wrows * p.wcp : 0);
-    ho = c.take<_Float16>(a.split ? 2 * p.np * p.dp : 0);
+    const int64_t esz = a.dt == DT_F32 ? 4 : 2;                    // (two halves take as much as an fp32 value)
+    wo = c.take<char>(a.split || p.pad_w ? p.wrows * p.wcp * esz : 0);
+    ho = c.take<char>(a.split || p.pad_h ? p.np * p.dp * esz : 0);
     bytes = c.at;
   }
 };
@@ -1043,7 +1078,7 @@ struct Work {
     const int64_t esz = a.dt == DT_F32 ? 4 : 2;
     coef = c.take<float>(a.N); G = c.take<char>(p.np * p.gcols * esz * (p.nt || p.pair ? 2 : 1));
     colsum = c.take<float>(a.want_b && !a.K ? (a.N + p.bm - 1) / p.bm * a.V : 0);
-    packed = c.take<char>(a.want_w && !a.split && !p.nt ? a.N * p.dp * esz : 0);
+    packed = c.take<char>(a.want_w && !a.split && !p.nt && !p.pad_h ? a.N * p.dp * esz : 0);
     ht = c.take<uint16_t>(a.want_w && p.nt ? a.D * p.np * (a.split ? 2 : 1) : 0);
     wtr = c.take<uint16_t>(a.want_h && p.nt && !a.wt ? a.D * p.vp * (a.split ? 2 : 1) : 0);
     const int64_t ht = tile_rows(p.dh_tile), wt = tile_rows(p.dw_tile), cols = p.gcols < a.V ? p.gcols : a.V;
@@ -1052,8 +1087,6 @@ struct Work {
     bwd = c.at;
   }
 };
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 #define VL_CHECK() do { const int e_ = (int)hipGetLastError(); if (e_) return e_; } while (0)
 
@@ -1126,8 +1159,7 @@ template <class C, int OT, bool SWAP, int SEG> int launch_dw(const DwP& p, hipSt
   return (int)hipGetLastError();
 }
 template <int DT, int OT, bool SWAP, int SEG> int rows_dw(const DwP& p, int tile, hipStream_t st) {
-  return tile == TILE_SMALL ? launch_dw<Small<DT>, OT, SWAP, SEG>(p, st) : tile == TILE_THIN ? launch_dw<Thin<DT>, OT, SWAP, SEG>(p, st)
-                            : launch_dw<Mid<DT>, OT, SWAP, SEG>(p, st);
+  return tile == TILE_SMALL ? launch_dw<Small<DT>, OT, SWAP, SEG>(p, st) : launch_dw<Mid<DT>, OT, SWAP, SEG>(p, st);
 }
 template <bool SWAP> int dispatch_dw(const DwP& p, int tile, int op, bool split, bool pair, hipStream_t st) {
   const bool big = tile == TILE_BIG;
@@ -1144,9 +1176,7 @@ int check(const Args& a, bool bwd) {
   if (a.dt < 0 || a.dt > 2 || a.bdt < 0 || a.bdt > 2 || (a.split && a.dt != DT_F32) || a.K < 0 || a.K > KMAX) return -2;
   if (!a.H || !a.W || !a.state || !a.ws || !a.loss || !aligned16(a.state) || !aligned16(a.ws)) return -2;
   if (a.K ? !a.idx || !a.t || a.tdt < 0 || a.tdt > 2 : !a.labels) return -2;
-  const int64_t ch = a.dt == DT_F32 ? 4 : 8, wc = a.wt ? a.V : a.D;
-  if (a.split ? a.ldh < a.D || a.ldw < wc                        // halves are made from any row stride
-              : a.ldh % ch || a.ldw % ch || a.ldh < up(a.D, ch) || a.ldw < up(wc, ch) || !aligned16(a.H) || !aligned16(a.W)) return -2;
+  if (a.ldh < a.D || a.ldw < (a.wt ? a.V : a.D)) return -2;
   if (bwd && (!a.dloss || (a.want_h && !a.dh) || (a.want_w && !a.dw) || (a.want_b && (!a.db || !a.bias)))) return -2;
   return 0;
 }
@@ -1157,8 +1187,8 @@ void operands(const Args& a, const Plan& p, const State& s, Operand& H, Operand&
     H = Operand{(const char*)s.ho, p.dp * 2, p.np * p.dp * 2, 0, nullptr};
     W = Operand{(const char*)s.wo, p.wcp * 2, p.wrows * p.wcp * 2, 0, nullptr};
   } else {
-    H = Operand{(const char*)a.H, a.ldh * esz, 0, 0, s.rows};
-    W = Operand{(const char*)a.W, a.ldw * esz, 0, 0, nullptr};
+    H = p.pad_h ? Operand{s.ho, p.dp * esz, 0, 0, nullptr} : Operand{(const char*)a.H, a.ldh * esz, 0, 0, s.rows};
+    W = p.pad_w ? Operand{s.wo, p.wcp * esz, 0, 0, nullptr} : Operand{(const char*)a.W, a.ldw * esz, 0, 0, nullptr};
   }
 }
 
@@ -1191,8 +1221,16 @@ int forward(const Args& a, const float* f, hipStream_t st) {
     hipLaunchKernelGGL(amax_kernel, dim3(AMAX_W + AMAX_H), dim3(256), 0, st, (const float*)a.W, a.ldw, wr, wc, (const float*)a.H, a.ldh, (int)a.D, s.rows,
                        s.count, w.amax);
     VL_CHECK();
-    SplitP q{(const float*)a.W, a.ldw, wr, wc, (int)p.wcp, s.wo, (const float*)a.H, a.ldh, (int)a.D, (int)p.dp, s.ho, (int)p.np, s.rows, s.count, w.amax, s.sc, 2048};
+    SplitP q{(const float*)a.W, a.ldw, wr, wc, (int)p.wcp, (_Float16*)s.wo, (const float*)a.H, a.ldh, (int)a.D, (int)p.dp, (_Float16*)s.ho, (int)p.np, s.rows, s.count, w.amax, s.sc, 2048};
     hipLaunchKernelGGL(split_kernel, dim3(2048 + 256), dim3(256), 0, st, q);
+    VL_CHECK();
+  }
+  if (p.pad_w || p.pad_h) {
+    const PadP q{(const char*)a.W, a.ldw, (int)p.wrows, (int)(a.wt ? a.V : a.D), s.wo, p.wcp, (const char*)a.H, a.ldh, (int)a.D, s.ho, p.dp, s.rows, s.count,
+                 p.pad_w ? 1024 : 0};
+    const dim3 grid(q.gw + (p.pad_h ? 256 : 0));
+    if (a.dt == DT_F32) hipLaunchKernelGGL((pad_kernel<4>), grid, dim3(256), 0, st, q);
+    else hipLaunchKernelGGL((pad_kernel<2>), grid, dim3(256), 0, st, q);
     VL_CHECK();
   }
   ScoreP q = score_args(a, s, f);
@@ -1219,7 +1257,7 @@ int backward(const Args& a, const float* f, hipStream_t st) {
   operands(a, p, s, H, W);
   Operand packed = H;
   const int64_t rb = up(a.D, 16 / esz) * esz;
-  const bool pack = a.want_w && !a.split && !p.nt;
+  const bool pack = a.want_w && !a.split && !p.nt && !p.pad_h;
   if (a.N <= 1024) {
     hipLaunchKernelGGL(prepare_kernel, dim3((unsigned)a.N), dim3(256), 0, st, a.dloss, s.rows, s.count, f[0], top, w.coef, s.sc, (const char*)a.H, a.ldh * esz,
                        pack ? w.packed : nullptr, rb, p.dp * esz);
@@ -1298,10 +1336,6 @@ int backward(const Args& a, const float* f, hipStream_t st) {
 }
 
 }  // namespace
-
-#ifdef VL_TUNE
-DL4J_API void dl4j_vl_tune(int i, int v) { g_tune[i] = v; }
-#endif
 
 // bytes of the state, the forward workspace and the backward workspace
 DL4J_API void dl4j_linear_loss_bytes(const int64_t* args, int64_t* out) {
