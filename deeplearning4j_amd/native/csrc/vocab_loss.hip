@@ -216,12 +216,12 @@ __global__ void __launch_bounds__(256) amax_kernel(const float* __restrict__ W, 
   if (threadIdx.x == 0) out[blockIdx.x] = m;
 }
 
-// a power of two that puts m into [2^13, 2^14)
-__device__ __forceinline__ float scale_for(float m) {
-  if (!(m > 0.f)) return 1.f;
+// the power of two that puts m into [2^13, 2^14)
+__device__ __forceinline__ int scale_for(float m) {
+  if (!(m > 0.f)) return 0;
   int e;
   frexpf(m, &e);
-  return ldexpf(1.f, min(max(14 - e, -100), 100));
+  return max(14 - e, -114);
 }
 
 __device__ __forceinline__ void halves(float v, _Float16& hi, _Float16& lo) {
@@ -243,7 +243,10 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitP p) {
   float mw = 0.f, mh = 0.f;
   for (int i = threadIdx.x; i < AMAX_W; i += 256) mw = fmaxf(mw, p.amax[i]);
   for (int i = threadIdx.x; i < AMAX_H; i += 256) mh = fmaxf(mh, p.amax[AMAX_W + i]);
-  const float sw = scale_for(block_max(mw, red)), sh = scale_for(block_max(mh, red));
+  // both together 2^100 at most, since a bias enters the accumulators times both: below that the smaller operand's low bits go first
+  const int ew = scale_for(block_max(mw, red)), eh = scale_for(block_max(mh, red));
+  const bool cap = ew + eh > 100;
+  const float sw = ldexpf(1.f, cap ? min(ew, max(50, 100 - eh)) : ew), sh = ldexpf(1.f, cap ? min(eh, max(50, 100 - ew)) : eh);
   if (blockIdx.x == 0 && threadIdx.x == 0) { p.sc->h = sh; p.sc->w = sw; p.sc->z = 1.f / sh / sw; }
   const bool is_w = (int)blockIdx.x < p.gw;
   const int c = *p.count;
@@ -1174,8 +1177,8 @@ template <bool SWAP> int dispatch_dw(const DwP& p, int tile, int op, bool split,
 int check(const Args& a, bool bwd) {
   if (a.N <= 0 || a.N > 0x7fffffff - 512 || a.D <= 0 || a.D > 0x7fffffff - 512 || a.V <= 0 || a.V > 0x7fffffff - 512) return -2;
   if (a.dt < 0 || a.dt > 2 || a.bdt < 0 || a.bdt > 2 || (a.split && a.dt != DT_F32) || a.K < 0 || a.K > KMAX) return -2;
-  if (!a.H || !a.W || !a.state || !a.ws || !a.loss || !aligned16(a.state) || !aligned16(a.ws)) return -2;
-  if (a.K ? !a.idx || !a.t || a.tdt < 0 || a.tdt > 2 : !a.labels) return -2;
+  if (!a.H || !a.W || !a.state || !a.ws || !aligned16(a.state) || !aligned16(a.ws)) return -2;
+  if (!bwd && (!a.loss || (a.K ? !a.idx || !a.t || a.tdt < 0 || a.tdt > 2 : !a.labels))) return -2;
   if (a.ldh < a.D || a.ldw < (a.wt ? a.V : a.D)) return -2;
   if (bwd && (!a.dloss || (a.want_h && !a.dh) || (a.want_w && !a.dw) || (a.want_b && (!a.db || !a.bias)))) return -2;
   return 0;
@@ -1204,6 +1207,7 @@ ScoreP score_args(const Args& a, const State& s, const float* f) {
 
 int forward(const Args& a, const float* f, hipStream_t st) {
   if (const int e = check(a, false)) return e;
+  if (!(f[0] > 0.f)) return -2;
   const Plan p = plan(a);
   const State s(a, p);
   const Work w(a, p);

@@ -216,7 +216,7 @@ class _LinearLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weights, bias, first, second, ignore, smoothing, temperature):
         loss, ((h, w, state), call) = _linear_forward(hidden, weights, bias, first, second, ignore, smoothing, temperature, ctx.needs_input_grad[:3])
-        ctx.save_for_backward(h, w, bias, first, second, loss, state)
+        ctx.save_for_backward(h, w, bias, state)                       # (labels and teacher are in the state: their tensors may change)
         ctx.call, ctx.shape = call, hidden.shape
         return loss
 
@@ -232,7 +232,7 @@ class _LinearLoss(torch.autograd.Function):
 
 
 def _linear_backward(ctx, dloss):
-    h, w, bias = ctx.saved_tensors[:3]
+    h, w, bias, state = ctx.saved_tensors
     a, f, size, dv = ctx.call
     a = _Block.from_buffer_copy(a)                                      # (a graph kept alive may be walked from two threads)
     dev = h.device
@@ -242,7 +242,7 @@ def _linear_backward(ctx, dloss):
     dw = torch.empty(w.shape, dtype=h.dtype, device=dev) if want_w else None
     db = torch.empty_like(bias) if want_b else None
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    for name, t in (("ws", ws), ("dloss", g), ("dh", dh), ("dw", dw), ("db", db)):
+    for name, t in (("state", state), ("ws", ws), ("dloss", g), ("dh", dh), ("dw", dw), ("db", db)):
         if t is not None:
             a[_AT[name]] = t.data_ptr()
     _launch(_lib().dl4j_linear_loss_bwd, "linear_loss_bwd", dev, a, f)

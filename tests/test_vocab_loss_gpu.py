@@ -438,3 +438,61 @@ def test_refusals():
                  lambda: VL.linear_topk_distillation(h, w, torch.zeros(4, 1025, dtype=torch.int64, device=DEV), torch.zeros(4, 1025, device=DEV))):
         with pytest.raises(ND4JIllegalArgumentException):
             call()
+
+
+@pytest.mark.parametrize("layout", ["vd", "dv"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("n", [1, 17, 32])
+def test_few_rows_against_a_wide_vocabulary(n, dtype, layout):
+    d, v = 137, 16399
+    h, w, b, dl = _linear_inputs(n, d, v, dtype, n, True, layout)
+    y = _labels(n, v, 0.2, n)
+    _both(lambda h, w, b: VL.linear_cross_entropy(h, w, y, b), lambda h, w, b: VL.linear_cross_entropy_reference(h, w, y, b), [h, w, b], dl)
+    idx, t = _teacher(n, v, 33, n)
+    _both(lambda h, w, b: VL.linear_topk_distillation(h, w, idx, t, b, 1.5),
+          lambda h, w, b: VL.linear_topk_distillation_reference(h, w, idx, t, b, 1.5), [h, w, b], dl)
+
+
+def test_one_row_without_a_row_axis():
+    h, w, b, dl = _linear_inputs(1, 72, 300, torch.float32, 5, True, "vd")
+    h, dl, y = h[0], dl[0], torch.tensor(7, device=DEV)
+    idx, t = torch.tensor([3, 299, -1], device=DEV), torch.tensor([0.5, 1.5, 9.0], device=DEV)
+    _both(lambda h, w, b: VL.linear_cross_entropy(h, w, y, b), lambda h, w, b: VL.linear_cross_entropy_reference(h, w, y, b), [h, w, b], dl)
+    _both(lambda h, w, b: VL.linear_topk_distillation(h, w, idx, t, b), lambda h, w, b: VL.linear_topk_distillation_reference(h, w, idx, t, b), [h, w, b], dl)
+    _both(lambda z: VL.topk_distillation(z, idx, t), lambda z: VL.topk_distillation_reference(z, idx, t), [b], dl, names=("logits",))
+
+
+@pytest.mark.parametrize("exponent", [-70, -110])
+def test_tiny_hidden_states_beside_a_large_bias(exponent):
+    """fp32 operands in scaled halves: the bias, up to some 10^5, is scaled with them."""
+    n, d, v = 600, 512, 1000
+    h, w, b, dl = _linear_inputs(n, d, v, torch.float32, 4, True, "vd")
+    h, b = h * 2.0 ** exponent, b * 3e4
+    y = b.argsort(descending=True)[:3].repeat(n // 3)
+    loss, grads = _grads(lambda h, w, b: VL.linear_cross_entropy(h, w, y, b, label_smoothing=0.1), [h, w, b], dl)
+    want, wgrads = _grads(lambda h, w, b: VL.linear_cross_entropy_reference(h, w, y, b, label_smoothing=0.1), [t.double() for t in (h, w, b)], dl)
+    _losses_close(loss, want)
+    for k, (a, e) in enumerate(zip(grads, wgrads)):
+        if k == 1 and exponent < -100:                                  # products of the hidden states alone: 2^-24 of the scaled range is gone
+            assert torch.isfinite(a).all()
+        else:
+            _close(a, e, LIMIT[torch.float32], ("hidden", "weights", "bias")[k])
+
+
+def test_the_loss_and_the_labels_may_be_changed_before_the_backward_pass():
+    h, w, b, dl = _linear_inputs(50, 64, 500, torch.bfloat16, 6, True, "vd")
+    y = _labels(50, 500, 0.2, 6)
+    idx, t = _teacher(50, 500, 9, 6)
+    for fn, held in ((lambda *p: VL.linear_cross_entropy(p[0], p[1], y, p[2]), (y,)),
+                     (lambda *p: VL.linear_topk_distillation(p[0], p[1], idx, t, p[2]), (idx, t))):
+        want = _grads(fn, [h, w, b], dl * 0.5)[1]
+        leaves = [x.detach().requires_grad_() for x in (h, w, b)]
+        loss = fn(*leaves)
+        loss.mul_(0.5)
+        kept = [x.clone() for x in held]
+        for x in held:
+            x.zero_()
+        got = torch.autograd.grad(loss, leaves, dl)
+        for x, k in zip(held, kept):
+            x.copy_(k)
+        assert all(torch.equal(a, e) for a, e in zip(got, want))
