@@ -19,7 +19,7 @@
 //   K-contiguous operand   the core's image: 256 rows x 128 bytes, half-tile h = rows g * 128 + h * 64 + 0..63 (A) / cols wn * 64 + h * 32 + 0..31 (B)
 //   K-major operand        each half-tile is an image of its own, [64 k][128 x] with a pitch of 256 bytes: 16 KiB, two 1-KiB pieces per
 //                          wave like the other, so the counted waits hold unchanged; the fragments come from transposing LDS reads
-//                          (8192 x 2048 x 16384: 25 to 40 % longer than K-contiguous ones)
+//                          (one such operand: up to 20 % longer than K-contiguous ones, at 8192 x 2048 x 32768; two: 40 %)
 //
 // A product of fp32 operands runs on the 16-bit matrix cores as three products of halves, a = a1 + a2 with a1 = fp16(a), a2 = fp16(a - a1)
 // (operands scaled by a power of two so that the largest is below 2^14):  a . b = a1 b1 + a1 b2 + a2 b1, what is left out is 2^-24 of |a||b|.

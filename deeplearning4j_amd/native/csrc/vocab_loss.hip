@@ -69,31 +69,42 @@ struct Scales {
 // ------------------------------------------------------------------------------------------------------------------------ rows
 // rows[0 .. count) = rows that take part, in order, lab their labels (-1: outside the vocabulary, or none); rows[count .. N) = the others;
 // loss of the others = 0.
-// One workgroup: a scan of N flags, 1024 at a time.
+// One workgroup: a scan of N flags, 1024 at a time behind the loads of 8192.
+constexpr int SCAN = 8;
 __global__ void __launch_bounds__(1024) rows_kernel(const void* __restrict__ labels, int lab64, int64_t ignore, const float* __restrict__ mass, int N,
                                                     int V, int* __restrict__ rows, int* __restrict__ lab, int* __restrict__ count,
                                                     Scales* __restrict__ sc, float* __restrict__ loss) {
-  __shared__ int wsum[16];
+  __shared__ int wsum[2][16];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   int done = 0;
-  for (int64_t base = 0; base < N; base += 1024) {
-    const int64_t n = base + tid;
-    bool ok = false;
-    int64_t y = -1;
-    if (n < N && labels) { y = load_index(labels, n, lab64); ok = y != ignore; }
-    else if (n < N) ok = mass[n] != 0.f;
-    const unsigned long long b = __ballot(ok);
-    if (lane == 0) wsum[wid] = __popcll(b);
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int w = 0; w < 16; ++w) { if (w < wid) before += wsum[w]; all += wsum[w]; }
-    const int at = done + before + __popcll(b & ((1ull << lane) - 1));
-    if (n < N) {
-      if (ok) { rows[at] = (int)n; lab[at] = y >= 0 && y < V ? (int)y : -1; }
-      else { rows[N - 1 - (n - at)] = (int)n; loss[n] = 0.f; }   // n - at rows before this one do not take part
+  for (int64_t base = 0; base < N; base += 1024 * SCAN) {
+    int y[SCAN];                                                     // label; -1: none inside the vocabulary; -2: takes no part
+#pragma unroll
+    for (int j = 0; j < SCAN; ++j) {
+      const int64_t n = base + j * 1024 + tid;
+      y[j] = -2;
+      if (n < N && labels) {
+        const int64_t l = load_index(labels, n, lab64);
+        if (l != ignore) y[j] = l >= 0 && l < V ? (int)l : -1;
+      } else if (n < N && mass[n] != 0.f) y[j] = -1;
     }
-    done += all;
-    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < SCAN; ++j) {
+      const int64_t n = base + j * 1024 + tid;
+      if (n - tid >= N) break;
+      const unsigned long long b = __ballot(y[j] != -2);
+      if (lane == 0) wsum[j & 1][wid] = __popcll(b);
+      __syncthreads();                                               // (the other array was read in front of the barrier before this one)
+      int before = 0, all = 0;
+#pragma unroll
+      for (int w = 0; w < 16; ++w) { const int c = wsum[j & 1][w]; if (w < wid) before += c; all += c; }
+      const int at = done + before + __popcll(b & ((1ull << lane) - 1));
+      if (n < N) {
+        if (y[j] != -2) { rows[at] = (int)n; lab[at] = y[j]; }
+        else { rows[N - 1 - (n - at)] = (int)n; loss[n] = 0.f; }   // n - at rows before this one do not take part
+      }
+      done += all;
+    }
   }
   if (tid == 0) { *count = done; *sc = Scales{1.f, 1.f, 1.f, 1.f, 1.f, 1.f}; }
 }
@@ -321,15 +332,17 @@ __global__ void __launch_bounds__(256) pack_kernel(const char* __restrict__ h, i
 }
 
 // out[c][r] = in[row r][c] of 16-bit values, R x C, 64 x 64 at a time through LDS; blockIdx.z: the halves of a pair. `count`: R on the device,
-// and `rows` the row of position r (both or none); positions from R to the next multiple of 64 become zeros.
+// and `rows` the row of position r (both or none); positions from R to the next multiple of 64 become zeros. `gate`: only where *gate >= least.
 struct TransposeP {
   const uint16_t* in; int64_t ldi, half_in;
   uint16_t* out; int64_t ldo, half_out;
   int R, C;
   const int* count; const int* rows;
+  const int* gate; int least;
 };
 __global__ void __launch_bounds__(256) transpose_kernel(const TransposeP p) {
   __shared__ uint16_t tile[64][64 + 2];
+  if (p.gate && *p.gate < p.least) return;
   const int R = p.count ? *p.count : p.R, r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
   if (r0 >= R) return;
   const uint16_t* in = p.in + blockIdx.z * p.half_in;
@@ -756,17 +769,24 @@ __global__ void __launch_bounds__(1024) coef_kernel(const float* __restrict__ dl
                                                     float T, float top, float* __restrict__ coef, Scales* __restrict__ sc) {
   __shared__ float red[16];
   const int c = *count;
-  float s = 1.f;
+  float s = 1.f, v[8];                                             // the first 8192 rows stay in registers
+#pragma unroll
+  for (int j = 0; j < 8; ++j) { const int m = j * 1024 + threadIdx.x; v[j] = m < c ? dloss[rows[m]] * T : 0.f; }
   if (top > 0.f) {
     float mx = 0.f;
-    for (int m = threadIdx.x; m < c; m += 1024) {
-      const float v = fabsf(dloss[rows[m]] * T);
-      if (v < __builtin_inff()) mx = fmaxf(mx, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (fabsf(v[j]) < __builtin_inff()) mx = fmaxf(mx, fabsf(v[j]));
+    for (int m = 8192 + threadIdx.x; m < c; m += 1024) {
+      const float x = fabsf(dloss[rows[m]] * T);
+      if (x < __builtin_inff()) mx = fmaxf(mx, x);
     }
     mx = block_max(mx, red);
     if (mx > 0.f) s = fminf(top / mx, 1e37f);
   }
-  for (int m = threadIdx.x; m < c; m += 1024) coef[m] = dloss[rows[m]] * T * s;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) { const int m = j * 1024 + threadIdx.x; if (m < c) coef[m] = v[j] * s; }
+  for (int m = 8192 + threadIdx.x; m < c; m += 1024) coef[m] = dloss[rows[m]] * T * s;
   if (threadIdx.x == 0) { sc->db = 1.f / s; sc->dh = 1.f / s / sc->w; sc->dw = 1.f / s / sc->h; }
 }
 
@@ -813,8 +833,11 @@ __global__ void __launch_bounds__(256) bias_rows_kernel(const char* __restrict__
 
 // dh: unit u of the grid owns output tile u % tiles and share u / tiles of the piece's columns; its fp32 tile lives in slab u and is added
 // to by the following pieces. Which unit owns what depends on the number of rows alone, so the sum's order is fixed.
+//
+// Large tile, W by rows ([V, D]): read as it is (K-major, transposing LDS reads), or transposed first where `many` rows pay for that.
 struct DhP {
-  Operand G, W;
+  Operand G, W, WT;
+  int many;
   const int* count;
   int D, vc, units, most, accum;         // most: shares at most (each has some k-tiles to work on)
   float* slab;
@@ -852,7 +875,8 @@ __global__ void __launch_bounds__(C::NT) dh_kernel(const DhP p) {
   const int ktiles = k_tiles<C, SEG>(p.vc), per = (ktiles + shares - 1) / shares;
   const int k0 = min(ktiles, share * per), k1 = min(ktiles, k0 + per);
   typename C::acc_t acc[C::TM][C::TN];
-  product<C, TA, TB, SEG>(smem, p.G, p.W, mt * C::BM, nt * C::BN, p.vc, k0, k1, acc);
+  if (is_pp<C>() && TB && count >= p.many) product<C, TA, false, SEG>(smem, p.G, p.WT, mt * C::BM, nt * C::BN, p.vc, k0, k1, acc);
+  else product<C, TA, TB, SEG>(smem, p.G, p.W, mt * C::BM, nt * C::BN, p.vc, k0, k1, acc);
   to_slab<C>(p.slab + (int64_t)u * C::BM * C::BN, acc, p.accum);
 }
 
@@ -984,6 +1008,7 @@ struct Plan {
   bool pad_w, pad_h;                     // operands that are copied to whole 16-byte chunks (H: packed) by the forward call
   bool pair;                             // 16-bit operands: the scores' gradient in two halves
   bool nt;                               // backward products on 256 x 256 tiles from operands laid out along the sum's axis
+  bool wtr; int many;                    // dh: W is transposed first, for calls of `many` rows that take part
   int bm, bn, tiles;                     // tiles of the scores
   int64_t np, dp, wcp, wrows, vp;           // padded rows / columns of the packed H and of the halves of W
   int pieces, step;
@@ -1022,6 +1047,10 @@ Plan plan(const Args& a) {
   p.pieces = (int)((a.V + p.step - 1) / p.step);
   p.gcols = up(a.V < p.step ? a.V : p.step, 256);
   p.nt = p.tile == TILE_BIG && a.N >= 512 && a.D >= 256;
+  // W as it lies, through transposing LDS reads, against W transposed first: 2100 rows x 1000 of 50001 words 231 us against 207 + 98; 4096 x 1024 of
+  // 32000: 242 and 226 + 47; 8192 x 2048 of 65536: 1820 and 1520 + 188. The transpose costs the same for any number of rows.
+  p.many = 6144;
+  p.wtr = a.want_h && p.nt && !a.wt && a.N >= p.many;
   p.pair = bits16 && !a.split && a.N <= 256;
   const int seg = a.split ? 3 : p.pair ? 2 : 1, bk = bits16 ? 64 : 32;
   const int64_t vk = seg * (up(p.step, bk) / bk), nk = seg * (up(a.N, bk) / bk);   // k-tiles of the two products' sums
@@ -1083,7 +1112,7 @@ struct Work {
     colsum = c.take<float>(a.want_b && !a.K ? (a.N + p.bm - 1) / p.bm * a.V : 0);
     packed = c.take<char>(a.want_w && !a.split && !p.nt && !p.pad_h ? a.N * p.dp * esz : 0);
     ht = c.take<uint16_t>(a.want_w && p.nt ? a.D * p.np * (a.split ? 2 : 1) : 0);
-    wtr = c.take<uint16_t>(a.want_h && p.nt && !a.wt ? a.D * p.vp * (a.split ? 2 : 1) : 0);
+    wtr = c.take<uint16_t>(p.wtr ? a.D * p.vp * (a.split ? 2 : 1) : 0);
     const int64_t ht = tile_rows(p.dh_tile), wt = tile_rows(p.dw_tile), cols = p.gcols < a.V ? p.gcols : a.V;
     dh_slab = c.take<float>(a.want_h ? p.units * ht * ht : 0);
     dw_slab = c.take<float>(a.want_w && p.shares > 1 ? up(cols, wt) * up(a.D, wt) * p.shares : 0);
@@ -1132,15 +1161,16 @@ template <class C, bool TA, bool TB, int SEG> int launch_dh(const DhP& p, hipStr
   hipLaunchKernelGGL((dh_kernel<C, TA, TB, SEG>), dim3(p.units), dim3(C::NT), LDS, st, p);
   return (int)hipGetLastError();
 }
-// 256 x 256: both operands K-contiguous (p.nt); smaller tiles: the gradient and the [V, D] table are walked row by row
+// 256 x 256: the gradient K-contiguous (p.nt); smaller tiles: the gradient and the [V, D] table are walked row by row
 template <int DT, int SEG> int rows_dh(const DhP& p, int tile, bool wt, hipStream_t st) {
   if (tile == TILE_SMALL) return wt ? launch_dh<Small<DT>, true, false, SEG>(p, st) : launch_dh<Small<DT>, true, true, SEG>(p, st);
   return wt ? launch_dh<Mid<DT>, true, false, SEG>(p, st) : launch_dh<Mid<DT>, true, true, SEG>(p, st);
 }
+template <bool TB> int big_dh(const DhP& p, int op, bool split, hipStream_t st) {
+  return split ? launch_dh<Big<DT_F16>, false, TB, 3>(p, st) : op == DT_BF16 ? launch_dh<Big<DT_BF16>, false, TB, 1>(p, st) : launch_dh<Big<DT_F16>, false, TB, 1>(p, st);
+}
 int dispatch_dh(const DhP& p, int tile, int op, bool split, bool pair, bool wt, hipStream_t st) {
-  if (tile == TILE_BIG)
-    return split ? launch_dh<Big<DT_F16>, false, false, 3>(p, st) : op == DT_BF16 ? launch_dh<Big<DT_BF16>, false, false, 1>(p, st)
-                                                                                 : launch_dh<Big<DT_F16>, false, false, 1>(p, st);
+  if (tile == TILE_BIG) return wt ? big_dh<false>(p, op, split, st) : big_dh<true>(p, op, split, st);
   if (split) return rows_dh<DT_F16, 3>(p, tile, wt, st);
   if (op == DT_F32) return rows_dh<DT_F32, 1>(p, tile, wt, st);
   if (op == DT_BF16) return pair ? rows_dh<DT_BF16, 2>(p, tile, wt, st) : rows_dh<DT_BF16, 1>(p, tile, wt, st);
@@ -1276,18 +1306,18 @@ int backward(const Args& a, const float* f, hipStream_t st) {
   }
   if (pack) packed = Operand{w.packed, p.dp * esz, 0, 0, nullptr};
   if (a.want_w && p.nt) {
-    TransposeP t{(const uint16_t*)H.p, H.ld / 2, H.lo / 2, w.ht, p.np, a.D * p.np, (int)a.N, (int)a.D, s.count, H.rows};
+    TransposeP t{(const uint16_t*)H.p, H.ld / 2, H.lo / 2, w.ht, p.np, a.D * p.np, (int)a.N, (int)a.D, s.count, H.rows, nullptr, 0};
     hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)((a.N + 63) / 64), (unsigned)((a.D + 63) / 64), a.split ? 2 : 1), dim3(256), 0, st, t);
     VL_CHECK();
     packed = Operand{(const char*)w.ht, p.np * 2, a.split ? a.D * p.np * 2 : 0, 0, nullptr};
   }
   packed.xlim = (int)a.D;
-  Operand wh = W;                                                  // W for the dh product
-  if (a.want_h && p.nt && !a.wt) {
-    TransposeP t{(const uint16_t*)W.p, W.ld / 2, W.lo / 2, w.wtr, p.vp, a.D * p.vp, (int)a.V, (int)a.D, nullptr, nullptr};
+  Operand wt = W;                                                  // W along the sum's axis of the dh product
+  if (p.wtr) {
+    TransposeP t{(const uint16_t*)W.p, W.ld / 2, W.lo / 2, w.wtr, p.vp, a.D * p.vp, (int)a.V, (int)a.D, nullptr, nullptr, s.count, p.many};
     hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)((a.V + 63) / 64), (unsigned)((a.D + 63) / 64), a.split ? 2 : 1), dim3(256), 0, st, t);
     VL_CHECK();
-    wh = Operand{(const char*)w.wtr, p.vp * 2, a.split ? a.D * p.vp * 2 : 0, 0, nullptr};
+    wt = Operand{(const char*)w.wtr, p.vp * 2, a.split ? a.D * p.vp * 2 : 0, (int)a.D, nullptr};
   }
   const int64_t ldg = p.np * gsz, glo = a.split || p.pair ? p.gcols * ldg : 0;
   const int64_t ldr = p.gcols * gsz, rlo = a.split ? p.np * ldr : 0;   // the same row by row (p.nt)
@@ -1310,9 +1340,12 @@ int backward(const Args& a, const float* f, hipStream_t st) {
     if (a.want_h) {
       DhP d;
       d.G = p.nt ? Operand{rows_g, ldr, rlo, 0, nullptr} : G;
-      d.G.xlim = (int)p.np; d.W = wh;
-      d.W.p += p.nt || a.wt ? (int64_t)v0 * gsz : v0 * wh.ld;
+      d.G.xlim = (int)p.np; d.W = W;
+      d.W.p += a.wt ? (int64_t)v0 * gsz : v0 * W.ld;
       d.W.xlim = (int)a.D;
+      d.WT = wt;
+      d.WT.p += (int64_t)v0 * gsz;
+      d.many = p.wtr ? p.many : 0x7fffffff;
       d.count = s.count; d.D = (int)a.D; d.vc = vc; d.units = p.units; d.most = p.most; d.accum = k > 0; d.slab = w.dh_slab;
       const int e = dispatch_dh(d, p.dh_tile, p.op, a.split, p.pair, a.wt, st);
       if (e) return e;
