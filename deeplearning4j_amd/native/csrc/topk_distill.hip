@@ -5,7 +5,8 @@
 //
 // Bound by the logits: forward reads them once (running maximum and sum of the softmax), backward reads them once and writes dz. One
 // workgroup per row; 16-byte loads behind a peeled head, since rows of an odd vocabulary start anywhere. The teacher's softmax is K
-// values: both directions compute it in LDS instead of passing it through memory.
+// values: both directions compute it in LDS instead of passing it through memory. 8192 x 65536 bf16, 128 entries: forward 238 us (4.5 TB/s),
+// backward 478 us (4.5 TB/s; a copy reaches 5.0); 4096 x 30522, a fifth of the rows without entries: 60 and 93 us.
 #include "common.h"
 
 namespace {

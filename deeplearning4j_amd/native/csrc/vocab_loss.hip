@@ -6,6 +6,10 @@
 //
 // with q = exp(z - lse), p = softmax over the K teacher logits / T and P_n = sum_k p_k (1, or 0 for a row without entries).
 //
+// What bounds it: the products. A step is four of 2 N D V operations (scores twice, since they are not kept, and the two gradients). bf16, 8192 x
+// 2048 of 65536 words: 8.8 TFLOP, 6.7 ms (1310 TF/s; the loop alone reaches 1605). One forward of a few rows reads W once: 1 x 768 of 30522 words,
+// 47 MB, 12 us (3.9 TB/s) of 19.
+//
 // Forward: a product tile h W^T stays in the accumulators; its epilogue leaves one (max, sum of exp) pair per row and column tile, which
 // combine_kernel joins. Backward: the same product again, piece by piece of the vocabulary; the epilogue turns the accumulators into dz
 // (a piece of at most some hundred MiB), and two products consume it: dh += dz W and dW = dz^T h. Rows without a label / teacher entry
@@ -69,7 +73,7 @@ struct Scales {
 // ------------------------------------------------------------------------------------------------------------------------ rows
 // rows[0 .. count) = rows that take part, in order, lab their labels (-1: outside the vocabulary, or none); rows[count .. N) = the others;
 // loss of the others = 0.
-// One workgroup: a scan of N flags, 1024 at a time behind the loads of 8192.
+// One workgroup: a scan of N flags, 1024 at a time behind the loads of 8192 (bound by their latency: 4096 rows 7 us, 8192 rows 11 us).
 constexpr int SCAN = 8;
 __global__ void __launch_bounds__(1024) rows_kernel(const void* __restrict__ labels, int lab64, int64_t ignore, const float* __restrict__ mass, int N,
                                                     int V, int* __restrict__ rows, int* __restrict__ lab, int* __restrict__ count,
@@ -122,7 +126,7 @@ struct TeacherP {
 };
 // One wave per row: p = softmax(teacher / T) over the entries with an index >= 0, ent = sum p log p, mass = 1, or 0 where no entry has a
 // weight. The entries are sorted by index (a bitonic sort in LDS), so that a column tile finds its own between first[t] and first[t + 1],
-// and psum, the summed p of all entries with one index, is a run. An index outside the vocabulary, a NaN or +inf makes ent NaN.
+// and psum, the summed p of all entries with one index, is a run. K log^2 K steps of LDS: 4096 rows x 64 entries 18 us. An index outside the vocabulary, a NaN or +inf makes ent NaN.
 __global__ void __launch_bounds__(256) teacher_kernel(const TeacherP p) {
   extern __shared__ char smem[];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
@@ -200,6 +204,8 @@ __global__ void __launch_bounds__(256) teacher_kernel(const TeacherP p) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------------ operands
+// Bound by reading W (30522 x 768 fp32, 94 MB: 25 us, 3.7 TB/s); the same pass cannot convert, since one factor serves the whole of W: the
+// gradient products sum over its rows.
 // largest finite |x| of W (workgroups 0 .. AMAX_W - 1) and of the rows of H that take part (the others): one value per workgroup
 constexpr int AMAX_W = 1024, AMAX_H = 128;
 __global__ void __launch_bounds__(256) amax_kernel(const float* __restrict__ W, int64_t ldw, int wr, int wc, const float* __restrict__ H, int64_t ldh,
@@ -241,6 +247,7 @@ __device__ __forceinline__ void halves(float v, _Float16& hi, _Float16& lo) {
   lo = (_Float16)(d == d ? d : 0.f);                    // inf - inf: an infinity stays in the first half alone
 }
 
+// Bound by memory: W read once, written once in halves (30522 x 768: 188 MB, 35 us, 5.3 TB/s from what the caches keep of the pass before).
 // W and the packed rows of H as scaled halves, 4 values per thread and step; columns [C, Cp) are zeros. Workgroups [0, gw) take W, the others H.
 struct SplitP {
   const float* W; int64_t ldw; int wr, wc, wcp; _Float16* wo;
@@ -285,7 +292,7 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitP p) {
 }
 
 // Copies of operands whose rows do not start on 16 bytes or do not end on them: rows of Cp elements with zeros behind C. Workgroups [0, gw)
-// take W, the others the rows of H that take part, one after the other.
+// take W, the others the rows of H that take part, one after the other. (Bound by memory; 1600 rows x 512 and 512 x 98 words in fp32: 3 us.)
 struct PadP {
   const char* W; int64_t ldw; int wr, wc; char* wo; int64_t wcp;       // elements
   const char* H; int64_t ldh; int D; char* ho; int64_t dp;
@@ -331,6 +338,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const char* __restrict__ h, i
   for (int64_t b = threadIdx.x * 16; b < row_bytes; b += 256 * 16) *reinterpret_cast<f32x4*>(out + m * ldo_bytes + b) = *reinterpret_cast<const f32x4*>(src + b);
 }
 
+// Bound by memory (65536 x 2048 bf16, 537 MB: 190 us, 2.9 TB/s).
 // out[c][r] = in[row r][c] of 16-bit values, R x C, 64 x 64 at a time through LDS; blockIdx.z: the halves of a pair. `count`: R on the device,
 // and `rows` the row of position r (both or none); positions from R to the next multiple of 64 become zeros. `gate`: only where *gate >= least.
 struct TransposeP {
@@ -406,7 +414,10 @@ template <class C> constexpr int score_lds(bool grad) {
 // tile), instead of the row's maximum: four cross-lane steps in all instead of four per row, and no row waits for its own maximum. A sum of
 // exponentials 2^-100 below the reference is still a sound fp32 number; a row that lies lower makes the workgroup take the tile again with a
 // reference per row. The 16 lanes that share a row leave their partial sums in LDS, where one thread per row adds them.
-// Epilogue of a 256 x 256 tile: 11 us with a maximum and a sum reduced over the lanes for every row (product of one k-tile: 1.5 us).
+// (A maximum and a sum reduced over the lanes for every row, as the fallback does it, made the epilogue of a 256 x 256 tile as long as seven
+// of its k-tiles.)
+// Bound by the matrix cores: forward of 8192 x 2048 of 65536 words in bf16 1.72 ms (1280 TF/s), 4096 x 1024 of 32000 0.31 ms (860 TF/s: 16 k-tiles
+// to an epilogue). With the gradient (exponentials, 2 or 4 bytes per score written through LDS) 1.94 and 0.35 ms.
 // SEG 3: operands and gradient in halves; 2: the gradient in halves (its rounding to 16 bits then counts for nothing: few rows do not
 // average it out, and for them a second pass over the gradient costs little beside W).
 template <class C, bool TB, bool GRAD, int SEG>
@@ -700,6 +711,7 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
   }
 }
 
+// Bound by latency: 8 bytes per row and column tile (4096 rows x 125 tiles 8 us, one row x 239 tiles 4 us).
 // joins the (max, sum) pairs of a row's column tiles; R rows x 256 / R tile groups per workgroup
 struct CombineP {
   const float2* part; const float* zs; const float* tz;
@@ -762,6 +774,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineP p) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------------ backward
+// Bound by the latency of one workgroup (4096 rows: 7 us).
 // coef[m] = dloss[rows[m]] * T * s with the largest at `top` (0: s = 1). The scores' gradient is rounded to 16 bits: at a label it is close to
 // its coefficient, and with the largest coefficient at a power of two the large ones sit at the end of their binade, where a rounding counts
 // least; fp16 takes 2^14, so that entries down to 2^-38 of the largest stay above its smallest step.
@@ -817,6 +830,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const float* __restrict__ 
     for (int64_t b = threadIdx.x * 16; b < row_bytes; b += 256 * 16) *reinterpret_cast<f32x4*>(out + m * ldo_bytes + b) = *reinterpret_cast<const f32x4*>(src + b);
 }
 
+// Bound by reading the gradient (96 rows x 30522 words in halves: 10 us).
 // db from the gradient itself (both halves), one wave per word: with teacher entries the tiles' column sums do not hold them
 __global__ void __launch_bounds__(256) bias_rows_kernel(const char* __restrict__ G, int64_t ldg, int64_t glo, int dt, int vc, const int* __restrict__ count,
                                                         const Scales* __restrict__ sc, void* __restrict__ db, int bdt) {
@@ -832,7 +846,7 @@ __global__ void __launch_bounds__(256) bias_rows_kernel(const char* __restrict__
 }
 
 // dh: unit u of the grid owns output tile u % tiles and share u / tiles of the piece's columns; its fp32 tile lives in slab u and is added
-// to by the following pieces. Which unit owns what depends on the number of rows alone, so the sum's order is fixed.
+// to by the following pieces. 8192 x 2048 of 65536 words in bf16 1.53 ms (1440 TF/s), 4096 x 1024 of 32000 0.238 ms (1130 TF/s). Which unit owns what depends on the number of rows alone, so the sum's order is fixed.
 //
 // Large tile, W by rows ([V, D]): read as it is (K-major, transposing LDS reads), or transposed first where `many` rows pay for that.
 struct DhP {
@@ -880,7 +894,7 @@ __global__ void __launch_bounds__(C::NT) dh_kernel(const DhP p) {
   to_slab<C>(p.slab + (int64_t)u * C::BM * C::BN, acc, p.accum);
 }
 
-// What is left: workgroups [0, N) one row of dh each from the slabs, in the order of the shares (rows that take no part get zeros), those
+// What is left, bound by memory (8192 x 2048: 100 MB, 26 us): workgroups [0, N) one row of dh each from the slabs, in the order of the shares (rows that take no part get zeros), those
 // behind them 256 words of db = scale * sum over the row tiles' column sums.
 struct FinishP {
   const float* slab; const int* rows; const int* count; const Scales* sc;
@@ -922,7 +936,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishP p) {
 }
 
 // dW[v0 .. v0 + vc) = scale * dz^T h (SWAP 0, [V, D]) or its transpose (SWAP 1, [D, V]): the gradient is read along its
-// rows (the sum's axis); h is walked row by row by the 128 x 128 tiles, and read along the rows of its transpose by the 256 x 256 ones.
+// rows (the sum's axis; 8192 x 2048 of 65536 words in bf16 1.5 ms, 1470 TF/s); h is walked row by row by the 128 x 128 tiles, and read along the rows of its transpose by the 256 x 256 ones.
 // shares > 1 (small outputs): the rows' range is cut, fp32 tiles go to a slab and dw_sum_kernel adds them in order.
 struct DwP {
   Operand G, H;
@@ -1024,9 +1038,14 @@ Plan plan(const Args& a) {
   // (its operands are addressed with 32-bit offsets: rows of all of them, and H's indirect ones together, have to be short of that)
   const bool near = up(a.N, 256) * 2 < BUF_LD && up(a.V, 256) * 2 < BUF_LD && a.ldh * 4 < BUF_LD && a.ldw * 4 < BUF_LD && up(a.D, 8) * 4 < BUF_LD && (a.split || a.N * a.ldh * 2 < BUF_SPAN);
   const int64_t mid_tiles = up(a.N, 128) / 128 * (up(a.V, 128) / 128);
-  // 256 x 256 tiles once they cover two thirds of the 256 CUs; 32 rows where few rows meet a large vocabulary (W streams through, a tile per
-  // CU at 32768 words); 64 x 64 tiles with four stages where 128 x 128 ones would leave CUs idle (the time is a chain of k-tiles then)
-  p.tile = bits16 && big_tiles >= 176 && a.N > 128 && near ? TILE_BIG : a.N <= 32 && a.V >= 16384 ? TILE_FEW : mid_tiles < 176 ? TILE_SMALL : TILE_MID;
+  // Tile of the scores (times of calls with D = 1024 in bf16, 128 x 128 against the other):
+  //   256 x 256 once such tiles cover two thirds of the 256 CUs: forward of 300 rows x 22500 words (176 tiles) 44.3 and 38.9 us, x 16000 (126) 31.3
+  //   and 36.3; step of 1000 x 11300 168 and 153 us; not for half a tile of rows: 100 x 50000 30.1 and 36.3
+  //   32 x 128, four stages, where few rows meet a large vocabulary and W streams through: 1 x 768 of 30522 words 23.3 and 18.9 us, fp32 32 x 50000
+  //   153 and 67 (64 x 64: 19.2 and 96)
+  //   64 x 64, four stages, where 128 x 128 ones leave CUs idle and the time is one chain of k-tiles: 300 x 5000 (120 tiles) 24.8 and 19.1 us, x 7000
+  //   (165) 24.9 and 27.0; fp32, whose larger tile leaves one wave to a SIMD: 300 x 300 of 12000 (282) 59.9 and 44.7, of 20000 (471) 51.8 and 66.8
+  p.tile = bits16 && big_tiles >= 176 && a.N > 128 && near ? TILE_BIG : a.N <= 32 && a.V >= 16384 ? TILE_FEW : mid_tiles < (bits16 ? 144 : 384) ? TILE_SMALL : TILE_MID;
   if (a.split && p.tile == TILE_FEW) p.tile = TILE_MID;
   if (!bits16 && p.tile == TILE_BIG) p.tile = TILE_MID;
   p.bm = tile_rows(p.tile);
@@ -1041,22 +1060,27 @@ Plan plan(const Args& a) {
   p.pad_h = !a.split && (a.D % ch || a.ldh % ch || !aligned16(a.H));
   p.wcp = up(a.wt ? a.V : a.D, 8);
   const int64_t esz = a.dt == DT_F32 ? 4 : 2;                    // halves take as much as fp32
+  // a piece's gradient: 512 MiB (step of 8192 x 2048 of 65536 words: 6.95 ms with 128 MiB, 6.82 with 256, 6.76 with 512, 6.72 with 1024)
   const int64_t most = ((int64_t)512 << 20) / (p.np * esz) / 256 * 256;
   p.pieces = (int)(most >= 256 ? (a.V + most - 1) / most : up(a.V, 256) / 256);
   p.step = (int)up((a.V + p.pieces - 1) / p.pieces, 256);
   p.pieces = (int)((a.V + p.step - 1) / p.step);
   p.gcols = up(a.V < p.step ? a.V : p.step, 256);
-  p.nt = p.tile == TILE_BIG && a.N >= 512 && a.D >= 256;
+  // The backward products on 256 x 256 tiles, for which the scores' gradient is written a second time, row by row, and H transposed; against
+  // 128 x 128 tiles without that: step of 600 rows x 4096 of 40000 words 858 against 962 us, x 1024 280 and 288, 1024 x 512 of 32000 198 and 205,
+  // 2048 x 256 271 and 241, 400 x 1024 of 40000 248 and 238.
+  p.nt = p.tile == TILE_BIG && a.N >= 512 && a.D >= 512;
   // W as it lies, through transposing LDS reads, against W transposed first: 2100 rows x 1000 of 50001 words 231 us against 207 + 98; 4096 x 1024 of
   // 32000: 242 and 226 + 47; 8192 x 2048 of 65536: 1820 and 1520 + 188. The transpose costs the same for any number of rows.
   p.many = 6144;
   p.wtr = a.want_h && p.nt && !a.wt && a.N >= p.many;
-  p.pair = bits16 && !a.split && a.N <= 256;
+  p.pair = bits16 && !a.split && a.N <= 256;                       // (see score_kernel)
   const int seg = a.split ? 3 : p.pair ? 2 : 1, bk = bits16 ? 64 : 32;
   const int64_t vk = seg * (up(p.step, bk) / bk), nk = seg * (up(a.N, bk) / bk);   // k-tiles of the two products' sums
   const int64_t cols = p.gcols < a.V ? p.gcols : a.V;
   auto tiles = [](int64_t m, int64_t n, int t) { return up(m, t) / t * (up(n, t) / t); };
-  // the same for the backward products, whose sums can be cut into shares of four k-tiles
+  // 64 x 64 tiles in the backward products by the same reasoning; their sums can be cut into shares of four k-tiles. Step of 700 rows x 304 of
+  // 400 words: dh 41.3 (128 x 128) and 38.7 us, dw 41.8 and 38.7; 30 x 2048 of 10000, dw: 89 and 100.
   p.dh_tile = p.nt ? TILE_BIG : tiles(a.N, a.D, 128) * (vk / 4 + 1) < 256 ? TILE_SMALL : TILE_MID;
   p.dw_tile = p.nt ? TILE_BIG : tiles(cols, a.D, 128) * (nk / 4 + 1) < 256 ? TILE_SMALL : TILE_MID;
   const int want_h = p.dh_tile == TILE_BIG ? 256 : p.dh_tile == TILE_SMALL ? 1024 : 512, want_w = p.dw_tile == TILE_SMALL ? 1024 : 512;
@@ -1137,9 +1161,9 @@ template <int DT, bool TB, bool GRAD, int SEG> int score_tile(const ScoreP& p, i
   return tile == TILE_SMALL ? launch_score<Small<DT>, TB, GRAD, SEG>(p, st) : launch_score<Mid<DT>, TB, GRAD, SEG>(p, st);
 }
 template <int DT, bool TB, bool GRAD> int score16(const ScoreP& p, int tile, bool pair, hipStream_t st) {
-  if (tile == TILE_BIG) return launch_score<Big<DT>, TB, GRAD, 1>(p, st);
   if constexpr (GRAD)
-    if (pair) return score_tile<DT, TB, GRAD, 2>(p, tile, st);
+    if (pair) return tile == TILE_BIG ? launch_score<Big<DT>, TB, GRAD, 2>(p, st) : score_tile<DT, TB, GRAD, 2>(p, tile, st);
+  if (tile == TILE_BIG) return launch_score<Big<DT>, TB, GRAD, 1>(p, st);
   if (GRAD || tile != TILE_FEW) return tile == TILE_SMALL ? launch_score<Small<DT>, TB, GRAD, 1>(p, st) : launch_score<Mid<DT>, TB, GRAD, 1>(p, st);
   return launch_score<Few<DT>, TB, false, 1>(p, st);
 }

@@ -496,3 +496,19 @@ def test_the_loss_and_the_labels_may_be_changed_before_the_backward_pass():
         for x, k in zip(held, kept):
             x.copy_(k)
         assert all(torch.equal(a, e) for a, e in zip(got, want))
+
+
+@pytest.mark.parametrize("layout", ["vd", "dv"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [129, 256])
+def test_gradient_halves_on_large_tiles(n, dtype, layout):
+    """Up to 256 rows the scores' gradient comes in two halves, whatever the tile that forms it. What is left of its rounding is u^2, so the
+    weights' and hidden states' gradients are off by their own rounding alone."""
+    d, v = 72, 45057
+    h, w, b, dl = _linear_inputs(n, d, v, dtype, n, True, layout)
+    y = _labels(n, v, 0.1, n)
+    _both(lambda h, w, b: VL.linear_cross_entropy(h, w, y, b), lambda h, w, b: VL.linear_cross_entropy_reference(h, w, y, b), [h, w, b], dl,
+          limit=LIMIT[dtype] / 2)
+    idx, t = _teacher(n, v, 17, n)
+    _both(lambda h, w, b: VL.linear_topk_distillation(h, w, idx, t, b), lambda h, w, b: VL.linear_topk_distillation_reference(h, w, idx, t, b), [h, w, b], dl,
+          limit=LIMIT[dtype] / 2)
