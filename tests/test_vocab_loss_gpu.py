@@ -512,3 +512,20 @@ def test_gradient_halves_on_large_tiles(n, dtype, layout):
     idx, t = _teacher(n, v, 17, n)
     _both(lambda h, w, b: VL.linear_topk_distillation(h, w, idx, t, b), lambda h, w, b: VL.linear_topk_distillation_reference(h, w, idx, t, b), [h, w, b], dl,
           limit=LIMIT[dtype] / 2)
+
+
+@pytest.mark.parametrize("n,d,v", [(1, 64, 17001), (3, 1, 16387), (27, 1085, 16595), (32, 33, 20000), (30, 130, 1003), (64, 257, 5001), (33, 31, 2)])
+@pytest.mark.parametrize("layout", ["vd", "dv"])
+def test_forward_of_few_rows_reads_weights_off_16_bytes(n, d, v, layout):
+    """fp32 weights cut out of a larger table at an odd place: every row starts and ends on 4 bytes only; what lies around them is NaN."""
+    h, w, b, _ = _linear_inputs(n, d, v, torch.float32, n, True, "vd")
+    rows, cols = (v, d) if layout == "vd" else (d, v)
+    table = torch.full((rows + 2, cols + 3), math.nan, device=DEV)
+    part = table[1:1 + rows, 1:1 + cols]
+    part.copy_(w if layout == "vd" else w.t())
+    w = part if layout == "vd" else part.t()
+    y = _labels(n, v, 0.2, n)
+    _losses_close(VL.linear_cross_entropy(h, w, y, b), VL.linear_cross_entropy_reference(h.double(), w.double(), y, b.double()))
+    k = min(9, v)
+    idx, t = _teacher(n, v, k, n)
+    _losses_close(VL.linear_topk_distillation(h, w, idx, t, b), VL.linear_topk_distillation_reference(h.double(), w.double(), idx, t, b.double()))
