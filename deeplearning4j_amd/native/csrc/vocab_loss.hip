@@ -830,19 +830,39 @@ __global__ void __launch_bounds__(256) prepare_kernel(const float* __restrict__ 
     for (int64_t b = threadIdx.x * 16; b < row_bytes; b += 256 * 16) *reinterpret_cast<f32x4*>(out + m * ldo_bytes + b) = *reinterpret_cast<const f32x4*>(src + b);
 }
 
-// Bound by reading the gradient (96 rows x 30522 words in halves: 10 us).
-// db from the gradient itself (both halves), one wave per word: with teacher entries the tiles' column sums do not hold them
+// db from the gradient itself (both halves): with teacher entries the tiles' column sums do not hold them. Eight lanes to a word, 16 bytes each at a
+// time. Bound by reading the gradient (96 rows x 30522 words in halves: 6.6 us; a wave to a word, two bytes a lane, took 10.4).
 __global__ void __launch_bounds__(256) bias_rows_kernel(const char* __restrict__ G, int64_t ldg, int64_t glo, int dt, int vc, const int* __restrict__ count,
                                                         const Scales* __restrict__ sc, void* __restrict__ db, int bdt) {
-  const int v = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, c = *count;
-  if (v >= vc) return;
+  const int v = blockIdx.x * 32 + (threadIdx.x >> 3), c = *count, ch = dt == DT_F32 ? 4 : 8;
   float s = 0.f;
-  for (int m = lane; m < c; m += 64) {
-    s += load_f(G + v * ldg, m, dt);
-    if (glo) s += load_f(G + glo + v * ldg, m, dt);
+  auto add = [&](const char* at, int m) {
+    const f32x4 raw = *reinterpret_cast<const f32x4*>(at);
+    if (dt == DT_F32) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += m + e < c ? raw[e] : 0.f;
+    } else {
+      const s16x8 x = __builtin_bit_cast(s16x8, raw);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint16_t u = (uint16_t)x[e];
+        s += m + e < c ? (dt == DT_BF16 ? bf2f(u) : (float)__builtin_bit_cast(_Float16, u)) : 0.f;
+      }
+    }
+  };
+  if (v < vc) {
+    const char* row = G + v * ldg;
+#pragma unroll 2
+    for (int m = (threadIdx.x & 7) * ch; m < c; m += 8 * ch) {
+      const char* at = row + (int64_t)m * (16 / ch);
+      add(at, m);
+      if (glo) add(at + glo, m);
+    }
   }
-  s = wave_sum(s);
-  if (lane == 0) store_f(db, v, bdt, s * sc->db);
+  s += __shfl_xor(s, 4, 64);
+  s += __shfl_xor(s, 2, 64);
+  s += __shfl_xor(s, 1, 64);
+  if (v < vc && (threadIdx.x & 7) == 0) store_f(db, v, bdt, s * sc->db);
 }
 
 // dh: unit u of the grid owns output tile u % tiles and share u / tiles of the piece's columns; its fp32 tile lives in slab u and is added
@@ -894,20 +914,23 @@ __global__ void __launch_bounds__(C::NT) dh_kernel(const DhP p) {
   to_slab<C>(p.slab + (int64_t)u * C::BM * C::BN, acc, p.accum);
 }
 
-// What is left, bound by memory (8192 x 2048: 100 MB, 26 us): workgroups [0, N) one row of dh each from the slabs, in the order of the shares (rows that take no part get zeros), those
-// behind them 256 words of db = scale * sum over the row tiles' column sums.
+// What is left, bound by memory (8192 x 2048: 100 MB, 26 us): workgroups [0, N * blocks) dh from the slabs, in the order of the shares
+// (rows that take no part get zeros): 1024 columns of a row, or, where a call of few rows leaves many shares, 256 columns with a quarter of the shares
+// to each wave (96 rows x 768 from 85 shares 12.9 and 8.0 us; 4096 x 1024 from 4 shares 20.6 and 24.7).
+// Those behind them 256 words of db = scale * sum over the row tiles' column sums.
 struct FinishP {
   const float* slab; const int* rows; const int* count; const Scales* sc;
-  int N, D, units, most;
+  int N, D, units, most, blocks;         // blocks of a row
   void* dh; int dt;
   const float* colsum; int bm; int V;
   void* db; int bdt;
 };
-template <int BM, int BN>
+template <int BM, int BN, bool QUARTERS>
 __global__ void __launch_bounds__(256) finish_kernel(const FinishP p) {
+  __shared__ f32x4 quarter[QUARTERS ? 3 : 1][64];
   const int c = *p.count;
-  if ((int)blockIdx.x >= p.N) {
-    const int v = ((int)blockIdx.x - p.N) * 256 + threadIdx.x, tiles = (c + p.bm - 1) / p.bm;
+  if ((int)blockIdx.x >= p.N * p.blocks) {
+    const int v = ((int)blockIdx.x - p.N * p.blocks) * 256 + threadIdx.x, tiles = (c + p.bm - 1) / p.bm;
     if (v >= p.V) return;
     float s = 0.f;
 #pragma unroll 4
@@ -915,24 +938,32 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishP p) {
     store_f(p.db, v, p.bdt, s * p.sc->db);
     return;
   }
-  const int m = blockIdx.x, n = p.rows[m];
+  const int m = blockIdx.x / p.blocks, b = blockIdx.x - m * p.blocks;
   const int mtiles = (c + BM - 1) / BM, ntiles = (p.D + BN - 1) / BN, tiles = mtiles * ntiles;
-  const int shares = tiles ? shares_of(tiles, p.units, p.most) : 1;
-  const float s = p.sc->dh;
-  for (int d = threadIdx.x * 4; d < p.D; d += 1024) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (m < c) {
-      const int mt = m / BM, nt = d / BN;
-      const int g = mt / 8, rowsg = min(8, mtiles - g * 8);       // tile_coords with 8 row tiles to a group
-      const int t = g * 8 * ntiles + nt * rowsg + (mt - g * 8);
-      const float* x = p.slab + ((int64_t)t * BM + (m - mt * BM)) * BN + (d - nt * BN);
+  const int shares = m < c ? shares_of(tiles, p.units, p.most) : 1;
+  const int wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int d = QUARTERS ? b * 256 + lane * 4 : b * 1024 + (int)threadIdx.x * 4;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (m < c && d < p.D) {
+    const int mt = m / BM, nt = d / BN;
+    const int g = mt / 8, rowsg = min(8, mtiles - g * 8);         // tile_coords with 8 row tiles to a group
+    const int t = g * 8 * ntiles + nt * rowsg + (mt - g * 8);
+    const float* x = p.slab + ((int64_t)t * BM + (m - mt * BM)) * BN + (d - nt * BN);
+    const int per = QUARTERS ? (shares + 3) / 4 : shares, k0 = QUARTERS ? wid * per : 0, k1 = min(shares, k0 + per);
 #pragma unroll 4
-      for (int k = 0; k < shares; ++k) v += *reinterpret_cast<const f32x4*>(x + (int64_t)k * tiles * BM * BN);
-      v *= s;
-    }
-    const int64_t o = (int64_t)n * p.D + d;
-    for (int j = 0; j < 4 && d + j < p.D; ++j) store_f(p.dh, o + j, p.dt, v[j]);
+    for (int k = k0; k < k1; ++k) v += *reinterpret_cast<const f32x4*>(x + (int64_t)k * tiles * BM * BN);
   }
+  if constexpr (QUARTERS) {
+    if (wid > 0) quarter[wid - 1][lane] = v;
+    __syncthreads();
+    if (wid > 0) return;
+    v = (v + quarter[0][lane]) + (quarter[1][lane] + quarter[2][lane]);
+  }
+  v *= p.sc->dh;
+  const int64_t o = (int64_t)p.rows[m] * p.D + d;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (d + j < p.D) store_f(p.dh, o + j, p.dt, v[j]);
 }
 
 // dW[v0 .. v0 + vc) = scale * dz^T h (SWAP 0, [V, D]) or its transpose (SWAP 1, [D, V]): the gradient is read along its
@@ -1027,6 +1058,7 @@ struct Plan {
   int64_t np, dp, wcp, wrows, vp;           // padded rows / columns of the packed H and of the halves of W
   int pieces, step;
   int units, most, shares;
+  bool quarters;                         // finish_kernel
   int64_t gcols;
 };
 
@@ -1087,6 +1119,7 @@ Plan plan(const Args& a) {
   const int64_t ht = tiles(a.N, a.D, tile_rows(p.dh_tile)), wt = tiles(cols, a.D, tile_rows(p.dw_tile));
   p.units = (int)(ht > want_h ? ht : want_h);
   p.most = (int)((vk + 3) / 4);
+  p.quarters = (ht >= p.units ? 1 : p.units / ht < p.most ? p.units / ht : p.most) >= 16;
   int64_t sh = p.dw_tile == TILE_BIG ? 1 : want_w / wt;
   if (sh > nk / 4) sh = nk / 4;
   p.shares = (int)(sh < 1 ? 1 : sh);
@@ -1304,6 +1337,11 @@ int forward(const Args& a, const float* f, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
+template <int B> void launch_finish(const FinishP& q, bool quarters, dim3 grid, hipStream_t st) {
+  if (quarters) hipLaunchKernelGGL((finish_kernel<B, B, true>), grid, dim3(256), 0, st, q);
+  else hipLaunchKernelGGL((finish_kernel<B, B, false>), grid, dim3(256), 0, st, q);
+}
+
 int backward(const Args& a, const float* f, hipStream_t st) {
   if (const int e = check(a, true)) return e;
   const Plan p = plan(a);
@@ -1356,7 +1394,7 @@ int backward(const Args& a, const float* f, hipStream_t st) {
     if (a.want_b && !a.K) { q.colsum = w.colsum; q.ldc = a.V; }
     if (const int e = scores<true>(q, p.tile, p.op, a.split, p.pair, a.wt, st)) return e;
     if (a.want_b && a.K) {
-      hipLaunchKernelGGL(bias_rows_kernel, dim3((vc + 3) / 4), dim3(256), 0, st, w.G, ldg, glo, a.split ? (int)DT_F16 : (int)a.dt, vc, s.count, s.sc,
+      hipLaunchKernelGGL(bias_rows_kernel, dim3((vc + 31) / 32), dim3(256), 0, st, w.G, ldg, glo, a.split ? (int)DT_F16 : (int)a.dt, vc, s.count, s.sc,
                          (char*)a.db + (int64_t)v0 * (a.bdt == DT_F32 ? 4 : 2), (int)a.bdt);
       VL_CHECK();
     }
@@ -1387,11 +1425,13 @@ int backward(const Args& a, const float* f, hipStream_t st) {
   }
   const bool sums = a.want_b && !a.K;
   if (a.want_h || sums) {
-    const FinishP q{w.dh_slab, s.rows, s.count, s.sc, a.want_h ? (int)a.N : 0, (int)a.D, p.units, p.most, a.dh, (int)a.dt, w.colsum, p.bm, (int)a.V, a.db, (int)a.bdt};
-    const dim3 grid((unsigned)(q.N + (sums ? (a.V + 255) / 256 : 0)));
-    if (p.dh_tile == TILE_BIG) hipLaunchKernelGGL((finish_kernel<256, 256>), grid, dim3(256), 0, st, q);
-    else if (p.dh_tile == TILE_SMALL) hipLaunchKernelGGL((finish_kernel<64, 64>), grid, dim3(256), 0, st, q);
-    else hipLaunchKernelGGL((finish_kernel<128, 128>), grid, dim3(256), 0, st, q);
+    const int64_t cols = p.quarters ? 256 : 1024, blocks = (a.D + cols - 1) / cols;
+    if (a.N * blocks + (a.V + 255) / 256 > 0x7fffffff) return -2;
+    const FinishP q{w.dh_slab, s.rows, s.count, s.sc, a.want_h ? (int)a.N : 0, (int)a.D, p.units, p.most, (int)blocks, a.dh, (int)a.dt, w.colsum, p.bm, (int)a.V, a.db, (int)a.bdt};
+    const dim3 grid((unsigned)(q.N * blocks + (sums ? (a.V + 255) / 256 : 0)));
+    if (p.dh_tile == TILE_BIG) launch_finish<256>(q, p.quarters, grid, st);
+    else if (p.dh_tile == TILE_SMALL) launch_finish<64>(q, p.quarters, grid, st);
+    else launch_finish<128>(q, p.quarters, grid, st);
   }
   return (int)hipGetLastError();
 }
