@@ -909,8 +909,10 @@ __global__ void __launch_bounds__(C::NT) dh_kernel(const DhP p) {
   const int ktiles = k_tiles<C, SEG>(p.vc), per = (ktiles + shares - 1) / shares;
   const int k0 = min(ktiles, share * per), k1 = min(ktiles, k0 + per);
   typename C::acc_t acc[C::TM][C::TN];
-  if (is_pp<C>() && TB && count >= p.many) product<C, TA, false, SEG>(smem, p.G, p.WT, mt * C::BM, nt * C::BN, p.vc, k0, k1, acc);
-  else product<C, TA, TB, SEG>(smem, p.G, p.W, mt * C::BM, nt * C::BN, p.vc, k0, k1, acc);
+  Operand G = p.G;
+  G.xlim = (count + 7) & ~7;                                       // (whole chunks; what lies behind is not read)
+  if (is_pp<C>() && TB && count >= p.many) product<C, TA, false, SEG>(smem, G, p.WT, mt * C::BM, nt * C::BN, p.vc, k0, k1, acc);
+  else product<C, TA, TB, SEG>(smem, G, p.W, mt * C::BM, nt * C::BN, p.vc, k0, k1, acc);
   to_slab<C>(p.slab + (int64_t)u * C::BM * C::BN, acc, p.accum);
 }
 
@@ -1402,7 +1404,7 @@ int backward(const Args& a, const float* f, hipStream_t st) {
     if (a.want_h) {
       DhP d;
       d.G = p.nt ? Operand{rows_g, ldr, rlo, 0, nullptr} : G;
-      d.G.xlim = (int)p.np; d.W = W;
+      d.W = W;
       d.W.p += a.wt ? (int64_t)v0 * gsz : v0 * W.ld;
       d.W.xlim = (int)a.D;
       d.WT = wt;
