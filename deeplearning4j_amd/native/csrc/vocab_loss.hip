@@ -1031,7 +1031,7 @@ __global__ void __launch_bounds__(256) dw_sum_kernel(const float* __restrict__ s
 
 // ------------------------------------------------------------------------------------------------------------------------ host side
 template <int DT> using Big = Cfg<256, 256, 2, 4, 2, 16, DT>;
-template <int DT> using Mid = Cfg<128, 128, 2, 2, 2, 16, DT>;
+template <int DT> using Mid = Cfg<128, 128, 2, 4, 2, 16, DT>;   // eight waves: step of 32 rows x 1024, 50000 words 138 us with four, 132 with eight
 template <int DT> using Few = Cfg<32, 128, 1, 4, 4, 16, DT>;
 template <int DT> using Small = Cfg<64, 64, 2, 2, 4, 16, DT>;
 enum { TILE_BIG = 0, TILE_MID = 1, TILE_FEW = 2, TILE_SMALL = 3 };
@@ -1073,12 +1073,12 @@ Plan plan(const Args& a) {
   const bool near = up(a.N, 256) * 2 < BUF_LD && up(a.V, 256) * 2 < BUF_LD && a.ldh * 4 < BUF_LD && a.ldw * 4 < BUF_LD && up(a.D, 8) * 4 < BUF_LD && (a.split || a.N * a.ldh * 2 < BUF_SPAN);
   const int64_t mid_tiles = up(a.N, 128) / 128 * (up(a.V, 128) / 128);
   // Tile of the scores (times of calls with D = 1024 in bf16, 128 x 128 against the other):
-  //   256 x 256 once such tiles cover two thirds of the 256 CUs: forward of 300 rows x 22500 words (176 tiles) 44.3 and 38.9 us, x 16000 (126) 31.3
-  //   and 36.3; step of 1000 x 11300 168 and 153 us; not for half a tile of rows: 100 x 50000 30.1 and 36.3
-  //   32 x 128, four stages, where few rows meet a large vocabulary and W streams through: 1 x 768 of 30522 words 23.3 and 18.9 us, fp32 32 x 50000
-  //   153 and 67 (64 x 64: 19.2 and 96)
-  //   64 x 64, four stages, where 128 x 128 ones leave CUs idle and the time is one chain of k-tiles: 300 x 5000 (120 tiles) 24.8 and 19.1 us, x 7000
-  //   (165) 24.9 and 27.0; fp32, whose larger tile leaves one wave to a SIMD: 300 x 300 of 12000 (282) 59.9 and 44.7, of 20000 (471) 51.8 and 66.8
+  //   256 x 256 once such tiles cover two thirds of the 256 CUs: forward of 300 rows x 22500 words (176 tiles) 41.8 and 39.2 us, x 16000 (126) 30.5
+  //   and 37.3; step of 1000 x 11300 159 and 151 us; not for half a tile of rows: 100 x 50000 30.1 and 36.3
+  //   32 x 128, four stages, where few rows meet a large vocabulary and W streams through: 1 x 768 of 30522 words 22.2 and 18.4 us, fp32 32 x 50000
+  //   150 and 67 (64 x 64: 18.6 and 96)
+  //   64 x 64, four stages, where 128 x 128 ones leave CUs idle and the time is one chain of k-tiles: 300 x 5000 (120 tiles) 22.5 and 19.0 us, x 7000
+  //   (165) 22.6 and 26.8; fp32, whose chains are longer: 300 x 300 of 12000 (282) 59.3 and 44.3, of 20000 (471) 51.7 and 67.0
   p.tile = bits16 && big_tiles >= 176 && a.N > 128 && near ? TILE_BIG : a.N <= 32 && a.V >= 16384 ? TILE_FEW : mid_tiles < (bits16 ? 144 : 384) ? TILE_SMALL : TILE_MID;
   if (a.split && p.tile == TILE_FEW) p.tile = TILE_MID;
   if (!bits16 && p.tile == TILE_BIG) p.tile = TILE_MID;
@@ -1101,8 +1101,8 @@ Plan plan(const Args& a) {
   p.pieces = (int)((a.V + p.step - 1) / p.step);
   p.gcols = up(a.V < p.step ? a.V : p.step, 256);
   // The backward products on 256 x 256 tiles, for which the scores' gradient is written a second time, row by row, and H transposed; against
-  // 128 x 128 tiles without that: step of 600 rows x 4096 of 40000 words 858 against 962 us, x 1024 280 and 288, 1024 x 512 of 32000 198 and 205,
-  // 2048 x 256 271 and 241, 400 x 1024 of 40000 248 and 238.
+  // 128 x 128 tiles without that: step of 600 rows x 4096 of 40000 words 841 against 939 us, x 1024 277 and 285, 4096 x 512 of 32000 634 and 683,
+  // 2048 x 256 271 and 244, 400 x 1024 of 40000 243 and 240.
   p.nt = p.tile == TILE_BIG && a.N >= 512 && a.D >= 512;
   // W as it lies, through transposing LDS reads, against W transposed first: 2100 rows x 1000 of 50001 words 231 us against 207 + 98; 4096 x 1024 of
   // 32000: 242 and 226 + 47; 8192 x 2048 of 65536: 1820 and 1520 + 188. The transpose costs the same for any number of rows.
@@ -1114,7 +1114,7 @@ Plan plan(const Args& a) {
   const int64_t cols = p.gcols < a.V ? p.gcols : a.V;
   auto tiles = [](int64_t m, int64_t n, int t) { return up(m, t) / t * (up(n, t) / t); };
   // 64 x 64 tiles in the backward products by the same reasoning; their sums can be cut into shares of four k-tiles. Step of 700 rows x 304 of
-  // 400 words: dh 41.3 (128 x 128) and 38.7 us, dw 41.8 and 38.7; 30 x 2048 of 10000, dw: 89 and 100.
+  // 400 words: dh 40.8 (128 x 128) and 38.6 us, dw 41.6 and 38.5; 30 x 2048 of 10000, dw: 81 and 95.
   p.dh_tile = p.nt ? TILE_BIG : tiles(a.N, a.D, 128) * (vk / 4 + 1) < 256 ? TILE_SMALL : TILE_MID;
   p.dw_tile = p.nt ? TILE_BIG : tiles(cols, a.D, 128) * (nk / 4 + 1) < 256 ? TILE_SMALL : TILE_MID;
   const int want_h = p.dh_tile == TILE_BIG ? 256 : p.dh_tile == TILE_SMALL ? 1024 : 512, want_w = p.dw_tile == TILE_SMALL ? 1024 : 512;
