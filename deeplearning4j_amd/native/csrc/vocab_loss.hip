@@ -1041,6 +1041,7 @@ int tile_cols(int tile) { return tile == TILE_BIG ? 256 : tile == TILE_SMALL ? 6
 // One call: sizes, layout and pointers (ops/vocab_loss.py _ARGS lists the same fields in the same order)
 struct Args {
   int64_t N, D, V, dt, split, wt, bdt, ldh, ldw, lab64, ignore, idx64, tdt, K, want_h, want_w, want_b;
+  int64_t pad_h, pad_w;                  // operands that are copied to whole 16-byte chunks (H: packed) by the forward call: set by layout()
   const void *H, *W, *bias, *labels, *idx, *t;
   float* loss; char* state; char* ws;
   const float* dloss; void *dh, *dw, *db;
@@ -1052,7 +1053,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 struct Plan {
   int tile, dh_tile, dw_tile;            // TILE_*
   int op;                                // operand type of the products
-  bool pad_w, pad_h;                     // operands that are copied to whole 16-byte chunks (H: packed) by the forward call
+  bool pad_w, pad_h;
   bool pair;                             // 16-bit operands: the scores' gradient in two halves
   bool nt;                               // backward products on 256 x 256 tiles from operands laid out along the sum's axis
   bool wtr; int many;                    // dh: W is transposed first, for calls of `many` rows that take part
@@ -1063,6 +1064,13 @@ struct Plan {
   bool quarters;                         // finish_kernel
   int64_t gcols;
 };
+
+// What the operands' addresses decide. The forward call's decision, since the backward call may get the same values at another place.
+void layout(Args& a) {
+  const int64_t ch = a.dt == DT_F32 ? 4 : 8, wc = a.wt ? a.V : a.D;
+  a.pad_w = !a.split && (wc % ch || a.ldw % ch || !aligned16(a.W));
+  a.pad_h = !a.split && (a.D % ch || a.ldh % ch || !aligned16(a.H));
+}
 
 Plan plan(const Args& a) {
   Plan p;
@@ -1089,9 +1097,8 @@ Plan plan(const Args& a) {
   p.vp = up(a.V, 64);
   p.dp = up(a.D, 8);
   p.wrows = a.wt ? a.D : a.V;
-  const int64_t ch = a.dt == DT_F32 ? 4 : 8, wc = a.wt ? a.V : a.D;
-  p.pad_w = !a.split && (wc % ch || a.ldw % ch || !aligned16(a.W));
-  p.pad_h = !a.split && (a.D % ch || a.ldh % ch || !aligned16(a.H));
+  p.pad_w = a.pad_w;
+  p.pad_h = a.pad_h;
   p.wcp = up(a.wt ? a.V : a.D, 8);
   const int64_t esz = a.dt == DT_F32 ? 4 : 2;                    // halves take as much as fp32
   // a piece's gradient: 512 MiB (step of 8192 x 2048 of 65536 words: 6.95 ms with 128 MiB, 6.82 with 256, 6.76 with 512, 6.72 with 1024)
@@ -1269,6 +1276,9 @@ int check(const Args& a, bool bwd) {
   if (!a.H || !a.W || !a.state || !a.ws || !aligned16(a.state) || !aligned16(a.ws)) return -2;
   if (!bwd && (!a.loss || (a.K ? !a.idx || !a.t || a.tdt < 0 || a.tdt > 2 : !a.labels))) return -2;
   if (a.ldh < a.D || a.ldw < (a.wt ? a.V : a.D)) return -2;
+  Args now = a;
+  layout(now);
+  if ((now.pad_w && !a.pad_w) || (now.pad_h && !a.pad_h)) return -2;
   if (bwd && (!a.dloss || (a.want_h && !a.dh) || (a.want_w && !a.dw) || (a.want_b && (!a.db || !a.bias)))) return -2;
   return 0;
 }
@@ -1440,9 +1450,10 @@ int backward(const Args& a, const float* f, hipStream_t st) {
 
 }  // namespace
 
-// bytes of the state, the forward workspace and the backward workspace
-DL4J_API void dl4j_linear_loss_bytes(const int64_t* args, int64_t* out) {
-  const Args& a = *reinterpret_cast<const Args*>(args);
+// bytes of the state, the forward workspace and the backward workspace; sets the fields of the call that layout() decides
+DL4J_API void dl4j_linear_loss_bytes(int64_t* args, int64_t* out) {
+  Args& a = *reinterpret_cast<Args*>(args);
+  layout(a);
   const Plan p = plan(a);
   const Work w(a, p);
   out[0] = State(a, p).bytes;

@@ -120,13 +120,14 @@ def linear_topk_distillation_reference(hidden, weights, teacher_indices, teacher
 
 # ------------------------------------------------------------------------------------------------------------------ kernel calls
 # the fields of struct Args in native/csrc/vocab_loss.hip, in order
-_ARGS = ("N D V dt split wt bdt ldh ldw lab64 ignore idx64 tdt K want_h want_w want_b "
+_ARGS = ("N D V dt split wt bdt ldh ldw lab64 ignore idx64 tdt K want_h want_w want_b pad_h pad_w "
          "H W bias labels idx t loss state ws dloss dh dw db").split()
 _AT = {n: k for k, n in enumerate(_ARGS)}
 _Block = ctypes.c_int64 * len(_ARGS)
 _Floats = ctypes.c_float * 2
 _Sizes = ctypes.c_int64 * 3
 _STATE, _WS = _AT["state"], _AT["ws"]
+_H, _W, _BIAS, _LDH, _LDW, _SPLIT, _PAD_H, _PAD_W = (_AT[n] for n in "H W bias ldh ldw split pad_h pad_w".split())
 # struct DistillArgs in native/csrc/topk_distill.hip: N V K ldz dt idx64 tdt z idx t loss lse dloss dz
 _TopkBlock = ctypes.c_int64 * 14
 
@@ -151,6 +152,14 @@ def _split(rows, hidden, vocabulary, training):
     and 121 us, of 128 rows: 78 and 91 us."""
     work = hidden * vocabulary
     return (rows - 40) * work > 150e6 if training else (rows - 150) * work > 600e6
+
+
+def _as_before(t, ld, any_start):
+    """``t``, or its values with rows ``ld`` apart and on 16 bytes (unless any start will do). Saved tensors come back from hooks (recomputation,
+    offload) in other memory, and the forward call's choices hold for its own row distance and alignment."""
+    if (t.shape[1] == 1 or t.stride(1) == 1) and (t.shape[0] == 1 or t.stride(0) == ld) and (any_start or t.data_ptr() % 16 == 0):
+        return t
+    return torch.empty_strided(t.shape, (ld, 1), dtype=t.dtype, device=t.device).copy_(t)
 
 
 def _launch(fn, what, dev, *args):
@@ -193,7 +202,7 @@ def _linear_forward(hidden, weights, bias, first, second, ignore, smoothing, tem
     teacher = second is not None
     is64, at = first.dtype == torch.int64, first.data_ptr()
     a = _Block(N, D, weights.shape[0], _DT[h.dtype], split, dv, 0 if bias is None else _DT[bias.dtype], _ld(h), _ld(w), is64, ignore, is64,
-               _DT[second.dtype] if teacher else 0, first.shape[1] if teacher else 0, *want,
+               _DT[second.dtype] if teacher else 0, first.shape[1] if teacher else 0, *want, 0, 0,
                h.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if teacher else at, at if teacher else 0,
                second.data_ptr() if teacher else 0, loss.data_ptr(), 0, 0, 0, 0, 0, 0)
     f = _Floats(temperature, smoothing)
@@ -207,7 +216,7 @@ def _linear_forward(hidden, weights, bias, first, second, ignore, smoothing, tem
         a[_STATE] = both.data_ptr()
         a[_WS] = a[_STATE] + size[0]
     _launch(lib.dl4j_linear_loss_fwd, "linear_loss_fwd", dev, a, f)
-    return loss, ((h, w, state), (a, f, size[2], dv)) if training else None
+    return loss, ((h, w, state), (a, f, size[0], size[2], dv)) if training else None
 
 
 class _LinearLoss(torch.autograd.Function):
@@ -232,9 +241,16 @@ class _LinearLoss(torch.autograd.Function):
 
 
 def _linear_backward(ctx, dloss):
-    h, w, bias, state = ctx.saved_tensors
-    a, f, size, dv = ctx.call
+    h, w, bias, state = ctx.saved_tensors                               # (the forward call's own, or what hooks make of them)
+    a, f, state_size, size, dv = ctx.call
     a = _Block.from_buffer_copy(a)                                      # (a graph kept alive may be walked from two threads)
+    _need(state.numel() == state_size, "linear loss: the saved state is another call's (%d bytes for %d)" % (state.numel(), state_size))
+    split = a[_SPLIT]
+    h, w = _as_before(h, a[_LDH], split or a[_PAD_H]), _as_before(w, a[_LDW], split or a[_PAD_W])
+    a[_H], a[_W] = h.data_ptr(), w.data_ptr()
+    if bias is not None:
+        bias = bias.contiguous()
+        a[_BIAS] = bias.data_ptr()
     dev = h.device
     g = _dloss(dloss)
     want_h, want_w, want_b = ctx.needs_input_grad[:3]
@@ -286,11 +302,13 @@ class _TopkDistillation(torch.autograd.Function):
 
 
 def _topk_backward(ctx, dloss):
-    z = ctx.saved_tensors[0]                                            # (unpacked: a changed tensor is refused)
+    z, idx, t, lse = ctx.saved_tensors                                  # (the forward call's own, or what hooks make of them)
+    z, idx, t, lse = _rows(z), idx.contiguous(), t.contiguous(), lse.contiguous()
     a, f = ctx.call
     a = _TopkBlock.from_buffer_copy(a)
     g = _dloss(dloss)
     dz = torch.empty(ctx.shape, dtype=z.dtype, device=z.device)
+    a[3], a[7], a[8], a[9], a[11] = z.stride(0), z.data_ptr(), idx.data_ptr(), t.data_ptr(), lse.data_ptr()
     a[10], a[12], a[13] = 0, g.data_ptr(), dz.data_ptr()
     _launch(_lib().dl4j_topk_distill, "topk_distill", z.device, a, f)
     return dz, None, None, None
