@@ -7,7 +7,7 @@
 
 namespace gemmcore {
 
-enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU_TANH = 2, ACT_GELU_ERF = 3, ACT_TANH = 4, ACT_SIGMOID = 5 };
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU_TANH = 2, ACT_GELU_ERF = 3, ACT_TANH = 4, ACT_SIGMOID = 5, ACT_KEEP = 6 };
 enum { OT_BF16 = 0, OT_F16 = 1, OT_F32 = 2 };
 
 __device__ __forceinline__ float apply_act(float v, int act) {
@@ -51,7 +51,7 @@ struct EpiP {
 
 // RowOff: int64 element offset of tile row r's first column (n0) in `out`, or -1 when the row is out of range.
 // vrows: number of valid rows of this tile (rows >= vrows are padding: excluded from the statistics, never stored).
-template <class C, int OT, int ACTK, int STATS, class RowOff>   // ACTK: ACT_NONE = linear / ReLU, else that activation; STATS: 0 never, 1 always, 2 run time (e.stats)
+template <class C, int OT, int ACTK, int STATS, class RowOff>   // ACTK: ACT_NONE = linear / ReLU, ACT_KEEP = linear with NaN kept, else that activation; STATS: 0 never, 1 always, 2 run time (e.stats)
 __device__ __forceinline__ void epilogue_impl(char* smem, typename C::acc_t (&acc)[C::TM][C::TN], int mt, int n0, int N, int vrows,
                                               const EpiP& e, RowOff rowoff) {
   typedef Out<OT> O;
@@ -71,6 +71,7 @@ __device__ __forceinline__ void epilogue_impl(char* smem, typename C::acc_t (&ac
   // ACTK == ACT_NONE (no activation or ReLU): branch-free, v = max(alpha * acc + bias, lo) with lo = 0 or -inf. Inlined per element (128
   // accumulators per lane on the 256 x 256 tile) the six-way activation switch makes the epilogue ~30k instructions / ~2000
   // branches, far beyond the instruction cache (+10 us per output tile, measured): only the transcendental activations pay that.
+  // (That maximum turns a NaN into lo; ACT_KEEP has none.)
   const float lo = e.act == ACT_RELU ? 0.f : -__builtin_inff();
 #pragma unroll
   for (int j = 0; j < C::TN; ++j) {

@@ -1008,9 +1008,9 @@ __global__ void __launch_bounds__(C::NT) dw_kernel(const DwP p) {
   }
   EpiP e;
   e.out = p.out; e.residual = nullptr; e.bias = nullptr; e.stats = nullptr; e.stat_shift = nullptr;
-  e.alpha = p.sc->dw; e.act = ACT_NONE; e.accum = 0;
+  e.alpha = p.sc->dw; e.act = ACT_KEEP; e.accum = 0;
   const int64_t ldo = p.ldo;
-  epilogue_impl<C, OT, ACT_NONE, 0>(smem, acc, mt, n0, N, M - m0, e, [=](int r) -> int64_t {
+  epilogue_impl<C, OT, ACT_KEEP, 0>(smem, acc, mt, n0, N, M - m0, e, [=](int r) -> int64_t {
     return m0 + r < M ? (int64_t)(m0 + r) * ldo + n0 : (int64_t)-1;
   });
 }
