@@ -138,10 +138,11 @@ def _up(n, m):
 
 def _rows(t):
     """[R, C] with contiguous rows, ``t`` itself where they are. (Rows that do not start or end on 16 bytes are copied by the native call.)"""
-    return t if t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+    return t if (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
 
 
 def _ld(t):
+    """From one row of ``_rows(t)`` to the next; the stride of a single row says nothing."""
     return t.stride(0) if t.shape[0] > 1 else _up(t.shape[1], 16 // t.element_size())
 
 
@@ -277,11 +278,11 @@ _TOPK_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 def _topk_forward(logits, idx, t, temperature):
     z = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
-    z = z if z.stride(1) == 1 and z.stride(0) >= z.shape[1] else z.contiguous()
+    z = _rows(z)
     N, dev = z.shape[0], z.device
     loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
     lse = torch.empty(N, dtype=torch.float32, device=dev)
-    a = _TopkBlock(N, z.shape[1], idx.shape[1], z.stride(0), _TOPK_DT[z.dtype], idx.dtype == torch.int64, _TOPK_DT[t.dtype], z.data_ptr(), idx.data_ptr(),
+    a = _TopkBlock(N, z.shape[1], idx.shape[1], _ld(z), _TOPK_DT[z.dtype], idx.dtype == torch.int64, _TOPK_DT[t.dtype], z.data_ptr(), idx.data_ptr(),
                    t.data_ptr(), loss.data_ptr(), lse.data_ptr(), 0, 0)
     f = _Floats(temperature, 0.0)
     _launch(_lib().dl4j_topk_distill, "topk_distill", dev, a, f)
@@ -308,7 +309,7 @@ def _topk_backward(ctx, dloss):
     a = _TopkBlock.from_buffer_copy(a)
     g = _dloss(dloss)
     dz = torch.empty(ctx.shape, dtype=z.dtype, device=z.device)
-    a[3], a[7], a[8], a[9], a[11] = z.stride(0), z.data_ptr(), idx.data_ptr(), t.data_ptr(), lse.data_ptr()
+    a[3], a[7], a[8], a[9], a[11] = _ld(z), z.data_ptr(), idx.data_ptr(), t.data_ptr(), lse.data_ptr()
     a[10], a[12], a[13] = 0, g.data_ptr(), dz.data_ptr()
     _launch(_lib().dl4j_topk_distill, "topk_distill", z.device, a, f)
     return dz, None, None, None

@@ -132,3 +132,23 @@ def test_a_state_of_another_call_is_refused(calls):
         loss = VL.linear_cross_entropy(h, w, torch.zeros(5, dtype=torch.int64))
     with pytest.raises(VL.ND4JIllegalArgumentException, match="state"):
         _backward(loss)
+
+
+@pytest.mark.parametrize("v", [1, 7, 24])
+@pytest.mark.parametrize("row", [lambda v: torch.randn(v, 1).t(), lambda v: torch.randn(v).expand(3, v)[1:2], lambda v: torch.randn(v, 3).t()[1:2]])
+def test_one_row_of_logits_has_a_row_distance_whatever_its_stride(calls, v, row):
+    z = row(v).requires_grad_()
+    _backward(VL.topk_distillation(z, torch.zeros(1, 3, dtype=torch.int64), torch.zeros(1, 3)))
+    for _, c in calls:
+        assert c["ldz"] >= v
+
+
+@pytest.mark.parametrize("rows", [2, 5])
+def test_rows_of_one_logit_lie_as_far_apart_as_they_do(calls, rows):
+    z = torch.randn(rows, 4)[:, 1:2].requires_grad_()                      # strides (4, 1)
+    _backward(VL.topk_distillation(z, torch.zeros(rows, 3, dtype=torch.int64), torch.zeros(rows, 3)))
+    assert [c["ldz"] for _, c in calls] == [4, 4]
+    del calls[:]
+    z = torch.randn(3, rows).t()[:, 1:2].requires_grad_()                  # strides (1, rows): the inner one says nothing
+    _backward(VL.topk_distillation(z, torch.zeros(rows, 3, dtype=torch.int64), torch.zeros(rows, 3)))
+    assert [c["ldz"] for _, c in calls] == [1, 1]
