@@ -22,7 +22,8 @@
 //                          (one such operand: up to 20 % longer than K-contiguous ones, at 8192 x 2048 x 32768; two: 40 %)
 //
 // A product of fp32 operands runs on the 16-bit matrix cores as three products of halves, a = a1 + a2 with a1 = fp16(a), a2 = fp16(a - a1)
-// (operands scaled by a power of two so that the largest is below 2^14):  a . b = a1 b1 + a1 b2 + a2 b1, what is left out is 2^-24 of |a||b|.
+// (operands scaled by powers of two so that the largest is below 2^15):  a . b = a1 b1 + a1 b2 + a2 b1. What is left out of an element is 2^-24 of it,
+// or 2^-40 of the largest element that shares its factor (the second half's smallest step) where that is more.
 // The three are one long product whose k-tiles come in threes, (a1, b1), (a1, b2), (a2, b1), so that what a k-tile reads again is still in L2.
 #pragma once
 #include "gemm_trans.h"

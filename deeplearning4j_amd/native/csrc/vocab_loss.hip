@@ -29,6 +29,7 @@ constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x); }
 constexpr int KMAX = 1024;                              // teacher entries per row
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float load_f(const void* p, int64_t i, int dt) {
   if (dt == DT_F32) return reinterpret_cast<const float*>(p)[i];
@@ -63,12 +64,31 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   m = nm;
 }
 
-// Factors that the halves' scaling (fp32, powers of two) and the normalised coefficients of the backward pass bring in.
-struct Scales {
-  float z;          // scores = z * product
-  float h, w;       // of the operands' halves
-  float dh, dw, db; // gradients = factor * product (sum)
+// fp32 operands in halves: a row of H is scaled by a power of two of its own, 2^eh, that puts its largest value into [2^14, 2^15), so that no
+// row costs another one its low bits (one factor for all of H: a row 10^6 times as large as the others left their scores off by 5e-5, 10^9 by
+// 0.05). A score is 2^-(eh + ew) * product + bias.
+// A word of W has 2^ew, with 2^lo, the largest word's, unless its largest value lies NEAR powers of two below that word's: such a word's exponent
+// goes up to WORD beyond lo. The gradient of the hidden states sums over the words, and takes the rest, 2^(lo - ew), with a copy of the scores'
+// gradient that is written for it alone, where there is such a word (`wide`). A score of halves is off by 2^-40 of the factors' range, so a word
+// 10^6 times smaller than the largest keeps 2^-32 of its own largest value, one 10^9 times smaller 2^-22; the gradient's copy keeps 2^-27 of a row's
+// coefficient.
+constexpr int NEAR = 8, WORD = 12, ZERO_ROW = 127;                 // ZERO_ROW: the exponent of a row of zeros
+struct Scales { float top; int wide; };                            // top: the largest finite |w|
+// the exponent that puts m into [2^14, 2^15)
+__device__ __forceinline__ int scale_for(float m) {
+  if (!(m > 0.f)) return 0;
+  int e;
+  frexpf(m, &e);
+  return min(15 - e, 126);
+}
+__device__ __forceinline__ int lowest_word(const Scales* sc) { return scale_for(sc->top); }
+__device__ __forceinline__ int word_scale(float m, int lo) { return m > 0.f ? lo + min(max(scale_for(m) - lo - NEAR, 0), min(WORD, 126 - lo)) : lo; }
+// What the backward pass multiplies its products with.
+struct Grad {
+  float inv;        // gradients = inv * product (sum)
+  int hlo;          // dW: exponent of the rows' factors, all brought to the one of the largest row
 };
+__device__ __forceinline__ float pow2(float v, int e) { return __builtin_amdgcn_ldexpf(v, e); }
 
 // ------------------------------------------------------------------------------------------------------------------------ rows
 // rows[0 .. count) = rows that take part, in order, lab their labels (-1: outside the vocabulary, or none); rows[count .. N) = the others;
@@ -110,7 +130,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(const void* __restrict__ lab
       done += all;
     }
   }
-  if (tid == 0) { *count = done; *sc = Scales{1.f, 1.f, 1.f, 1.f, 1.f, 1.f}; }
+  if (tid == 0) { *count = done; *sc = Scales{0.f, 0}; }
 }
 
 // ------------------------------------------------------------------------------------------------------------------------ teacher
@@ -204,90 +224,174 @@ __global__ void __launch_bounds__(256) teacher_kernel(const TeacherP p) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------------ operands
-// Bound by reading W (30522 x 768 fp32, 94 MB: 25 us, 3.7 TB/s); the same pass cannot convert, since one factor serves the whole of W: the
-// gradient products sum over its rows.
-// largest finite |x| of W (workgroups 0 .. AMAX_W - 1) and of the rows of H that take part (the others): one value per workgroup
-constexpr int AMAX_W = 1024, AMAX_H = 128;
-__global__ void __launch_bounds__(256) amax_kernel(const float* __restrict__ W, int64_t ldw, int wr, int wc, const float* __restrict__ H, int64_t ldh,
-                                                   int D, const int* __restrict__ rows, const int* __restrict__ count, float* __restrict__ out) {
-  __shared__ float red[16];
-  const bool is_w = blockIdx.x < AMAX_W;
-  const int R = is_w ? wr : *count, C = is_w ? wc : D, q = (C + 3) / 4;
-  const int64_t n = (int64_t)R * q, step = (is_w ? AMAX_W : AMAX_H) * 256;
-  float m = 0.f;
-#pragma unroll 4
-  for (int64_t i = (int64_t)(is_w ? blockIdx.x : blockIdx.x - AMAX_W) * 256 + threadIdx.x; i < n; i += step) {
-    const int r = (int)(i / q), c = (int)(i - (int64_t)r * q) * 4;
-    const float* x = (is_w ? W + r * ldw : H + rows[r] * ldh) + c;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (c + 4 <= C && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
-      const f32x4 f = *reinterpret_cast<const f32x4*>(x);
-      v[0] = f[0]; v[1] = f[1]; v[2] = f[2]; v[3] = f[3];
-    } else {
-      for (int j = 0; j < 4; ++j) v[j] = c + j < C ? x[j] : 0.f;
-    }
+// Values and halves, four at a time; columns [C, ..) are zeros.
+__device__ __forceinline__ void load4(const float* x, int c, int C, float (&v)[4]) {
+  if (c + 4 <= C && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+    const f32x4 f = *reinterpret_cast<const f32x4*>(x);
+    v[0] = f[0]; v[1] = f[1]; v[2] = f[2]; v[3] = f[3];
+  } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { const float t = fabsf(v[j]); m = fmaxf(m, t < __builtin_inff() ? t : 0.f); }
+    for (int j = 0; j < 4; ++j) v[j] = c + j < C ? x[j] : 0.f;
   }
-  m = block_max(m, red);
-  if (threadIdx.x == 0) out[blockIdx.x] = m;
 }
-
-// the power of two that puts m into [2^13, 2^14)
-__device__ __forceinline__ int scale_for(float m) {
-  if (!(m > 0.f)) return 0;
-  int e;
-  frexpf(m, &e);
-  return max(14 - e, -114);
-}
-
+__device__ __forceinline__ float finite_max(float m, float x) { const float t = fabsf(x); return fmaxf(m, t < __builtin_inff() ? t : 0.f); }
 __device__ __forceinline__ void halves(float v, _Float16& hi, _Float16& lo) {
   hi = (_Float16)v;
   const float d = v - (float)hi;
   lo = (_Float16)(d == d ? d : 0.f);                    // inf - inf: an infinity stays in the first half alone
 }
 
-// Bound by memory: W read once, written once in halves (30522 x 768: 188 MB, 35 us, 5.3 TB/s from what the caches keep of the pass before).
-// W and the packed rows of H as scaled halves, 4 values per thread and step; columns [C, Cp) are zeros. Workgroups [0, gw) take W, the others H.
 struct SplitP {
-  const float* W; int64_t ldw; int wr, wc, wcp; _Float16* wo;
-  const float* H; int64_t ldh; int D, Dp; _Float16* ho; int hcap;      // hcap: rows of one half of ho
-  const int* rows; const int* count; const float* amax;
-  Scales* sc;
-  int gw;
+  const float* W; int64_t ldw; int wt, V, D;             // [V, D], or [D, V] with wt
+  _Float16* wo; int64_t wcp;                             // halves of W, rows of wcp
+  const float* H; int64_t ldh; _Float16* ho; int64_t dp, hcap;   // the rows that take part, packed; hcap: rows of one half
+  const int* rows; const int* count;
+  Scales* sc; int *eh, *ew;
+  float* wmax; int chunks;                               // largest finite |w| of every word ([D, V]: of each of `chunks` cuts of the rows)
+  float* tops;                                           // the same of every workgroup of W in amax_kernel
+  int gw;                                                // workgroups of W, the others are H's
 };
-__global__ void __launch_bounds__(256) split_kernel(const SplitP p) {
+constexpr int CHUNKS = 16, AMAX_W = 2048;
+// Bound by reading W (30522 x 768 fp32, 94 MB: 25 us, 3.7 TB/s); the same pass cannot convert, since a word's factor depends on the largest word.
+// Rows of H and words of a [V, D] table: a wave to a row. Words of a [D, V] table: a lane to four columns, workgroups of 256 columns x a cut of the rows.
+__global__ void __launch_bounds__(256) amax_kernel(const SplitP p) {
   __shared__ float red[16];
-  float mw = 0.f, mh = 0.f;
-  for (int i = threadIdx.x; i < AMAX_W; i += 256) mw = fmaxf(mw, p.amax[i]);
-  for (int i = threadIdx.x; i < AMAX_H; i += 256) mh = fmaxf(mh, p.amax[AMAX_W + i]);
-  // both together 2^100 at most, since a bias enters the accumulators times both: below that the smaller operand's low bits go first
-  const int ew = scale_for(block_max(mw, red)), eh = scale_for(block_max(mh, red));
-  const bool cap = ew + eh > 100;
-  const float sw = ldexpf(1.f, cap ? min(ew, max(50, 100 - eh)) : ew), sh = ldexpf(1.f, cap ? min(eh, max(50, 100 - ew)) : eh);
-  if (blockIdx.x == 0 && threadIdx.x == 0) { p.sc->h = sh; p.sc->w = sw; p.sc->z = 1.f / sh / sw; }
+  __shared__ f32x4 part[4][64];
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const bool is_w = (int)blockIdx.x < p.gw;
-  const int c = *p.count;
-  const int R = is_w ? p.wr : c, C = is_w ? p.wc : p.D, q = (is_w ? p.wcp : p.Dp) / 4;
-  const float s = is_w ? sw : sh;
-  const int64_t n = (int64_t)R * q, step = (int64_t)(is_w ? p.gw : gridDim.x - p.gw) * 256;
-  _Float16* out = is_w ? p.wo : p.ho;
-  const int64_t half = (int64_t)(is_w ? p.wr : p.hcap) * q * 4;
-  for (int64_t i = (int64_t)(is_w ? blockIdx.x : blockIdx.x - p.gw) * 256 + threadIdx.x; i < n; i += step) {
-    const int r = (int)(i / q), d = (int)(i - (int64_t)r * q) * 4;
-    const float* x = is_w ? p.W + r * p.ldw + d : p.H + p.rows[r] * p.ldh + d;
-    _Float16 hi[4], lo[4];
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (d + 4 <= C && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
-      const f32x4 f = *reinterpret_cast<const f32x4*>(x);
-      v[0] = f[0]; v[1] = f[1]; v[2] = f[2]; v[3] = f[3];
-    } else {
-      for (int j = 0; j < 4; ++j) v[j] = d + j < C ? x[j] : 0.f;
-    }
+  float top = 0.f;
+  if (is_w && p.wt) {
+    const int per = (p.D + p.chunks - 1) / p.chunks, units = (p.V + 255) / 256 * p.chunks;
+    for (int u = blockIdx.x; u < units; u += p.gw) {
+      const int strip = u / p.chunks, chunk = u - strip * p.chunks, c = strip * 256 + lane * 4, r1 = min(p.D, (chunk + 1) * per);
+      float m[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int r = chunk * per + wid; r < r1; r += 4) {
+        float v[4];
+        load4(p.W + r * p.ldw + c, c, p.V, v);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) halves(v[j] * s, hi[j], lo[j]);
-    __builtin_memcpy(out + i * 4, hi, 8);
-    __builtin_memcpy(out + half + i * 4, lo, 8);
+        for (int j = 0; j < 4; ++j) m[j] = finite_max(m[j], v[j]);
+      }
+      part[wid][lane] = f32x4{m[0], m[1], m[2], m[3]};
+      __syncthreads();
+      if (wid == 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = fmaxf(fmaxf(part[0][lane][j], part[1][lane][j]), fmaxf(part[2][lane][j], part[3][lane][j]));
+          if (c + j < p.V) p.wmax[(int64_t)chunk * p.V + c + j] = x;
+          top = fmaxf(top, x);
+        }
+      }
+      __syncthreads();
+    }
+  } else {
+    constexpr int G = 4;                                           // rows of a wave at a time: their loads are in flight together
+    const int R = is_w ? p.V : *p.count, step = (is_w ? p.gw : gridDim.x - p.gw) * 4 * G;
+    const bool whole = ((reinterpret_cast<uintptr_t>(is_w ? p.W : p.H) | (uintptr_t)((is_w ? p.ldw : p.ldh) * 4) | (uintptr_t)p.D * 4) & 15) == 0;   // 16 bytes at a time
+    for (int64_t r0 = ((is_w ? blockIdx.x : blockIdx.x - p.gw) * 4 + wid) * G; r0 < R; r0 += step) {
+      const float* x[G];
+      float m[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const int64_t r = r0 + g < R ? r0 + g : R - 1;
+        x[g] = is_w ? p.W + r * p.ldw : p.H + p.rows[r] * p.ldh;
+        m[g] = 0.f;
+      }
+      if (whole) {
+#pragma unroll 4
+        for (int c = lane * 4; c < p.D; c += 256)
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(x[g] + c);
+            m[g] = finite_max(finite_max(finite_max(finite_max(m[g], v[0]), v[1]), v[2]), v[3]);
+          }
+      } else {
+        for (int c = lane * 4; c < p.D; c += 256)
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            float v[4];
+            load4(x[g] + c, c, p.D, v);
+            m[g] = finite_max(finite_max(finite_max(finite_max(m[g], v[0]), v[1]), v[2]), v[3]);
+          }
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float t = wave_max(m[g]);
+        if (lane == 0 && r0 + g < R) {
+          if (is_w) p.wmax[r0 + g] = t;
+          else p.eh[r0 + g] = t > 0.f ? scale_for(t) : ZERO_ROW;
+        }
+        top = fmaxf(top, t);
+      }
+    }
+  }
+  if (!is_w) return;
+  top = block_max(top, red);
+  if (threadIdx.x == 0) p.tops[blockIdx.x] = top;
+}
+
+// Bound by memory: W read once, written once in halves (30522 x 768: 188 MB, 35 us, 5.3 TB/s from what the caches keep of the pass before).
+// W and the packed rows of H as scaled halves, cut into workgroups as amax_kernel cuts them.
+__global__ void __launch_bounds__(256) split_kernel(const SplitP p) {
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  __shared__ float red[16];
+  const bool is_w = (int)blockIdx.x < p.gw;
+  float top = 0.f;
+  for (int i = threadIdx.x; i < p.gw; i += 256) top = fmaxf(top, p.tops[i]);
+  top = block_max(top, red);
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.sc->top = top;
+  const int lo = scale_for(top);
+  auto store4 = [](_Float16* out, int64_t half, const float (&v)[4], const float (&f)[4]) {
+    _Float16 a[4], b[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) halves(v[j] * f[j], a[j], b[j]);
+    __builtin_memcpy(out, a, 8);
+    __builtin_memcpy(out + half, b, 8);
+  };
+  if (is_w && p.wt) {
+    const int per = (p.D + p.chunks - 1) / p.chunks, units = (p.V + 255) / 256 * p.chunks;
+    for (int u = blockIdx.x; u < units; u += p.gw) {
+      const int strip = u / p.chunks, chunk = u - strip * p.chunks, c = strip * 256 + lane * 4, r1 = min(p.D, (chunk + 1) * per);
+      if (c >= p.wcp) continue;
+      float f[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float m = 0.f;
+        if (c + j < p.V)
+          for (int k = 0; k < p.chunks; ++k) m = fmaxf(m, p.wmax[(int64_t)k * p.V + c + j]);
+        const int e = word_scale(m, lo);
+        f[j] = pow2(1.f, e);
+        if (chunk == 0 && wid == 0 && c + j < p.V) {
+          p.ew[c + j] = e;
+          if (e != lo) p.sc->wide = 1;
+        }
+      }
+#pragma unroll 2
+      for (int r = chunk * per + wid; r < r1; r += 4) {
+        float v[4];
+        load4(p.W + r * p.ldw + c, c, p.V, v);
+        store4(p.wo + r * p.wcp + c, (int64_t)p.D * p.wcp, v, f);
+      }
+    }
+    return;
+  }
+  const int R = is_w ? p.V : *p.count, step = (is_w ? p.gw : gridDim.x - p.gw) * 4;
+  const int64_t ldo = is_w ? p.wcp : p.dp, half = is_w ? p.V * p.wcp : p.hcap * p.dp;
+  for (int64_t r = (is_w ? blockIdx.x : blockIdx.x - p.gw) * 4 + wid; r < R; r += step) {
+    const float* x = is_w ? p.W + r * p.ldw : p.H + p.rows[r] * p.ldh;
+    _Float16* out = (is_w ? p.wo : p.ho) + r * ldo;
+    const int e = is_w ? word_scale(p.wmax[r], lo) : p.eh[r] == ZERO_ROW ? 0 : p.eh[r];
+    const float s = pow2(1.f, e), f[4] = {s, s, s, s};
+    if (is_w && lane == 0) {
+      p.ew[r] = e;
+      if (e != lo) p.sc->wide = 1;
+    }
+#pragma unroll 2
+    for (int c = lane * 4; c < ldo; c += 256) {
+      float v[4];
+      load4(x + c, c, p.D, v);
+      store4(out + c, half, v, f);
+    }
   }
 }
 
@@ -329,24 +433,49 @@ __global__ void __launch_bounds__(256) pad_kernel(const PadP p) {
   }
 }
 
-// the rows that take part, packed
-__global__ void __launch_bounds__(256) pack_kernel(const char* __restrict__ h, int64_t ldh_bytes, const int* __restrict__ rows,
-                                                   const int* __restrict__ count, char* __restrict__ out, int64_t row_bytes, int64_t ldo_bytes) {
-  const int c = *count, m = blockIdx.x;
-  if (m >= c) return;
-  const char* src = h + rows[m] * ldh_bytes;
-  for (int64_t b = threadIdx.x * 16; b < row_bytes; b += 256 * 16) *reinterpret_cast<f32x4*>(out + m * ldo_bytes + b) = *reinterpret_cast<const f32x4*>(src + b);
+// The rows that take part, packed, for the weights' gradient. Operands in halves are packed already; there they are brought to one factor, 2^hlo,
+// since the product sums over the rows (a row's low bits are lost against the largest row's where it is smaller, as in the sum itself).
+struct PackP {
+  const char* h; int64_t ldh, half_in;                             // bytes
+  const int* rows;                                                 // or null: packed already
+  char* out; int64_t ldo, half_out, row_bytes;
+  const int* eh;                                                   // exponents of halves, or null
+};
+__device__ __forceinline__ s16x8 halves_pow2(s16x8 v, int e) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const short x = v[j];                                          // (a bit cast of the vector's element itself reads element 0)
+    v[j] = __builtin_bit_cast(short, (_Float16)pow2((float)__builtin_bit_cast(_Float16, x), e));
+  }
+  return v;
+}
+__device__ __forceinline__ void pack_row(const PackP& p, int m, int hlo) {
+  const char* src = p.h + (p.rows ? p.rows[m] : m) * p.ldh;
+  char* out = p.out + m * p.ldo;
+  for (int64_t b = threadIdx.x * 16; b < p.row_bytes; b += 256 * 16) {
+    if (p.eh) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+        *reinterpret_cast<s16x8*>(out + half * p.half_out + b) = halves_pow2(*reinterpret_cast<const s16x8*>(src + half * p.half_in + b), hlo - p.eh[m]);
+    } else *reinterpret_cast<f32x4*>(out + b) = *reinterpret_cast<const f32x4*>(src + b);
+  }
+}
+__global__ void __launch_bounds__(256) pack_kernel(const PackP p, const int* __restrict__ count, const Grad* __restrict__ gr) {
+  const int m = blockIdx.x;
+  if (m < *count) pack_row(p, m, gr->hlo);
 }
 
 // Bound by memory (65536 x 2048 bf16, 537 MB: 190 us, 2.9 TB/s).
 // out[c][r] = in[row r][c] of 16-bit values, R x C, 64 x 64 at a time through LDS; blockIdx.z: the halves of a pair. `count`: R on the device,
-// and `rows` the row of position r (both or none); positions from R to the next multiple of 64 become zeros. `gate`: only where *gate >= least.
+// and `rows` the row of position r (both or none); positions from R to the next multiple of 64 become zeros. `gate`: only where *gate >= least. `eh`: exponents of
+// positions that are brought to one factor, 2^hlo (pack_kernel), or null.
 struct TransposeP {
   const uint16_t* in; int64_t ldi, half_in;
   uint16_t* out; int64_t ldo, half_out;
   int R, C;
   const int* count; const int* rows;
   const int* gate; int least;
+  const int* eh; const Grad* gr;
 };
 __global__ void __launch_bounds__(256) transpose_kernel(const TransposeP p) {
   __shared__ uint16_t tile[64][64 + 2];
@@ -361,6 +490,7 @@ __global__ void __launch_bounds__(256) transpose_kernel(const TransposeP p) {
   for (int h = 0; h < 2; ++h) {
     s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
     if (src && c0 + q + h * 8 < p.C) v = *reinterpret_cast<const s16x8*>(src + h * 8);      // rows are readable in whole chunks
+    if (src && p.eh) v = halves_pow2(v, p.gr->hlo - p.eh[r0 + r]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) tile[r][q + h * 8 + e] = (uint16_t)v[e];
   }
@@ -381,7 +511,8 @@ __global__ void __launch_bounds__(256) transpose_kernel(const TransposeP p) {
 struct ScoreP {
   Operand H, W;                          // H: [rows, D] (xlim is the count, set on the device); W: columns of the vocabulary
   const void* bias; int bdt;
-  const int* rows; const int* count; const Scales* sc;
+  const int* rows; const int* count;
+  const Scales* sc; const int *eh, *ew;  // operands in halves: exponents per position in `rows` and per word
   const int* lab;                        // per position in `rows`
   int N, D, v0, v1;                      // columns [v0, v1) of the vocabulary
   float invT, smooth_v;                  // 1 / T;  e / V
@@ -391,6 +522,7 @@ struct ScoreP {
   float keep;                            // 1 - e
   char* G; int64_t ldg, glo;             // [v - v0][ldg bytes]: position m at element m; second half glo bytes behind
   char* R; int64_t ldr, rlo;             // the gradient once more, row by row: [m][v - v0] (or null; 256 x 256 tiles)
+  char* G2;                              // operands in halves, smaller tiles: the copy like G for the hidden states' gradient (or null)
   float* colsum; int64_t ldc;            // [row tiles][ldc] column sums of the gradient, or null
   // teacher entries (first != null)
   const unsigned short* first; const int* sidx; const float* psum; float* zk; int K;
@@ -404,11 +536,11 @@ constexpr int larger(int a, int b) { return a > b ? a : b; }
 template <class C> constexpr int score_over(bool grad) {
   return larger(C::STAGES * C::STAGE_BYTES, grad ? C::BN * grad_pitch<C>() : larger(C::WN * 16 * (C::BM + 16), C::BM / C::WM * (C::BN + 4)) * 4);
 }
-template <class C> constexpr int score_lds(bool grad) {
-  return score_over<C>(grad) + (grad ? 4 * C::BM + C::WM * C::BN : C::BM * (1 + 3 * C::WN) + 4 * C::NW + 1) * 4;
-}
+template <class C> constexpr int score_side(bool grad) { return grad ? 4 * C::BM + C::WM * C::BN : C::BM * (1 + 3 * C::WN) + 4 * C::NW + 4; }
+template <class C> constexpr int score_lds(bool grad, int seg) { return score_over<C>(grad) + (score_side<C>(grad) + (seg == 3 ? C::BM : 0)) * 4; }
 
-// The bias is where the accumulators start (-inf for columns past the vocabulary), so that a score is accumulator * zscale.
+// The bias is where the accumulators start (-inf for columns past the vocabulary), so that a score is accumulator * zscale. (Operands in halves:
+// the accumulators are brought to 2^-(eh + ew) * accumulator + bias behind the product.)
 //
 // Statistics: every exponential is taken against ONE reference per quarter wave, the largest score of its 32 rows x 64 columns (on the large
 // tile), instead of the row's maximum: four cross-lane steps in all instead of four per row, and no row waits for its own maximum. A sum of
@@ -433,34 +565,50 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
   const int wm = wid / C::WN, wn = wid - wm * C::WN, lc = lane & 15;
   const int row0 = wm * (C::BM / C::WM) + (lane >> 4) * 4, col0 = wn * (C::BN / C::WN) + lc;
   constexpr int OSZ = C::ESZ, PITCH = grad_pitch<C>(), RW = C::BM / C::WM, CW = C::BN / C::WN;
-  const float zscale = p.sc->z * p.invT * LOG2E;
+  const float zscale = p.invT * LOG2E;
   // the rows' label, coefficient and normaliser: on their way while the product runs
   int lab = -1;
   float rc = 0.f, rl = 3e38f, rq = 0.f;                            // rows past the end: exp2(z - ref) = 0
+  int re = 0;
+  if (SEG == 3 && tid < C::BM) re = p.eh[min(m0 + tid, count - 1)];    // (rows past the end repeat the last one)
   if (tid < C::BM && m0 + tid < count) {
     lab = p.lab[m0 + tid] - n0;
     if constexpr (GRAD) { rc = p.coef[m0 + tid]; rl = p.ref[m0 + tid]; rq = rc * p.inv[m0 + tid]; }
   }
   typename C::acc_t acc[C::TM][C::TN];
-  {
-    float init[C::TN];
+  float bj[C::TN];                                                 // the columns' bias
+  int ej[C::TN];                                                   // and exponents
 #pragma unroll
-    for (int j = 0; j < C::TN; ++j) {
-      const int col = n0 + col0 + j * 16;
-      init[j] = col < p.v1 ? (p.bias ? load_f(p.bias, col, p.bdt) / p.sc->z : 0.f) : NEG_INF;
-    }
+  for (int j = 0; j < C::TN; ++j) {
+    const int col = n0 + col0 + j * 16;
+    bj[j] = col < p.v1 ? (p.bias ? load_f(p.bias, col, p.bdt) : 0.f) : NEG_INF;
+    ej[j] = SEG == 3 && col < p.v1 ? p.ew[col] : 0;
+  }
+  {
     Operand H = p.H;
     H.xlim = count;
-    constexpr int PSEG = SEG == 3 ? 3 : 1;
-    product<C, false, TB, PSEG>(smem, H, p.W, m0, n0, p.D, 0, k_tiles<C, PSEG>(p.D), acc, init);
+    if constexpr (SEG == 3) product<C, false, TB, 3>(smem, H, p.W, m0, n0, p.D, 0, k_tiles<C, 3>(p.D), acc);
+    else product<C, false, TB, 1>(smem, H, p.W, m0, n0, p.D, 0, k_tiles<C, 1>(p.D), acc, bj);
   }
   float* sf = reinterpret_cast<float*>(smem + score_over<C>(GRAD));
   int* slab = reinterpret_cast<int*>(sf);                          // label's column inside the tile, or none of them
+  int* sE = slab + score_side<C>(GRAD);                            // exponents of the rows
   if (tid < C::BM) {
+    if constexpr (SEG == 3) sE[tid] = re;
     slab[tid] = lab < C::BN && lab + n0 < p.v1 ? lab : -1;
     if constexpr (GRAD) { sf[C::BM + tid] = rc; sf[2 * C::BM + tid] = rl; sf[3 * C::BM + tid] = rq; }
   }
   __syncthreads();
+  if constexpr (SEG == 3) {
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) {
+      const i32x4 e = *reinterpret_cast<const i32x4*>(sE + row0 + i * 16);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j) acc[i][j][q] = pow2(acc[i][j][q], -(e[q] + ej[j])) + bj[j];
+    }
+  }
   // a label's score is rare in a wave's part of the tile: whether there is one at all is asked once
   bool labelled = false;
   for (int r = lane; r < RW; r += 64) labelled |= (unsigned)(slab[wm * RW + r] - wn * CW) < (unsigned)CW;
@@ -635,66 +783,88 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
     // there: 255 -> 264 us)
     const bool stream = (int64_t)count * (p.v1 - p.v0) > (32 << 20);
     constexpr int CPR = C::BM * OSZ / 16;
-#pragma unroll
-    for (int half = 0; half < (SEG > 1 ? 2 : 1); ++half) {
-      if (half == 1) __syncthreads();
-#pragma unroll
-      for (int i = 0; i < C::TM; ++i)
+    // copy 0: the gradient; copy 1 (where words have factors): the hidden states' own, times 2^(lo - ew)
+    const bool wide = SEG == 3 && p.sc->wide && (p.R || p.G2);
+    const int lo = SEG == 3 ? lowest_word(p.sc) : 0;
+#pragma unroll 1
+    for (int copy = 0; copy < (SEG == 3 && wide ? 2 : 1); ++copy) {
+      if (SEG == 3 && copy == 1) {
+        __syncthreads();
+        out = p.G2 ? p.G2 + (out - p.G) : nullptr;
 #pragma unroll
         for (int j = 0; j < C::TN; ++j) {
-          Pack v;
+          const float f = n0 + col0 + j * 16 < p.v1 ? pow2(1.f, lo - p.ew[n0 + col0 + j * 16]) : 0.f;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            v[q] = O::cv(acc[i][j][q]);
-            if constexpr (SEG > 1) acc[i][j][q] -= O::fl(v[q]);
-          }
-          *reinterpret_cast<Pack*>(smem + (col0 + j * 16) * PITCH + (row0 + i * 16) * OSZ) = v;
+          for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[i][j][q] *= f;
         }
-      __syncthreads();
-      if (p.first) {
-        // the teacher's entries of this tile, from their exact scores: entries with one index write the same value
-        if (tid < C::BM && m0 + tid < count) {
-          const int n = p.rows[m0 + tid];
-          const int64_t t = nt + p.v0 / C::BN;
-          const int e1 = p.first[(t + 1) * p.N + n];
-          for (int e = p.first[t * p.N + n]; e < e1; ++e) {
-            const int64_t o = (int64_t)n * p.K + e;
-            float g = sf[3 * C::BM + tid] * exp2_(p.zk[o] - sf[2 * C::BM + tid]) - sf[C::BM + tid] * p.psum[o];
-            if (half == 1) g -= O::fl(O::cv(g));
-            *reinterpret_cast<OTy*>(smem + (p.sidx[o] - n0) * PITCH + tid * OSZ) = O::cv(g);
+      }
+#pragma unroll
+      for (int half = 0; half < (SEG > 1 ? 2 : 1); ++half) {
+        if (half == 1) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j) {
+            Pack v;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              v[q] = O::cv(acc[i][j][q]);
+              if constexpr (SEG == 2) acc[i][j][q] -= O::fl(v[q]);
+              else if (half == 1) v[q] = O::cv(acc[i][j][q] - O::fl(v[q]));   // (the accumulators are needed again)
+            }
+            *reinterpret_cast<Pack*>(smem + (col0 + j * 16) * PITCH + (row0 + i * 16) * OSZ) = v;
           }
-        }
         __syncthreads();
-      }
-      char* o = out + half * p.glo;
-      const int rows_there = min(C::BN, p.v1 - n0) * CPR;
-      if (stream) {
-        for (int idx = tid; idx < rows_there; idx += C::NT) {
-          const int v = idx / CPR, ch = idx - v * CPR;
-          __builtin_nontemporal_store(*reinterpret_cast<const f32x4*>(smem + v * PITCH + ch * 16), reinterpret_cast<f32x4*>(o + v * p.ldg + ch * 16));
+        if (p.first) {
+          // the teacher's entries of this tile, from their exact scores: entries with one index write the same value
+          if (tid < C::BM && m0 + tid < count) {
+            const int n = p.rows[m0 + tid];
+            const int64_t t = nt + p.v0 / C::BN;
+            const int e1 = p.first[(t + 1) * p.N + n];
+            for (int e = p.first[t * p.N + n]; e < e1; ++e) {
+              const int64_t o = (int64_t)n * p.K + e;
+              float g = sf[3 * C::BM + tid] * exp2_(p.zk[o] - sf[2 * C::BM + tid]) - sf[C::BM + tid] * p.psum[o];
+              if (SEG == 3 && copy == 1) g = pow2(g, lo - p.ew[p.sidx[o]]);
+              if (half == 1) g -= O::fl(O::cv(g));
+              *reinterpret_cast<OTy*>(smem + (p.sidx[o] - n0) * PITCH + tid * OSZ) = O::cv(g);
+            }
+          }
+          __syncthreads();
         }
-      } else {
-        for (int idx = tid; idx < rows_there; idx += C::NT) {
-          const int v = idx / CPR, ch = idx - v * CPR;
-          *reinterpret_cast<f32x4*>(o + v * p.ldg + ch * 16) = *reinterpret_cast<const f32x4*>(smem + v * PITCH + ch * 16);
+        if (out) {
+          char* o = out + half * p.glo;
+          const int rows_there = min(C::BN, p.v1 - n0) * CPR;
+          if (stream) {
+            for (int idx = tid; idx < rows_there; idx += C::NT) {
+              const int v = idx / CPR, ch = idx - v * CPR;
+              __builtin_nontemporal_store(*reinterpret_cast<const f32x4*>(smem + v * PITCH + ch * 16), reinterpret_cast<f32x4*>(o + v * p.ldg + ch * 16));
+            }
+          } else {
+            for (int idx = tid; idx < rows_there; idx += C::NT) {
+              const int v = idx / CPR, ch = idx - v * CPR;
+              *reinterpret_cast<f32x4*>(o + v * p.ldg + ch * 16) = *reinterpret_cast<const f32x4*>(smem + v * PITCH + ch * 16);
+            }
+          }
         }
-      }
-      if constexpr (is_pp<C>()) {
-        if (p.R) {
-          // rows again: transposing LDS reads give a lane 4 + 4 words of one position; a wave writes 16 positions x 32 words at a time
-          char* orow = p.R + half * p.rlo + (int64_t)m0 * p.ldr + (int64_t)(n0 - p.v0) * OSZ;
-          const int x = lane & 15, g4 = lane >> 4;
-          const char* base = smem + (g4 * 8 + (x >> 2)) * PITCH + (x & 3) * 8;
+        if constexpr (is_pp<C>()) {
+          if (p.R && (!wide || copy == 1)) {
+            // rows again: transposing LDS reads give a lane 4 + 4 words of one position; a wave writes 16 positions x 32 words at a time
+            char* orow = p.R + half * p.rlo + (int64_t)m0 * p.ldr + (int64_t)(n0 - p.v0) * OSZ;
+            const int x = lane & 15, g4 = lane >> 4;
+            const char* base = smem + (g4 * 8 + (x >> 2)) * PITCH + (x & 3) * 8;
 #pragma unroll 4
-          for (int b = wid; b < 128; b += 8) {
-            const int v = (b & 7) * 32, m = (b >> 3) * 16;
-            const char* a0 = base + v * PITCH + m * 2;
-            typedef s16x4 __attribute__((address_space(3))) * lds_ptr_t;
-            const s16x4 t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr_t)(a0));
-            const s16x4 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr_t)(a0 + 4 * PITCH));
-            s16x8 t;
-            t[0] = t0[0]; t[1] = t0[1]; t[2] = t0[2]; t[3] = t0[3]; t[4] = t1[0]; t[5] = t1[1]; t[6] = t1[2]; t[7] = t1[3];
-            *reinterpret_cast<s16x8*>(orow + (int64_t)(m + x) * p.ldr + (v + g4 * 8) * 2) = t;
+            for (int b = wid; b < 128; b += 8) {
+              const int v = (b & 7) * 32, m = (b >> 3) * 16;
+              const char* a0 = base + v * PITCH + m * 2;
+              typedef s16x4 __attribute__((address_space(3))) * lds_ptr_t;
+              const s16x4 t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr_t)(a0));
+              const s16x4 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr_t)(a0 + 4 * PITCH));
+              s16x8 t;
+              t[0] = t0[0]; t[1] = t0[1]; t[2] = t0[2]; t[3] = t0[3]; t[4] = t1[0]; t[5] = t1[1]; t[6] = t1[2]; t[7] = t1[3];
+              *reinterpret_cast<s16x8*>(orow + (int64_t)(m + x) * p.ldr + (v + g4 * 8) * 2) = t;
+            }
           }
         }
       }
@@ -775,11 +945,11 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineP p) {
 
 // ------------------------------------------------------------------------------------------------------------------------ backward
 // Bound by the latency of one workgroup (4096 rows: 7 us).
-// coef[m] = dloss[rows[m]] * T * s with the largest at `top` (0: s = 1). The scores' gradient is rounded to 16 bits: at a label it is close to
+// coef[m] = dloss[rows[m]] * T * s with the largest at `top` (0: s = 1), and gr (eh: exponents of operands in halves, or null). The scores' gradient is rounded to 16 bits: at a label it is close to
 // its coefficient, and with the largest coefficient at a power of two the large ones sit at the end of their binade, where a rounding counts
 // least; fp16 takes 2^14, so that entries down to 2^-38 of the largest stay above its smallest step.
 __global__ void __launch_bounds__(1024) coef_kernel(const float* __restrict__ dloss, const int* __restrict__ rows, const int* __restrict__ count,
-                                                    float T, float top, float* __restrict__ coef, Scales* __restrict__ sc) {
+                                                    float T, float top, const int* __restrict__ eh, float* __restrict__ coef, Grad* __restrict__ gr) {
   __shared__ float red[16];
   const int c = *count;
   float s = 1.f, v[8];                                             // the first 8192 rows stay in registers
@@ -800,40 +970,46 @@ __global__ void __launch_bounds__(1024) coef_kernel(const float* __restrict__ dl
 #pragma unroll
   for (int j = 0; j < 8; ++j) { const int m = j * 1024 + threadIdx.x; if (m < c) coef[m] = v[j] * s; }
   for (int m = 8192 + threadIdx.x; m < c; m += 1024) coef[m] = dloss[rows[m]] * T * s;
-  if (threadIdx.x == 0) { sc->db = 1.f / s; sc->dh = 1.f / s / sc->w; sc->dw = 1.f / s / sc->h; }
+  int hlo = 0;
+  if (eh) {
+    int e = ZERO_ROW;
+    for (int m = threadIdx.x; m < c; m += 1024) e = min(e, eh[m]);
+    hlo = -(int)block_max((float)-e, red);
+  }
+  if (threadIdx.x == 0) *gr = Grad{1.f / s, hlo};
 }
 
 // coef_kernel and pack_kernel in one launch for few rows: a workgroup per row, each finds the largest coefficient for itself
 __global__ void __launch_bounds__(256) prepare_kernel(const float* __restrict__ dloss, const int* __restrict__ rows, const int* __restrict__ count,
-                                                      float T, float top, float* __restrict__ coef, Scales* __restrict__ sc,
-                                                      const char* __restrict__ h, int64_t ldh_bytes, char* __restrict__ out, int64_t row_bytes,
-                                                      int64_t ldo_bytes) {
+                                                      float T, float top, const int* __restrict__ eh, float* __restrict__ coef, Grad* __restrict__ gr,
+                                                      const PackP p) {
   __shared__ float red[16];
   const int c = *count, m = blockIdx.x;
   if (m >= c && m > 0) return;
   float s = 1.f;
+  int hlo = 0;
   if (top > 0.f) {
     float mx = 0.f;
+    int e = ZERO_ROW;
     for (int k = threadIdx.x; k < c; k += 256) {
       const float v = fabsf(dloss[rows[k]] * T);
       if (v < __builtin_inff()) mx = fmaxf(mx, v);
+      if (eh) e = min(e, eh[k]);
     }
     mx = block_max(mx, red);
     if (mx > 0.f) s = fminf(top / mx, 1e37f);
+    if (eh) hlo = -(int)block_max((float)-e, red);
   }
-  if (m == 0 && threadIdx.x == 0) { sc->db = 1.f / s; sc->dh = 1.f / s / sc->w; sc->dw = 1.f / s / sc->h; }
+  if (m == 0 && threadIdx.x == 0) *gr = Grad{1.f / s, hlo};
   if (m >= c) return;
-  const int n = rows[m];
-  if (threadIdx.x == 0) coef[m] = dloss[n] * T * s;
-  const char* src = h + n * ldh_bytes;
-  if (out)
-    for (int64_t b = threadIdx.x * 16; b < row_bytes; b += 256 * 16) *reinterpret_cast<f32x4*>(out + m * ldo_bytes + b) = *reinterpret_cast<const f32x4*>(src + b);
+  if (threadIdx.x == 0) coef[m] = dloss[rows[m]] * T * s;
+  if (p.out) pack_row(p, m, hlo);
 }
 
 // db from the gradient itself (both halves): with teacher entries the tiles' column sums do not hold them. Eight lanes to a word, 16 bytes each at a
 // time. Bound by reading the gradient (96 rows x 30522 words in halves: 6.6 us; a wave to a word, two bytes a lane, took 10.4).
 __global__ void __launch_bounds__(256) bias_rows_kernel(const char* __restrict__ G, int64_t ldg, int64_t glo, int dt, int vc, const int* __restrict__ count,
-                                                        const Scales* __restrict__ sc, void* __restrict__ db, int bdt) {
+                                                        const Grad* __restrict__ gr, void* __restrict__ db, int bdt) {
   const int v = blockIdx.x * 32 + (threadIdx.x >> 3), c = *count, ch = dt == DT_F32 ? 4 : 8;
   float s = 0.f;
   auto add = [&](const char* at, int m) {
@@ -862,7 +1038,7 @@ __global__ void __launch_bounds__(256) bias_rows_kernel(const char* __restrict__
   s += __shfl_xor(s, 4, 64);
   s += __shfl_xor(s, 2, 64);
   s += __shfl_xor(s, 1, 64);
-  if (v < vc && (threadIdx.x & 7) == 0) store_f(db, v, bdt, s * sc->db);
+  if (v < vc && (threadIdx.x & 7) == 0) store_f(db, v, bdt, s * gr->inv);
 }
 
 // dh: unit u of the grid owns output tile u % tiles and share u / tiles of the piece's columns; its fp32 tile lives in slab u and is added
@@ -871,6 +1047,7 @@ __global__ void __launch_bounds__(256) bias_rows_kernel(const char* __restrict__
 // Large tile, W by rows ([V, D]): read as it is (K-major, transposing LDS reads), or transposed first where `many` rows pay for that.
 struct DhP {
   Operand G, W, WT;
+  const char* wide_g; const Scales* sc;  // operands in halves: the gradient's copy for words with factors (or null)
   int many;
   const int* count;
   int D, vc, units, most, accum;         // most: shares at most (each has some k-tiles to work on)
@@ -910,6 +1087,7 @@ __global__ void __launch_bounds__(C::NT) dh_kernel(const DhP p) {
   const int k0 = min(ktiles, share * per), k1 = min(ktiles, k0 + per);
   typename C::acc_t acc[C::TM][C::TN];
   Operand G = p.G;
+  if (SEG == 3 && p.wide_g && p.sc->wide) G.p = p.wide_g;
   G.xlim = (count + 7) & ~7;                                       // (whole chunks; what lies behind is not read)
   if (is_pp<C>() && TB && count >= p.many) product<C, TA, false, SEG>(smem, G, p.WT, mt * C::BM, nt * C::BN, p.vc, k0, k1, acc);
   else product<C, TA, TB, SEG>(smem, G, p.W, mt * C::BM, nt * C::BN, p.vc, k0, k1, acc);
@@ -921,7 +1099,8 @@ __global__ void __launch_bounds__(C::NT) dh_kernel(const DhP p) {
 // to each wave (96 rows x 768 from 85 shares 12.9 and 8.0 us; 4096 x 1024 from 4 shares 20.6 and 24.7).
 // Those behind them 256 words of db = scale * sum over the row tiles' column sums.
 struct FinishP {
-  const float* slab; const int* rows; const int* count; const Scales* sc;
+  const float* slab; const int* rows; const int* count;
+  const Scales* sc; const Grad* gr;      // sc: of operands in halves, or null
   int N, D, units, most, blocks;         // blocks of a row
   void* dh; int dt;
   const float* colsum; int bm; int V;
@@ -937,7 +1116,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishP p) {
     float s = 0.f;
 #pragma unroll 4
     for (int t = 0; t < tiles; ++t) s += p.colsum[(int64_t)t * p.V + v];
-    store_f(p.db, v, p.bdt, s * p.sc->db);
+    store_f(p.db, v, p.bdt, s * p.gr->inv);
     return;
   }
   const int m = blockIdx.x / p.blocks, b = blockIdx.x - m * p.blocks;
@@ -961,7 +1140,10 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishP p) {
     if (wid > 0) return;
     v = (v + quarter[0][lane]) + (quarter[1][lane] + quarter[2][lane]);
   }
-  v *= p.sc->dh;
+  const int lo = p.sc ? lowest_word(p.sc) : 0;
+  const float inv = p.gr->inv;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = pow2(v[j], -lo) * inv;
   const int64_t o = (int64_t)p.rows[m] * p.D + d;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -973,7 +1155,8 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishP p) {
 // shares > 1 (small outputs): the rows' range is cut, fp32 tiles go to a slab and dw_sum_kernel adds them in order.
 struct DwP {
   Operand G, H;
-  const int* count; const Scales* sc;
+  const int* count;
+  const Grad* gr;
   void* out; int64_t ldo;
   int D, vc, shares;
   float* slab;
@@ -993,10 +1176,19 @@ __global__ void __launch_bounds__(C::NT) dw_kernel(const DwP p) {
   typename C::acc_t acc[C::TM][C::TN];
   product<C, SWAP && !is_pp<C>(), !SWAP && !is_pp<C>(), SEG>(smem, SWAP ? p.H : p.G, SWAP ? p.G : p.H, m0, n0, K, k0, k1, acc);
   if (p.shares > 1) { to_slab<C>(p.slab + (int64_t)u * C::BM * C::BN, acc, false); return; }
+  if constexpr (SEG == 3) {                                        // the rows' factor
+    const int e = -p.gr->hlo;
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[i][j][q] = pow2(acc[i][j][q], e);
+  }
   if constexpr (is_pp<C>() && OT == OT_F32) {                      // an fp32 tile is more than LDS: stores of 16 columns from the accumulators
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, wm = wid / C::WN, wn = wid - wm * C::WN;
     const int r0 = m0 + wm * (C::BM / C::WM) + (lane >> 4) * 4, c0 = n0 + wn * (C::BN / C::WN) + (lane & 15);
-    const float s = p.sc->dw;
+    const float s = p.gr->inv;
 #pragma unroll
     for (int i = 0; i < C::TM; ++i)
 #pragma unroll
@@ -1008,14 +1200,14 @@ __global__ void __launch_bounds__(C::NT) dw_kernel(const DwP p) {
   }
   EpiP e;
   e.out = p.out; e.residual = nullptr; e.bias = nullptr; e.stats = nullptr; e.stat_shift = nullptr;
-  e.alpha = p.sc->dw; e.act = ACT_KEEP; e.accum = 0;
+  e.alpha = p.gr->inv; e.act = ACT_KEEP; e.accum = 0;
   const int64_t ldo = p.ldo;
   epilogue_impl<C, OT, ACT_KEEP, 0>(smem, acc, mt, n0, N, M - m0, e, [=](int r) -> int64_t {
     return m0 + r < M ? (int64_t)(m0 + r) * ldo + n0 : (int64_t)-1;
   });
 }
 template <int BM, int BN>
-__global__ void __launch_bounds__(256) dw_sum_kernel(const float* __restrict__ slab, int shares, int M, int N, const Scales* __restrict__ sc,
+__global__ void __launch_bounds__(256) dw_sum_kernel(const float* __restrict__ slab, int shares, int M, int N, const Grad* __restrict__ gr,
                                                      void* __restrict__ out, int64_t ldo, int dt) {
   const int mtiles = (M + BM - 1) / BM, ntiles = (N + BN - 1) / BN, tiles = mtiles * ntiles;
   const int m = blockIdx.x, mt = m / BM, g = mt / 8, rowsg = min(8, mtiles - g * 8);
@@ -1025,7 +1217,7 @@ __global__ void __launch_bounds__(256) dw_sum_kernel(const float* __restrict__ s
     float v = 0.f;
 #pragma unroll 4
     for (int k = 0; k < shares; ++k) v += x[(int64_t)k * tiles * BM * BN];
-    store_f(out, (int64_t)m * ldo + n, dt, v * sc->dw);
+    store_f(out, (int64_t)m * ldo + n, dt, pow2(v, -gr->hlo) * gr->inv);
   }
 }
 
@@ -1062,6 +1254,7 @@ struct Plan {
   int pieces, step;
   int units, most, shares;
   bool quarters;                         // finish_kernel
+  bool pack;                             // dW: the rows of H that take part are packed first (halves: brought to one factor)
   int64_t gcols;
 };
 
@@ -1116,6 +1309,7 @@ Plan plan(const Args& a) {
   p.many = 6144;
   p.wtr = a.want_h && p.nt && !a.wt && a.N >= p.many;
   p.pair = bits16 && !a.split && a.N <= 256;                       // (see score_kernel)
+  p.pack = a.want_w && !p.nt && !p.pad_h;
   const int seg = a.split ? 3 : p.pair ? 2 : 1, bk = bits16 ? 64 : 32;
   const int64_t vk = seg * (up(p.step, bk) / bk), nk = seg * (up(a.N, bk) / bk);   // k-tiles of the two products' sums
   const int64_t cols = p.gcols < a.V ? p.gcols : a.V;
@@ -1146,7 +1340,7 @@ struct Carve {
   }
 };
 struct State {
-  Scales* sc; int *count, *rows, *lab; float *ref, *inv;
+  Scales* sc; int *count, *rows, *lab; float *ref, *inv; int *eh, *ew;
   int* sidx; float *sp, *psum, *zk, *ent, *mass; unsigned short* first;
   char *wo, *ho;
   int64_t bytes;
@@ -1158,25 +1352,27 @@ struct State {
     ent = c.take<float>(a.K ? a.N : 0); mass = c.take<float>(a.K ? a.N : 0);
     first = c.take<unsigned short>(a.K ? (int64_t)(p.tiles + 1) * a.N : 0);
     const int64_t esz = a.dt == DT_F32 ? 4 : 2;                    // (two halves take as much as an fp32 value)
+    eh = c.take<int>(a.split ? a.N : 0); ew = c.take<int>(a.split ? a.V : 0);
     wo = c.take<char>(a.split || p.pad_w ? p.wrows * p.wcp * esz : 0);
     ho = c.take<char>(a.split || p.pad_h ? p.np * p.dp * esz : 0);
     bytes = c.at;
   }
 };
 struct Work {
-  float2* part; float *tz, *zs, *amax;                           // forward
-  float *coef, *colsum; char* G; char* packed; uint16_t *ht, *wtr; float *dh_slab, *dw_slab;  // backward
+  float2* part; float *tz, *zs, *wmax, *tops;                         // forward
+  Grad* gr; float *coef, *colsum; char* G; char* packed; uint16_t *ht, *wtr; float *dh_slab, *dw_slab;  // backward
   int64_t fwd, bwd;
   Work(const Args& a, const Plan& p) {
     Carve c(a.ws);
     part = c.take<float2>((int64_t)p.tiles * a.N); tz = c.take<float>(a.N); zs = c.take<float>((int64_t)p.tiles * a.N);
-    amax = c.take<float>(a.split ? AMAX_W + AMAX_H : 0);
+    wmax = c.take<float>(a.split ? a.V * (a.wt ? CHUNKS : 1) : 0);
+    tops = c.take<float>(a.split ? AMAX_W : 0);
     fwd = c.at;
     c.at = 0;
     const int64_t esz = a.dt == DT_F32 ? 4 : 2;
-    coef = c.take<float>(a.N); G = c.take<char>(p.np * p.gcols * esz * (p.nt || p.pair ? 2 : 1));
+    gr = c.take<Grad>(1); coef = c.take<float>(a.N); G = c.take<char>(p.np * p.gcols * esz * (p.nt || p.pair || (a.split && a.want_h) ? 2 : 1));
     colsum = c.take<float>(a.want_b && !a.K ? (a.N + p.bm - 1) / p.bm * a.V : 0);
-    packed = c.take<char>(a.want_w && !a.split && !p.nt && !p.pad_h ? a.N * p.dp * esz : 0);
+    packed = c.take<char>(p.pack ? a.N * p.dp * esz : 0);
     ht = c.take<uint16_t>(a.want_w && p.nt ? a.D * p.np * (a.split ? 2 : 1) : 0);
     wtr = c.take<uint16_t>(p.wtr ? a.D * p.vp * (a.split ? 2 : 1) : 0);
     const int64_t ht = tile_rows(p.dh_tile), wt = tile_rows(p.dw_tile), cols = p.gcols < a.V ? p.gcols : a.V;
@@ -1191,7 +1387,7 @@ struct Work {
 template <class C, bool TB, bool GRAD, int SEG> int launch_score(const ScoreP& p, hipStream_t st) {
   const int64_t grid = (int64_t)((p.N + C::BM - 1) / C::BM) * ((p.v1 - p.v0 + C::BN - 1) / C::BN);
   if (grid > 0x7fffffff) return -2;
-  constexpr int LDS = score_lds<C>(GRAD);
+  constexpr int LDS = score_lds<C>(GRAD, SEG);
   static_assert(LDS <= 160 * 1024, "tile does not fit the 160 KiB LDS");
   static DeviceOnceLds once;
   once.ensure(reinterpret_cast<const void*>(&score_kernel<C, TB, GRAD, SEG>), LDS);
@@ -1253,7 +1449,7 @@ template <class C, int OT, bool SWAP, int SEG> int launch_dw(const DwP& p, hipSt
   hipLaunchKernelGGL((dw_kernel<C, OT, SWAP, SEG>), dim3(tiles * p.shares), dim3(C::NT), LDS, st, p);
   VL_CHECK();
   if (p.shares > 1)
-    hipLaunchKernelGGL((dw_sum_kernel<C::BM, C::BN>), dim3(M), dim3(256), 0, st, p.slab, p.shares, M, N, p.sc, p.out, p.ldo,
+    hipLaunchKernelGGL((dw_sum_kernel<C::BM, C::BN>), dim3(M), dim3(256), 0, st, p.slab, p.shares, M, N, p.gr, p.out, p.ldo,
                        OT == OT_F32 ? (int)DT_F32 : OT == OT_F16 ? (int)DT_F16 : (int)DT_BF16);
   return (int)hipGetLastError();
 }
@@ -1296,7 +1492,7 @@ void operands(const Args& a, const Plan& p, const State& s, Operand& H, Operand&
 
 ScoreP score_args(const Args& a, const State& s, const float* f) {
   ScoreP q = {};
-  q.bias = a.bias; q.bdt = (int)a.bdt; q.rows = s.rows; q.count = s.count; q.sc = s.sc;
+  q.bias = a.bias; q.bdt = (int)a.bdt; q.rows = s.rows; q.count = s.count; q.sc = s.sc; q.eh = s.eh; q.ew = s.ew;
   q.lab = s.lab;
   q.N = (int)a.N; q.D = (int)a.D;
   q.invT = 1.f / f[0]; q.smooth_v = f[1] / (float)a.V; q.keep = 1.f - f[1];
@@ -1320,12 +1516,13 @@ int forward(const Args& a, const float* f, hipStream_t st) {
   hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, a.K ? nullptr : a.labels, (int)a.lab64, a.ignore, s.mass, (int)a.N, (int)a.V, s.rows, s.lab, s.count, s.sc, a.loss);
   VL_CHECK();
   if (a.split) {
-    const int wr = (int)p.wrows, wc = (int)(a.wt ? a.V : a.D);
-    hipLaunchKernelGGL(amax_kernel, dim3(AMAX_W + AMAX_H), dim3(256), 0, st, (const float*)a.W, a.ldw, wr, wc, (const float*)a.H, a.ldh, (int)a.D, s.rows,
-                       s.count, w.amax);
+    const int chunks = (int)(a.D < CHUNKS ? 1 : CHUNKS);             // ([D, V]: cuts of the rows)
+    const int64_t units = up(a.V, 256) / 256 * chunks;
+    SplitP q{(const float*)a.W, a.ldw, (int)a.wt, (int)a.V, (int)a.D, (_Float16*)s.wo, p.wcp, (const float*)a.H, a.ldh, (_Float16*)s.ho, p.dp, p.np,
+             s.rows, s.count, s.sc, s.eh, s.ew, w.wmax, chunks, w.tops, (int)(a.wt && units < AMAX_W ? units : AMAX_W)};
+    hipLaunchKernelGGL(amax_kernel, dim3(q.gw + 256), dim3(256), 0, st, q);
     VL_CHECK();
-    SplitP q{(const float*)a.W, a.ldw, wr, wc, (int)p.wcp, (_Float16*)s.wo, (const float*)a.H, a.ldh, (int)a.D, (int)p.dp, (_Float16*)s.ho, (int)p.np, s.rows, s.count, w.amax, s.sc, 2048};
-    hipLaunchKernelGGL(split_kernel, dim3(2048 + 256), dim3(256), 0, st, q);
+    hipLaunchKernelGGL(split_kernel, dim3(q.gw + 256), dim3(256), 0, st, q);
     VL_CHECK();
   }
   if (p.pad_w || p.pad_h) {
@@ -1360,27 +1557,27 @@ int backward(const Args& a, const float* f, hipStream_t st) {
   const State s(a, p);
   const Work w(a, p);
   const int esz = a.dt == DT_F32 ? 4 : 2, gsz = a.split ? 2 : esz;
-  const float top = p.op == DT_F16 ? 16384.f : p.op == DT_BF16 ? 1.f : 0.f;
+  const float top = a.split ? 32768.f : p.op == DT_F16 ? 16384.f : p.op == DT_BF16 ? 1.f : 0.f;
   Operand H, W;
   operands(a, p, s, H, W);
   Operand packed = H;
-  const int64_t rb = up(a.D, 16 / esz) * esz;
-  const bool pack = a.want_w && !a.split && !p.nt && !p.pad_h;
+  const int* eh = a.split ? s.eh : nullptr;
+  PackP pk{H.p, H.ld, H.lo, H.rows, p.pack ? w.packed : nullptr, p.dp * gsz, a.split ? a.N * p.dp * 2 : 0, p.dp * gsz, eh};
+  if (!a.split) pk.row_bytes = up(a.D, 16 / esz) * esz;
   if (a.N <= 1024) {
-    hipLaunchKernelGGL(prepare_kernel, dim3((unsigned)a.N), dim3(256), 0, st, a.dloss, s.rows, s.count, f[0], top, w.coef, s.sc, (const char*)a.H, a.ldh * esz,
-                       pack ? w.packed : nullptr, rb, p.dp * esz);
+    hipLaunchKernelGGL(prepare_kernel, dim3((unsigned)a.N), dim3(256), 0, st, a.dloss, s.rows, s.count, f[0], top, eh, w.coef, w.gr, pk);
     VL_CHECK();
   } else {
-    hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, st, a.dloss, s.rows, s.count, f[0], top, w.coef, s.sc);
+    hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, st, a.dloss, s.rows, s.count, f[0], top, eh, w.coef, w.gr);
     VL_CHECK();
-    if (pack) {
-      hipLaunchKernelGGL(pack_kernel, dim3((unsigned)a.N), dim3(256), 0, st, (const char*)a.H, a.ldh * esz, s.rows, s.count, w.packed, rb, p.dp * esz);
+    if (p.pack) {
+      hipLaunchKernelGGL(pack_kernel, dim3((unsigned)a.N), dim3(256), 0, st, pk, s.count, w.gr);
       VL_CHECK();
     }
   }
-  if (pack) packed = Operand{w.packed, p.dp * esz, 0, 0, nullptr};
+  if (p.pack) packed = Operand{w.packed, pk.ldo, pk.half_out, 0, nullptr};
   if (a.want_w && p.nt) {
-    TransposeP t{(const uint16_t*)H.p, H.ld / 2, H.lo / 2, w.ht, p.np, a.D * p.np, (int)a.N, (int)a.D, s.count, H.rows, nullptr, 0};
+    TransposeP t{(const uint16_t*)H.p, H.ld / 2, H.lo / 2, w.ht, p.np, a.D * p.np, (int)a.N, (int)a.D, s.count, H.rows, nullptr, 0, eh, w.gr};
     hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)((a.N + 63) / 64), (unsigned)((a.D + 63) / 64), a.split ? 2 : 1), dim3(256), 0, st, t);
     VL_CHECK();
     packed = Operand{(const char*)w.ht, p.np * 2, a.split ? a.D * p.np * 2 : 0, 0, nullptr};
@@ -1388,14 +1585,14 @@ int backward(const Args& a, const float* f, hipStream_t st) {
   packed.xlim = (int)a.D;
   Operand wt = W;                                                  // W along the sum's axis of the dh product
   if (p.wtr) {
-    TransposeP t{(const uint16_t*)W.p, W.ld / 2, W.lo / 2, w.wtr, p.vp, a.D * p.vp, (int)a.V, (int)a.D, nullptr, nullptr, s.count, p.many};
+    TransposeP t{(const uint16_t*)W.p, W.ld / 2, W.lo / 2, w.wtr, p.vp, a.D * p.vp, (int)a.V, (int)a.D, nullptr, nullptr, s.count, p.many, nullptr, nullptr};
     hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)((a.V + 63) / 64), (unsigned)((a.D + 63) / 64), a.split ? 2 : 1), dim3(256), 0, st, t);
     VL_CHECK();
     wt = Operand{(const char*)w.wtr, p.vp * 2, a.split ? a.D * p.vp * 2 : 0, (int)a.D, nullptr};
   }
   const int64_t ldg = p.np * gsz, glo = a.split || p.pair ? p.gcols * ldg : 0;
   const int64_t ldr = p.gcols * gsz, rlo = a.split ? p.np * ldr : 0;   // the same row by row (p.nt)
-  char* rows_g = w.G + p.np * p.gcols * esz;
+  char* rows_g = w.G + p.np * p.gcols * esz;                       // that layout, or the copy G2
   for (int k = 0; k < p.pieces; ++k) {
     const int v0 = k * p.step, v1 = (int)(a.V < v0 + (int64_t)p.step ? a.V : v0 + p.step), vc = v1 - v0;
     ScoreP q = score_args(a, s, f);
@@ -1403,10 +1600,11 @@ int backward(const Args& a, const float* f, hipStream_t st) {
     q.W.xlim = (int)a.V;
     q.v0 = v0; q.v1 = v1; q.ref = s.ref; q.inv = s.inv; q.coef = w.coef; q.G = w.G; q.ldg = ldg; q.glo = glo;
     if (p.nt && a.want_h) { q.R = rows_g; q.ldr = ldr; q.rlo = rlo; }
+    else if (a.split && a.want_h) q.G2 = rows_g;
     if (a.want_b && !a.K) { q.colsum = w.colsum; q.ldc = a.V; }
     if (const int e = scores<true>(q, p.tile, p.op, a.split, p.pair, a.wt, st)) return e;
     if (a.want_b && a.K) {
-      hipLaunchKernelGGL(bias_rows_kernel, dim3((vc + 31) / 32), dim3(256), 0, st, w.G, ldg, glo, a.split ? (int)DT_F16 : (int)a.dt, vc, s.count, s.sc,
+      hipLaunchKernelGGL(bias_rows_kernel, dim3((vc + 31) / 32), dim3(256), 0, st, w.G, ldg, glo, a.split ? (int)DT_F16 : (int)a.dt, vc, s.count, w.gr,
                          (char*)a.db + (int64_t)v0 * (a.bdt == DT_F32 ? 4 : 2), (int)a.bdt);
       VL_CHECK();
     }
@@ -1414,6 +1612,7 @@ int backward(const Args& a, const float* f, hipStream_t st) {
     if (a.want_h) {
       DhP d;
       d.G = p.nt ? Operand{rows_g, ldr, rlo, 0, nullptr} : G;
+      d.wide_g = q.G2; d.sc = s.sc;
       d.W = W;
       d.W.p += a.wt ? (int64_t)v0 * gsz : v0 * W.ld;
       d.W.xlim = (int)a.D;
@@ -1427,7 +1626,7 @@ int backward(const Args& a, const float* f, hipStream_t st) {
     if (a.want_w) {
       DwP d;
       d.G = G; d.G.xlim = vc;
-      d.H = packed; d.count = s.count; d.sc = s.sc;
+      d.H = packed; d.count = s.count; d.gr = w.gr;
       d.out = (char*)a.dw + (a.wt ? (int64_t)v0 : v0 * a.D) * esz;
       d.ldo = a.wt ? a.V : a.D;
       d.D = (int)a.D; d.vc = vc; d.shares = p.shares; d.slab = w.dw_slab;
@@ -1439,7 +1638,7 @@ int backward(const Args& a, const float* f, hipStream_t st) {
   if (a.want_h || sums) {
     const int64_t cols = p.quarters ? 256 : 1024, blocks = (a.D + cols - 1) / cols;
     if (a.N * blocks + (a.V + 255) / 256 > 0x7fffffff) return -2;
-    const FinishP q{w.dh_slab, s.rows, s.count, s.sc, a.want_h ? (int)a.N : 0, (int)a.D, p.units, p.most, (int)blocks, a.dh, (int)a.dt, w.colsum, p.bm, (int)a.V, a.db, (int)a.bdt};
+    const FinishP q{w.dh_slab, s.rows, s.count, a.split ? s.sc : nullptr, w.gr, a.want_h ? (int)a.N : 0, (int)a.D, p.units, p.most, (int)blocks, a.dh, (int)a.dt, w.colsum, p.bm, (int)a.V, a.db, (int)a.bdt};
     const dim3 grid((unsigned)(q.N * blocks + (sums ? (a.V + 255) / 256 : 0)));
     if (p.dh_tile == TILE_BIG) launch_finish<256>(q, p.quarters, grid, st);
     else if (p.dh_tile == TILE_SMALL) launch_finish<64>(q, p.quarters, grid, st);
