@@ -86,8 +86,9 @@ __device__ __forceinline__ int word_scale(float m, int lo) { return m > 0.f ? lo
 // What the backward pass multiplies its products with.
 struct Grad {
   float inv;        // gradients = inv * product (sum)
-  int hlo;          // dW: exponent of the rows' factors, all brought to the one of the largest row
+  int hlo;          // dW: exponent of the rows' factors, all brought to the one of the row that counts most
 };
+constexpr int NO_ROW = 254;                                        // the exponent of a row that adds nothing to dW
 __device__ __forceinline__ float pow2(float v, int e) { return __builtin_amdgcn_ldexpf(v, e); }
 
 // ------------------------------------------------------------------------------------------------------------------------ rows
@@ -433,13 +434,13 @@ __global__ void __launch_bounds__(256) pad_kernel(const PadP p) {
   }
 }
 
-// The rows that take part, packed, for the weights' gradient. Operands in halves are packed already; there they are brought to one factor, 2^hlo,
-// since the product sums over the rows (a row's low bits are lost against the largest row's where it is smaller, as in the sum itself).
+// The rows that take part, packed, for the weights' gradient. fp16 values and halves are brought to one factor, 2^hlo, since the product sums
+// over the rows (a row's low bits are lost against the row's that counts most where it counts less, as in the sum itself).
 struct PackP {
   const char* h; int64_t ldh, half_in;                             // bytes
   const int* rows;                                                 // or null: packed already
   char* out; int64_t ldo, half_out, row_bytes;
-  const int* eh;                                                   // exponents of halves, or null
+  int halves;                                                      // 1 or 2
 };
 __device__ __forceinline__ s16x8 halves_pow2(s16x8 v, int e) {
 #pragma unroll
@@ -449,25 +450,23 @@ __device__ __forceinline__ s16x8 halves_pow2(s16x8 v, int e) {
   }
   return v;
 }
-__device__ __forceinline__ void pack_row(const PackP& p, int m, int hlo) {
+__device__ __forceinline__ void pack_row(const PackP& p, int m, int e) {
   const char* src = p.h + (p.rows ? p.rows[m] : m) * p.ldh;
   char* out = p.out + m * p.ldo;
-  for (int64_t b = threadIdx.x * 16; b < p.row_bytes; b += 256 * 16) {
-    if (p.eh) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-        *reinterpret_cast<s16x8*>(out + half * p.half_out + b) = halves_pow2(*reinterpret_cast<const s16x8*>(src + half * p.half_in + b), hlo - p.eh[m]);
-    } else *reinterpret_cast<f32x4*>(out + b) = *reinterpret_cast<const f32x4*>(src + b);
-  }
+  for (int half = 0; half < p.halves; ++half)
+    for (int64_t b = threadIdx.x * 16; b < p.row_bytes; b += 256 * 16) {
+      const s16x8 v = *reinterpret_cast<const s16x8*>(src + half * p.half_in + b);
+      *reinterpret_cast<s16x8*>(out + half * p.half_out + b) = e == 0 ? v : halves_pow2(v, e);
+    }
 }
-__global__ void __launch_bounds__(256) pack_kernel(const PackP p, const int* __restrict__ count, const Grad* __restrict__ gr) {
+__global__ void __launch_bounds__(256) pack_kernel(const PackP p, const int* __restrict__ count, const int* __restrict__ t, const Grad* __restrict__ gr) {
   const int m = blockIdx.x;
-  if (m < *count) pack_row(p, m, gr->hlo);
+  if (m < *count) pack_row(p, m, t ? gr->hlo - t[m] : 0);
 }
 
 // Bound by memory (65536 x 2048 bf16, 537 MB: 190 us, 2.9 TB/s).
 // out[c][r] = in[row r][c] of 16-bit values, R x C, 64 x 64 at a time through LDS; blockIdx.z: the halves of a pair. `count`: R on the device,
-// and `rows` the row of position r (both or none); positions from R to the next multiple of 64 become zeros. `gate`: only where *gate >= least. `eh`: exponents of
+// and `rows` the row of position r (both or none); positions from R to the next multiple of 64 become zeros. `gate`: only where *gate >= least. `t`: exponents of
 // positions that are brought to one factor, 2^hlo (pack_kernel), or null.
 struct TransposeP {
   const uint16_t* in; int64_t ldi, half_in;
@@ -475,7 +474,7 @@ struct TransposeP {
   int R, C;
   const int* count; const int* rows;
   const int* gate; int least;
-  const int* eh; const Grad* gr;
+  const int* t; const Grad* gr;
 };
 __global__ void __launch_bounds__(256) transpose_kernel(const TransposeP p) {
   __shared__ uint16_t tile[64][64 + 2];
@@ -490,7 +489,7 @@ __global__ void __launch_bounds__(256) transpose_kernel(const TransposeP p) {
   for (int h = 0; h < 2; ++h) {
     s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
     if (src && c0 + q + h * 8 < p.C) v = *reinterpret_cast<const s16x8*>(src + h * 8);      // rows are readable in whole chunks
-    if (src && p.eh) v = halves_pow2(v, p.gr->hlo - p.eh[r0 + r]);
+    if (src && p.t) v = halves_pow2(v, p.gr->hlo - p.t[r0 + r]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) tile[r][q + h * 8 + e] = (uint16_t)v[e];
   }
@@ -518,7 +517,7 @@ struct ScoreP {
   float invT, smooth_v;                  // 1 / T;  e / V
   float2* part; float* tz; float* zs;    // statistics: part [ntiles][N]; target score [N]; zs [ntiles][N] = sum of z * e / V (or null)
   // gradient, per position in `rows`: coefficient; q = exp2(z - ref) * inv
-  const float* ref; const float* inv; const float* coef;
+  const float* ref; const float* inv; const float* coef; const int* g;   // g: exponents inside the coefficients (fp16, halves)
   float keep;                            // 1 - e
   char* G; int64_t ldg, glo;             // [v - v0][ldg bytes]: position m at element m; second half glo bytes behind
   char* R; int64_t ldr, rlo;             // the gradient once more, row by row: [m][v - v0] (or null; 256 x 256 tiles)
@@ -537,7 +536,9 @@ template <class C> constexpr int score_over(bool grad) {
   return larger(C::STAGES * C::STAGE_BYTES, grad ? C::BN * grad_pitch<C>() : larger(C::WN * 16 * (C::BM + 16), C::BM / C::WM * (C::BN + 4)) * 4);
 }
 template <class C> constexpr int score_side(bool grad) { return grad ? 4 * C::BM + C::WM * C::BN : C::BM * (1 + 3 * C::WN) + 4 * C::NW + 4; }
-template <class C> constexpr int score_lds(bool grad, int seg) { return score_over<C>(grad) + (score_side<C>(grad) + (seg == 3 ? C::BM : 0)) * 4; }
+template <class C> constexpr int score_lds(bool grad, int seg) {
+  return score_over<C>(grad) + (score_side<C>(grad) + (seg == 3 ? C::BM : 0) + (grad && C::DT == DT_F16 ? C::BM : 0)) * 4;
+}
 
 // The bias is where the accumulators start (-inf for columns past the vocabulary), so that a score is accumulator * zscale. (Operands in halves:
 // the accumulators are brought to 2^-(eh + ew) * accumulator + bias behind the product.)
@@ -570,10 +571,12 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
   int lab = -1;
   float rc = 0.f, rl = 3e38f, rq = 0.f;                            // rows past the end: exp2(z - ref) = 0
   int re = 0;
+  float rg = 1.f;
   if (SEG == 3 && tid < C::BM) re = p.eh[min(m0 + tid, count - 1)];    // (rows past the end repeat the last one)
   if (tid < C::BM && m0 + tid < count) {
     lab = p.lab[m0 + tid] - n0;
     if constexpr (GRAD) { rc = p.coef[m0 + tid]; rl = p.ref[m0 + tid]; rq = rc * p.inv[m0 + tid]; }
+    if (GRAD && C::DT == DT_F16) rg = pow2(1.f, -p.g[m0 + tid]);
   }
   typename C::acc_t acc[C::TM][C::TN];
   float bj[C::TN];                                                 // the columns' bias
@@ -593,8 +596,10 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
   float* sf = reinterpret_cast<float*>(smem + score_over<C>(GRAD));
   int* slab = reinterpret_cast<int*>(sf);                          // label's column inside the tile, or none of them
   int* sE = slab + score_side<C>(GRAD);                            // exponents of the rows
+  float* sG = sf + score_side<C>(GRAD) + (SEG == 3 ? C::BM : 0);   // 2^-g
   if (tid < C::BM) {
     if constexpr (SEG == 3) sE[tid] = re;
+    if constexpr (GRAD && C::DT == DT_F16) sG[tid] = rg;
     slab[tid] = lab < C::BN && lab + n0 < p.v1 ? lab : -1;
     if constexpr (GRAD) { sf[C::BM + tid] = rc; sf[2 * C::BM + tid] = rl; sf[3 * C::BM + tid] = rq; }
   }
@@ -772,7 +777,12 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
       for (int j = 0; j < C::TN; ++j) {
         float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < C::TM; ++i) s += (acc[i][j][0] + acc[i][j][1]) + (acc[i][j][2] + acc[i][j][3]);
+        for (int i = 0; i < C::TM; ++i) {
+          if constexpr (C::DT == DT_F16) {
+            const f32x4 g = *reinterpret_cast<const f32x4*>(sG + row0 + i * 16);
+            s += (acc[i][j][0] * g[0] + acc[i][j][1] * g[1]) + (acc[i][j][2] * g[2] + acc[i][j][3] * g[3]);
+          } else s += (acc[i][j][0] + acc[i][j][1]) + (acc[i][j][2] + acc[i][j][3]);
+        }
         s += __shfl_xor(s, 16, 64);
         s += __shfl_xor(s, 32, 64);
         if (lane < 16) sC[wm * C::BN + col0 + j * 16] = s;
@@ -945,71 +955,109 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineP p) {
 
 // ------------------------------------------------------------------------------------------------------------------------ backward
 // Bound by the latency of one workgroup (4096 rows: 7 us).
-// coef[m] = dloss[rows[m]] * T * s with the largest at `top` (0: s = 1), and gr (eh: exponents of operands in halves, or null). The scores' gradient is rounded to 16 bits: at a label it is close to
+// coef[m] = dloss[rows[m]] * T * s with the largest at `top` (0: s = 1). The scores' gradient is rounded to 16 bits: at a label it is close to
 // its coefficient, and with the largest coefficient at a power of two the large ones sit at the end of their binade, where a rounding counts
-// least; fp16 takes 2^14, so that entries down to 2^-38 of the largest stay above its smallest step.
-__global__ void __launch_bounds__(1024) coef_kernel(const float* __restrict__ dloss, const int* __restrict__ rows, const int* __restrict__ count,
-                                                    float T, float top, const int* __restrict__ eh, float* __restrict__ coef, Grad* __restrict__ gr) {
+// least.
+// fp16 takes top = 2^14, and its smallest step, 2^-24, is what is left of a row whose coefficient is small. So a row has a power of two
+// of its own, 2^g, which the sums over the words carry and give back: halves (slack 0) put every coefficient into [2^14, 2^15), fp16 operands,
+// whose gradients keep 11 bits, only those below 2^-12 of the largest (raised to that). With one factor for all, a row weighted 10^-6 of the
+// largest had its hidden states' gradient off by 2e-4 in fp32, one weighted 10^-7 by 5e-3 in fp16. For dW, which sums over the rows, t = g + eh is
+// the whole exponent of a row, and the rows of H are brought to the lowest t. (A value of dW so holds 2^-40 of the largest |coefficient| |h| of a row.)
+struct CoefP {
+  const float* dloss; const int* rows; const int* count;
+  float T, top;
+  const int* eh;                         // exponents of operands in halves, or null
+  float* coef; int *g, *t; int slack;    // g, t: or null (bf16, fp32)
+  Grad* gr;
+};
+__device__ __forceinline__ int row_scale(const CoefP& p, float c) {
+  const float x = fabsf(c);
+  if (!p.g || !(x > 0.f && x < __builtin_inff())) return 0;
+  int e;
+  frexpf(x, &e);
+  return min(max(15 - e - p.slack, 0), 126);
+}
+__device__ __forceinline__ int row_total(const CoefP& p, int m, float c, int g) {
+  if (!p.t) return 0;
+  const int e = p.eh ? p.eh[m] : 0;
+  return c == 0.f || e == ZERO_ROW ? NO_ROW : g + e;
+}
+// Bound by the latency of one workgroup (4096 rows: 7 us).
+__global__ void __launch_bounds__(1024) coef_kernel(const CoefP p) {
   __shared__ float red[16];
-  const int c = *count;
+  const int c = *p.count;
   float s = 1.f, v[8];                                             // the first 8192 rows stay in registers
 #pragma unroll
-  for (int j = 0; j < 8; ++j) { const int m = j * 1024 + threadIdx.x; v[j] = m < c ? dloss[rows[m]] * T : 0.f; }
-  if (top > 0.f) {
+  for (int j = 0; j < 8; ++j) { const int m = j * 1024 + threadIdx.x; v[j] = m < c ? p.dloss[p.rows[m]] * p.T : 0.f; }
+  if (p.top > 0.f) {
     float mx = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (fabsf(v[j]) < __builtin_inff()) mx = fmaxf(mx, fabsf(v[j]));
     for (int m = 8192 + threadIdx.x; m < c; m += 1024) {
-      const float x = fabsf(dloss[rows[m]] * T);
+      const float x = fabsf(p.dloss[p.rows[m]] * p.T);
       if (x < __builtin_inff()) mx = fmaxf(mx, x);
     }
     mx = block_max(mx, red);
-    if (mx > 0.f) s = fminf(top / mx, 1e37f);
+    if (mx > 0.f) s = fminf(p.top / mx, 1e37f);
   }
+  int low = NO_ROW;
+  auto row = [&](int m, float x) {
+    const int g = row_scale(p, x * s);
+    p.coef[m] = pow2(x * s, g);
+    if (p.g) {
+      const int t = row_total(p, m, x, g);
+      p.g[m] = g;
+      p.t[m] = t;
+      low = min(low, t);
+    }
+  };
 #pragma unroll
-  for (int j = 0; j < 8; ++j) { const int m = j * 1024 + threadIdx.x; if (m < c) coef[m] = v[j] * s; }
-  for (int m = 8192 + threadIdx.x; m < c; m += 1024) coef[m] = dloss[rows[m]] * T * s;
-  int hlo = 0;
-  if (eh) {
-    int e = ZERO_ROW;
-    for (int m = threadIdx.x; m < c; m += 1024) e = min(e, eh[m]);
-    hlo = -(int)block_max((float)-e, red);
-  }
-  if (threadIdx.x == 0) *gr = Grad{1.f / s, hlo};
+  for (int j = 0; j < 8; ++j) { const int m = j * 1024 + threadIdx.x; if (m < c) row(m, v[j]); }
+  for (int m = 8192 + threadIdx.x; m < c; m += 1024) row(m, p.dloss[p.rows[m]] * p.T);
+  if (p.g) low = -(int)block_max((float)-low, red);
+  if (threadIdx.x == 0) *p.gr = Grad{1.f / s, p.g ? low : 0};
 }
 
-// coef_kernel and pack_kernel in one launch for few rows: a workgroup per row, each finds the largest coefficient for itself
-__global__ void __launch_bounds__(256) prepare_kernel(const float* __restrict__ dloss, const int* __restrict__ rows, const int* __restrict__ count,
-                                                      float T, float top, const int* __restrict__ eh, float* __restrict__ coef, Grad* __restrict__ gr,
-                                                      const PackP p) {
+// coef_kernel and pack_kernel in one launch for few rows: a workgroup per row, each finds the largest coefficient and the lowest t for itself
+__global__ void __launch_bounds__(256) prepare_kernel(const CoefP p, const PackP pk) {
   __shared__ float red[16];
-  const int c = *count, m = blockIdx.x;
+  const int c = *p.count, m = blockIdx.x;
   if (m >= c && m > 0) return;
   float s = 1.f;
-  int hlo = 0;
-  if (top > 0.f) {
+  if (p.top > 0.f) {
     float mx = 0.f;
-    int e = ZERO_ROW;
     for (int k = threadIdx.x; k < c; k += 256) {
-      const float v = fabsf(dloss[rows[k]] * T);
+      const float v = fabsf(p.dloss[p.rows[k]] * p.T);
       if (v < __builtin_inff()) mx = fmaxf(mx, v);
-      if (eh) e = min(e, eh[k]);
     }
     mx = block_max(mx, red);
-    if (mx > 0.f) s = fminf(top / mx, 1e37f);
-    if (eh) hlo = -(int)block_max((float)-e, red);
+    if (mx > 0.f) s = fminf(p.top / mx, 1e37f);
   }
-  if (m == 0 && threadIdx.x == 0) *gr = Grad{1.f / s, hlo};
+  int low = 0;
+  if (p.g) {
+    low = NO_ROW;
+    for (int k = threadIdx.x; k < c; k += 256) {
+      const float v = p.dloss[p.rows[k]] * p.T;
+      low = min(low, row_total(p, k, v, row_scale(p, v * s)));
+    }
+    low = -(int)block_max((float)-low, red);
+  }
+  if (m == 0 && threadIdx.x == 0) *p.gr = Grad{1.f / s, low};
   if (m >= c) return;
-  if (threadIdx.x == 0) coef[m] = dloss[rows[m]] * T * s;
-  if (p.out) pack_row(p, m, hlo);
+  const float x = p.dloss[p.rows[m]] * p.T;
+  const int g = row_scale(p, x * s), t = row_total(p, m, x, g);
+  if (threadIdx.x == 0) {
+    p.coef[m] = pow2(x * s, g);
+    if (p.g) { p.g[m] = g; p.t[m] = t; }
+  }
+  if (pk.out) pack_row(pk, m, low - t);
 }
 
 // db from the gradient itself (both halves): with teacher entries the tiles' column sums do not hold them. Eight lanes to a word, 16 bytes each at a
 // time. Bound by reading the gradient (96 rows x 30522 words in halves: 6.6 us; a wave to a word, two bytes a lane, took 10.4).
 __global__ void __launch_bounds__(256) bias_rows_kernel(const char* __restrict__ G, int64_t ldg, int64_t glo, int dt, int vc, const int* __restrict__ count,
-                                                        const Grad* __restrict__ gr, void* __restrict__ db, int bdt) {
+                                                        const int* __restrict__ g, const Grad* __restrict__ gr, void* __restrict__ db, int bdt) {
   const int v = blockIdx.x * 32 + (threadIdx.x >> 3), c = *count, ch = dt == DT_F32 ? 4 : 8;
   float s = 0.f;
   auto add = [&](const char* at, int m) {
@@ -1019,10 +1067,12 @@ __global__ void __launch_bounds__(256) bias_rows_kernel(const char* __restrict__
       for (int e = 0; e < 4; ++e) s += m + e < c ? raw[e] : 0.f;
     } else {
       const s16x8 x = __builtin_bit_cast(s16x8, raw);
+      i32x4 g0 = {0, 0, 0, 0}, g1 = {0, 0, 0, 0};
+      if (dt == DT_F16) { g0 = *reinterpret_cast<const i32x4*>(g + m); g1 = *reinterpret_cast<const i32x4*>(g + m + 4); }   // (readable in 64s)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const uint16_t u = (uint16_t)x[e];
-        s += m + e < c ? (dt == DT_BF16 ? bf2f(u) : (float)__builtin_bit_cast(_Float16, u)) : 0.f;
+        s += m + e < c ? (dt == DT_BF16 ? bf2f(u) : pow2((float)__builtin_bit_cast(_Float16, u), -(e < 4 ? g0[e & 3] : g1[e & 3]))) : 0.f;
       }
     }
   };
@@ -1100,7 +1150,7 @@ __global__ void __launch_bounds__(C::NT) dh_kernel(const DhP p) {
 // Those behind them 256 words of db = scale * sum over the row tiles' column sums.
 struct FinishP {
   const float* slab; const int* rows; const int* count;
-  const Scales* sc; const Grad* gr;      // sc: of operands in halves, or null
+  const Scales* sc; const int* g; const Grad* gr;   // sc: of operands in halves, or null; g: or null
   int N, D, units, most, blocks;         // blocks of a row
   void* dh; int dt;
   const float* colsum; int bm; int V;
@@ -1140,10 +1190,10 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishP p) {
     if (wid > 0) return;
     v = (v + quarter[0][lane]) + (quarter[1][lane] + quarter[2][lane]);
   }
-  const int lo = p.sc ? lowest_word(p.sc) : 0;
+  const int e = (p.sc ? lowest_word(p.sc) : 0) + (p.g && m < c ? p.g[m] : 0);
   const float inv = p.gr->inv;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = pow2(v[j], -lo) * inv;
+  for (int j = 0; j < 4; ++j) v[j] = pow2(v[j], -e) * inv;
   const int64_t o = (int64_t)p.rows[m] * p.D + d;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -1176,7 +1226,7 @@ __global__ void __launch_bounds__(C::NT) dw_kernel(const DwP p) {
   typename C::acc_t acc[C::TM][C::TN];
   product<C, SWAP && !is_pp<C>(), !SWAP && !is_pp<C>(), SEG>(smem, SWAP ? p.H : p.G, SWAP ? p.G : p.H, m0, n0, K, k0, k1, acc);
   if (p.shares > 1) { to_slab<C>(p.slab + (int64_t)u * C::BM * C::BN, acc, false); return; }
-  if constexpr (SEG == 3) {                                        // the rows' factor
+  if constexpr (C::DT == DT_F16) {                                 // the rows' factor
     const int e = -p.gr->hlo;
 #pragma unroll
     for (int i = 0; i < C::TM; ++i)
@@ -1254,7 +1304,7 @@ struct Plan {
   int pieces, step;
   int units, most, shares;
   bool quarters;                         // finish_kernel
-  bool pack;                             // dW: the rows of H that take part are packed first (halves: brought to one factor)
+  bool pack;                             // dW: the rows of H that take part are packed first (fp16, halves: brought to one factor)
   int64_t gcols;
 };
 
@@ -1309,7 +1359,7 @@ Plan plan(const Args& a) {
   p.many = 6144;
   p.wtr = a.want_h && p.nt && !a.wt && a.N >= p.many;
   p.pair = bits16 && !a.split && a.N <= 256;                       // (see score_kernel)
-  p.pack = a.want_w && !p.nt && !p.pad_h;
+  p.pack = a.want_w && !p.nt && (!p.pad_h || p.op == DT_F16);
   const int seg = a.split ? 3 : p.pair ? 2 : 1, bk = bits16 ? 64 : 32;
   const int64_t vk = seg * (up(p.step, bk) / bk), nk = seg * (up(a.N, bk) / bk);   // k-tiles of the two products' sums
   const int64_t cols = p.gcols < a.V ? p.gcols : a.V;
@@ -1360,7 +1410,7 @@ struct State {
 };
 struct Work {
   float2* part; float *tz, *zs, *wmax, *tops;                         // forward
-  Grad* gr; float *coef, *colsum; char* G; char* packed; uint16_t *ht, *wtr; float *dh_slab, *dw_slab;  // backward
+  Grad* gr; int *g, *t; float *coef, *colsum; char* G; char* packed; uint16_t *ht, *wtr; float *dh_slab, *dw_slab;  // backward
   int64_t fwd, bwd;
   Work(const Args& a, const Plan& p) {
     Carve c(a.ws);
@@ -1370,7 +1420,7 @@ struct Work {
     fwd = c.at;
     c.at = 0;
     const int64_t esz = a.dt == DT_F32 ? 4 : 2;
-    gr = c.take<Grad>(1); coef = c.take<float>(a.N); G = c.take<char>(p.np * p.gcols * esz * (p.nt || p.pair || (a.split && a.want_h) ? 2 : 1));
+    gr = c.take<Grad>(1); g = c.take<int>(p.op == DT_F16 ? a.N : 0); t = c.take<int>(p.op == DT_F16 ? a.N : 0); coef = c.take<float>(a.N); G = c.take<char>(p.np * p.gcols * esz * (p.nt || p.pair || (a.split && a.want_h) ? 2 : 1));
     colsum = c.take<float>(a.want_b && !a.K ? (a.N + p.bm - 1) / p.bm * a.V : 0);
     packed = c.take<char>(p.pack ? a.N * p.dp * esz : 0);
     ht = c.take<uint16_t>(a.want_w && p.nt ? a.D * p.np * (a.split ? 2 : 1) : 0);
@@ -1557,27 +1607,28 @@ int backward(const Args& a, const float* f, hipStream_t st) {
   const State s(a, p);
   const Work w(a, p);
   const int esz = a.dt == DT_F32 ? 4 : 2, gsz = a.split ? 2 : esz;
-  const float top = a.split ? 32768.f : p.op == DT_F16 ? 16384.f : p.op == DT_BF16 ? 1.f : 0.f;
+  const float top = p.op == DT_F16 ? 16384.f : p.op == DT_BF16 ? 1.f : 0.f;
   Operand H, W;
   operands(a, p, s, H, W);
   Operand packed = H;
-  const int* eh = a.split ? s.eh : nullptr;
-  PackP pk{H.p, H.ld, H.lo, H.rows, p.pack ? w.packed : nullptr, p.dp * gsz, a.split ? a.N * p.dp * 2 : 0, p.dp * gsz, eh};
-  if (!a.split) pk.row_bytes = up(a.D, 16 / esz) * esz;
+  const bool f16 = p.op == DT_F16;
+  const CoefP cp{a.dloss, s.rows, s.count, f[0], top, a.split ? s.eh : nullptr, w.coef, f16 ? w.g : nullptr, f16 ? w.t : nullptr, a.split ? 0 : 12, w.gr};
+  PackP pk{H.p, H.ld, H.lo, H.rows, p.pack ? w.packed : nullptr, p.dp * gsz, a.split ? a.N * p.dp * 2 : 0, a.split || p.pad_h ? p.dp * gsz : up(a.D, 16 / esz) * esz,
+           a.split ? 2 : 1};
   if (a.N <= 1024) {
-    hipLaunchKernelGGL(prepare_kernel, dim3((unsigned)a.N), dim3(256), 0, st, a.dloss, s.rows, s.count, f[0], top, eh, w.coef, w.gr, pk);
+    hipLaunchKernelGGL(prepare_kernel, dim3((unsigned)a.N), dim3(256), 0, st, cp, pk);
     VL_CHECK();
   } else {
-    hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, st, a.dloss, s.rows, s.count, f[0], top, eh, w.coef, w.gr);
+    hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, st, cp);
     VL_CHECK();
     if (p.pack) {
-      hipLaunchKernelGGL(pack_kernel, dim3((unsigned)a.N), dim3(256), 0, st, pk, s.count, w.gr);
+      hipLaunchKernelGGL(pack_kernel, dim3((unsigned)a.N), dim3(256), 0, st, pk, s.count, cp.t, w.gr);
       VL_CHECK();
     }
   }
   if (p.pack) packed = Operand{w.packed, pk.ldo, pk.half_out, 0, nullptr};
   if (a.want_w && p.nt) {
-    TransposeP t{(const uint16_t*)H.p, H.ld / 2, H.lo / 2, w.ht, p.np, a.D * p.np, (int)a.N, (int)a.D, s.count, H.rows, nullptr, 0, eh, w.gr};
+    TransposeP t{(const uint16_t*)H.p, H.ld / 2, H.lo / 2, w.ht, p.np, a.D * p.np, (int)a.N, (int)a.D, s.count, H.rows, nullptr, 0, cp.t, w.gr};
     hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)((a.N + 63) / 64), (unsigned)((a.D + 63) / 64), a.split ? 2 : 1), dim3(256), 0, st, t);
     VL_CHECK();
     packed = Operand{(const char*)w.ht, p.np * 2, a.split ? a.D * p.np * 2 : 0, 0, nullptr};
@@ -1598,13 +1649,13 @@ int backward(const Args& a, const float* f, hipStream_t st) {
     ScoreP q = score_args(a, s, f);
     q.H = H; q.W = W;
     q.W.xlim = (int)a.V;
-    q.v0 = v0; q.v1 = v1; q.ref = s.ref; q.inv = s.inv; q.coef = w.coef; q.G = w.G; q.ldg = ldg; q.glo = glo;
+    q.v0 = v0; q.v1 = v1; q.ref = s.ref; q.inv = s.inv; q.coef = w.coef; q.g = w.g; q.G = w.G; q.ldg = ldg; q.glo = glo;
     if (p.nt && a.want_h) { q.R = rows_g; q.ldr = ldr; q.rlo = rlo; }
     else if (a.split && a.want_h) q.G2 = rows_g;
     if (a.want_b && !a.K) { q.colsum = w.colsum; q.ldc = a.V; }
     if (const int e = scores<true>(q, p.tile, p.op, a.split, p.pair, a.wt, st)) return e;
     if (a.want_b && a.K) {
-      hipLaunchKernelGGL(bias_rows_kernel, dim3((vc + 31) / 32), dim3(256), 0, st, w.G, ldg, glo, a.split ? (int)DT_F16 : (int)a.dt, vc, s.count, w.gr,
+      hipLaunchKernelGGL(bias_rows_kernel, dim3((vc + 31) / 32), dim3(256), 0, st, w.G, ldg, glo, a.split ? (int)DT_F16 : (int)a.dt, vc, s.count, w.g, w.gr,
                          (char*)a.db + (int64_t)v0 * (a.bdt == DT_F32 ? 4 : 2), (int)a.bdt);
       VL_CHECK();
     }
@@ -1638,7 +1689,7 @@ int backward(const Args& a, const float* f, hipStream_t st) {
   if (a.want_h || sums) {
     const int64_t cols = p.quarters ? 256 : 1024, blocks = (a.D + cols - 1) / cols;
     if (a.N * blocks + (a.V + 255) / 256 > 0x7fffffff) return -2;
-    const FinishP q{w.dh_slab, s.rows, s.count, a.split ? s.sc : nullptr, w.gr, a.want_h ? (int)a.N : 0, (int)a.D, p.units, p.most, (int)blocks, a.dh, (int)a.dt, w.colsum, p.bm, (int)a.V, a.db, (int)a.bdt};
+    const FinishP q{w.dh_slab, s.rows, s.count, a.split ? s.sc : nullptr, cp.g, w.gr, a.want_h ? (int)a.N : 0, (int)a.D, p.units, p.most, (int)blocks, a.dh, (int)a.dt, w.colsum, p.bm, (int)a.V, a.db, (int)a.bdt};
     const dim3 grid((unsigned)(q.N * blocks + (sums ? (a.V + 255) / 256 : 0)));
     if (p.dh_tile == TILE_BIG) launch_finish<256>(q, p.quarters, grid, st);
     else if (p.dh_tile == TILE_SMALL) launch_finish<64>(q, p.quarters, grid, st);

@@ -1,9 +1,9 @@
-"""The linear vocabulary losses on values of very different size: rows and words that lie many powers of ten apart must not disturb one another.
-Against the definition in 64 bits; sizes reach the fp32 cores, the products of halves on both tiles and both layouts.
+"""The linear vocabulary losses on values of very different size: rows, words and row weights that lie many powers of ten apart must not
+disturb one another. Against the definition in 64 bits; sizes reach the fp32 cores, the products of halves on both tiles and both layouts.
 
 Tolerances. Losses of single rows: 4e-6 of the row's own size (at least of 1), as the sum of D = 512 fp32 products and a normaliser of V terms
 gives it. Gradients of single rows in the 2-norm: fp32 4e-6 (2e-6 for a whole tensor; a row of 64 or more values spreads around that by less than
-a factor of two)."""
+a factor of two), fp16 two roundings of 2^-11."""
 import math
 
 import pytest
@@ -13,7 +13,7 @@ from deeplearning4j_amd.ops import vocab_loss as VL
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
-ROW = {torch.float32: 4e-6}
+ROW = {torch.float32: 4e-6, torch.float16: 2 * 2.0 ** -11}
 
 
 def _gen(seed):
@@ -108,3 +108,45 @@ def test_words_of_very_different_size(n, d, v, layout, distil):
         assert float((a.double() - e).norm()) <= 2e-6 * float(e.norm()), what
     labelled = y.unique() if not distil else idx.reshape(-1).unique()
     _rows_close(got[2][labelled], want[2][labelled], ROW[torch.float32], "weights")
+
+
+@pytest.mark.parametrize("layout", ["vd", "dv"])
+@pytest.mark.parametrize("n,d,v", SIZES)
+@pytest.mark.parametrize("distil", [False, True])
+def test_row_weights_from_1_to_1e_8(n, d, v, layout, distil):
+    h, w, b, y, idx, t, dl = _inputs(n, d, v, torch.float32, layout)
+    dl *= 10.0 ** -(torch.arange(n, device=DEV) % 9).float()
+    dl[5] = 0.0
+    got, want = _both(distil, h, w, b, y, idx, t, dl, layout)
+    assert (got[1][5] == 0).all()
+    _rows_close(got[1], want[1], ROW[torch.float32], "hidden")
+    for a, e, what in zip(got[2:], want[2:], ("weights", "bias")):
+        assert float((a.double() - e).norm()) <= 2e-6 * float(e.norm()), what
+
+
+@pytest.mark.parametrize("layout", ["vd", "dv"])
+@pytest.mark.parametrize("n,d,v", [(300, 64, 900), (700, 520, 30000), (300, 101, 1003)])
+@pytest.mark.parametrize("distil", [False, True])
+def test_row_weights_from_1_to_1e_7_in_half_precision(n, d, v, layout, distil):
+    h, w, b, y, idx, t, dl = _inputs(n, d, v, torch.float32, layout)
+    # (weights of some 10 and hidden states of some 0.1, and a loss scale: the small rows' gradients are then normal fp16 numbers)
+    h, w = (h * (0.25 / math.sqrt(d))).half(), (w * (10 / 2.5 * math.sqrt(d))).half()
+    dl *= 1e3 * 10.0 ** -(torch.arange(n, device=DEV) % 8).float()
+    got, want = _both(distil, h, w, b.half(), y, idx, t, dl, layout)
+    _rows_close(got[1], want[1], ROW[torch.float16], "hidden")
+    for a, e, what in zip(got[2:], want[2:], ("weights", "bias")):
+        assert float((a.double() - e).norm()) <= ROW[torch.float16] * float(e.norm()), what
+
+
+@pytest.mark.parametrize("layout", ["vd", "dv"])
+@pytest.mark.parametrize("n,d,v", SIZES)
+@pytest.mark.parametrize("scale", [0.0, 1e-34, 1e30])
+def test_all_row_weights_tiny_huge_or_zero(n, d, v, scale, layout):
+    """One row's huge hidden states count for nothing where its weight is zero."""
+    h, w, b, y, idx, t, dl = _inputs(n, d, v, torch.float32, layout)
+    h[n // 2] *= 1e6
+    dl *= scale
+    dl[n // 2] = 0.0
+    got, want = _both(False, h, w, b, y, idx, t, dl, layout)
+    for a, e, what in zip(got[1:], want[1:], ("hidden", "weights", "bias")):
+        assert torch.isfinite(a).all() and float((a.double() - e).norm()) <= 2e-6 * float(e.norm()), what
