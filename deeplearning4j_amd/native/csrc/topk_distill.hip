@@ -34,6 +34,14 @@ __device__ __forceinline__ float load_any(const void* p, int64_t i, int dt) {   
   return dt == 1 ? bf2f(v) : (float)__builtin_bit_cast(_Float16, v);
 }
 
+// exp(z / T - ref) of a rounded z / T against a reference that is one: 1 at most. Fused to one instruction, the exact product stands against a
+// rounded one, and half a step of a logit of 2^30 is more than an exponential holds.
+__device__ __forceinline__ float exp_below(float z, float invT, float ref) {
+#pragma clang fp contract(off)
+  const float t = z * invT;
+  return __expf(t - ref);
+}
+
 // the teacher's weights of row n in LDS: si[k] index (-1: none), sp[k] = p_k; returns (P, sum p log p) to all threads. NaN or +inf among
 // the row's logits makes both NaN.
 template <int NT>
@@ -87,13 +95,13 @@ __global__ void __launch_bounds__(NT) distill_fwd_kernel(const T* __restrict__ z
   const int head = min(V, (int)(((16 - (reinterpret_cast<uintptr_t>(zr) & 15)) & 15) / sizeof(T)));
   const int nv = (V - head) / E, tail = head + nv * E;
   float m = NEG_INF, s = 0.f;
-  auto one = [&](float v) {
-    const float nm = fmaxf(m, v);
-    if (nm != NEG_INF) s = s * __expf(m - nm) + __expf(v - nm); else s += v != v ? v : 0.f;
+  auto one = [&](float z) {
+    const float nm = fmaxf(m, z * invT);
+    if (nm != NEG_INF) s = s * __expf(m - nm) + exp_below(z, invT, nm); else s += z != z ? z : 0.f;
     m = nm;
   };
-  if (tid < head) one(El<T>::ld(zr[tid]) * invT);
-  if (tail + tid < V) one(El<T>::ld(zr[tail + tid]) * invT);
+  if (tid < head) one(El<T>::ld(zr[tid]));
+  if (tail + tid < V) one(El<T>::ld(zr[tail + tid]));
   const f32x4* vp = reinterpret_cast<const f32x4*>(zr + head);
 #pragma unroll 4
   for (int i = tid; i < nv; i += NT) {
@@ -102,11 +110,11 @@ __global__ void __launch_bounds__(NT) distill_fwd_kernel(const T* __restrict__ z
     __builtin_memcpy(e, &raw, 16);
     float f[E], mx = NEG_INF;
 #pragma unroll
-    for (int j = 0; j < E; ++j) { f[j] = El<T>::ld(e[j]) * invT; mx = fmaxf(mx, f[j]); }
+    for (int j = 0; j < E; ++j) { f[j] = El<T>::ld(e[j]); mx = fmaxf(mx, f[j] * invT); }
     const float nm = fmaxf(m, mx), ref = nm == NEG_INF ? 0.f : nm;
     float a = 0.f;
 #pragma unroll
-    for (int j = 0; j < E; ++j) a += __expf(f[j] - ref);
+    for (int j = 0; j < E; ++j) a += exp_below(f[j], invT, ref);
     s = s * __expf(m - ref) + a;                        // m = -inf: s is 0 (or NaN) there
     m = nm;
   }
@@ -145,7 +153,7 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const T* __restrict__ z
   const bool alike = ((reinterpret_cast<uintptr_t>(zr) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
   const int head = alike ? min(V, (int)(((16 - (reinterpret_cast<uintptr_t>(zr) & 15)) & 15) / sizeof(T))) : V;
   const int nv = (V - head) / E, tail = head + nv * E;
-  auto one = [&](int j) { out[j] = El<T>::st(none ? 0.f : cp * __expf(El<T>::ld(zr[j]) * invT - L)); };
+  auto one = [&](int j) { out[j] = El<T>::st(none ? 0.f : cp * exp_below(El<T>::ld(zr[j]), invT, L)); };
   for (int j = tid; j < head; j += NT) one(j);
   if (tail + tid < V) one(tail + tid);
   const f32x4* vp = reinterpret_cast<const f32x4*>(zr + head);
@@ -160,7 +168,7 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const T* __restrict__ z
     T e[E];
     __builtin_memcpy(e, &raw, 16);
 #pragma unroll
-    for (int j = 0; j < E; ++j) e[j] = El<T>::st(cp * __expf(El<T>::ld(e[j]) * invT - L));
+    for (int j = 0; j < E; ++j) e[j] = El<T>::st(cp * exp_below(El<T>::ld(e[j]), invT, L));
     __builtin_memcpy(&raw, e, 16);
     op[i] = raw;
   }
@@ -170,7 +178,7 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const T* __restrict__ z
     if (i < 0 || i >= V || sp[k] == 0.f) continue;
     float q = 0.f;
     for (int j = 0; j < K; ++j) q += si[j] == i ? sp[j] : 0.f;     // an index may come twice: all its entries write the same value
-    out[i] = El<T>::st(c * (pt.x * __expf(El<T>::ld(zr[i]) * invT - L) - q));
+    out[i] = El<T>::st(c * (pt.x * exp_below(El<T>::ld(zr[i]), invT, L) - q));
   }
 }
 

@@ -28,6 +28,18 @@ constexpr float NEG_INF = -__builtin_inff();
 constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x); }
+// A score x * scale against a reference that is one. In one instruction the exact product stands against a rounded one: what is off by half a step of
+// the reference is the same for a whole row and leaves its softmax as it is, as long as an exponential holds it. Beyond LARGE (a step of 1/2; at
+// 2^30 half a step is 64) the score is rounded first, so that it is 0 at most. (Always rounding first made the statistics kernel 4 % longer.)
+constexpr float LARGE = 0x1p22f;
+template <bool ROUND> __device__ __forceinline__ float below(float x, float scale, float ref) {
+  if constexpr (ROUND) {
+#pragma clang fp contract(off)
+    const float z = x * scale;
+    return z - ref;
+  } else return __builtin_fmaf(x, scale, -ref);
+}
+template <bool B> struct Bool { static constexpr bool value = B; };
 constexpr int KMAX = 1024;                              // teacher entries per row
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
@@ -545,8 +557,8 @@ template <class C> constexpr int score_lds(bool grad, int seg) {
 //
 // Statistics: every exponential is taken against ONE reference per quarter wave, the largest score of its 32 rows x 64 columns (on the large
 // tile), instead of the row's maximum: four cross-lane steps in all instead of four per row, and no row waits for its own maximum. A sum of
-// exponentials 2^-100 below the reference is still a sound fp32 number; a row that lies lower makes the workgroup take the tile again with a
-// reference per row. The 16 lanes that share a row leave their partial sums in LDS, where one thread per row adds them.
+// exponentials 2^-100 below the reference is still a sound fp32 number; a row that lies lower, or a reference beyond LARGE, makes the workgroup take
+// the tile again with a reference per row and rounded scores. The 16 lanes that share a row leave their partial sums in LDS, where one thread per row adds them.
 // (A maximum and a sum reduced over the lanes for every row, as the fallback does it, made the epilogue of a 256 x 256 tile as long as seven
 // of its k-tiles.)
 // Bound by the matrix cores: forward of 8192 x 2048 of 65536 words in bf16 1.72 ms (1280 TF/s), 4096 x 1024 of 32000 0.31 ms (860 TF/s: 16 k-tiles
@@ -640,7 +652,7 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
 #pragma unroll
       for (int j = 0; j < C::TN; ++j)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) s[q] += exp2_(acc[i][j][q] * zscale - ref);   // (the reference passes over a NaN score, the sum keeps it)
+        for (int q = 0; q < 4; ++q) s[q] += exp2_(below<false>(acc[i][j][q], zscale, ref));   // (the reference passes over a NaN score, the sum keeps it)
       *reinterpret_cast<f32x4*>(sP + (wn * 16 + lc) * (C::BM + 16) + row0 + i * 16) = s;
     }
     __syncthreads();
@@ -651,9 +663,10 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
         float s = 0.f;
 #pragma unroll
         for (int k = 0; k < 16; ++k) s += sP[(w * 16 + k) * (C::BM + 16) + tid];
-        sM[w * C::BM + tid] = sR[(tid / RW * C::WN + w) * 4 + ((tid >> 2) & 3)];
+        const float r = sR[(tid / RW * C::WN + w) * 4 + ((tid >> 2) & 3)];
+        sM[w * C::BM + tid] = r;
         sS[w * C::BM + tid] = s;
-        low |= s < 0x1p-100f && n0 + w * CW < p.v1;
+        low |= (s < 0x1p-100f && n0 + w * CW < p.v1) || fabsf(r) >= LARGE;
       }
       if (low) *again = 1;
     }
@@ -669,7 +682,7 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
           mr = max16(mr) * zscale;
           const float rr = mr == NEG_INF ? 0.f : mr;
 #pragma unroll
-          for (int j = 0; j < C::TN; ++j) s += exp2_(acc[i][j][q] * zscale - rr);
+          for (int j = 0; j < C::TN; ++j) s += exp2_(below<true>(acc[i][j][q], zscale, rr));
           s = sum16(s);
           if (lc == 0) { sM[wn * C::BM + row0 + i * 16 + q] = mr; sS[wn * C::BM + row0 + i * 16 + q] = s; }
         }
@@ -744,10 +757,17 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
 #pragma unroll
     for (int i = 0; i < C::TM; ++i) {
       const f32x4 c = *reinterpret_cast<const f32x4*>(sf + 3 * C::BM + row0 + i * 16), l = *reinterpret_cast<const f32x4*>(sf + 2 * C::BM + row0 + i * 16);
+      auto probabilities = [&](auto round) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
-        for (int j = 0; j < C::TN; ++j) acc[i][j][q] = c[q] * exp2_(acc[i][j][q] * zscale - l[q]);
+          for (int j = 0; j < C::TN; ++j) acc[i][j][q] = c[q] * exp2_(below<decltype(round)::value>(acc[i][j][q], zscale, l[q]));
+      };
+      // (rows past the end have a reference of 3e38: either way a probability of 0)
+      bool large = false;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) large |= fabsf(l[q]) >= LARGE && l[q] < 3e38f;
+      if (__any(large)) probabilities(Bool<true>()); else probabilities(Bool<false>());
     }
     if (p.smooth_v != 0.f) {
 #pragma unroll
