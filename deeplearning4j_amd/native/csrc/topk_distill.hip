@@ -43,19 +43,19 @@ __device__ __forceinline__ float exp_below(float z, float invT, float ref) {
 }
 
 // the teacher's weights of row n in LDS: si[k] index (-1: none), sp[k] = p_k; returns (P, sum p log p) to all threads. NaN or +inf among
-// the row's logits makes both NaN.
+// the row's logits, or an entry outside the vocabulary (with any logit but -inf), makes both NaN.
 template <int NT>
-__device__ __forceinline__ float2 teacher_row(const void* idx, int idx64, const void* t, int tdt, int64_t n, int K, float invT, int* si, float* sp,
-                                              float* red) {
+__device__ __forceinline__ float2 teacher_row(const void* idx, int idx64, const void* t, int tdt, int64_t n, int V, int K, float invT, int* si,
+                                              float* sp, float* red) {
   const int tid = threadIdx.x;
   float m = NEG_INF, bad = 0.f;
   for (int k = tid; k < K; k += NT) {
     const int64_t o = n * K + k;
     const int64_t i = idx64 ? reinterpret_cast<const int64_t*>(idx)[o] : (int64_t)reinterpret_cast<const int*>(idx)[o];
-    const float v = i < 0 ? NEG_INF : load_any(t, o, tdt) * invT;
+    const float l = i < 0 ? NEG_INF : load_any(t, o, tdt), v = l * invT;
     si[k] = i < 0 ? -1 : i > 0x7fffffff ? 0x7fffffff : (int)i;
     sp[k] = v;
-    if (!(v < __builtin_inff())) bad = 1.f;
+    if (!(v < __builtin_inff()) || (i >= V && l != NEG_INF)) bad = 1.f;
     m = fmaxf(m, v);
   }
   m = block_max(m, red);
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(NT) distill_fwd_kernel(const T* __restrict__ z
   const int64_t n = blockIdx.x;
   const T* zr = z + n * ldz;
   const int tid = threadIdx.x;
-  const float2 pt = teacher_row<NT>(idx, idx64, t, tdt, n, K, invT, si, sp, red);
+  const float2 pt = teacher_row<NT>(idx, idx64, t, tdt, n, V, K, invT, si, sp, red);
   if (pt.x == 0.f) {                                    // no entry: the row takes no part
     if (tid == 0) { loss[n] = 0.f; lse[n] = 0.f; }
     return;
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(NT) distill_fwd_kernel(const T* __restrict__ z
   for (int k = tid; k < K; k += NT) {
     const float w = sp[k];
     if (w == 0.f) continue;
-    c += w * (si[k] < V ? El<T>::ld(zr[si[k]]) * invT : __builtin_nanf(""));
+    c += si[k] < V ? w * (El<T>::ld(zr[si[k]]) * invT) : __builtin_nanf("");   // (w is NaN too)
   }
   c = block_sum(c, red);
   if (tid == 0) {
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const T* __restrict__ z
   const T* zr = z + n * ldz;
   T* out = dz + n * V;
   const int tid = threadIdx.x;
-  const float2 pt = teacher_row<NT>(idx, idx64, t, tdt, n, K, invT, si, sp, red);
+  const float2 pt = teacher_row<NT>(idx, idx64, t, tdt, n, V, K, invT, si, sp, red);
   const bool none = pt.x == 0.f;
   const float c = dloss[n] * Tm, cp = c * pt.x, L = lse[n];
   // the heads of the two rows differ where ldz is not V: whole 16-byte pieces only where both are aligned alike

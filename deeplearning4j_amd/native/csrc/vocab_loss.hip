@@ -175,8 +175,9 @@ __global__ void __launch_bounds__(256) teacher_kernel(const TeacherP p) {
     if (k < p.K) {
       const int64_t o = (int64_t)n * p.K + k, i = load_index(p.idx, o, p.idx64);
       if (i >= 0) {
-        v = load_f(p.t, o, p.tdt) * p.invT;
-        bad |= !(v < __builtin_inff()) || (i >= p.V && v != NEG_INF);
+        const float l = load_f(p.t, o, p.tdt);
+        v = l * p.invT;
+        bad |= !(v < __builtin_inff()) || (i >= p.V && l != NEG_INF);
         if (i < p.V) q = (uint64_t)i << 10 | (uint64_t)k;
       }
     }

@@ -93,7 +93,7 @@ def _distill_rows(z, indices, teacher_logits, temperature):
     at = z.gather(1, indices.long().clamp(0, V - 1))
     at = torch.where(p != 0, at, torch.zeros_like(at))                 # a score of -inf that the teacher gives no weight
     cross = (p * (torch.logsumexp(z, 1, keepdim=True) - at)).sum(1)
-    outside = ((indices >= V) & (p != 0)).any(1)
+    outside = ((indices >= V) & (teacher_logits.detach() != -math.inf)).any(1)
     return temperature * temperature * (torch.xlogy(p, p).sum(1) + cross) * torch.where(outside, math.nan, 1.0)
 
 
@@ -362,7 +362,7 @@ def linear_topk_distillation(hidden, weights, teacher_indices, teacher_logits, b
     teacher_indices [..., K] INT32 / INT64 and teacher_logits [..., K] name the teacher's K best words of every row in any order; the
     teacher's softmax runs over them alone. Entries with a negative index are padding; a logit of -inf counts as none; an index that comes
     twice counts twice. A row without entries has loss 0 and no gradient. A row with an index >= V, or a teacher logit that is NaN or +inf,
-    has loss and gradients NaN. No gradient goes to the teacher. Other arguments, types and result as :func:`linear_cross_entropy`."""
+    has loss and gradients NaN, however little the teacher gives it. No gradient goes to the teacher. Other arguments, types and result as :func:`linear_cross_entropy`."""
     name = "linear_topk_distillation"
     _check_linear(hidden, weights, bias, name)
     _check_teacher(hidden.shape[:-1], hidden.device, teacher_indices, teacher_logits, temperature, name)
