@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -174,13 +175,21 @@ def _launch(fn, what, dev, *args):
         L.check(code, what)
 
 
+_LIB, _LOCK = None, threading.Lock()
+
+
 def _lib():
-    lib = L.hip()
-    if lib.dl4j_linear_loss_fwd.argtypes is None:
-        for fn in (lib.dl4j_linear_loss_fwd, lib.dl4j_linear_loss_bwd, lib.dl4j_topk_distill):
-            fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
-        lib.dl4j_linear_loss_bytes.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
-    return lib
+    """The kernel library with the calls' signatures declared, for every thread alike."""
+    global _LIB
+    if _LIB is None:
+        with _LOCK:
+            if _LIB is None:
+                lib = L.hip()
+                for fn in (lib.dl4j_linear_loss_fwd, lib.dl4j_linear_loss_bwd, lib.dl4j_topk_distill):
+                    fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+                lib.dl4j_linear_loss_bytes.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+                _LIB = lib
+    return _LIB
 
 
 def _dloss(g):
