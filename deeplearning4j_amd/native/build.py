@@ -59,6 +59,28 @@ def _newer(src: Path, dst: Path, extra=()) -> bool:
     return any(p.stat().st_mtime > t for p in (src, *extra))
 
 
+def _note(obj: Path) -> Path:
+    """Beside each object: the command that made it, so that other flags compile it again."""
+    return obj.with_suffix(".cmd")
+
+
+def _text(cmd) -> str:
+    return " ".join(map(str, cmd)).replace(str(HERE), ".")
+
+
+def _stale(src: Path, obj: Path, cmd, headers) -> bool:
+    note = _note(obj)
+    return _newer(src, obj, headers) or not note.exists() or note.read_text() != _text(cmd)
+
+
+def _compile(task):
+    obj, cmd = task
+    _note(obj).unlink(missing_ok=True)          # (a compilation that does not end leaves none)
+    out = _run(cmd)
+    _note(obj).write_text(_text(cmd))
+    return out
+
+
 def _run(cmd):
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if r.returncode != 0:
@@ -78,18 +100,18 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -
     tasks = []
     for s in hip_srcs:
         o = OBJ / (s.stem + ".hip.o")
-        if force or _newer(s, o, headers):
-            tasks.append([hipcc, f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17", "-fvisibility=hidden",
-                          "-Wno-unused-result", "-Wno-unused-value", *EXTRA_FLAGS.get(s.name, HIP_FLAGS), "-I", str(CSRC), "-c", str(s),
-                          "-o", str(o)])
+        cmd = [hipcc, f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17", "-fvisibility=hidden",
+               "-Wno-unused-result", "-Wno-unused-value", *EXTRA_FLAGS.get(s.name, HIP_FLAGS), "-I", str(CSRC), "-c", str(s), "-o", str(o)]
+        if force or _stale(s, o, cmd, headers):
+            tasks.append((o, cmd))
     for s in cpp_srcs:
         o = OBJ / (s.stem + ".cpp.o")
-        if force or _newer(s, o, headers):
-            tasks.append(["g++", "-O2", "-fPIC", "-std=c++17", "-fvisibility=hidden", "-pthread", "-I", str(CSRC),
-                          "-c", str(s), "-o", str(o)])
+        cmd = ["g++", "-O2", "-fPIC", "-std=c++17", "-fvisibility=hidden", "-pthread", "-I", str(CSRC), "-c", str(s), "-o", str(o)]
+        if force or _stale(s, o, cmd, headers):
+            tasks.append((o, cmd))
     if tasks:
         with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-            for out in ex.map(_run, tasks):
+            for out in ex.map(_compile, tasks):
                 if verbose and out.strip():
                     print(out)
     hip_objs = [str(OBJ / (s.stem + ".hip.o")) for s in hip_srcs if s.name not in DEV_SRCS]
