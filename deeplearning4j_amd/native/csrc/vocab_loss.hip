@@ -1318,6 +1318,7 @@ struct Plan {
   int op;                                // operand type of the products
   bool pad_w, pad_h;
   bool pair;                             // 16-bit operands: the scores' gradient in two halves
+  int copies;                            // of the scores' gradient: two halves, two layouts, or one copy for each product that reads it
   bool nt;                               // backward products on 256 x 256 tiles from operands laid out along the sum's axis
   bool wtr; int many;                    // dh: W is transposed first, for calls of `many` rows that take part
   int bm, bn, tiles;                     // tiles of the scores
@@ -1365,21 +1366,23 @@ Plan plan(const Args& a) {
   p.pad_h = a.pad_h;
   p.wcp = up(a.wt ? a.V : a.D, 8);
   const int64_t esz = a.dt == DT_F32 ? 4 : 2;                    // halves take as much as fp32
-  // a piece's gradient: 512 MiB (step of 8192 x 2048 of 65536 words: 6.95 ms with 128 MiB, 6.82 with 256, 6.76 with 512, 6.72 with 1024)
-  const int64_t most = ((int64_t)512 << 20) / (p.np * esz) / 256 * 256;
-  p.pieces = (int)(most >= 256 ? (a.V + most - 1) / most : up(a.V, 256) / 256);
-  p.step = (int)up((a.V + p.pieces - 1) / p.pieces, 256);
-  p.pieces = (int)((a.V + p.step - 1) / p.step);
-  p.gcols = up(a.V < p.step ? a.V : p.step, 256);
   // The backward products on 256 x 256 tiles, for which the scores' gradient is written a second time, row by row, and H transposed; against
   // 128 x 128 tiles without that: step of 600 rows x 4096 of 40000 words 841 against 939 us, x 1024 277 and 285, 4096 x 512 of 32000 634 and 683,
   // 2048 x 256 271 and 244, 400 x 1024 of 40000 243 and 240.
   p.nt = p.tile == TILE_BIG && a.N >= 512 && a.D >= 512;
+  p.pair = bits16 && !a.split && a.N <= 256;                       // (see score_kernel)
+  // A piece's gradient with all its copies: 640 MiB. Step of 8192 x 2048 of 65536 words, two copies: 6.95 ms with 256 MiB, 6.82 with 512, 6.76 with 1024
+  // (its 16-bit logits: 1024 MiB); 3001 x 1000 of 50001: 0.99 ms in one piece of 588 MiB, 1.09 in two.
+  p.copies = p.nt || p.pair || (a.split && a.want_h) ? 2 : 1;
+  const int64_t most = ((int64_t)640 << 20) / (p.np * esz * p.copies) / 256 * 256;
+  p.pieces = (int)(most >= 256 ? (a.V + most - 1) / most : up(a.V, 256) / 256);
+  p.step = (int)up((a.V + p.pieces - 1) / p.pieces, 256);
+  p.pieces = (int)((a.V + p.step - 1) / p.step);
+  p.gcols = up(a.V < p.step ? a.V : p.step, 256);
   // W as it lies, through transposing LDS reads, against W transposed first: 2100 rows x 1000 of 50001 words 231 us against 207 + 98; 4096 x 1024 of
   // 32000: 242 and 226 + 47; 8192 x 2048 of 65536: 1820 and 1520 + 188. The transpose costs the same for any number of rows.
   p.many = 6144;
   p.wtr = a.want_h && p.nt && !a.wt && a.N >= p.many;
-  p.pair = bits16 && !a.split && a.N <= 256;                       // (see score_kernel)
   p.pack = a.want_w && !p.nt && (!p.pad_h || p.op == DT_F16);
   const int seg = a.split ? 3 : p.pair ? 2 : 1, bk = bits16 ? 64 : 32;
   const int64_t vk = seg * (up(p.step, bk) / bk), nk = seg * (up(a.N, bk) / bk);   // k-tiles of the two products' sums
@@ -1441,7 +1444,7 @@ struct Work {
     fwd = c.at;
     c.at = 0;
     const int64_t esz = a.dt == DT_F32 ? 4 : 2;
-    gr = c.take<Grad>(1); g = c.take<int>(p.op == DT_F16 ? a.N : 0); t = c.take<int>(p.op == DT_F16 ? a.N : 0); coef = c.take<float>(a.N); G = c.take<char>(p.np * p.gcols * esz * (p.nt || p.pair || (a.split && a.want_h) ? 2 : 1));
+    gr = c.take<Grad>(1); g = c.take<int>(p.op == DT_F16 ? a.N : 0); t = c.take<int>(p.op == DT_F16 ? a.N : 0); coef = c.take<float>(a.N); G = c.take<char>(p.np * p.gcols * esz * p.copies);
     colsum = c.take<float>(a.want_b && !a.K ? (a.N + p.bm - 1) / p.bm * a.V : 0);
     packed = c.take<char>(p.pack ? a.N * p.dp * esz : 0);
     ht = c.take<uint16_t>(a.want_w && p.nt ? a.D * p.np * (a.split ? 2 : 1) : 0);
