@@ -7,7 +7,7 @@
 // with q = exp(z - lse), p = softmax over the K teacher logits / T and P_n = sum_k p_k (1, or 0 for a row without entries).
 //
 // What bounds it: the products. A step is four of 2 N D V operations (scores twice, since they are not kept, and the two gradients). bf16, 8192 x
-// 2048 of 65536 words: 8.8 TFLOP, 6.7 ms (1310 TF/s; the loop alone reaches 1605). One forward of a few rows reads W once: 1 x 768 of 30522 words,
+// 2048 of 65536 words: 8.8 TFLOP, 6.95 ms (1265 TF/s; the loop alone reaches 1605). One forward of a few rows reads W once: 1 x 768 of 30522 words,
 // 47 MB, 12 us (3.9 TB/s) of 19.
 //
 // Forward: a product tile h W^T stays in the accumulators; its epilogue leaves one (max, sum of exp) pair per row and column tile, which
@@ -266,7 +266,7 @@ struct SplitP {
   int gw;                                                // workgroups of W, the others are H's
 };
 constexpr int CHUNKS = 16, AMAX_W = 2048;
-// Bound by reading W (30522 x 768 fp32, 94 MB: 25 us, 3.7 TB/s); the same pass cannot convert, since a word's factor depends on the largest word.
+// Bound by reading W (30522 x 768 fp32, 94 MB: 27 us, 3.5 TB/s); the same pass cannot convert, since a word's factor depends on the largest word.
 // Rows of H and words of a [V, D] table: a wave to a row. Words of a [D, V] table: a lane to four columns, workgroups of 256 columns x a cut of the rows.
 __global__ void __launch_bounds__(256) amax_kernel(const SplitP p) {
   __shared__ float red[16];
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(256) amax_kernel(const SplitP p) {
   if (threadIdx.x == 0) p.tops[blockIdx.x] = top;
 }
 
-// Bound by memory: W read once, written once in halves (30522 x 768: 188 MB, 35 us, 5.3 TB/s from what the caches keep of the pass before).
+// Bound by memory: W read once, written once in halves (30522 x 768: 188 MB, 37 us, 5.1 TB/s from what the caches keep of the pass before).
 // W and the packed rows of H as scaled halves, cut into workgroups as amax_kernel cuts them.
 __global__ void __launch_bounds__(256) split_kernel(const SplitP p) {
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
@@ -1076,7 +1076,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const CoefP p, const PackP
 }
 
 // db from the gradient itself (both halves): with teacher entries the tiles' column sums do not hold them. Eight lanes to a word, 16 bytes each at a
-// time. Bound by reading the gradient (96 rows x 30522 words in halves: 6.6 us; a wave to a word, two bytes a lane, took 10.4).
+// time. Bound by reading the gradient (96 rows x 30522 words in halves: 7.2 us; a wave to a word, two bytes a lane, took 10.4).
 __global__ void __launch_bounds__(256) bias_rows_kernel(const char* __restrict__ G, int64_t ldg, int64_t glo, int dt, int vc, const int* __restrict__ count,
                                                         const int* __restrict__ g, const Grad* __restrict__ gr, void* __restrict__ db, int bdt) {
   const int v = blockIdx.x * 32 + (threadIdx.x >> 3), c = *count, ch = dt == DT_F32 ? 4 : 8;
@@ -1113,7 +1113,7 @@ __global__ void __launch_bounds__(256) bias_rows_kernel(const char* __restrict__
 }
 
 // dh: unit u of the grid owns output tile u % tiles and share u / tiles of the piece's columns; its fp32 tile lives in slab u and is added
-// to by the following pieces. 8192 x 2048 of 65536 words in bf16 1.53 ms (1440 TF/s), 4096 x 1024 of 32000 0.238 ms (1130 TF/s). Which unit owns what depends on the number of rows alone, so the sum's order is fixed.
+// to by the following pieces. 8192 x 2048 of 65536 words in bf16 1.69 ms in four pieces (1300 TF/s; 1.54 in two), 4096 x 1024 of 32000 0.238 ms (1130 TF/s). Which unit owns what depends on the number of rows alone, so the sum's order is fixed.
 //
 // Large tile, W by rows ([V, D]): read as it is (K-major, transposing LDS reads), or transposed first where `many` rows pay for that.
 struct DhP {

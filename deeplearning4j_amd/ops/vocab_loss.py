@@ -150,8 +150,8 @@ def _ld(t):
 def _split(rows, hidden, vocabulary, training):
     """fp32 operands as pairs of halves on the 16-bit matrix cores: three products there take a quarter of one on the fp32 cores, once the rows
     pay for the conversion of the weights (12 bytes an element) and the call for its two launches. Step of 96 rows x 768 against 30522 words:
-    281 us in fp32, 217 us in halves; 64 rows x 512 against 8000 words: 94 and 101 us; one forward of 512 rows x 768 against 30522 words: 232
-    and 121 us, of 128 rows: 78 and 91 us."""
+    261 us in fp32, 204 us in halves, of 40 rows: 186 and 189 us; 64 rows x 512 against 8000 words: 147 and 152 us; one forward of 512 rows x 768
+    against 30522 words: 221 and 121 us, of 128 rows: 74 and 91 us."""
     work = hidden * vocabulary
     return (rows - 40) * work > 150e6 if training else (rows - 150) * work > 600e6
 
@@ -351,7 +351,9 @@ def linear_cross_entropy(hidden, weights, labels, bias=None, ignore_index=-100, 
     Returns the rows' losses (fp32; fp64 for fp64 operands). Differentiable in hidden, weights and bias.
 
     16-bit operands: scores, softmax and all sums in fp32, the scores' gradient is rounded to the operands' type for the two gradient
-    products (fp16: scaled to its range first; up to 256 rows it is kept in two halves). ``plain``: the plain form, whatever the operands."""
+    products (fp16: scaled to its range first; up to 256 rows it is kept in two halves). fp32 operands may run as scaled pairs of fp16 halves, which
+    hold 2^-24 of a value, or 2^-40 of the largest value of the row of hidden states, of the words within 2^8 of the largest one, of the row's
+    gradient. ``plain``: the plain form, whatever the operands."""
     name = "linear_cross_entropy"
     _check_linear(hidden, weights, bias, name)
     _need(labels.dtype in (torch.int32, torch.int64), "%s: labels must be INT32 or INT64" % name)
