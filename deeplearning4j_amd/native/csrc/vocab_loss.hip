@@ -558,8 +558,9 @@ template <class C> constexpr int score_lds(bool grad, int seg) {
 //
 // Statistics: every exponential is taken against ONE reference per quarter wave, the largest score of its 32 rows x 64 columns (on the large
 // tile), instead of the row's maximum: four cross-lane steps in all instead of four per row, and no row waits for its own maximum. A sum of
-// exponentials 2^-100 below the reference is still a sound fp32 number; a row that lies lower, or a reference beyond LARGE, makes the workgroup take
-// the tile again with a reference per row and rounded scores. The 16 lanes that share a row leave their partial sums in LDS, where one thread per row adds them.
+// exponentials down to 2^-64 below the reference keeps what words 2^-62 of it add (at 2^-100 a row that is sure of its word lost all the others,
+// 1.7e-4 of its loss); a row that lies lower, or a reference beyond LARGE, makes the workgroup take the tile again with a reference per row and
+// rounded scores. The 16 lanes that share a row leave their partial sums in LDS, where one thread per row adds them.
 // (A maximum and a sum reduced over the lanes for every row, as the fallback does it, made the epilogue of a 256 x 256 tile as long as seven
 // of its k-tiles.)
 // Bound by the matrix cores: forward of 8192 x 2048 of 65536 words in bf16 1.72 ms (1280 TF/s), 4096 x 1024 of 32000 0.31 ms (860 TF/s: 16 k-tiles
@@ -667,7 +668,7 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
         const float r = sR[(tid / RW * C::WN + w) * 4 + ((tid >> 2) & 3)];
         sM[w * C::BM + tid] = r;
         sS[w * C::BM + tid] = s;
-        low |= (s < 0x1p-100f && n0 + w * CW < p.v1) || fabsf(r) >= LARGE;
+        low |= (s < 0x1p-64f && n0 + w * CW < p.v1) || fabsf(r) >= LARGE;
       }
       if (low) *again = 1;
     }
@@ -745,7 +746,7 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
           const int e1 = p.first[(t + 1) * p.N + n];
           for (int e = p.first[t * p.N + n] + tid % TPR; e < e1; e += TPR) {
             const int64_t o = (int64_t)n * p.K + e;
-            p.zk[o] = sz[r * P4 + p.sidx[o] - n0] * zscale;
+            p.zk[o] = sz[r * P4 + p.sidx[o] - n0];
           }
         }
         __syncthreads();
@@ -856,7 +857,8 @@ __global__ void __launch_bounds__(C::NT) score_kernel(const ScoreP p) {
             const int e1 = p.first[(t + 1) * p.N + n];
             for (int e = p.first[t * p.N + n]; e < e1; ++e) {
               const int64_t o = (int64_t)n * p.K + e;
-              float g = sf[3 * C::BM + tid] * exp2_(p.zk[o] - sf[2 * C::BM + tid]) - sf[C::BM + tid] * p.psum[o];
+              const float l = sf[2 * C::BM + tid], z = fabsf(l) >= LARGE ? below<true>(p.zk[o], zscale, l) : below<false>(p.zk[o], zscale, l);
+              float g = sf[3 * C::BM + tid] * exp2_(z) - sf[C::BM + tid] * p.psum[o];
               if (SEG == 3 && copy == 1) g = pow2(g, lo - p.ew[p.sidx[o]]);
               if (half == 1) g -= O::fl(O::cv(g));
               *reinterpret_cast<OTy*>(smem + (p.sidx[o] - n0) * PITCH + tid * OSZ) = O::cv(g);
@@ -920,7 +922,7 @@ struct CombineP {
   const int* lab;
   const float* ent; const float* sp; const float* zk; int K;    // distillation (ent != null)
   int N, ntiles;
-  float keep, T;
+  float keep, T, zscale;                                        // zscale: of the entries' scores zk
   float* ref; float* inv; float* loss;
 };
 template <int R>
@@ -944,7 +946,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineP p) {
     if (p.ent)
       for (int k = g; k < p.K; k += GR) {
         const float w = p.sp[(int64_t)n * p.K + k];
-        if (w > 0.f) z += w * p.zk[(int64_t)n * p.K + k];
+        if (w > 0.f) z += w * (p.zk[(int64_t)n * p.K + k] * p.zscale);
       }
   }
   sm[g][r] = mx; ss[g][r] = s; sz[g][r] = z;
@@ -959,14 +961,16 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineP p) {
   if (g != 0 || m >= count) return;
   // The normaliser is kept as (reference, 1 / sum): as one number of the size of the scores its rounding would be the row's, some 2^-24 |lse|
   // of every probability at once.
+  // The reference may lie up to 2^64 above the row: the sum's exponent goes to it (exactly, towards the row's own scores), the mantissa has the logarithm.
   float loss;
+  const float top = mx + (float)__builtin_amdgcn_frexp_expf(s), ls = log2_(__builtin_amdgcn_frexp_mantf(s));
   if (p.ent) {
     const float h = p.ent[n];
-    loss = p.T * p.T * (h + LN2 * ((mx - z) + log2_(s)));
+    loss = p.T * p.T * (h + LN2 * ((top - z) + ls));
     if (h != h) mx = h;                                          // nothing sound to distil from: the row's gradient is NaN too
   } else {
     const bool in = p.lab[m] >= 0;
-    loss = in ? LN2 * ((mx - p.keep * p.tz[m] - z) + log2_(s)) : __builtin_nanf("");
+    loss = in ? LN2 * ((top - p.keep * p.tz[m] - z) + ls) : __builtin_nanf("");
     if (!in) mx = loss;                                          // a label outside the vocabulary: loss and gradient of the row are NaN
   }
   p.ref[m] = mx;
@@ -1614,7 +1618,7 @@ int forward(const Args& a, const float* f, hipStream_t st) {
   q.part = w.part; q.tz = w.tz; q.zs = q.smooth_v != 0.f ? w.zs : nullptr;
   if (const int e = scores<false>(q, p.tile, p.op, a.split, false, a.wt, st)) return e;
   CombineP c{w.part, q.zs, w.tz, s.rows, s.count, s.lab, a.K ? s.ent : nullptr, s.sp, s.zk, (int)a.K, (int)a.N, p.tiles, q.keep, f[0],
-             s.ref, s.inv, a.loss};
+             q.invT * LOG2E, s.ref, s.inv, a.loss};
   if (a.N <= 256) hipLaunchKernelGGL((combine_kernel<1>), dim3((unsigned)a.N), dim3(256), 0, st, c);
   else hipLaunchKernelGGL((combine_kernel<8>), dim3((unsigned)((a.N + 7) / 8)), dim3(256), 0, st, c);
   return (int)hipGetLastError();
