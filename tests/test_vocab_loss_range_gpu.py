@@ -150,3 +150,29 @@ def test_all_row_weights_tiny_huge_or_zero(n, d, v, scale, layout):
     got, want = _both(False, h, w, b, y, idx, t, dl, layout)
     for a, e, what in zip(got[1:], want[1:], ("hidden", "weights", "bias")):
         assert torch.isfinite(a).all() and float((a.double() - e).norm()) <= 2e-6 * float(e.norm()), what
+
+
+@pytest.mark.parametrize("layout", ["vd", "dv"])
+@pytest.mark.parametrize("n,d,v", SIZES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("distil", [False, True])
+def test_each_gradient_alone_is_that_of_the_whole_step(n, d, v, dtype, layout, distil):
+    """With words and row weights far enough apart for factors and copies: what is not asked for is left out, the rest has the same bits."""
+    h, w, b, y, idx, t, dl = _inputs(n, d, v, torch.float32, layout)
+    if dtype == torch.float32:
+        w *= 10.0 ** (-6 * torch.rand(v, 1, generator=_gen(5), device=DEV))
+    dl *= 10.0 ** -(torch.arange(n, device=DEV) % 6).float()
+    h, w, b = h.to(dtype), w.to(dtype), b.to(dtype)
+    w = w if layout == "vd" else w.t().contiguous().t()
+
+    def grads(wanted):
+        x = [a.detach().requires_grad_(k in wanted) for k, a in enumerate((h, w, b))]
+        if distil:
+            loss = VL.linear_topk_distillation(x[0], x[1], idx, t, x[2], temperature=1.5)
+        else:
+            loss = VL.linear_cross_entropy(x[0], x[1], y, x[2])
+        return dict(zip(wanted, torch.autograd.grad(loss, [x[k] for k in wanted], dl)))
+    whole = grads((0, 1, 2))
+    for wanted in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2)):
+        for k, g in grads(wanted).items():
+            assert torch.equal(g, whole[k]), (wanted, k)
