@@ -238,10 +238,11 @@ __global__ void __launch_bounds__(256) teacher_kernel(const TeacherP p) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------------ operands
-// Values and halves, four at a time; columns [C, ..) are zeros.
+// Values and halves, four at a time; columns [C, ..) are zeros. (Vector loads from global memory take any multiple of 4 bytes.)
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 __device__ __forceinline__ void load4(const float* x, int c, int C, float (&v)[4]) {
-  if (c + 4 <= C && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
-    const f32x4 f = *reinterpret_cast<const f32x4*>(x);
+  if (c + 4 <= C) {
+    const f32x4 f = *reinterpret_cast<const f32x4_any*>(x);
     v[0] = f[0]; v[1] = f[1]; v[2] = f[2]; v[3] = f[3];
   } else {
 #pragma unroll
@@ -255,19 +256,22 @@ __device__ __forceinline__ void halves(float v, _Float16& hi, _Float16& lo) {
   lo = (_Float16)(d == d ? d : 0.f);                    // inf - inf: an infinity stays in the first half alone
 }
 
+__device__ __forceinline__ int64_t up4(int n) { return ((int64_t)n + 3) / 4 * 4; }   // words of a cut's maxima
 struct SplitP {
   const float* W; int64_t ldw; int wt, V, D;             // [V, D], or [D, V] with wt
   _Float16* wo; int64_t wcp;                             // halves of W, rows of wcp
   const float* H; int64_t ldh; _Float16* ho; int64_t dp, hcap;   // the rows that take part, packed; hcap: rows of one half
   const int* rows; const int* count;
   Scales* sc; int *eh, *ew;
-  float* wmax; int chunks;                               // largest finite |w| of every word ([D, V]: of each of `chunks` cuts of the rows)
+  float* wmax; int cuts;                                 // largest finite |w| of every word ([D, V]: of each of `cuts` cuts of the rows)
+  int chunks;                                            // [D, V]: cuts of the rows among the kernel's workgroups
   float* tops;                                           // the same of every workgroup of W in amax_kernel
-  int gw;                                                // workgroups of W, the others are H's
+  int gw, tw;                                            // workgroups of W, the others are H's; values of tops
 };
-constexpr int CHUNKS = 16, AMAX_W = 2048;
+constexpr int CUTS = 32, TOPS = 2048;
 // Bound by reading W (30522 x 768 fp32, 94 MB: 27 us, 3.5 TB/s); the same pass cannot convert, since a word's factor depends on the largest word.
-// Rows of H and words of a [V, D] table: a wave to a row. Words of a [D, V] table: a lane to four columns, workgroups of 256 columns x a cut of the rows.
+// Rows of H and words of a [V, D] table: a wave to four rows at a time. Words of a [D, V] table: a lane to four columns, workgroups of 256 columns x a cut
+// of the rows.
 __global__ void __launch_bounds__(256) amax_kernel(const SplitP p) {
   __shared__ float red[16];
   __shared__ f32x4 part[4][64];
@@ -279,7 +283,7 @@ __global__ void __launch_bounds__(256) amax_kernel(const SplitP p) {
     for (int u = blockIdx.x; u < units; u += p.gw) {
       const int strip = u / p.chunks, chunk = u - strip * p.chunks, c = strip * 256 + lane * 4, r1 = min(p.D, (chunk + 1) * per);
       float m[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+#pragma unroll 8
       for (int r = chunk * per + wid; r < r1; r += 4) {
         float v[4];
         load4(p.W + r * p.ldw + c, c, p.V, v);
@@ -288,13 +292,14 @@ __global__ void __launch_bounds__(256) amax_kernel(const SplitP p) {
       }
       part[wid][lane] = f32x4{m[0], m[1], m[2], m[3]};
       __syncthreads();
-      if (wid == 0) {
+      if (wid == 0 && c < p.V) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float x = fmaxf(fmaxf(part[0][lane][j], part[1][lane][j]), fmaxf(part[2][lane][j], part[3][lane][j]));
-          if (c + j < p.V) p.wmax[(int64_t)chunk * p.V + c + j] = x;
+          m[j] = x;
           top = fmaxf(top, x);
         }
+        *reinterpret_cast<f32x4*>(p.wmax + chunk * up4(p.V) + c) = f32x4{m[0], m[1], m[2], m[3]};
       }
       __syncthreads();
     }
@@ -345,13 +350,13 @@ __global__ void __launch_bounds__(256) amax_kernel(const SplitP p) {
 }
 
 // Bound by memory: W read once, written once in halves (30522 x 768: 188 MB, 37 us, 5.1 TB/s from what the caches keep of the pass before).
-// W and the packed rows of H as scaled halves, cut into workgroups as amax_kernel cuts them.
+// W and the packed rows of H as scaled halves.
 __global__ void __launch_bounds__(256) split_kernel(const SplitP p) {
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   __shared__ float red[16];
   const bool is_w = (int)blockIdx.x < p.gw;
   float top = 0.f;
-  for (int i = threadIdx.x; i < p.gw; i += 256) top = fmaxf(top, p.tops[i]);
+  for (int i = threadIdx.x; i < p.tw; i += 256) top = fmaxf(top, p.tops[i]);
   top = block_max(top, red);
   if (blockIdx.x == 0 && threadIdx.x == 0) p.sc->top = top;
   const int lo = scale_for(top);
@@ -368,19 +373,25 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitP p) {
       const int strip = u / p.chunks, chunk = u - strip * p.chunks, c = strip * 256 + lane * 4, r1 = min(p.D, (chunk + 1) * per);
       if (c >= p.wcp) continue;
       float f[4];
+      f32x4 m = {0.f, 0.f, 0.f, 0.f};
+      if (c < p.V) {
+#pragma unroll 8
+        for (int k = 0; k < p.cuts; ++k) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(p.wmax + k * up4(p.V) + c);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) m[j] = fmaxf(m[j], x[j]);
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        float m = 0.f;
-        if (c + j < p.V)
-          for (int k = 0; k < p.chunks; ++k) m = fmaxf(m, p.wmax[(int64_t)k * p.V + c + j]);
-        const int e = word_scale(m, lo);
+        const int e = word_scale(m[j], lo);
         f[j] = pow2(1.f, e);
         if (chunk == 0 && wid == 0 && c + j < p.V) {
           p.ew[c + j] = e;
           if (e != lo) p.sc->wide = 1;
         }
       }
-#pragma unroll 2
+#pragma unroll 4
       for (int r = chunk * per + wid; r < r1; r += 4) {
         float v[4];
         load4(p.W + r * p.ldw + c, c, p.V, v);
@@ -389,23 +400,27 @@ __global__ void __launch_bounds__(256) split_kernel(const SplitP p) {
     }
     return;
   }
-  const int R = is_w ? p.V : *p.count, step = (is_w ? p.gw : gridDim.x - p.gw) * 4;
+  // a wave to 1024 values of a row, all its loads ahead of its stores
   const int64_t ldo = is_w ? p.wcp : p.dp, half = is_w ? p.V * p.wcp : p.hcap * p.dp;
-  for (int64_t r = (is_w ? blockIdx.x : blockIdx.x - p.gw) * 4 + wid; r < R; r += step) {
+  const int parts = (int)((ldo + 1023) / 1024);
+  const int64_t n = (int64_t)(is_w ? p.V : *p.count) * parts, step = (int64_t)(is_w ? p.gw : gridDim.x - p.gw) * 4;
+  for (int64_t u = (int64_t)(is_w ? blockIdx.x : blockIdx.x - p.gw) * 4 + wid; u < n; u += step) {
+    const int64_t r = u / parts;
+    const int c0 = (int)(u - r * parts) * 1024 + lane * 4;
     const float* x = is_w ? p.W + r * p.ldw : p.H + p.rows[r] * p.ldh;
-    _Float16* out = (is_w ? p.wo : p.ho) + r * ldo;
+    float v[4][4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) load4(x + c0 + k * 256, c0 + k * 256, p.D, v[k]);
     const int e = is_w ? word_scale(p.wmax[r], lo) : p.eh[r] == ZERO_ROW ? 0 : p.eh[r];
     const float s = pow2(1.f, e), f[4] = {s, s, s, s};
-    if (is_w && lane == 0) {
+    if (is_w && c0 == 0) {
       p.ew[r] = e;
       if (e != lo) p.sc->wide = 1;
     }
-#pragma unroll 2
-    for (int c = lane * 4; c < ldo; c += 256) {
-      float v[4];
-      load4(x + c, c, p.D, v);
-      store4(out + c, half, v, f);
-    }
+    _Float16* out = (is_w ? p.wo : p.ho) + r * ldo + c0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c0 + k * 256 < ldo) store4(out + k * 256, half, v[k], f);
   }
 }
 
@@ -1443,8 +1458,8 @@ struct Work {
   Work(const Args& a, const Plan& p) {
     Carve c(a.ws);
     part = c.take<float2>((int64_t)p.tiles * a.N); tz = c.take<float>(a.N); zs = c.take<float>((int64_t)p.tiles * a.N);
-    wmax = c.take<float>(a.split ? a.V * (a.wt ? CHUNKS : 1) : 0);
-    tops = c.take<float>(a.split ? AMAX_W : 0);
+    wmax = c.take<float>(a.split ? up(a.V, 4) * (a.wt ? CUTS : 1) : 0);
+    tops = c.take<float>(a.split ? TOPS : 0);
     fwd = c.at;
     c.at = 0;
     const int64_t esz = a.dt == DT_F32 ? 4 : 2;
@@ -1594,12 +1609,18 @@ int forward(const Args& a, const float* f, hipStream_t st) {
   hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, a.K ? nullptr : a.labels, (int)a.lab64, a.ignore, s.mass, (int)a.N, (int)a.V, s.rows, s.lab, s.count, s.sc, a.loss);
   VL_CHECK();
   if (a.split) {
-    const int chunks = (int)(a.D < CHUNKS ? 1 : CHUNKS);             // ([D, V]: cuts of the rows)
-    const int64_t units = up(a.V, 256) / 256 * chunks;
+    // [D, V]: as many cuts of the rows as fill the chip once for the largest values (2368 x 20592: 58 us with 25 cuts, 68 with 16), fewer for the
+    // conversion (84 us with 25, 75 with 16)
+    const int64_t strips = up(a.V, 256) / 256, fit = strips < 2048 ? 2048 / strips : 1, most = a.D < 64 ? 1 : CUTS;
+    const int cuts = (int)(fit < most ? fit : most);
+    auto groups = [&](int n) { return (int)(strips * n < TOPS ? strips * n : TOPS); };
     SplitP q{(const float*)a.W, a.ldw, (int)a.wt, (int)a.V, (int)a.D, (_Float16*)s.wo, p.wcp, (const float*)a.H, a.ldh, (_Float16*)s.ho, p.dp, p.np,
-             s.rows, s.count, s.sc, s.eh, s.ew, w.wmax, chunks, w.tops, (int)(a.wt && units < AMAX_W ? units : AMAX_W)};
+             s.rows, s.count, s.sc, s.eh, s.ew, w.wmax, cuts, cuts, w.tops, a.wt ? groups(cuts) : 1024, 0};
     hipLaunchKernelGGL(amax_kernel, dim3(q.gw + 256), dim3(256), 0, st, q);
     VL_CHECK();
+    q.tw = q.gw;
+    q.chunks = cuts < 16 ? cuts : 16;
+    q.gw = a.wt ? groups(q.chunks) : 2048;
     hipLaunchKernelGGL(split_kernel, dim3(q.gw + 256), dim3(256), 0, st, q);
     VL_CHECK();
   }
